@@ -631,6 +631,131 @@ int objb_deepseek_gate_device(const float *d_gate_weight, const float *d_gate_bi
                               size_t hidden_size, size_t top_k, int score_func, float route_scale,
                               int32_t *d_ids, float *d_weights, objb_stream_t stream);
 
+/* ---- dense products of many tokens (no counterpart in the reference, whose
+ * dense paths run one token: objb_gemv_bf16_device, objb_ffn_bf16_device).
+ *
+ * Types are OBJB_DTYPE_* (F32, F16, BF16).  Operands: x and w both BF16, both
+ * F16, x F32 with w BF16, or both F32; y (and residual, z, dy) F32 or, where x
+ * is a 16-bit type, that type; bias F32 or w's type.  Products of 16-bit
+ * operands are exact and summed in f32; an f32 operand enters as three bf16
+ * parts (8 + 8 + 8 bits), so f32 products keep f32's precision.  A non-finite
+ * operand makes its row and column of the product non-finite (Inf or NaN).
+ * Rows are contiguous; strides are in elements between rows, 0 for contiguous.
+ * Any sizes, strides and element-aligned addresses are taken: operands that
+ * the copy engine cannot read (16-byte aligned rows) are laid out again in
+ * the scratch, which costs one pass over them.  Scratch: 256-byte aligned, at
+ * least the matching *_scratch_bytes, in use until the stream has passed the
+ * call; NULL takes the per-(device, stream) workspace, under whose rules (no
+ * first use under capture; graphs captured on one stream share it). */
+enum {
+  OBJB_ACT_NONE = 0,
+  OBJB_ACT_RELU = 1,
+  OBJB_ACT_SILU = 2,
+  OBJB_ACT_GELU = 3,      /* v Phi(v), by erf */
+  OBJB_ACT_GELU_TANH = 4  /* its tanh form */
+};
+
+typedef struct {
+  size_t tokens, in_features, out_features;
+  int32_t x_dtype, w_dtype, y_dtype, bias_dtype;
+  int32_t activation;
+  int32_t reserved; /* 0 */
+  size_t x_stride, w_stride, y_stride, residual_stride, z_stride;
+} objb_linear_desc;
+
+/* y = act(x w^T + bias) + residual for x [tokens][in], w [out][in], bias
+ * [out] (may be NULL), residual [tokens][out] (may be NULL, or y itself with
+ * y's stride).  z (may be NULL) receives x w^T + bias in y's type. */
+int objb_linear_scratch_bytes(const objb_linear_desc *desc, size_t *bytes);
+int objb_linear_device(const objb_linear_desc *desc, const void *d_x, const void *d_w,
+                       const void *d_bias, const void *d_residual, void *d_y, void *d_z,
+                       void *d_scratch, size_t scratch_bytes, objb_stream_t stream);
+
+/* objb_linear_backward_desc.outputs */
+enum { OBJB_LINEAR_DX = 1, OBJB_LINEAR_DW = 2, OBJB_LINEAR_DBIAS = 4 };
+
+typedef struct {
+  size_t tokens, in_features, out_features;
+  int32_t x_dtype, w_dtype, dy_dtype, dw_dtype; /* dw: w's type or F32 */
+  int32_t activation;
+  int32_t outputs;    /* OBJB_LINEAR_* of the gradients wanted */
+  int32_t accumulate; /* nonzero: dw += and dbias +=, else they are set */
+  int32_t reserved;   /* 0 */
+  size_t dy_stride, z_stride, x_stride, w_stride, dx_stride, dw_stride;
+} objb_linear_backward_desc;
+
+/* The gradients of y = act(z), z = x w^T + bias, from dy [tokens][out]:
+ * dz = dy act'(z), dx = dz w (x's type), dw = dz^T x, dbias = sum_t dz (f32).
+ * z (dy's type) is the one objb_linear_device kept; without an activation it
+ * is not read.  Under a 16-bit dy, dz enters the two products rounded to that
+ * type, unless dw is F32 (then dz keeps f32's precision); dbias sums it
+ * unrounded.  The residual's gradient is dy.  F32 dy with F16 x is
+ * unsupported.  All sums are folded in a fixed order. */
+int objb_linear_backward_scratch_bytes(const objb_linear_backward_desc *desc, size_t *bytes);
+int objb_linear_backward_device(const objb_linear_backward_desc *desc, const void *d_dy,
+                                const void *d_z, const void *d_x, const void *d_w, void *d_dx,
+                                void *d_dw, float *d_dbias, void *d_scratch,
+                                size_t scratch_bytes, objb_stream_t stream);
+
+/* objb_ffn_bf16_device for num_tokens tokens (the shared expert of a batch):
+ * out[t] = residual[t] + down SwiGLU(gate x_t, up x_t), the SwiGLU (and its
+ * limit) as silu_mul computes it (moe.cu:2-22).  x [tokens][hidden], out and
+ * residual [tokens][out_dim] f32, contiguous; residual may be NULL, or out
+ * itself (routed output + shared output); weights bf16 as there. */
+int objb_ffn_bf16_tokens_scratch_bytes(size_t num_tokens, size_t hidden, size_t intermediate,
+                                       size_t out_dim, size_t *bytes);
+int objb_ffn_bf16_tokens_device(const void *d_gate, const void *d_up, const void *d_down,
+                                size_t hidden, size_t intermediate, size_t out_dim,
+                                const float *d_x, size_t num_tokens, const float *d_residual,
+                                float *d_out, float swiglu_limit, void *d_scratch,
+                                size_t scratch_bytes, objb_stream_t stream);
+
+/* ---- training the router on frozen experts (no counterpart in the reference).
+ * score_func: 0 softmax (the router), 1 sigmoid, 2 sqrt-softplus (the gate,
+ * with its branches), as objb_deepseek_gate_device.  Tokens that count: those
+ * of a sequence [d_seq_offsets[q], d_seq_offsets[q+1]) (ascending int32
+ * [num_seqs + 1]; NULL: all tokens are sequence 0) whose d_token_mask byte
+ * (may be NULL) is nonzero.  Ids outside 0..num_experts-1 count nowhere. */
+
+/* Per-expert counts [num_seqs][num_experts], counted tokens per sequence, and
+ * d_losses = { balance, z } with p the scores shared out to 1 per token:
+ *   balance = 1/S' sum_q sum_e (E counts[q][e] / (k n_q)) (1/n_q sum_t p[t][e])
+ *   z       = 1/N sum_t logsumexp(l_t)^2
+ * (n_q counted tokens of q, S' sequences that have any, N counted tokens; 0
+ * without any).  d_scales [num_seqs + 1] receives the gradients' factors
+ * E / (k n_q^2 S') and 2 / N for objb_router_backward_device.  Scratch as
+ * above.  Sums over tokens are folded in a fixed order. */
+int objb_balance_loss_scratch_bytes(size_t num_tokens, size_t num_experts, size_t num_seqs,
+                                    size_t *bytes);
+int objb_balance_loss_device(const float *d_logits, size_t logits_stride, const int32_t *d_ids,
+                             const uint8_t *d_token_mask, const int32_t *d_seq_offsets,
+                             size_t num_seqs, size_t num_tokens, size_t num_experts,
+                             size_t top_k, int score_func, int32_t *d_counts,
+                             int32_t *d_seq_tokens, float *d_losses, float *d_scales,
+                             void *d_scratch, size_t scratch_bytes, objb_stream_t stream);
+
+/* The whole gradient of the logits in one pass: through the routing weights
+ * w_j = route_scale * s[ids_j] (divided by sum_j s[ids_j] when renormalize;
+ * their gradient d_dweights [num_tokens][top_k] may be NULL), plus
+ * balance_grad and z_grad times the gradients of the two losses (d_counts and
+ * d_scales of objb_balance_loss_device; both NULL: no losses).  Rows of
+ * tokens that do not count become 0.  d_dlogits may be d_logits. */
+int objb_router_backward_device(const float *d_logits, size_t logits_stride,
+                                const int32_t *d_ids, const float *d_dweights,
+                                const uint8_t *d_token_mask, const int32_t *d_seq_offsets,
+                                size_t num_seqs, const int32_t *d_counts, const float *d_scales,
+                                size_t num_tokens, size_t num_experts, size_t top_k,
+                                int score_func, int renormalize, float route_scale,
+                                float balance_grad, float z_grad, float *d_dlogits,
+                                size_t dlogits_stride, objb_stream_t stream);
+
+/* The routing weights' gradient of objb_moe_combine_device: d_dweights[t][j] =
+ * sum_i d_dout[t][i] * d_v[d_slot_row[t][j]][i].  A row out of range is read
+ * as row 0 and flagged (device error word bit 8). */
+int objb_moe_combine_backward_device(const float *d_dout, const float *d_v, size_t v_rows,
+                                     const int32_t *d_slot_row, size_t num_tokens, size_t top_k,
+                                     size_t out_dim, float *d_dweights, objb_stream_t stream);
+
 /* ---- official DeepSeek arithmetic: activations quantized to F8_E4M3 with one
  * E8M0 scale per 128 values (deepseek.rs:1444-1525 for the codecs). */
 

@@ -1,0 +1,175 @@
+"""Training a router on frozen experts: load counts, balance and z losses, and
+the gradients of the router's logits and of the routing weights.
+
+A step over T tokens, beside ``router_topk_batched`` / ``deepseek_gate``,
+``ExpertParallelMoe`` or ``moe_pairs`` and ``moe_combine``::
+
+    logits = linear(x, w_router)                       # dense.py
+    ids, w = router_topk_batched(logits, k, renormalize=True)
+    bal = balance_loss(logits, ids)
+    ... v = moe_pairs(...); out = moe_combine(v, slot_row, w, out) ...
+    dw = moe_combine_backward(dout, v, slot_row)
+    dlogits = router_backward(logits, ids, dw, renormalize=True, balance=bal,
+                              balance_grad=1e-2, z_grad=1e-3)
+    _, dw_router, _ = linear_backward(dlogits, x, w_router, need_dx=False)
+
+The reference has no training; the scores are those of its router and gate
+(crates/objeta-cuda/src/bin/deepseek_single_layer_moe.rs:720-740, 768-881).
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+from . import _lib
+from ._launch import launch, on_device, row_stride
+from .ep import SOFTMAX
+
+c_size = ctypes.c_size_t
+c_int = ctypes.c_int
+c_float = ctypes.c_float
+c_void_p = ctypes.c_void_p
+
+_lib.register_signatures({
+    "objb_balance_loss_scratch_bytes": (c_int, [c_size, c_size, c_size, ctypes.POINTER(c_size)]),
+    "objb_balance_loss_device": (c_int, [c_void_p, c_size, c_void_p, c_void_p, c_void_p, c_size, c_size, c_size,
+                                         c_size, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size,
+                                         c_void_p]),
+    "objb_router_backward_device": (c_int, [c_void_p, c_size, c_void_p, c_void_p, c_void_p, c_void_p, c_size,
+                                            c_void_p, c_void_p, c_size, c_size, c_size, c_int, c_int, c_float,
+                                            c_float, c_float, c_void_p, c_size, c_void_p]),
+    "objb_moe_combine_backward_device": (c_int, [c_void_p, c_void_p, c_size, c_void_p, c_size, c_size, c_size,
+                                                 c_void_p, c_void_p]),
+})
+
+
+@dataclass
+class BalanceLoss:
+    """What ``balance_loss`` returns; ``router_backward`` takes it back."""
+    balance: object      # f32 scalar tensor
+    z: object            # f32 scalar tensor
+    counts: object       # int32 [S, E]: selections of each expert
+    tokens: object       # int32 [S]: counted tokens
+    scales: object       # f32 [S + 1]: gradient factors (E / (k n^2 S'), then 2 / N)
+    score_func: int
+    seq_offsets: object
+    token_mask: object
+
+
+def _p(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _routing(d_logits, d_ids, score_func, d_seq_offsets, d_token_mask):
+    import torch
+    dev = on_device("d_logits", d_logits, dtypes=(torch.float32,), contiguous=False)
+    ld = row_stride("d_logits", d_logits)
+    T, E = d_logits.shape
+    on_device("d_ids", d_ids, dev, (torch.int32,))
+    if d_ids.dim() != 2 or d_ids.shape[0] != T:
+        raise ValueError(f"d_ids has shape {tuple(d_ids.shape)}, expected ({T}, top_k)")
+    if d_token_mask is not None:
+        on_device("d_token_mask", d_token_mask, dev, (torch.bool, torch.uint8), (T,))
+    if d_seq_offsets is not None:
+        on_device("d_seq_offsets", d_seq_offsets, dev, (torch.int32,))
+        if d_seq_offsets.dim() != 1 or d_seq_offsets.numel() < 2:
+            raise ValueError("d_seq_offsets: expected [num_seqs + 1] offsets")
+    return dev, ld, T, E, d_ids.shape[1], 1 if d_seq_offsets is None else d_seq_offsets.numel() - 1
+
+
+def balance_loss(d_logits, d_ids, score_func: int = SOFTMAX, d_seq_offsets=None, d_token_mask=None,
+                 stream=None) -> BalanceLoss:
+    """Per-expert counts and the balance and z losses of a routed batch.
+
+    d_logits f32 [T, E] (rows may be strided), d_ids int32 [T, k] the selected
+    experts (entries outside 0..E-1, such as the gate's -1, count nowhere).
+    ``d_seq_offsets`` int32 [S + 1], ascending: sequence q holds tokens
+    [off[q], off[q+1]); tokens before the first and behind the last belong to
+    none.  Without it all tokens are one sequence.  ``d_token_mask`` bool [T]:
+    tokens to count.  With p the scores shared out to 1 per token, n_q the
+    counted tokens of q, S' the sequences that have any and N all of them:
+
+    * balance = 1/S' sum_q sum_e (E counts[q, e] / (k n_q)) (1/n_q sum_t p[t, e])
+    * z = 1/N sum_t logsumexp(l_t)^2
+
+    (both 0 where no token counts).  A token whose logits are all -inf counts
+    but adds nothing to either.  Sums over tokens are folded in a fixed order:
+    the same call gives the same bits.
+    """
+    import torch
+    dev, ld, T, E, k, S = _routing(d_logits, d_ids, score_func, d_seq_offsets, d_token_mask)
+    with launch(dev, stream) as st:
+        n = c_size()
+        _lib.call("objb_balance_loss_scratch_bytes", T, E, S, ctypes.byref(n))
+        scratch = torch.empty(int(n.value), dtype=torch.uint8, device=dev)
+        ints = torch.empty(S * (E + 1), dtype=torch.int32, device=dev)
+        floats = torch.empty(S + 3, dtype=torch.float32, device=dev)
+        counts, tokens = ints[:S * E].view(S, E), ints[S * E:]
+        losses, scales = floats[:2], floats[2:]
+        _lib.call("objb_balance_loss_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), _p(d_token_mask),
+                  _p(d_seq_offsets), S, T, E, k, int(score_func), counts.data_ptr(), tokens.data_ptr(),
+                  losses.data_ptr(), scales.data_ptr(), scratch.data_ptr(), scratch.numel(), st)
+    return BalanceLoss(losses[0], losses[1], counts, tokens, scales, int(score_func), d_seq_offsets, d_token_mask)
+
+
+def router_backward(d_logits, d_ids, d_dweights=None, score_func: int = SOFTMAX, renormalize: bool = False,
+                    route_scale: float = 1.0, balance: BalanceLoss | None = None, balance_grad: float = 0.0,
+                    z_grad: float = 0.0, d_token_mask=None, d_dlogits=None, stream=None):
+    """The gradient of the router's logits, f32 [T, E], in one pass.
+
+    ``d_dweights`` f32 [T, k] (or None): the gradient of the routing weights
+    w_j = route_scale * s[ids_j], divided by sum_j s[ids_j] with
+    ``renormalize`` (``router_topk_batched``: softmax, scale 1;
+    ``deepseek_gate``: its score function and scale, renormalised unless
+    softmax).  ``balance``: the ``balance_loss`` result of the same logits and
+    ids, whose two losses enter with the factors ``balance_grad`` and
+    ``z_grad``; its offsets and mask then say which tokens count (else
+    ``d_token_mask``).  Rows of tokens that do not count are zero.
+    ``d_dlogits`` may be ``d_logits`` itself.
+    """
+    import torch
+    off = None
+    if balance is not None:
+        if int(score_func) != balance.score_func:
+            raise ValueError(f"score_func {score_func} differs from the balance loss's {balance.score_func}")
+        if d_token_mask is not None:
+            raise ValueError("the token mask of a call with a balance loss is the balance loss's")
+        off, d_token_mask = balance.seq_offsets, balance.token_mask
+    dev, ld, T, E, k, S = _routing(d_logits, d_ids, score_func, off, d_token_mask)
+    if balance is not None:
+        on_device("balance.counts", balance.counts, dev, (torch.int32,), (S, E))
+    if d_dweights is not None:
+        on_device("d_dweights", d_dweights, dev, (torch.float32,), (T, k))
+    with launch(dev, stream) as st:
+        if d_dlogits is None:
+            d_dlogits = torch.empty(T, E, dtype=torch.float32, device=dev)
+        else:
+            on_device("d_dlogits", d_dlogits, dev, (torch.float32,), (T, E), contiguous=False)
+        _lib.call("objb_router_backward_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), _p(d_dweights),
+                  _p(d_token_mask), _p(off), S, _p(balance.counts) if balance is not None else None,
+                  _p(balance.scales) if balance is not None else None, T, E, k, int(score_func),
+                  int(bool(renormalize)), float(route_scale), float(balance_grad), float(z_grad),
+                  d_dlogits.data_ptr(), row_stride("d_dlogits", d_dlogits), st)
+    return d_dlogits
+
+
+def moe_combine_backward(d_dout, d_v, slot_row, d_dw=None, stream=None):
+    """The routing weights' gradient of ``moe_combine``: dw[t, j] = sum_o
+    d_dout[t, o] * d_v[slot_row[t, j], o], f32 [T, k].  A row outside d_v is
+    read as row 0 and flagged (device error word bit 8), as the combine does."""
+    import torch
+    dev = on_device("d_dout", d_dout, dtypes=(torch.float32,))
+    on_device("d_v", d_v, dev, (torch.float32,))
+    on_device("slot_row", slot_row, dev, (torch.int32,))
+    if d_dout.dim() != 2 or d_v.dim() != 2 or slot_row.dim() != 2:
+        raise ValueError("expected d_dout [T, O], d_v [V, O] and slot_row [T, k]")
+    T, k = slot_row.shape
+    on_device("d_dout", d_dout, dev, shape=(T, d_v.shape[1]))
+    with launch(dev, stream) as st:
+        if d_dw is None:
+            d_dw = torch.empty(T, k, dtype=torch.float32, device=dev)
+        else:
+            on_device("d_dw", d_dw, dev, (torch.float32,), (T, k))
+        _lib.call("objb_moe_combine_backward_device", d_dout.data_ptr(), d_v.data_ptr(), d_v.shape[0],
+                  slot_row.data_ptr(), T, k, d_v.shape[1], d_dw.data_ptr(), st)
+    return d_dw
