@@ -644,8 +644,8 @@ int objb_deepseek_gate_device(const float *d_gate_weight, const float *d_gate_bi
  * Any sizes, strides and element-aligned addresses are taken: operands that
  * the copy engine cannot read (16-byte aligned rows) are laid out again in
  * the scratch, which costs one pass over them.  Scratch: 256-byte aligned, at
- * least the matching *_scratch_bytes, in use until the stream has passed the
- * call; NULL takes the per-(device, stream) workspace, under whose rules (no
+ * least the matching *_scratch_bytes (of the same operands: their alignment
+ * counts, nothing is read), in use until the stream has passed the call; NULL takes the per-(device, stream) workspace, under whose rules (no
  * first use under capture; graphs captured on one stream share it). */
 enum {
   OBJB_ACT_NONE = 0,
@@ -666,7 +666,8 @@ typedef struct {
 /* y = act(x w^T + bias) + residual for x [tokens][in], w [out][in], bias
  * [out] (may be NULL), residual [tokens][out] (may be NULL, or y itself with
  * y's stride).  z (may be NULL) receives x w^T + bias in y's type. */
-int objb_linear_scratch_bytes(const objb_linear_desc *desc, size_t *bytes);
+int objb_linear_scratch_bytes(const objb_linear_desc *desc, const void *d_x, const void *d_w,
+                              size_t *bytes);
 int objb_linear_device(const objb_linear_desc *desc, const void *d_x, const void *d_w,
                        const void *d_bias, const void *d_residual, void *d_y, void *d_z,
                        void *d_scratch, size_t scratch_bytes, objb_stream_t stream);
@@ -689,9 +690,10 @@ typedef struct {
  * z (dy's type) is the one objb_linear_device kept; without an activation it
  * is not read.  Under a 16-bit dy, dz enters the two products rounded to that
  * type, unless dw is F32 (then dz keeps f32's precision); dbias sums it
- * unrounded.  The residual's gradient is dy.  F32 dy with F16 x is
- * unsupported.  All sums are folded in a fixed order. */
-int objb_linear_backward_scratch_bytes(const objb_linear_backward_desc *desc, size_t *bytes);
+ * unrounded.  The residual's gradient is dy.  All sums are folded in a fixed
+ * order. */
+int objb_linear_backward_scratch_bytes(const objb_linear_backward_desc *desc, const void *d_dy,
+                                       const void *d_x, const void *d_w, size_t *bytes);
 int objb_linear_backward_device(const objb_linear_backward_desc *desc, const void *d_dy,
                                 const void *d_z, const void *d_x, const void *d_w, void *d_dx,
                                 void *d_dw, float *d_dbias, void *d_scratch,
@@ -702,8 +704,9 @@ int objb_linear_backward_device(const objb_linear_backward_desc *desc, const voi
  * limit) as silu_mul computes it (moe.cu:2-22).  x [tokens][hidden], out and
  * residual [tokens][out_dim] f32, contiguous; residual may be NULL, or out
  * itself (routed output + shared output); weights bf16 as there. */
-int objb_ffn_bf16_tokens_scratch_bytes(size_t num_tokens, size_t hidden, size_t intermediate,
-                                       size_t out_dim, size_t *bytes);
+int objb_ffn_bf16_tokens_scratch_bytes(const void *d_gate, const void *d_up, const void *d_down,
+                                       size_t hidden, size_t intermediate, size_t out_dim,
+                                       size_t num_tokens, size_t *bytes);
 int objb_ffn_bf16_tokens_device(const void *d_gate, const void *d_up, const void *d_down,
                                 size_t hidden, size_t intermediate, size_t out_dim,
                                 const float *d_x, size_t num_tokens, const float *d_residual,

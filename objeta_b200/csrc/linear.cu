@@ -6,94 +6,142 @@
 //   y  [t][o]: A = w [o][i],       B = x  [t][i],       k = i
 //   dx [t][i]: A = w^T (k rows),   B = dz [t][o],       k = o
 //   dw [o][i]: A = x^T (k rows),   B = dz^T (k rows),   k = t
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <mutex>
 #include <string>
 
 #include "objb_common.h"
 #include "objb_host_launch.cuh"
 #include "objb_launch.h"
-#include "objb_linear.cuh"
-#include "objb_moe.cuh"
+#include "objb_linear_gemm.cuh"
 
 namespace objb {
 namespace dev {
 
-// An operand in memory: element (row, k) at row * ld + k, or k * ld + row
-// where k runs over the memory's rows.
-struct Operand {
-  const void* p;
-  size_t ld;
-  int dtype;
-  bool k_rows;
-};
-
-__device__ __forceinline__ float operand_at(const Operand& o, size_t row, size_t k) {
-  return load_elem(o.p, o.dtype, o.k_rows ? k * o.ld + row : row * o.ld + k);
-}
-
-// 64 x 64 tile, 16 x 16 threads of 4 x 4 elements, 16 of k at a time.
-__global__ void __launch_bounds__(256) gemm_kernel(const Operand A, const Operand B, int M, long long N, long long K,
-                                                   const LinearEpilogue epi) {
-  __shared__ float as[16][65], bs[16][65];
-  const int m0 = blockIdx.x * 64;
-  const long long n0 = static_cast<long long>(blockIdx.y) * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (long long k0 = 0; k0 < K; k0 += 16) {
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-      const int ra = A.k_rows ? i & 63 : i >> 4, ka = A.k_rows ? i >> 6 : i & 15;
-      const int rb = B.k_rows ? i & 63 : i >> 4, kb = B.k_rows ? i >> 6 : i & 15;
-      as[ka][ra] = m0 + ra < M && k0 + ka < K ? operand_at(A, m0 + ra, k0 + ka) : 0.0f;
-      bs[kb][rb] = n0 + rb < N && k0 + kb < K ? operand_at(B, n0 + rb, k0 + kb) : 0.0f;
+// 8 neighbouring elements as f32; VEC: their address is 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ void load8(const void* p, int dtype, size_t at, int n, float (&v)[8]) {
+  if constexpr (VEC) {
+    if (n >= 8) {
+      if (dtype == OBJB_DTYPE_F32) {
+        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+        const float4 a = q[0], b = q[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      } else {
+        const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint16_t h = static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)));
+          v[i] = dtype == OBJB_DTYPE_BF16 ? __uint_as_float(static_cast<uint32_t>(h) << 16)
+                                          : __half2float(__ushort_as_half(h));
+        }
+      }
+      return;
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[k][tx + 16 * j], bs[k][ty + 16 * i], acc[i][j]);
-    __syncthreads();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + tx + 16 * j;
-      const long long n = n0 + ty + 16 * i;
-      if (m < M && n < N) epi.put(m, n, acc[i][j]);
-    }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? load_elem(p, dtype, at + i) : 0.0f;
 }
 
-// dz = dy act'(z), rounded to dz's type, and column sums of runs of rows.
+// 8 elements of an image row (its pitch is a whole number of 16-byte quads):
+// one plane of `dtype`, or the first `planes` bf16 parts.
+__device__ __forceinline__ void store_image8(uint16_t* img, size_t plane, size_t at, int planes, int dtype,
+                                             const float (&v)[8]) {
+  uint32_t u[3][4] = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint16_t h[3] = {};
+    if (planes == 1) {
+      h[0] = dtype == OBJB_DTYPE_F16 ? __half_as_ushort(__float2half_rn(v[i]))
+                                     : __bfloat16_as_ushort(__float2bfloat16_rn(v[i]));
+    } else {
+      __nv_bfloat16 b[3];
+      split3(v[i], b);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) h[j] = __bfloat16_as_ushort(b[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) u[j][i >> 1] |= static_cast<uint32_t>(h[j]) << (16 * (i & 1));
+  }
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (j < planes)
+      *reinterpret_cast<uint4*>(img + j * plane + at) = make_uint4(u[j][0], u[j][1], u[j][2], u[j][3]);
+}
+
+// An operand laid out for the copy engine: rows of `pitch` elements (a multiple
+// of 8), f32 in planes.  8 elements per thread.
+template <bool VEC>
+__global__ void __launch_bounds__(256) image_kernel(const void* src, int dtype, size_t ld, long long rows, int cols,
+                                                    uint16_t* img, int pitch, int planes) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int quads = pitch / 8;
+  const long long n = rows * quads;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
+    const long long r = i / quads;
+    const int c = static_cast<int>(i - r * quads) * 8;
+    float v[8];
+    load8<VEC>(src, dtype, r * ld + c, cols - c, v);
+    store_image8(img, rows * static_cast<size_t>(pitch), r * static_cast<size_t>(pitch) + c, planes, dtype, v);
+  }
+}
+
+// dz = dy act'(z) as an image (may be null: only its sums), and the column
+// sums of each run of rows.  A block: 256 columns (8 per thread), 8 rows at a
+// time; the 8 row lanes are folded in order.
+template <bool VEC>
 __global__ void __launch_bounds__(256) dz_kernel(const void* dy, size_t ldy, const void* z, size_t ldz, int dtype,
-                                                 int act, long long T, int N, void* dz, int dz_dtype,
+                                                 int act, long long T, int N, uint16_t* img, int pitch, int planes,
                                                  long long rows_per, float* part) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= N) return;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float sm[8][256];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 256 + tx * 8;
   const long long r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < T ? r0 + rows_per : T;
-  float s = 0.0f;
-  for (long long r = r0; r < r1; ++r) {
-    float v = load_elem(dy, dtype, r * ldy + c);
-    if (act != OBJB_ACT_NONE) v *= act_grad(act, load_elem(z, dtype, r * ldz + c));
-    if (dz) store_elem(dz, dz_dtype, r * N + c, v);
-    s += v;
+  float s[8] = {};
+  if (c < N) {
+    for (long long r = r0 + ty; r < r1; r += 8) {
+      float v[8];
+      load8<VEC>(dy, dtype, r * ldy + c, N - c, v);
+      if (act != OBJB_ACT_NONE) {
+        float zz[8];
+        load8<VEC>(z, dtype, r * ldz + c, N - c, zz);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= act_grad(act, zz[i]);
+      }
+      if (img) store_image8(img, T * static_cast<size_t>(pitch), r * static_cast<size_t>(pitch) + c, planes, dtype, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += v[i];
+    }
   }
-  if (part) part[static_cast<size_t>(blockIdx.y) * N + c] = s;
+  if (!part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sm[ty][tx * 8 + i] = s[i];
+  __syncthreads();
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col >= N) return;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += sm[i][threadIdx.x];
+  part[static_cast<size_t>(blockIdx.y) * N + col] = sum;
 }
 
 __global__ void __launch_bounds__(256) dbias_kernel(const float* part, int parts, int N, float* db, int accumulate) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= N) return;
   float s = 0.0f;
+#pragma unroll 8
   for (int i = 0; i < parts; ++i) s += part[static_cast<size_t>(i) * N + c];
   db[c] = accumulate ? db[c] + s : s;
-}
-
-__global__ void __launch_bounds__(256) swiglu_kernel(const float* g, const float* u, float* act, size_t n,
-                                                     float limit) {
-  const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < n) act[i] = swiglu(g[i], u[i], limit);
 }
 
 }  // namespace dev
@@ -106,13 +154,197 @@ constexpr size_t kMaxTokens = size_t{1} << 30;
 size_t r256(size_t b) { return (b + 255) / 256 * 256; }
 size_t elem_bytes(int dtype) { return dtype == OBJB_DTYPE_F32 ? 4 : 2; }
 
-int gemm(const dev::Operand& A, const dev::Operand& B, size_t M, size_t N, size_t K, const dev::LinearEpilogue& e,
-         cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>((M + 63) / 64), static_cast<unsigned>((N + 63) / 64));
-  dev::gemm_kernel<<<grid, 256, 0, st>>>(A, B, static_cast<int>(M), static_cast<long long>(N),
-                                         static_cast<long long>(K), e);
-  OBJB_CUDA(cudaGetLastError(), "launch dense product");
+// A 16-bit matrix as the copy engine reads it: 16-byte aligned, rows of `ld`
+// elements (a multiple of 8), `planes` of them `rows * ld` apart.
+struct Image {
+  const void* p = nullptr;
+  size_t ld = 0, rows = 0, cols = 0;
+  int planes = 1;
+  int dtype = 0;  // OBJB_DTYPE_BF16 or F16
+};
+
+// How an operand becomes an image: as it lies, or laid out in the scratch.
+struct ImagePlan {
+  bool direct = false;
+  int planes = 1;
+  size_t pitch = 0, bytes = 0;
+};
+ImagePlan plan_image(const void* p, int dtype, size_t ld, size_t rows, size_t cols, int planes) {
+  ImagePlan i;
+  i.planes = planes;
+  i.direct = planes == 1 && dtype != OBJB_DTYPE_F32 && aligned16(p) && ld % 8 == 0;
+  i.pitch = i.direct ? ld : (cols + 7) / 8 * 8;
+  i.bytes = i.direct ? 0 : r256(static_cast<size_t>(planes) * rows * i.pitch * 2);
+  return i;
+}
+
+int make_image(const ImagePlan& pl, const void* p, int dtype, size_t ld, size_t rows, size_t cols, void* scratch,
+               const DeviceProps& props, cudaStream_t st, Image* out) {
+  out->rows = rows;
+  out->cols = cols;
+  out->planes = pl.planes;
+  out->ld = pl.pitch;
+  out->dtype = pl.planes > 1 || dtype == OBJB_DTYPE_F32 ? OBJB_DTYPE_BF16 : dtype;
+  if (pl.direct) {
+    out->p = p;
+    return OBJB_OK;
+  }
+  out->p = scratch;
+  const size_t n = rows * (pl.pitch / 8);
+  const int grid = static_cast<int>(std::min<size_t>((n + 255) / 256, static_cast<size_t>(props.sm_count) * 16));
+  const bool vec = aligned16(p) && ld % 8 == 0;
+  auto k = vec ? dev::image_kernel<true> : dev::image_kernel<false>;
+  return launch_pdl(k, grid, 256, 0, st, p, dtype, ld, static_cast<long long>(rows), static_cast<int>(cols),
+                    static_cast<uint16_t*>(scratch), static_cast<int>(pl.pitch), pl.planes);
+}
+
+// The tensor map of an image: box of 64 elements by `box_rows` rows.
+int encode(CUtensorMap* map, const Image& im, int box_rows) {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  if (!fn) return OBJB_FAIL(OBJB_ERR_DRIVER, "dense product", "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[3] = {im.cols, im.rows, static_cast<cuuint64_t>(im.planes)};
+  const cuuint64_t strides[2] = {im.ld * 2, im.rows * im.ld * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r =
+      fn(map, im.dtype == OBJB_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+         const_cast<void*>(im.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return OBJB_FAIL(OBJB_ERR_DRIVER, "dense product", "cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
   return OBJB_OK;
+}
+
+struct Product {
+  int maj = dev::kMajKK;
+  Image a, a2, b;  // a2: the up rows of a gated product
+  bool gated = false;
+  size_t M = 0, N = 0, K = 0;
+  dev::LinearEpilogue epi;
+  float swiglu_limit = 0.0f;
+};
+
+constexpr int kLinRing = 200 * 1024;  // bytes of stages
+
+template <int MAJ, int BN, int CG, bool GATED>
+int launch_gemm(const Product& p, dev::GemmArgs g, int device, const DeviceProps& props, cudaStream_t st) {
+  constexpr int kBPlane = BN / CG * 128;
+  const int mt = (GATED ? 64 : 128) * CG;
+  g.tiles_m = static_cast<int>((p.M + mt - 1) / mt);
+  g.tiles_n = static_cast<int>((p.N + BN - 1) / BN);
+  const uint32_t stage = p.a.planes * dev::kLinAPlane + p.b.planes * kBPlane;
+  g.nstages = std::max(2, std::min<int>(dev::kLinStagesMax, kLinRing / static_cast<int>(stage)));
+  const size_t smem = g.nstages * static_cast<size_t>(stage) + 1024;
+  const uint32_t half = p.a.dtype == OBJB_DTYPE_F16 ? 0 : 1;
+  g.idesc = (1u << 4) | (half << 7) | (half << 10) | (static_cast<uint32_t>(MAJ != dev::kMajKK) << 15) |
+            (static_cast<uint32_t>(MAJ == dev::kMajMN) << 16) | (static_cast<uint32_t>(BN >> 3) << 17) |
+            (static_cast<uint32_t>(128 * CG >> 4) << 24);
+  CUtensorMap ma, ma2, mb;
+  OBJB_TRY(encode(&ma, p.a, MAJ == dev::kMajKK ? (GATED ? 64 : 128) : 64));
+  if (GATED)
+    OBJB_TRY(encode(&ma2, p.a2, 64));
+  else
+    ma2 = ma;
+  OBJB_TRY(encode(&mb, p.b, MAJ == dev::kMajMN ? 64 : BN / CG));
+  auto kernel = dev::lin_gemm_kernel<MAJ, BN, CG, GATED>;
+  OBJB_TRY(ensure_smem_attr(kernel, device, smem));
+  const long long tiles = static_cast<long long>(g.tiles_m) * g.tiles_n;
+  const int csize = CG == 2 ? 2 : g.split;
+  const bool one_each = GATED || g.split > 1;
+  const long long clusters = one_each ? tiles : std::min<long long>(tiles, props.sm_count / csize);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * csize));
+  cfg.blockDim = dim3(dev::kLinThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = csize;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = csize > 1 ? 2 : 1;
+  OBJB_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, ma2, mb, g), "launch dense product");
+  return OBJB_OK;
+}
+
+// Which tile a product takes.  CTA pairs (256 x 256) where the result has 16
+// bits, the operands one plane and the pairs' tiles fill the SMs; else single
+// CTAs of 128 rows by N up to 128, a tile's k split over a cluster while that
+// leaves SMs free.
+int gemm(const Product& p, int device, const DeviceProps& props, cudaStream_t st) {
+  dev::GemmArgs g;
+  g.M = static_cast<int>(p.M);
+  g.N = static_cast<long long>(p.N);
+  g.nkb = static_cast<int>((p.K + 63) / 64);
+  g.pa = p.a.planes;
+  g.pb = p.b.planes;
+  g.split = 1;
+  g.swiglu_limit = p.swiglu_limit;
+  g.epi = p.epi;
+  OBJB_TRY(device_error_word(device, &g.err));
+  const bool y16 = p.epi.y_dtype != OBJB_DTYPE_F32;
+  const size_t pair_tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
+  if (!p.gated && y16 && g.pa == 1 && g.pb == 1 && pair_tiles * 4 >= static_cast<size_t>(props.sm_count)) {
+    g.chunk_kb = g.nkb;
+    switch (p.maj) {
+      case dev::kMajKK: return launch_gemm<dev::kMajKK, 256, 2, false>(p, g, device, props, st);
+      case dev::kMajMK: return launch_gemm<dev::kMajMK, 256, 2, false>(p, g, device, props, st);
+      default: return launch_gemm<dev::kMajMN, 256, 2, false>(p, g, device, props, st);
+    }
+  }
+  int bn = p.maj == dev::kMajMN ? 64 : 16;
+  while (bn < 128 && static_cast<size_t>(bn) < p.N) bn *= 2;
+  const size_t mt = p.gated ? 64 : 128;
+  const size_t tiles = ((p.M + mt - 1) / mt) * ((p.N + bn - 1) / bn);
+  while (g.split < 8 && tiles * g.split * 2 <= static_cast<size_t>(props.sm_count) && g.nkb >= g.split * 2 * 4 &&
+         bn / (g.split * 2) >= 2)
+    g.split *= 2;
+  g.chunk_kb = y16 ? 16 : 4;
+#define OBJB_GEMM(MAJ, BN, GATED) return launch_gemm<MAJ, BN, 1, GATED>(p, g, device, props, st)
+  if (p.gated) {
+    switch (bn) {
+      case 16: OBJB_GEMM(dev::kMajKK, 16, true);
+      case 32: OBJB_GEMM(dev::kMajKK, 32, true);
+      case 64: OBJB_GEMM(dev::kMajKK, 64, true);
+      default: OBJB_GEMM(dev::kMajKK, 128, true);
+    }
+  }
+  switch (p.maj) {
+    case dev::kMajKK:
+      switch (bn) {
+        case 16: OBJB_GEMM(dev::kMajKK, 16, false);
+        case 32: OBJB_GEMM(dev::kMajKK, 32, false);
+        case 64: OBJB_GEMM(dev::kMajKK, 64, false);
+        default: OBJB_GEMM(dev::kMajKK, 128, false);
+      }
+    case dev::kMajMK:
+      switch (bn) {
+        case 16: OBJB_GEMM(dev::kMajMK, 16, false);
+        case 32: OBJB_GEMM(dev::kMajMK, 32, false);
+        case 64: OBJB_GEMM(dev::kMajMK, 64, false);
+        default: OBJB_GEMM(dev::kMajMK, 128, false);
+      }
+    default:
+      if (bn == 64) OBJB_GEMM(dev::kMajMN, 64, false);
+      OBJB_GEMM(dev::kMajMN, 128, false);
+  }
+#undef OBJB_GEMM
+}
+
+int device_here(int* device, DeviceProps* props) {
+  OBJB_TRY(current_device(device));
+  return device_props(*device, props);
 }
 
 int check_sizes(const char* action, size_t T, size_t K, size_t N, int act) {
@@ -149,7 +381,9 @@ int check_stride(const char* action, const char* name, size_t stride, size_t col
 // The caller's scratch, or the stream's workspace.
 int take_scratch(const char* action, void* d_scratch, size_t have, size_t need, cudaStream_t st, uint8_t** out) {
   void* ws = d_scratch;
-  if (ws) {
+  if (need == 0) {
+    ws = nullptr;
+  } else if (ws) {
     if (have < need || (reinterpret_cast<uintptr_t>(ws) & 255u))
       return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action,
                        "scratch needs " + std::to_string(need) + " bytes, 256-byte aligned (got " +
@@ -175,8 +409,6 @@ int check_backward(const char* action, const objb_linear_backward_desc* d) {
   if (d->reserved) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "reserved must be 0");
   OBJB_TRY(check_sizes(action, d->tokens, d->in_features, d->out_features, d->activation));
   OBJB_TRY(check_types(action, d->x_dtype, d->w_dtype, d->dy_dtype, "dy"));
-  if (d->x_dtype == OBJB_DTYPE_F16 && d->dy_dtype == OBJB_DTYPE_F32)
-    return OBJB_FAIL(OBJB_ERR_UNSUPPORTED, action, "f32 dy with f16 x");
   if (d->dw_dtype != OBJB_DTYPE_F32 && d->dw_dtype != d->w_dtype)
     return OBJB_FAIL(OBJB_ERR_UNSUPPORTED, action, "dw is f32 or w's type");
   if ((d->outputs & ~7) || !d->outputs)
@@ -184,20 +416,67 @@ int check_backward(const char* action, const objb_linear_backward_desc* d) {
   return OBJB_OK;
 }
 
+struct LinearPlan {
+  ImagePlan x, w;
+  size_t total;
+};
+LinearPlan plan_linear(const objb_linear_desc& d, size_t ldx, size_t ldw, const void* x, const void* w) {
+  LinearPlan p;
+  p.x = plan_image(x, d.x_dtype, ldx, d.tokens, d.in_features, d.x_dtype == OBJB_DTYPE_F32 ? 3 : 1);
+  p.w = plan_image(w, d.w_dtype, ldw, d.out_features, d.in_features, d.w_dtype == OBJB_DTYPE_F32 ? 3 : 1);
+  p.total = p.x.bytes + p.w.bytes;
+  return p;
+}
+
+// dz enters the two products in dy's 16-bit type, or in three bf16 planes (f32
+// dy; f32 dw behind an activation); then f16 operands become two bf16 planes,
+// which hold their 11 bits exactly.
 struct BackwardPlan {
+  bool has_act, want_dx, want_dw, want_db, dz_direct;
   int parts;
   long long rows_per;
-  size_t dz, part, total;
-  int dz_dtype;
+  ImagePlan x, w, dz;
+  size_t part_bytes, total;
 };
-BackwardPlan plan_backward(const objb_linear_backward_desc* d) {
+BackwardPlan plan_backward(const objb_linear_backward_desc& d, size_t lddy, size_t ldx, size_t ldw, const void* dy,
+                           const void* x, const void* w, int sms) {
   BackwardPlan p;
-  p.parts = static_cast<int>(std::max<size_t>(1, std::min<size_t>(64, (d->tokens + 63) / 64)));
-  p.rows_per = static_cast<long long>((d->tokens + p.parts - 1) / p.parts);
-  p.dz_dtype = d->dw_dtype == OBJB_DTYPE_F32 ? OBJB_DTYPE_F32 : d->dy_dtype;
-  p.dz = 0;
-  p.part = r256(d->tokens * d->out_features * elem_bytes(p.dz_dtype));
-  p.total = p.part + r256(static_cast<size_t>(p.parts) * d->out_features * 4);
+  p.want_dx = d.outputs & OBJB_LINEAR_DX;
+  p.want_dw = d.outputs & OBJB_LINEAR_DW;
+  p.want_db = d.outputs & OBJB_LINEAR_DBIAS;
+  p.has_act = d.activation != OBJB_ACT_NONE;
+  const bool wide = d.dy_dtype == OBJB_DTYPE_F32 || (p.has_act && p.want_dw && d.dw_dtype == OBJB_DTYPE_F32);
+  p.dz = plan_image(dy, d.dy_dtype, lddy, d.tokens, d.out_features, wide ? 3 : 1);
+  p.dz_direct = !p.has_act && p.dz.direct;
+  if (p.has_act && p.dz.direct) p.dz = plan_image(nullptr, OBJB_DTYPE_F32, 0, d.tokens, d.out_features, 1);
+  if (!p.want_dx && !p.want_dw) p.dz.bytes = 0;
+  auto planes = [&](int dtype) { return dtype == OBJB_DTYPE_F32 ? 3 : dtype == OBJB_DTYPE_F16 && wide ? 2 : 1; };
+  p.x = plan_image(x, d.x_dtype, ldx, d.tokens, d.in_features, planes(d.x_dtype));
+  p.w = plan_image(w, d.w_dtype, ldw, d.out_features, d.in_features, planes(d.w_dtype));
+  if (!p.want_dw) p.x.bytes = 0;
+  if (!p.want_dx) p.w.bytes = 0;
+  // runs of rows of the column sums: enough blocks to fill the SMs, 32 rows or more in each
+  const size_t cols = (d.out_features + 255) / 256;
+  const size_t want = std::max<size_t>(1, (static_cast<size_t>(sms) * 4 + cols - 1) / cols);
+  p.parts = static_cast<int>(std::max<size_t>(1, std::min(want, (d.tokens + 31) / 32)));
+  p.rows_per = static_cast<long long>((d.tokens + p.parts - 1) / p.parts);
+  p.part_bytes = p.want_db ? r256(static_cast<size_t>(p.parts) * d.out_features * 4) : 0;
+  p.total = p.x.bytes + p.w.bytes + p.dz.bytes + p.part_bytes;
+  return p;
+}
+
+struct FfnPlan {
+  ImagePlan gate, up, down, x, act;
+  size_t total;
+};
+FfnPlan plan_ffn(size_t T, size_t H, size_t I, size_t O, const void* gate, const void* up, const void* down) {
+  FfnPlan p;
+  p.gate = plan_image(gate, OBJB_DTYPE_BF16, H, I, H, 1);
+  p.up = plan_image(up, OBJB_DTYPE_BF16, H, I, H, 1);
+  p.down = plan_image(down, OBJB_DTYPE_BF16, I, O, I, 1);
+  p.x = plan_image(nullptr, OBJB_DTYPE_F32, H, T, H, 3);
+  p.act = plan_image(nullptr, OBJB_DTYPE_F32, I, T, I, 3);
+  p.total = p.gate.bytes + p.up.bytes + p.down.bytes + p.x.bytes + p.act.bytes;
   return p;
 }
 
@@ -208,11 +487,15 @@ using namespace objb;
 
 extern "C" {
 
-int objb_linear_scratch_bytes(const objb_linear_desc* desc, size_t* bytes) {
+int objb_linear_scratch_bytes(const objb_linear_desc* desc, const void* d_x, const void* d_w, size_t* bytes) {
   clear_error();
-  OBJB_TRY(check_linear("objb_linear_scratch_bytes", desc));
-  if (!bytes) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, "objb_linear_scratch_bytes", "null output pointer");
-  *bytes = 0;
+  const char* action = "objb_linear_scratch_bytes";
+  OBJB_TRY(check_linear(action, desc));
+  if (!bytes) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null output pointer");
+  size_t ldx, ldw;
+  OBJB_TRY(check_stride(action, "x_stride", desc->x_stride, desc->in_features, &ldx));
+  OBJB_TRY(check_stride(action, "w_stride", desc->w_stride, desc->in_features, &ldw));
+  *bytes = plan_linear(*desc, ldx, ldw, d_x, d_w).total;
   return OBJB_OK;
 }
 
@@ -235,9 +518,20 @@ int objb_linear_device(const objb_linear_desc* desc, const void* d_x, const void
   if (!d_x || !d_w || !d_y) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null device pointer");
   if (d_residual == d_y && ldr != ldy)
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "a residual in place needs y's stride");
-  (void)d_scratch;
-  (void)scratch_bytes;
-  dev::LinearEpilogue e;
+  int device = 0;
+  DeviceProps props;
+  OBJB_TRY(device_here(&device, &props));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const LinearPlan pl = plan_linear(d, ldx, ldw, d_x, d_w);
+  uint8_t* ws = nullptr;
+  OBJB_TRY(take_scratch(action, d_scratch, scratch_bytes, pl.total, st, &ws));
+  Product p;
+  OBJB_TRY(make_image(pl.w, d_w, d.w_dtype, ldw, d.out_features, d.in_features, ws, props, st, &p.a));
+  OBJB_TRY(make_image(pl.x, d_x, d.x_dtype, ldx, d.tokens, d.in_features, ws + pl.w.bytes, props, st, &p.b));
+  p.M = d.out_features;
+  p.N = d.tokens;
+  p.K = d.in_features;
+  dev::LinearEpilogue& e = p.epi;
   e.bias = d_bias;
   e.bias_dtype = d.bias_dtype;
   e.residual = d_residual;
@@ -248,15 +542,31 @@ int objb_linear_device(const objb_linear_desc* desc, const void* d_x, const void
   e.ldz = ldz;
   e.y_dtype = d.y_dtype;
   e.act = d.activation;
-  return gemm({d_w, ldw, d.w_dtype, false}, {d_x, ldx, d.x_dtype, false}, d.out_features, d.tokens, d.in_features, e,
-              static_cast<cudaStream_t>(stream));
+  return gemm(p, device, props, st);
 }
 
-int objb_linear_backward_scratch_bytes(const objb_linear_backward_desc* desc, size_t* bytes) {
+static int backward_strides(const char* action, const objb_linear_backward_desc& d, size_t* lddy, size_t* ldz,
+                            size_t* ldx, size_t* ldw, size_t* lddx, size_t* lddw) {
+  OBJB_TRY(check_stride(action, "dy_stride", d.dy_stride, d.out_features, lddy));
+  OBJB_TRY(check_stride(action, "z_stride", d.z_stride, d.out_features, ldz));
+  OBJB_TRY(check_stride(action, "x_stride", d.x_stride, d.in_features, ldx));
+  OBJB_TRY(check_stride(action, "w_stride", d.w_stride, d.in_features, ldw));
+  OBJB_TRY(check_stride(action, "dx_stride", d.dx_stride, d.in_features, lddx));
+  return check_stride(action, "dw_stride", d.dw_stride, d.in_features, lddw);
+}
+
+int objb_linear_backward_scratch_bytes(const objb_linear_backward_desc* desc, const void* d_dy, const void* d_x,
+                                       const void* d_w, size_t* bytes) {
   clear_error();
-  OBJB_TRY(check_backward("objb_linear_backward_scratch_bytes", desc));
-  if (!bytes) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, "objb_linear_backward_scratch_bytes", "null output pointer");
-  *bytes = plan_backward(desc).total;
+  const char* action = "objb_linear_backward_scratch_bytes";
+  OBJB_TRY(check_backward(action, desc));
+  if (!bytes) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null output pointer");
+  size_t lddy, ldz, ldx, ldw, lddx, lddw;
+  OBJB_TRY(backward_strides(action, *desc, &lddy, &ldz, &ldx, &ldw, &lddx, &lddw));
+  int device = 0;
+  DeviceProps props;
+  OBJB_TRY(device_here(&device, &props));
+  *bytes = plan_backward(*desc, lddy, ldx, ldw, d_dy, d_x, d_w, props.sm_count).total;
   return OBJB_OK;
 }
 
@@ -267,17 +577,13 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
   const char* action = "objb_linear_backward_device";
   OBJB_TRY(check_backward(action, desc));
   const objb_linear_backward_desc& d = *desc;
-  const bool want_dx = d.outputs & OBJB_LINEAR_DX, want_dw = d.outputs & OBJB_LINEAR_DW,
-             want_db = d.outputs & OBJB_LINEAR_DBIAS, has_act = d.activation != OBJB_ACT_NONE;
   size_t lddy, ldz, ldx, ldw, lddx, lddw;
-  OBJB_TRY(check_stride(action, "dy_stride", d.dy_stride, d.out_features, &lddy));
-  OBJB_TRY(check_stride(action, "z_stride", d.z_stride, d.out_features, &ldz));
-  OBJB_TRY(check_stride(action, "x_stride", d.x_stride, d.in_features, &ldx));
-  OBJB_TRY(check_stride(action, "w_stride", d.w_stride, d.in_features, &ldw));
-  OBJB_TRY(check_stride(action, "dx_stride", d.dx_stride, d.in_features, &lddx));
-  OBJB_TRY(check_stride(action, "dw_stride", d.dw_stride, d.in_features, &lddw));
+  OBJB_TRY(backward_strides(action, d, &lddy, &ldz, &ldx, &ldw, &lddx, &lddw));
+  const bool want_dx = d.outputs & OBJB_LINEAR_DX, want_dw = d.outputs & OBJB_LINEAR_DW,
+             want_db = d.outputs & OBJB_LINEAR_DBIAS;
   if ((want_dw && !d_dw) || (want_db && !d_dbias) ||
-      (d.tokens && (!d_dy || (has_act && !d_z) || (want_dw && !d_x) || (want_dx && (!d_w || !d_dx)))))
+      (d.tokens && (!d_dy || (d.activation != OBJB_ACT_NONE && !d_z) || (want_dw && !d_x) ||
+                    (want_dx && (!d_w || !d_dx)))))
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null device pointer");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d.tokens == 0) {  // sums over nothing
@@ -288,35 +594,72 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
     if (want_db && !d.accumulate) OBJB_CUDA(cudaMemsetAsync(d_dbias, 0, d.out_features * 4, st), "clear dbias");
     return OBJB_OK;
   }
-  const BackwardPlan p = plan_backward(desc);
+  int device = 0;
+  DeviceProps props;
+  OBJB_TRY(device_here(&device, &props));
+  const BackwardPlan pl = plan_backward(d, lddy, ldx, ldw, d_dy, d_x, d_w, props.sm_count);
   uint8_t* ws = nullptr;
-  OBJB_TRY(take_scratch(action, d_scratch, scratch_bytes, p.total, st, &ws));
+  OBJB_TRY(take_scratch(action, d_scratch, scratch_bytes, pl.total, st, &ws));
+  uint8_t *ws_dz = ws, *ws_x = ws_dz + pl.dz.bytes, *ws_w = ws_x + pl.x.bytes, *ws_part = ws_w + pl.w.bytes;
   const int N = static_cast<int>(d.out_features);
-  const unsigned cols = (N + 255) / 256;
-  dev::dz_kernel<<<dim3(cols, p.parts), 256, 0, st>>>(d_dy, lddy, d_z, ldz, d.dy_dtype, d.activation,
-                                                      static_cast<long long>(d.tokens), N, ws + p.dz, p.dz_dtype,
-                                                      p.rows_per, reinterpret_cast<float*>(ws + p.part));
-  OBJB_CUDA(cudaGetLastError(), "launch dz");
-  if (want_db) {
-    dev::dbias_kernel<<<cols, 256, 0, st>>>(reinterpret_cast<float*>(ws + p.part), p.parts, N, d_dbias, d.accumulate);
-    OBJB_CUDA(cudaGetLastError(), "launch dbias");
+  const bool products = want_dx || want_dw;
+  Image dz;
+  dz.p = pl.dz_direct ? d_dy : ws_dz;
+  dz.ld = pl.dz.pitch;
+  dz.rows = d.tokens;
+  dz.cols = d.out_features;
+  dz.planes = pl.dz.planes;
+  dz.dtype = pl.dz.planes > 1 ? OBJB_DTYPE_BF16 : d.dy_dtype;
+  const bool image = products && !pl.dz_direct;
+  if (image || want_db) {
+    const bool vec = aligned16(d_dy) && lddy % 8 == 0 && (!pl.has_act || (aligned16(d_z) && ldz % 8 == 0));
+    const dim3 grid((N + 255) / 256, pl.parts);
+    auto k = vec ? dev::dz_kernel<true> : dev::dz_kernel<false>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    float* part = want_db ? reinterpret_cast<float*>(ws_part) : nullptr;
+    OBJB_CUDA(cudaLaunchKernelEx(&cfg, k, d_dy, lddy, d_z, ldz, static_cast<int>(d.dy_dtype),
+                                 static_cast<int>(d.activation), static_cast<long long>(d.tokens), N,
+                                 image ? reinterpret_cast<uint16_t*>(ws_dz) : nullptr, static_cast<int>(pl.dz.pitch),
+                                 pl.dz.planes, pl.rows_per, part),
+              "launch dz");
+    if (want_db)
+      OBJB_TRY(launch_pdl(dev::dbias_kernel, (N + 255) / 256, 256, 0, st, static_cast<const float*>(part), pl.parts, N,
+                          d_dbias, static_cast<int>(d.accumulate)));
   }
   if (want_dx) {
-    dev::LinearEpilogue e;
-    e.y = d_dx;
-    e.ldy = lddx;
-    e.y_dtype = d.x_dtype;
-    OBJB_TRY(gemm({d_w, ldw, d.w_dtype, true}, {ws + p.dz, d.out_features, p.dz_dtype, false}, d.in_features,
-                  d.tokens, d.out_features, e, st));
+    Product p;
+    p.maj = dev::kMajMK;
+    OBJB_TRY(make_image(pl.w, d_w, d.w_dtype, ldw, d.out_features, d.in_features, ws_w, props, st, &p.a));
+    p.b = dz;
+    p.M = d.in_features;
+    p.N = d.tokens;
+    p.K = d.out_features;
+    p.epi.y = d_dx;
+    p.epi.ldy = lddx;
+    p.epi.y_dtype = d.x_dtype;
+    OBJB_TRY(gemm(p, device, props, st));
   }
   if (want_dw) {
-    dev::LinearEpilogue e;
-    e.y = d_dw;
-    e.ldy = lddw;
-    e.y_dtype = d.dw_dtype;
-    if (d.accumulate) e.residual = d_dw, e.ldr = lddw;
-    OBJB_TRY(gemm({d_x, ldx, d.x_dtype, true}, {ws + p.dz, d.out_features, p.dz_dtype, true}, d.in_features,
-                  d.out_features, d.tokens, e, st));
+    Product p;
+    p.maj = dev::kMajMN;
+    OBJB_TRY(make_image(pl.x, d_x, d.x_dtype, ldx, d.tokens, d.in_features, ws_x, props, st, &p.a));
+    p.b = dz;
+    p.M = d.in_features;
+    p.N = d.out_features;
+    p.K = d.tokens;
+    p.epi.y = d_dw;
+    p.epi.ldy = lddw;
+    p.epi.y_dtype = d.dw_dtype;
+    if (d.accumulate) p.epi.residual = d_dw, p.epi.ldr = lddw;
+    OBJB_TRY(gemm(p, device, props, st));
   }
   return OBJB_OK;
 }
@@ -326,12 +669,13 @@ static int check_ffn(const char* action, size_t T, size_t H, size_t I, size_t O)
   return check_sizes(action, T, I, O, 0);
 }
 
-int objb_ffn_bf16_tokens_scratch_bytes(size_t num_tokens, size_t hidden, size_t intermediate, size_t out_dim,
-                                       size_t* bytes) {
+int objb_ffn_bf16_tokens_scratch_bytes(const void* d_gate, const void* d_up, const void* d_down, size_t hidden,
+                                       size_t intermediate, size_t out_dim, size_t num_tokens, size_t* bytes) {
   clear_error();
-  OBJB_TRY(check_ffn("objb_ffn_bf16_tokens_scratch_bytes", num_tokens, hidden, intermediate, out_dim));
-  if (!bytes) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, "objb_ffn_bf16_tokens_scratch_bytes", "null output pointer");
-  *bytes = 2 * r256(num_tokens * intermediate * 4);
+  const char* action = "objb_ffn_bf16_tokens_scratch_bytes";
+  OBJB_TRY(check_ffn(action, num_tokens, hidden, intermediate, out_dim));
+  if (!bytes) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null output pointer");
+  *bytes = plan_ffn(num_tokens, hidden, intermediate, out_dim, d_gate, d_up, d_down).total;
   return OBJB_OK;
 }
 
@@ -345,29 +689,48 @@ int objb_ffn_bf16_tokens_device(const void* d_gate, const void* d_up, const void
   if (num_tokens == 0) return OBJB_OK;
   if (!d_gate || !d_up || !d_down || !d_x || !d_out)
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null device pointer");
+  int device = 0;
+  DeviceProps props;
+  OBJB_TRY(device_here(&device, &props));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const FfnPlan pl = plan_ffn(num_tokens, hidden, intermediate, out_dim, d_gate, d_up, d_down);
   uint8_t* ws = nullptr;
-  const size_t half = r256(num_tokens * intermediate * 4);
-  OBJB_TRY(take_scratch(action, d_scratch, scratch_bytes, 2 * half, st, &ws));
-  float* g = reinterpret_cast<float*>(ws);
-  float* u = reinterpret_cast<float*>(ws + half);
-  dev::LinearEpilogue e;
-  e.y_dtype = OBJB_DTYPE_F32;
-  e.ldy = intermediate;
-  const dev::Operand x{d_x, hidden, OBJB_DTYPE_F32, false};
-  e.y = g;
-  OBJB_TRY(gemm({d_gate, hidden, OBJB_DTYPE_BF16, false}, x, intermediate, num_tokens, hidden, e, st));
-  e.y = u;
-  OBJB_TRY(gemm({d_up, hidden, OBJB_DTYPE_BF16, false}, x, intermediate, num_tokens, hidden, e, st));
-  const size_t n = num_tokens * intermediate;
-  dev::swiglu_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(g, u, g, n, swiglu_limit);
-  OBJB_CUDA(cudaGetLastError(), "launch SwiGLU");
-  e.y = d_out;
-  e.ldy = out_dim;
-  e.residual = d_residual;
-  e.ldr = out_dim;
-  return gemm({d_down, intermediate, OBJB_DTYPE_BF16, false}, {g, intermediate, OBJB_DTYPE_F32, false}, out_dim,
-              num_tokens, intermediate, e, st);
+  OBJB_TRY(take_scratch(action, d_scratch, scratch_bytes, pl.total, st, &ws));
+  const int bf = OBJB_DTYPE_BF16;
+  Product gu;
+  gu.gated = true;
+  OBJB_TRY(make_image(pl.gate, d_gate, bf, hidden, intermediate, hidden, ws, props, st, &gu.a));
+  ws += pl.gate.bytes;
+  OBJB_TRY(make_image(pl.up, d_up, bf, hidden, intermediate, hidden, ws, props, st, &gu.a2));
+  ws += pl.up.bytes;
+  Product dn;
+  OBJB_TRY(make_image(pl.down, d_down, bf, intermediate, out_dim, intermediate, ws, props, st, &dn.a));
+  ws += pl.down.bytes;
+  OBJB_TRY(make_image(pl.x, d_x, OBJB_DTYPE_F32, hidden, num_tokens, hidden, ws, props, st, &gu.b));
+  ws += pl.x.bytes;
+  gu.M = intermediate;
+  gu.N = num_tokens;
+  gu.K = hidden;
+  gu.swiglu_limit = swiglu_limit;
+  gu.epi.y = ws;  // the activations, as the planes that the down product reads
+  gu.epi.ldy = pl.act.pitch;
+  gu.epi.plane = num_tokens * pl.act.pitch;
+  OBJB_TRY(gemm(gu, device, props, st));
+  dn.b.p = ws;
+  dn.b.ld = pl.act.pitch;
+  dn.b.rows = num_tokens;
+  dn.b.cols = intermediate;
+  dn.b.planes = 3;
+  dn.b.dtype = bf;
+  dn.M = out_dim;
+  dn.N = num_tokens;
+  dn.K = intermediate;
+  dn.epi.y = d_out;
+  dn.epi.ldy = out_dim;
+  dn.epi.residual = d_residual;
+  dn.epi.ldr = out_dim;
+  dn.epi.y_dtype = OBJB_DTYPE_F32;
+  return gemm(dn, device, props, st);
 }
 
 }  // extern "C"

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/objeta_b200.h"
 
@@ -64,6 +65,19 @@ __device__ __forceinline__ float act_grad(int act, float v) {
   }
 }
 
+// The three bf16 parts of an f32: 8 bits of the significand each, cut off (not
+// rounded), so that they sum to it exactly and none overflows.  A non-finite
+// value is its first part alone.
+__device__ __forceinline__ void split3(float v, __nv_bfloat16 (&p)[3]) {
+  const float a = __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
+  const bool finite = fabsf(v) < __int_as_float(0x7F800000);
+  const float r = finite ? v - a : 0.0f;
+  const float b = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
+  p[0] = __float2bfloat16_rn(finite ? a : v);
+  p[1] = __float2bfloat16_rn(b);
+  p[2] = __float2bfloat16_rn(r - b);
+}
+
 // What happens to the product's element (row m of A, row n of B), whose place
 // in y, z and residual is [n][m]: + bias[m] -> z -> act -> + residual -> y.
 struct LinearEpilogue {
@@ -72,14 +86,86 @@ struct LinearEpilogue {
   void* y = nullptr;
   void* z = nullptr;
   size_t ldr = 0, ldy = 0, ldz = 0;
+  size_t plane = 0;  // put_planes: elements between y's planes
   int bias_dtype = 0, y_dtype = 0, act = 0;
 
-  __device__ __forceinline__ void put(int m, size_t n, float v) const {
-    if (bias) v += load_elem(bias, bias_dtype, m);
-    if (z) store_elem(z, y_dtype, n * ldz + m, v);
-    v = act_value(act, v);
-    if (residual) v += load_elem(residual, y_dtype, n * ldr + m);
-    store_elem(y, y_dtype, n * ldy + m, v);
+  template <class T, int C>
+  __device__ __forceinline__ void store(T* p, size_t ld, int m, long long n, long long N, const float (&v)[C]) const {
+    p += static_cast<size_t>(n) * ld + m;
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (n + i < N) {
+        if constexpr (sizeof(T) == 4)
+          p[i * ld] = v[i];
+        else if constexpr (std::is_same<T, __half>::value)
+          p[i * ld] = __float2half_rn(v[i]);
+        else
+          p[i * ld] = __float2bfloat16_rn(v[i]);
+      }
+  }
+  template <class T, int C>
+  __device__ __forceinline__ void add(const T* p, size_t ld, int m, long long n, long long N, float (&v)[C]) const {
+    p += static_cast<size_t>(n) * ld + m;
+    T r[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (n + i < N) r[i] = p[i * ld];
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (n + i < N) v[i] += static_cast<float>(r[i]);
+  }
+  template <int C>
+  __device__ __forceinline__ void store_any(void* p, size_t ld, int m, long long n, long long N,
+                                            const float (&v)[C]) const {
+    if (y_dtype == OBJB_DTYPE_F32)
+      store(static_cast<float*>(p), ld, m, n, N, v);
+    else if (y_dtype == OBJB_DTYPE_BF16)
+      store(static_cast<__nv_bfloat16*>(p), ld, m, n, N, v);
+    else
+      store(static_cast<__half*>(p), ld, m, n, N, v);
+  }
+
+  // C neighbouring n of one m (those below N).
+  template <int C>
+  __device__ __forceinline__ void put_columns(int m, long long n, long long N, float (&v)[C]) const {
+    if (n >= N) return;
+    if (bias) {
+      const float b = load_elem(bias, bias_dtype, m);
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] += b;
+    }
+    if (z) store_any(z, ldz, m, n, N, v);
+    switch (act) {
+#define OBJB_ACT_CASE(A)                                          \
+  case A:                                                         \
+    _Pragma("unroll") for (int i = 0; i < C; ++i) v[i] = act_value(A, v[i]); \
+    break
+      OBJB_ACT_CASE(OBJB_ACT_RELU);
+      OBJB_ACT_CASE(OBJB_ACT_SILU);
+      OBJB_ACT_CASE(OBJB_ACT_GELU);
+      OBJB_ACT_CASE(OBJB_ACT_GELU_TANH);
+#undef OBJB_ACT_CASE
+      default: break;
+    }
+    if (residual) {
+      if (y_dtype == OBJB_DTYPE_F32)
+        add(static_cast<const float*>(residual), ldr, m, n, N, v);
+      else if (y_dtype == OBJB_DTYPE_BF16)
+        add(static_cast<const __nv_bfloat16*>(residual), ldr, m, n, N, v);
+      else
+        add(static_cast<const __half*>(residual), ldr, m, n, N, v);
+    }
+    store_any(y, ldy, m, n, N, v);
+  }
+
+  // One f32 value as the three planes of the next product's operand.
+  __device__ __forceinline__ void put_planes(int m, long long n, float v) const {
+    __nv_bfloat16 p[3];
+    split3(v, p);
+    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(y) + static_cast<size_t>(n) * ldy + m;
+    o[0] = p[0];
+    o[plane] = p[1];
+    o[2 * plane] = p[2];
   }
 };
 

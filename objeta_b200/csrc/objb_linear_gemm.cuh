@@ -1,0 +1,459 @@
+// objb_linear_gemm.cuh -- the tensor-core product under the dense operators
+// (linear.cu): D[n][m] = sum_k A(m, k) B(n, k), f32 accumulation.
+//
+// A and B are 16-bit matrices in memory ("images"), each either with k along
+// its rows' elements (K-major) or with k along its rows (the transposed read
+// of the gradients, MN-major); an f32 operand has three bf16 planes (the upper,
+// middle and lower 8 bits of its significand), whose products are taken pair
+// by pair.  Rows of A are the rows m of an M 128 tcgen05.mma, rows of B its N,
+// so a tensor-memory lane is a row m and a warp's 32 lanes store 32
+// neighbouring elements of D's row n: no transposition on the way out.
+//
+// One warp issues TMA copies into a ring of 128-byte-swizzled stages (64 of k,
+// all planes), one warp the MMAs, eight warps the epilogue (32 rows by half
+// of the columns each):
+//   * Single CTAs (CG 1), N 16..128.  The tensor core adds into its f32
+//     accumulators with truncation, so their error grows with the number of
+//     MMAs in one accumulator; the epilogue warps therefore take the
+//     accumulators into registers every chunk_kb k-blocks (two buffers) and
+//     add there, rounded to nearest.  The planes' cross products are below
+//     2^-8 of the main one and stay in a buffer of their own.
+//   * CTA pairs (CG 2, cta_group::2), M 256, N 256, for large 16-bit results:
+//     straight from tensor memory into the epilogue, two buffers over a
+//     persistent grid.
+//   * Few tiles (CG 1): `split` CTAs of a cluster share a tile's k-blocks and
+//     fold their partial tiles through distributed shared memory in rank
+//     order: one launch, no atomics, no scratch.
+//   * GATED: A is 64 rows of the gate and the same 64 rows of up; the epilogue
+//     pairs lanes i and i + 64 through shared memory.
+#pragma once
+
+#include <cuda.h>
+
+#include "objb_linear.cuh"
+#include "objb_moe.cuh"
+#include "objb_pipe.cuh"
+#include "objb_tc.cuh"
+
+namespace objb {
+namespace dev {
+
+enum { kMajKK = 0, kMajMK = 1, kMajMN = 2 };  // A, B: K-major both; A MN-major; both MN-major
+
+constexpr int kLinBK = 64;        // k of a stage: 128 bytes, one swizzle row
+constexpr int kLinStagesMax = 12;
+constexpr int kLinThreads = 320;  // producer, MMA, eight epilogue warps
+constexpr int kLinAPlane = 128 * 128;
+
+struct GemmArgs {
+  int M;                  // rows of A (GATED: features)
+  long long N;            // rows of B
+  int nkb;                // k-blocks
+  int tiles_m, tiles_n;
+  int pa, pb;             // planes
+  int split;              // CTAs of a cluster per tile (CG 1)
+  int chunk_kb;           // k-blocks per accumulator chunk
+  int nstages;
+  uint32_t idesc;
+  float swiglu_limit;
+  unsigned* err;
+  LinearEpilogue epi;
+};
+
+// SWIZZLE_128B operand tiles.  K-major: rows of 128 bytes, 8-row groups 1024
+// bytes apart.  MN-major: 64 rows x 64 k as 64 k rows of 128 bytes; 8-k groups
+// 1024 bytes apart (stride offset), the next 64 rows 8192 bytes (leading).
+template <bool MN>
+__device__ __forceinline__ uint64_t lin_desc(uint32_t saddr) {
+  uint64_t d = static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>((MN ? 8192 : 16) >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+template <int CG>
+__device__ __forceinline__ void lin_mma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u));
+}
+
+// 3-D tiled load (x along a row, row, plane).  x is a multiple of 64 elements.
+// With CG 2 the bytes are counted on the even CTA's barrier.
+template <int CG>
+__device__ __forceinline__ void lin_tma(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+        "{%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t lin_mapa(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float lin_ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(taddr));
+}
+template <int G>
+__device__ __forceinline__ void tmem_ldf(uint32_t taddr, float (&r)[G]) {
+  if constexpr (G == 32) {
+    tmem_ld32(taddr, r);
+  } else {
+    uint32_t u[G];
+    if constexpr (G == 16)
+      tmem_ld16(taddr, u);
+    else
+      tmem_ld8(taddr, u);
+#pragma unroll
+    for (int i = 0; i < G; ++i) r[i] = __uint_as_float(u[i]);
+  }
+}
+
+// mbar_wait_bounded by a whole warp: all lanes go on or all give up.
+__device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code,
+                                         unsigned* abort) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar, parity, err, code, abort));
+}
+
+// Tile t of the grid, in bands of 8 tiles of n: the tiles that run together
+// share few rows of A and of B.
+__device__ __forceinline__ void lin_tile(const GemmArgs& g, int t, int* tm, int* tn) {
+  const int band = 8 * g.tiles_m;
+  const int b = t / band, r = t - b * band;
+  const int width = g.tiles_n - b * 8 < 8 ? g.tiles_n - b * 8 : 8;
+  *tm = r / width;
+  *tn = b * 8 + r - *tm * width;
+}
+
+template <int MAJ, int BN, int CG, bool GATED>
+__global__ void __launch_bounds__(kLinThreads, 1)
+    lin_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a2,
+                    const __grid_constant__ CUtensorMap map_b, const GemmArgs g) {
+  constexpr bool A_MN = MAJ != kMajKK, B_MN = MAJ == kMajMN;
+  constexpr bool PROMOTE = CG == 1;
+  constexpr int BNC = BN / CG;                 // rows of B in this CTA's shared memory
+  constexpr int kBPlane = BNC * 128;
+  constexpr int HN = BN / 2;                   // columns of an epilogue warp
+  constexpr int G = HN < 32 ? HN : 32;         // of one tensor-memory load
+  constexpr int P = G < 16 ? G : 16;           // of one step of the epilogue
+  constexpr uint32_t kCols = PROMOTE ? (4 * BN < 32 ? 32 : 4 * BN) : 2 * BN;  // main x 2 (, cross products x 2)
+  static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0, "tensor memory columns");
+  static_assert(!B_MN || BNC % 64 == 0, "MN-major B comes in 64-row chunks");
+  static_assert(!GATED || (MAJ == kMajKK && CG == 1), "gated products are K-major, single CTAs");
+
+  extern __shared__ uint8_t lin_smem[];
+  __shared__ alignas(8) uint64_t full[kLinStagesMax], empty[kLinStagesMax], t_full[2], t_empty[2], c_empty[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ unsigned s_abort;
+  uint8_t* stages = lin_smem + ((1024u - (smem_u32(lin_smem) & 1023u)) & 1023u);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 || g.split > 1 ? cluster_ctarank() : 0;
+  const int csize = CG == 2 ? 2 : g.split;
+
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < g.nstages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&t_full[i], 1), mbar_init(&t_empty[i], 8 * CG), mbar_init(&c_empty[i], 8);
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    if constexpr (CG == 1)
+      tmem_alloc(&s_tmem, kCols);
+    else
+      tmem_alloc_pair(&s_tmem, kCols);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (csize > 1) cluster_sync_all();  // the peers' barriers exist before any arrival
+  tc_fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int ntiles = g.tiles_m * g.tiles_n;
+  const int first = blockIdx.x / csize, step = gridDim.x / csize;
+  const int krank = CG == 1 ? static_cast<int>(rank) : 0;
+  const int kb0 = static_cast<int>(static_cast<long long>(g.nkb) * krank / g.split);
+  const int kb1 = static_cast<int>(static_cast<long long>(g.nkb) * (krank + 1) / g.split);
+  const uint32_t stage_bytes = g.pa * kLinAPlane + g.pb * kBPlane;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---- producer
+      int it = 0;
+      bool ok = true;
+      for (int t = first; t < ntiles && ok; t += step) {
+        int tm, tn;
+        lin_tile(g, t, &tm, &tn);
+        const int m0 = GATED ? tm * 64 : (tm * CG + (CG == 2 ? rank : 0)) * 128;
+        const int n0 = tn * BN + (CG == 2 ? rank * BNC : 0);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % g.nstages;
+          if (it >= g.nstages &&
+              !mbar_wait_bounded(&empty[st], (it / g.nstages - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
+            ok = false;
+            break;
+          }
+          uint32_t bar = smem_u32(&full[st]);
+          if (rank == 0 || CG == 1) mbar_arrive_expect_tx(&full[st], stage_bytes * CG);
+          if (CG == 2) bar = lin_mapa(bar, 0);
+          uint32_t dst = smem_u32(stages) + st * stage_bytes;
+          for (int p = 0; p < g.pa; ++p, dst += kLinAPlane) {
+            if constexpr (GATED) {
+              lin_tma<CG>(dst, &map_a, kb * 64, m0, p, bar);
+              lin_tma<CG>(dst + 8192, &map_a2, kb * 64, m0, p, bar);
+            } else if constexpr (A_MN) {
+              lin_tma<CG>(dst, &map_a, m0, kb * 64, p, bar);
+              lin_tma<CG>(dst + 8192, &map_a, m0 + 64, kb * 64, p, bar);
+            } else {
+              lin_tma<CG>(dst, &map_a, kb * 64, m0, p, bar);
+            }
+          }
+          for (int p = 0; p < g.pb; ++p, dst += kBPlane) {
+            if constexpr (B_MN) {
+#pragma unroll
+              for (int c = 0; c < BNC / 64; ++c) lin_tma<CG>(dst + c * 8192, &map_b, n0 + c * 64, kb * 64, p, bar);
+            } else {
+              lin_tma<CG>(dst, &map_b, kb * 64, n0, p, bar);
+            }
+          }
+        }
+      }
+      if (*reinterpret_cast<volatile unsigned*>(&s_abort)) {
+        // a wait ran out: let the copies in flight land before shared memory goes
+        for (int i = it > g.nstages ? it - g.nstages : 0; i < it && (CG == 1 || rank == 0); ++i)
+          mbar_wait_bounded(&full[i % g.nstages], (i / g.nstages) & 1, g.err, kErrDrainTimeout);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (CG == 1 || rank == 0) {
+      // ---- MMA issue
+      int it = 0, cc = 0, tt = 0;
+      bool ok = true;
+      const bool cross = g.pa + g.pb > 2;
+      for (int t = first; t < ntiles && ok; t += step, ++tt) {
+        const uint32_t d_cross = tmem + (2 + (tt & 1)) * BN;
+        bool cross_acc = false;
+        if (cross && tt >= 2)
+          ok = lin_wait(&c_empty[tt & 1], ((tt >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort);
+        for (int kb = kb0; kb < kb1 && ok; ++cc) {
+          const int buf = cc & 1;
+          if (cc >= 2 &&
+              !lin_wait(&t_empty[buf], ((cc >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t d_main = tmem + buf * BN;
+          const int end = kb + g.chunk_kb < kb1 ? kb + g.chunk_kb : kb1;
+          bool acc = false;
+          for (; kb < end; ++kb, ++it) {
+            const int st = it % g.nstages;
+            if (!lin_wait(&full[st], (it / g.nstages) & 1, g.err, kErrFullWaitTimeout, &s_abort)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            const uint32_t sa = smem_u32(stages) + st * stage_bytes, sb = sa + g.pa * kLinAPlane;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              lin_mma<CG>(d_main, lin_desc<A_MN>(sa + k * (A_MN ? 2048 : 32)),
+                          lin_desc<B_MN>(sb + k * (B_MN ? 2048 : 32)), g.idesc, acc);
+              acc = true;
+            }
+            if (PROMOTE && cross) {
+              // planes (i, j) with 0 < i + j <= 2: what is left out is below 2^-24
+              for (int i = 0; i < g.pa; ++i)
+                for (int j = i ? 0 : 1; j < g.pb && i + j <= 2; ++j) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    lin_mma<CG>(d_cross, lin_desc<A_MN>(sa + i * kLinAPlane + k * (A_MN ? 2048 : 32)),
+                                lin_desc<B_MN>(sb + j * kBPlane + k * (B_MN ? 2048 : 32)), g.idesc, cross_acc);
+                    cross_acc = true;
+                  }
+                }
+            }
+            if constexpr (CG == 1)
+              umma_commit(&empty[st]);
+            else
+              umma_commit_pair(&empty[st]);
+          }
+          if constexpr (CG == 1)
+            umma_commit(&t_full[buf]);
+          else
+            umma_commit_pair(&t_full[buf]);
+        }
+      }
+    }
+  } else {
+    // ---- epilogue
+    const int quarter = warp & 3;  // tensor-memory lanes 32 quarter ..
+    const int col0 = warp < 6 ? 0 : HN;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + col0;
+    const int row = quarter * 32 + lane;
+    int cc = 0, tt = 0;
+    bool ok = true;
+    const bool cross = g.pa + g.pb > 2;
+    for (int t = first; t < ntiles && ok; t += step, ++tt) {
+      int tm, tn;
+      lin_tile(g, t, &tm, &tn);
+      const long long n0 = static_cast<long long>(tn) * BN + col0;
+      const int m = GATED ? tm * 64 + (row & 63) : (tm * CG + (CG == 2 ? static_cast<int>(rank) : 0)) * 128 + row;
+      if constexpr (PROMOTE) {
+        float acc[HN];
+#pragma unroll
+        for (int i = 0; i < HN; ++i) acc[i] = 0.0f;
+        auto take = [&](uint32_t at) {
+#pragma unroll
+          for (int c = 0; c < HN; c += G) {
+            float v[G];
+            tmem_ldf<G>(at + c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < G; ++i) acc[c + i] += v[i];
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+        };
+        for (int kb = kb0; kb < kb1; kb += g.chunk_kb, ++cc) {
+          const int buf = cc & 1;
+          if (!lin_wait(&t_full[buf], (cc >> 1) & 1, g.err, kErrFullWaitTimeout, &s_abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          take(t_lane + buf * BN);
+          if (lane == 0) mbar_arrive(&t_empty[buf]);
+        }
+        if (cross && ok) {
+          take(t_lane + (2 + (tt & 1)) * BN);
+          if (lane == 0) mbar_arrive(&c_empty[tt & 1]);
+        }
+        if (GATED || g.split > 1) {
+          // one tile per CTA: its stages are done with, the partial tile goes there as [n][row]
+          float* ex = reinterpret_cast<float*>(stages) + col0 * 128 + row;
+#pragma unroll
+          for (int i = 0; i < HN; ++i) ex[i * 128] = acc[i];
+        } else if (ok && m < g.M) {
+#pragma unroll
+          for (int c = 0; c < HN; c += P) {
+            float v[P];
+#pragma unroll
+            for (int i = 0; i < P; ++i) v[i] = acc[c + i];
+            g.epi.put_columns<P>(m, n0 + c, g.N, v);
+          }
+        }
+      } else {
+        const int buf = tt & 1;
+        if (!lin_wait(&t_full[buf], (tt >> 1) & 1, g.err, kErrFullWaitTimeout, &s_abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+#pragma unroll 1
+        for (int c = 0; c < HN; c += P) {
+          float v[P];
+          tmem_ldf<P>(t_lane + buf * BN + c, v);
+          tmem_wait_ld();
+          if (c + P == HN) {  // the accumulator is read: the next tile may have it
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cta_relaxed(&t_empty[buf], 0);
+          }
+          if (m < g.M) g.epi.put_columns<P>(m, n0 + c, g.N, v);
+        }
+      }
+    }
+  }
+
+  if (GATED || (CG == 1 && g.split > 1)) {
+    __syncthreads();
+    if (g.split > 1) cluster_sync_all();  // every partial tile is in place
+    if (warp >= 2) {
+      int tm, tn;
+      lin_tile(g, first, &tm, &tn);
+      const uint32_t ex = smem_u32(stages);
+      const int per = BN / g.split, c0 = static_cast<int>(rank) * per;
+      const long long n0 = static_cast<long long>(tn) * BN;
+      if constexpr (GATED) {
+        const int tid = threadIdx.x - 64, f = tid & 63, m = tm * 64 + f;
+        for (int c = c0 + (tid >> 6); c < c0 + per; c += 4) {
+          float gate = 0.0f, up = 0.0f;
+          for (int s = 0; s < g.split; ++s) {
+            const uint32_t at = (g.split > 1 ? lin_mapa(ex, s) : ex) + (c * 128 + f) * 4;
+            gate += lin_ld_cluster(at);
+            up += lin_ld_cluster(at + 256);
+          }
+          if (m < g.M && n0 + c < g.N) g.epi.put_planes(m, n0 + c, swiglu(gate, up, g.swiglu_limit));
+        }
+      } else {
+        // threads of 128 rows by two halves of this CTA's columns
+        const int tid = threadIdx.x - 64, row = tid & 127, m = tm * 128 + row;
+        auto fold = [&](auto cnt) {
+          constexpr int C = decltype(cnt)::value;
+          for (int c = c0 + (tid >> 7) * C; c < c0 + per; c += 2 * C) {
+            float v[C];
+#pragma unroll
+            for (int i = 0; i < C; ++i) v[i] = 0.0f;
+            for (int s = 0; s < g.split; ++s) {
+              const uint32_t at = lin_mapa(ex, s) + (c * 128 + row) * 4;
+#pragma unroll
+              for (int i = 0; i < C; ++i) v[i] += lin_ld_cluster(at + i * 512);
+            }
+            if (m < g.M) g.epi.put_columns<C>(m, n0 + c, g.N, v);
+          }
+        };
+        if (per % 8 == 0)
+          fold(std::integral_constant<int, 4>{});
+        else
+          fold(std::integral_constant<int, 1>{});
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (csize > 1) cluster_sync_all();  // no CTA leaves while a peer may still signal or read it
+  tc_fence_after_sync();
+  if (warp == 1) {
+    if constexpr (CG == 1)
+      tmem_dealloc(tmem, kCols);
+    else
+      tmem_dealloc_pair(tmem, kCols);
+  }
+}
+
+}  // namespace dev
+}  // namespace objb

@@ -38,11 +38,11 @@ class _LinearBackwardDesc(ctypes.Structure):
 
 
 _lib.register_signatures({
-    "objb_linear_scratch_bytes": (c_int, [c_void_p, ctypes.POINTER(c_size)]),
+    "objb_linear_scratch_bytes": (c_int, [c_void_p, c_void_p, c_void_p, ctypes.POINTER(c_size)]),
     "objb_linear_device": (c_int, [c_void_p] * 8 + [c_size, c_void_p]),
-    "objb_linear_backward_scratch_bytes": (c_int, [c_void_p, ctypes.POINTER(c_size)]),
+    "objb_linear_backward_scratch_bytes": (c_int, [c_void_p] * 4 + [ctypes.POINTER(c_size)]),
     "objb_linear_backward_device": (c_int, [c_void_p] * 9 + [c_size, c_void_p]),
-    "objb_ffn_bf16_tokens_scratch_bytes": (c_int, [c_size, c_size, c_size, c_size, ctypes.POINTER(c_size)]),
+    "objb_ffn_bf16_tokens_scratch_bytes": (c_int, [c_void_p] * 3 + [c_size] * 4 + [ctypes.POINTER(c_size)]),
     "objb_ffn_bf16_tokens_device": (c_int, [c_void_p, c_void_p, c_void_p, c_size, c_size, c_size, c_void_p, c_size,
                                             c_void_p, c_void_p, c_float, c_void_p, c_size, c_void_p]),
 })
@@ -119,7 +119,7 @@ def linear(d_x, d_w, d_bias=None, activation: str = "none", d_residual=None, out
             on_device("d_z", d_z, dev, (d_y.dtype,), contiguous=False)
             d.z_stride = _rows("d_z", d_z, dev, (T, N))
         ref = ctypes.byref(d)
-        scratch = _scratch("objb_linear_scratch_bytes", dev, ref)
+        scratch = _scratch("objb_linear_scratch_bytes", dev, ref, d_x.data_ptr(), d_w.data_ptr())
         _lib.call("objb_linear_device", ref, d_x.data_ptr(), d_w.data_ptr(), _p(d_bias), _p(d_residual),
                   d_y.data_ptr(), _p(d_z), _p(scratch), scratch.numel() if scratch is not None else 0, st)
     return d_y
@@ -180,7 +180,8 @@ def linear_backward(d_dy, d_x, d_w, d_z=None, activation: str = "none", need_dx:
         if need_dw:
             d.dw_stride = _rows("d_dw", d_dw, dev, (N, K))
         ref = ctypes.byref(d)
-        scratch = _scratch("objb_linear_backward_scratch_bytes", dev, ref)
+        scratch = _scratch("objb_linear_backward_scratch_bytes", dev, ref, d_dy.data_ptr(), d_x.data_ptr(),
+                           d_w.data_ptr())
         _lib.call("objb_linear_backward_device", ref, d_dy.data_ptr(), _p(d_z) if act else None, d_x.data_ptr(),
                   d_w.data_ptr(), _p(d_dx) if need_dx else None, _p(d_dw) if need_dw else None,
                   _p(d_dbias) if need_dbias else None, _p(scratch), scratch.numel() if scratch is not None else 0, st)
@@ -217,7 +218,8 @@ def ffn_bf16_tokens(d_gate, d_up, d_down, d_x, d_residual=None, d_out=None, swig
             d_out = torch.empty(T, O, dtype=torch.float32, device=dev)
         else:
             on_device("d_out", d_out, dev, (torch.float32,), (T, O))
-        scratch = _scratch("objb_ffn_bf16_tokens_scratch_bytes", dev, T, H, I, O)
+        scratch = _scratch("objb_ffn_bf16_tokens_scratch_bytes", dev, d_gate.data_ptr(), d_up.data_ptr(),
+                           d_down.data_ptr(), H, I, O, T)
         _lib.call("objb_ffn_bf16_tokens_device", d_gate.data_ptr(), d_up.data_ptr(), d_down.data_ptr(), H, I, O,
                   d_x.data_ptr(), T, _p(d_residual), d_out.data_ptr(), float(swiglu_limit), _p(scratch),
                   scratch.numel() if scratch is not None else 0, st)

@@ -146,7 +146,7 @@ def test_linear_empty_and_repeat(cuda_device):
 
 BPAIRS = [("bf16", "bf16", "bf16", "bf16"), ("bf16", "bf16", "bf16", "f32"), ("bf16", "bf16", "f32", "f32"),
           ("bf16", "bf16", "f32", "bf16"), ("f16", "f16", "f16", "f16"), ("f16", "f16", "f16", "f32"),
-          ("f32", "bf16", "f32", "f32"), ("f32", "bf16", "f32", "bf16"), ("f32", "f32", "f32", "f32")]
+          ("f16", "f16", "f32", "f16"), ("f32", "bf16", "f32", "f32"), ("f32", "bf16", "f32", "bf16"), ("f32", "f32", "f32", "f32")]
 
 
 def _run_backward(T, K, N, xd, wd, yd, dwd, act, seed=0):
@@ -325,3 +325,28 @@ def test_c_entry_with_the_streams_workspace(cuda_device):
     _lib.call("objb_linear_device", ctypes.byref(d), x.data_ptr(), w.data_ptr(), None, None, y.data_ptr(), None, None,
               0, torch.cuda.current_stream().cuda_stream)
     assert torch.equal(y, linear(x, w))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_large_tiles(cuda_device, dt):
+    """Results that fill the SMs with 256 x 256 tiles, ragged on both sides,
+    more tiles than the grid holds at once, one k-block and many."""
+    from objeta_b200.dense import linear
+    for T, K, N, act in ((1500, 200, 1800, "none"), (2049, 40, 1537, "silu"), (2600, 1000, 2570, "gelu_tanh"),
+                         (8000, 64, 1000, "relu")):
+        x, w = _case(T, K, N, dt, dt, 4)
+        yt = U.DT[dt]
+        b, r = U.randn((N,), yt, seed=8), U.randn((T, N), yt, seed=9)
+        z = torch.empty(T, N, dtype=yt, device="cuda")
+        y = linear(x, w, b, activation=act, d_residual=r, d_z=z)
+        rz, bz, ry, by = U.linear_ref(x, w, b, act, r, yt)
+        U.check(z, rz, bz, "z")
+        U.check(y, ry, by, "y")
+        assert torch.equal(y, linear(x, w, b, activation=act, d_residual=r))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_large_tiles_backward(cuda_device, dt):
+    _run_backward(1600, 1704, 1601, dt, dt, dt, dt, "none", 3)
+    _run_backward(1603, 1801, 2056, dt, dt, dt, dt, "silu", 4)
+    _run_backward(130, 2700, 2600, dt, dt, dt, dt, "none", 5)
