@@ -144,8 +144,16 @@ def check(status: int) -> None:
         raise CudaError(status, msg or f"status {status}")
 
 
+_fns: dict = {}  # entry point name -> bound function, filled on first use
+
+
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args))
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load(), name)
+    status = fn(*args)
+    if status != OK:
+        check(status)
 
 
 def stream_handle(stream) -> int | None:

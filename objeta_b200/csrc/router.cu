@@ -95,13 +95,25 @@ enum { kSoftmax = 0, kSigmoid = 1, kSqrtSoftplus = 2 };
 
 __device__ __forceinline__ float neg_inf() { return -__int_as_float(0x7F800000); }
 
+// exp by the special-function unit: 2 ulp, plus |x| half steps from the product.
+__device__ __forceinline__ float exp_sfu(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+__device__ __forceinline__ float rcp_sfu(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // The gate's sigmoid and sqrt-softplus scores and their derivatives.  The
 // sqrt-softplus keeps the gate's branches, log1p(exp(-l)) below -20 among
 // them, so the derivative is that of the score as it is computed.
 __device__ __forceinline__ float score_of(int func, float l, float* d) {
   if (func == kSigmoid) {
-    const float t = expf(-fabsf(l));
-    const float r = 1.0f / (1.0f + t);
+    const float t = exp_sfu(-fabsf(l));
+    const float r = rcp_sfu(1.0f + t);
     *d = t * r * r;
     return l >= 0.0f ? r : t * r;
   }
@@ -116,6 +128,35 @@ __device__ __forceinline__ float score_of(int func, float l, float* d) {
   const float sg = low ? 1.0f / (1.0f + expf(l)) : ex / (1.0f + ex);
   *d = (low ? -0.5f : 0.5f) * sg / s;
   return s;
+}
+
+// A token's logits l become exp(l - base); returns their sum.  Where none is
+// above 64 and one above -64 (every trained router), base is 0: no maximum has
+// to be found first, and the exponentials serve the sigmoid too (*direct).
+template <class TM, int EPL>
+__device__ __forceinline__ float exponentials(float (&l)[EPL], float* red, float* base, bool* direct) {
+  *base = 0.0f;
+  *direct = false;
+  if (TM::kThreads == 32) {
+    float m = l[0];
+#pragma unroll
+    for (int i = 1; i < EPL; ++i) m = fmaxf(m, l[i]);
+    *direct = !__any_sync(0xFFFFFFFFu, m > 64.0f) && __any_sync(0xFFFFFFFFu, m > -64.0f);
+  }
+  if (!*direct) {
+    float m = neg_inf();
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) m = fmaxf(m, l[i]);
+    m = TM::max(m, red);
+    *base = m > neg_inf() ? m : 0.0f;  // a row of -inf: every exponential is 0
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    l[i] = exp_sfu(l[i] - *base);
+    sum += l[i];
+  }
+  return TM::sum(sum, red);
 }
 
 // The sequence of token t: -1 before the first, S behind the last.  Offsets
@@ -152,16 +193,146 @@ struct BalanceArgs {
   unsigned* ticket;
 };
 
+struct BalanceFinishArgs {
+  BalanceArgs a;
+  int groups;          // 32-expert groups
+  bool alone;          // one block does the partial pass and this one
+  double* bal_part;    // [S][groups] sum_e c P
+  double* seq_z;       // [S]
+  int32_t* counts;     // [S][E]
+  int32_t* tokens;     // [S]
+  float* losses;       // balance, z
+  float* scales;       // [S + 1]: E / (k n_q^2 S'), then 2 / N
+};
+
+// Sums of up to four values per thread over the block, in a fixed order.
+template <int N>
+__device__ __forceinline__ void block_sums(double (&v)[N], double (*red)[32]) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], o);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (lane == 0) red[i][w] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = 0.0;
+    for (int j = 0; j < warps; ++j) v[i] += red[i][j];
+  }
+}
+
+struct FinishSmem {
+  double p[16][32];
+  int c[16][32];
+  double red[4][32];
+  bool last;
+};
+
+// One (sequence, 32 experts) item per block and turn: the partial rows of the
+// sequence are summed in block order (interleaved over the warps, the runs
+// folded in order), in double.  The block that finishes last (`alone`: the
+// only one) folds the sequences' sums into the losses.
+__device__ __forceinline__ void balance_finish(const BalanceFinishArgs& f, FinishSmem& sm, bool alone) {
+  const BalanceArgs& a = f.a;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  for (int item = alone ? 0 : blockIdx.x; item < a.S * f.groups; item += alone ? 1 : gridDim.x) {
+    const int q = item / f.groups, g = item - q * f.groups;
+    const int e = g * 32 + lane;
+    long long b = a.off ? a.off[q] : 0, end = a.off ? a.off[q + 1] : a.T;
+    b = b > 0 ? b : 0;
+    end = end < a.T ? end : a.T;
+    const int c0 = static_cast<int>(b / a.chunk), c1 = end > b ? static_cast<int>((end - 1) / a.chunk) : c0 - 1;
+    double p = 0.0;
+    int c = 0;
+    if (e < a.E) {
+      const float* pp = a.part_p + (static_cast<size_t>(c0) + q) * a.E + e;
+      const int32_t* pc = a.part_c + (static_cast<size_t>(c0) + q) * a.E + e;
+#pragma unroll 8
+      for (int i = w; i <= c1 - c0; i += warps) {
+        p += pp[static_cast<size_t>(i) * a.E];
+        c += pc[static_cast<size_t>(i) * a.E];
+      }
+    }
+    sm.p[w][lane] = p;
+    sm.c[w][lane] = c;
+    if (g == 0) {
+      double zn[2] = {};
+      for (int i = c0 + threadIdx.x; i <= c1; i += blockDim.x) {
+        zn[0] += a.part_z[static_cast<size_t>(i) + q];
+        zn[1] += a.part_n[static_cast<size_t>(i) + q];
+      }
+      block_sums(zn, sm.red);
+      if (threadIdx.x == 0) {
+        f.seq_z[q] = zn[0];
+        f.tokens[q] = static_cast<int32_t>(zn[1]);
+      }
+    }
+    __syncthreads();
+    if (w == 0) {
+      for (int i = 1; i < warps; ++i) p += sm.p[i][lane], c += sm.c[i][lane];
+      if (e < a.E) f.counts[static_cast<size_t>(q) * a.E + e] = c;
+      double v = p * c;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+      if (lane == 0) f.bal_part[item] = v;
+    }
+    __syncthreads();
+  }
+  if (!alone) {
+    if (threadIdx.x == 0) {
+      __threadfence();
+      sm.last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+      __threadfence();
+    }
+    __syncthreads();
+    if (!sm.last) return;
+  }
+  double t[4] = {};  // S', N, sum of z, sum of the sequences' balances
+  for (int i = threadIdx.x; i < a.S; i += blockDim.x) {
+    const int n = __ldcg(f.tokens + i);
+    if (n == 0) continue;
+    t[0] += 1.0;
+    t[1] += n;
+    t[2] += __ldcg(f.seq_z + i);
+    double v = 0.0;
+    for (int j = 0; j < f.groups; ++j) v += __ldcg(f.bal_part + static_cast<size_t>(i) * f.groups + j);
+    t[3] += v * a.E / (static_cast<double>(a.k) * n * n);
+  }
+  block_sums(t, sm.red);
+  for (int i = threadIdx.x; i < a.S; i += blockDim.x) {
+    const double n = __ldcg(f.tokens + i);
+    f.scales[i] = n > 0.0 ? static_cast<float>(a.E / (a.k * n * n * t[0])) : 0.0f;
+  }
+  if (threadIdx.x == 0) {
+    f.losses[0] = t[0] > 0.0 ? static_cast<float>(t[3] / t[0]) : 0.0f;
+    f.losses[1] = t[1] > 0.0 ? static_cast<float>(t[2] / t[1]) : 0.0f;
+    f.scales[a.S] = t[1] > 0.0 ? static_cast<float>(2.0 / t[1]) : 0.0f;
+  }
+}
+
+__global__ void __launch_bounds__(256) balance_finish_kernel(const BalanceFinishArgs f) {
+  __shared__ FinishSmem sm;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  balance_finish(f, sm, false);
+}
+
 template <int EPL, int WPT, bool V4, int THREADS>
-__global__ void __launch_bounds__(THREADS) balance_partial_kernel(const BalanceArgs a) {
+__global__ void __launch_bounds__(THREADS, EPL <= 8 ? 3 : 1) balance_partial_kernel(const BalanceFinishArgs f) {
   using TM = Team<EPL, WPT, V4>;
   constexpr int kTeams = THREADS / TM::kThreads;
   extern __shared__ __align__(16) uint8_t router_smem[];
+  const BalanceArgs& a = f.a;
   int32_t* hist = reinterpret_cast<int32_t*>(router_smem);             // [E]
   float* acc_sm = reinterpret_cast<float*>(hist + (a.E + 3) / 4 * 4);  // [kTeams][E], warp teams
   __shared__ float red[kTeamWarps];
   __shared__ double z_sm[kTeams];
   __shared__ int n_sm[kTeams];
+  __shared__ FinishSmem fin;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
@@ -187,47 +358,65 @@ __global__ void __launch_bounds__(THREADS) balance_partial_kernel(const BalanceA
     double z = 0.0;
     int n = 0;
     float nxt[EPL];
-    if (pos + team < end) TM::load(a.logits + (pos + team) * a.ld, E, neg_inf(), nxt);
+    int id_nxt = -1;  // slot r of the team's next token
+    bool in_nxt = false;
+    auto fetch = [&](long long t) {
+      if (t >= end) return;
+      TM::load(a.logits + t * a.ld, E, neg_inf(), nxt);
+      id_nxt = r < a.k ? a.ids[t * a.k + r] : -1;
+      in_nxt = !a.mask || a.mask[t];
+    };
+    fetch(pos + team);
     for (long long t = pos + team; t < end; t += kTeams) {
       float l[EPL];
 #pragma unroll
       for (int i = 0; i < EPL; ++i) l[i] = nxt[i];
-      if (t + kTeams < end) TM::load(a.logits + (t + kTeams) * a.ld, E, neg_inf(), nxt);
-      if (a.mask && !a.mask[t]) continue;
+      const int id = id_nxt;
+      const bool in = in_nxt;
+      fetch(t + kTeams);
+      if (!in) continue;
       ++n;
-      for (int j = r; j < a.k; j += TM::kThreads) {
+      if (id >= 0 && id < E) atomicAdd(&hist[id], 1);
+      for (int j = r + TM::kThreads; j < a.k; j += TM::kThreads) {
         const int e = a.ids[t * a.k + j];
         if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
       }
-      float m = neg_inf();
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) m = fmaxf(m, l[i]);
-      m = TM::max(m, red);
-      const float base = m > neg_inf() ? m : 0.0f;  // a row of -inf: every exponential is 0
-      float sum = 0.0f, ssum = 0.0f;
-      float ex[EPL];
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        ex[i] = expf(l[i] - base);
-        sum += ex[i];
-      }
-      sum = TM::sum(sum, red);
+      float base, s[EPL];
+      bool direct;
       if (a.func != kSoftmax) {
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-          float d;
-          ex[i] = TM::expert(i, r) < E ? score_of(a.func, l[i], &d) : 0.0f;
-          ssum += ex[i];
+        for (int i = 0; i < EPL; ++i) s[i] = l[i];
+      }
+      const float sum = exponentials<TM, EPL>(l, red, &base, &direct);
+      float ssum = sum;
+      if (a.func != kSoftmax) {
+        ssum = 0.0f;
+        if (a.func == kSigmoid && direct) {
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) {
+            s[i] = l[i] * rcp_sfu(1.0f + l[i]);
+            ssum += s[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) {
+            float d;
+            s[i] = TM::expert(i, r) < E ? score_of(a.func, s[i], &d) : 0.0f;
+            ssum += s[i];
+          }
         }
         ssum = TM::sum(ssum, red);
       } else {
-        ssum = sum;
-      }
-      const float inv = ssum > 0.0f ? 1.0f / ssum : (ssum == 0.0f ? 0.0f : ssum);  // nothing to share out: p = 0
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) acc[i] = fmaf(ex[i], inv, acc[i]);
-      const float lse = m + logf(sum);
-      if (sum != 0.0f) z += static_cast<double>(lse) * lse;
+        for (int i = 0; i < EPL; ++i) s[i] = l[i];
+      }
+      const float inv = ssum == 0.0f ? 0.0f : 1.0f / ssum;  // nothing to share out: p = 0
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) acc[i] = fmaf(s[i], inv, acc[i]);
+      if (r == 0 && sum != 0.0f) {
+        const float lse = base + logf(sum);
+        z += static_cast<double>(lse) * lse;
+      }
     }
     const size_t row = static_cast<size_t>(blockIdx.x) + q;
     if (r == 0) {
@@ -246,9 +435,10 @@ __global__ void __launch_bounds__(THREADS) balance_partial_kernel(const BalanceA
     int32_t* cr = a.part_c + row * E;
     if (WPT == 1) {
       for (int e = threadIdx.x; e < E; e += THREADS) {
-        float s = 0.0f;
-        for (int w = 0; w < kTeams; ++w) s += acc_sm[w * E + e];
-        pr[e] = s;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kTeams; ++w) v += acc_sm[w * E + e];
+        pr[e] = v;
       }
     } else {
 #pragma unroll
@@ -268,114 +458,7 @@ __global__ void __launch_bounds__(THREADS) balance_partial_kernel(const BalanceA
     __syncthreads();
     pos = end;
   }
-}
-
-struct BalanceFinishArgs {
-  BalanceArgs a;
-  int groups;          // 32-expert groups
-  double* bal_part;    // [S][groups] sum_e c P
-  double* seq_z;       // [S]
-  int32_t* counts;     // [S][E]
-  int32_t* tokens;     // [S]
-  float* losses;       // balance, z
-  float* scales;       // [S + 1]: E / (k n_q^2 S'), then 2 / N
-};
-
-__device__ __forceinline__ double block_sum(double v, double* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < 8; ++w) v += red[w];
-  return v;
-}
-
-// One block per (sequence, 32 experts): the partial rows of the sequence are
-// summed in block order (8 interleaved runs, then those in order), in double.
-// The block that finishes last folds the sequences' sums into the losses.
-__global__ void __launch_bounds__(256) balance_finish_kernel(const BalanceFinishArgs f) {
-  const BalanceArgs& a = f.a;
-  __shared__ double p_sm[8][32];
-  __shared__ int c_sm[8][32];
-  __shared__ double red[8];
-  __shared__ bool last;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int q = blockIdx.x / f.groups, g = blockIdx.x % f.groups;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int e = g * 32 + lane;
-  long long b = a.off ? a.off[q] : 0, end = a.off ? a.off[q + 1] : a.T;
-  b = b > 0 ? b : 0;
-  end = end < a.T ? end : a.T;
-  const long long c0 = b / a.chunk, c1 = end > b ? (end - 1) / a.chunk : c0 - 1;
-  double p = 0.0;
-  int c = 0;
-  for (long long i = c0 + w; i <= c1; i += 8) {
-    const size_t row = static_cast<size_t>(i) + q;
-    if (e < a.E) {
-      p += a.part_p[row * a.E + e];
-      c += a.part_c[row * a.E + e];
-    }
-  }
-  p_sm[w][lane] = p;
-  c_sm[w][lane] = c;
-  if (g == 0) {
-    double z = 0.0;
-    int n = 0;
-    for (long long i = c0 + threadIdx.x; i <= c1; i += 256) {
-      z += a.part_z[static_cast<size_t>(i) + q];
-      n += a.part_n[static_cast<size_t>(i) + q];
-    }
-    z = block_sum(z, red);
-    const double nn = block_sum(static_cast<double>(n), red);
-    if (threadIdx.x == 0) {
-      f.seq_z[q] = z;
-      f.tokens[q] = static_cast<int32_t>(nn);
-    }
-  }
-  __syncthreads();
-  if (w == 0) {
-    for (int i = 1; i < 8; ++i) p += p_sm[i][lane], c += c_sm[i][lane];
-    if (e < a.E) f.counts[static_cast<size_t>(q) * a.E + e] = c;
-    double v = p * c;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    if (lane == 0) f.bal_part[blockIdx.x] = v;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
-    __threadfence();
-  }
-  __syncthreads();
-  if (!last) return;
-  double some = 0.0, N = 0.0, z = 0.0, bal = 0.0;
-  for (int i = threadIdx.x; i < a.S; i += 256) {
-    const int n = __ldcg(f.tokens + i);
-    if (n == 0) continue;
-    some += 1.0;
-    N += n;
-    z += __ldcg(f.seq_z + i);
-    double v = 0.0;
-    for (int j = 0; j < f.groups; ++j) v += __ldcg(f.bal_part + static_cast<size_t>(i) * f.groups + j);
-    bal += v * a.E / (static_cast<double>(a.k) * n * n);
-  }
-  some = block_sum(some, red);
-  N = block_sum(N, red);
-  z = block_sum(z, red);
-  bal = block_sum(bal, red);
-  for (int i = threadIdx.x; i < a.S; i += 256) {
-    const double n = __ldcg(f.tokens + i);
-    f.scales[i] = n > 0.0 ? static_cast<float>(a.E / (a.k * n * n * some)) : 0.0f;
-  }
-  if (threadIdx.x == 0) {
-    f.losses[0] = some > 0.0 ? static_cast<float>(bal / some) : 0.0f;
-    f.losses[1] = N > 0.0 ? static_cast<float>(z / N) : 0.0f;
-    f.scales[a.S] = N > 0.0 ? static_cast<float>(2.0 / N) : 0.0f;
-  }
+  if (f.alone) balance_finish(f, fin, true);  // its own rows are all there are
 }
 
 struct RouterBackwardArgs {
@@ -397,99 +480,140 @@ struct RouterBackwardArgs {
 };
 
 template <int EPL, int WPT, bool V4>
-__global__ void __launch_bounds__(256) router_backward_kernel(const RouterBackwardArgs a) {
+__global__ void __launch_bounds__(256, EPL <= 8 ? 3 : 1) router_backward_kernel(const RouterBackwardArgs a) {
   using TM = Team<EPL, WPT, V4>;
   extern __shared__ __align__(16) uint8_t router_smem[];
   __shared__ float red[kTeamWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int E = a.E, r = TM::rank();
   const int team = WPT == 1 ? threadIdx.x >> 5 : 0;
   const int Epad = (E + 3) / 4 * 4;
   float* g = reinterpret_cast<float*>(router_smem) + static_cast<size_t>(team) * Epad;  // dL/ds of the selected experts
   for (int e = r; e < Epad; e += TM::kThreads) g[e] = 0.0f;
   TM::sync();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long t0 = (static_cast<long long>(blockIdx.x) * (256 / TM::kThreads) + team) * a.per_team;
   const long long t1 = t0 + a.per_team < a.T ? t0 + a.per_team : a.T;
   float B[EPL];
 #pragma unroll
   for (int i = 0; i < EPL; ++i) B[i] = 0.0f;
-  int have = -1;
-  const float zc = a.counts && a.z_grad != 0.0f ? a.z_grad * a.scales[a.S] : 0.0f;
-  float nxt[EPL];
-  if (t0 < t1) TM::load(a.logits + t0 * a.ld, E, neg_inf(), nxt);
+  const bool losses = a.counts != nullptr;
+  const float zc = losses && a.z_grad != 0.0f ? a.z_grad * a.scales[a.S] : 0.0f;
+  // the team's next token: its logits, and its slot r
+  float nxt[EPL], w_nxt = 0.0f;
+  int id_nxt = -1;
+  bool in_nxt = false;
+  auto fetch = [&](long long t) {
+    if (t >= t1) return;
+    TM::load(a.logits + t * a.ld, E, neg_inf(), nxt);
+    in_nxt = !a.mask || a.mask[t];
+    if (a.dw) {
+      id_nxt = r < a.k ? a.ids[t * a.k + r] : -1;
+      w_nxt = r < a.k ? a.dw[t * a.k + r] : 0.0f;
+    }
+  };
+  fetch(t0);
+  int q = -1;
+  long long q_end = t0;  // where the sequence q ends
   for (long long t = t0; t < t1; ++t) {
-    float l[EPL];
+    float l[EPL], s[EPL], d[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) l[i] = nxt[i];
-    if (t + 1 < t1) TM::load(a.logits + (t + 1) * a.ld, E, neg_inf(), nxt);
-    const int q = sequence_of(a.off, a.S, t);
-    const bool valid = q >= 0 && q < a.S && (!a.mask || a.mask[t]);
+    const int id0 = id_nxt >= 0 && id_nxt < E ? id_nxt : -1;
+    const float w0 = w_nxt;
+    const bool in = in_nxt;
+    const float le0 = a.dw && id0 >= 0 ? a.logits[t * a.ld + id0] : 0.0f;
+    fetch(t + 1);
+    if (t >= q_end) {
+      q = sequence_of(a.off, a.S, t);
+      q_end = !a.off || q >= a.S ? a.T : a.off[q < 0 ? 0 : q + 1];
+      const bool some = losses && q >= 0 && q < a.S;
+      const float c = some ? a.balance_grad * a.scales[q] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        const int e = TM::expert(i, r);
+        B[i] = some && e < E ? c * static_cast<float>(a.counts[static_cast<size_t>(q) * E + e]) : 0.0f;
+      }
+    }
     float dl[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) dl[i] = 0.0f;
-    if (valid) {
-      if (a.counts && q != have) {
-        const float c = a.balance_grad * a.scales[q];
+    if (in && q >= 0 && q < a.S) {
+      // exponentials, where the score or the z loss wants them
+      float base = 0.0f, inv = 0.0f, lse = 0.0f;
+      bool direct = false;
+      const bool exps = a.func != kSqrtSoftplus || zc != 0.0f;
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-          const int e = TM::expert(i, r);
-          B[i] = e < E ? c * static_cast<float>(a.counts[static_cast<size_t>(q) * E + e]) : 0.0f;
-        }
-        have = q;
-      }
-      // softmax, where the score or the z loss wants it
-      float m = neg_inf();
-      float p[EPL];
-      float inv = 0.0f, lse = 0.0f, base = 0.0f;
-      if (a.func == kSoftmax || zc != 0.0f) {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) m = fmaxf(m, l[i]);
-        m = TM::max(m, red);
-        base = m > neg_inf() ? m : 0.0f;
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-          p[i] = expf(l[i] - base);
-          sum += p[i];
-        }
-        sum = TM::sum(sum, red);
+      for (int i = 0; i < EPL; ++i) s[i] = l[i];
+      if (exps) {
+        const float sum = exponentials<TM, EPL>(l, red, &base, &direct);
         inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row of -inf: no probabilities, no gradient
-        lse = sum == 0.0f ? 0.0f : m + logf(sum);
+        if (zc != 0.0f) lse = sum == 0.0f ? 0.0f : base + logf(sum);
+      }
+      // scores and their derivatives
+      if (a.func == kSigmoid) {
+        if (direct) {
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) p[i] *= inv;
+          for (int i = 0; i < EPL; ++i) {
+            const float rc = rcp_sfu(1.0f + l[i]);
+            s[i] = l[i] * rc;
+            d[i] = s[i] * rc;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) s[i] = score_of(kSigmoid, s[i], &d[i]);
+        }
+      } else if (a.func == kSqrtSoftplus) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+          d[i] = 0.0f;
+          s[i] = TM::expert(i, r) < E ? score_of(kSqrtSoftplus, s[i], &d[i]) : 0.0f;
+        }
       }
       // dL/ds of the selected experts, scattered into g
       if (a.dw) {
-        float Q = 0.0f, GQ = 0.0f;
+        auto score_at = [&](float le) {
+          float dd;
+          return a.func == kSoftmax ? exp_sfu(le - base) * inv : score_of(a.func, le, &dd);
+        };
+        float c = a.route_scale, mean = 0.0f;
         if (a.renorm) {
-          for (int j = r; j < a.k; j += TM::kThreads) {
+          float Q = 0.0f, GQ = 0.0f;
+          if (id0 >= 0) {
+            Q = score_at(le0);
+            GQ = w0 * Q;
+          }
+          for (int j = r + TM::kThreads; j < a.k; j += TM::kThreads) {
             const int e = a.ids[t * a.k + j];
             if (e >= 0 && e < E) {
-              float d;
-              const float le = a.logits[t * a.ld + e];
-              const float s = a.func == kSoftmax ? expf(le - base) * inv : score_of(a.func, le, &d);
-              Q += s;
-              GQ = fmaf(a.dw[t * a.k + j], s, GQ);
+              const float v = score_at(a.logits[t * a.ld + e]);
+              Q += v;
+              GQ = fmaf(a.dw[t * a.k + j], v, GQ);
             }
           }
           Q = TM::sum(Q, red);
           GQ = TM::sum(GQ, red);
+          if (Q > 0.0f) {  // as the gate: a sum of 0 divides nothing
+            const float iq = 1.0f / Q;
+            c *= iq;
+            mean = GQ * iq;
+          }
         }
-        const bool norm = a.renorm && Q > 0.0f;  // as the gate: a sum of 0 divides nothing
-        const float c = norm ? a.route_scale / Q : a.route_scale;
-        const float mean = norm ? GQ / Q : 0.0f;
-        // 32 slots at a time; equal ids of a group are folded in slot order by the lowest
+        // 32 slots at a time; equal ids of a group are added in slot order
         if (WPT == 1 || threadIdx.x < 32) {
           const int lane = threadIdx.x & 31;
           for (int j0 = 0; j0 < a.k; j0 += 32) {
-            const int j = j0 + lane;
-            int e = j < a.k ? a.ids[t * a.k + j] : -1;
-            if (e < 0 || e >= E) e = -1;
-            const float v = e >= 0 ? c * (a.dw[t * a.k + j] - mean) : 0.0f;
+            int e = id0;
+            float v = w0;
+            if (j0) {
+              const int j = j0 + lane;
+              e = j < a.k ? a.ids[t * a.k + j] : -1;
+              if (e < 0 || e >= E) e = -1;
+              v = e >= 0 ? a.dw[t * a.k + j] : 0.0f;
+            }
+            v = c * (v - mean);
             const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
-            const bool alone = (same & (same - 1)) == 0;
-            if (__all_sync(0xFFFFFFFFu, alone || e < 0)) {
+            if (__all_sync(0xFFFFFFFFu, (same & (same - 1)) == 0 || e < 0)) {
               if (e >= 0) g[e] += v;
             } else {
               for (int i = 0; i < 32; ++i) {
@@ -501,53 +625,51 @@ __global__ void __launch_bounds__(256) router_backward_kernel(const RouterBackwa
           }
         }
         TM::sync();
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+          const int e = TM::expert(i, r);
+          dl[i] = e < E ? g[e] : 0.0f;
+        }
+        TM::sync();
+        if (id0 >= 0) g[id0] = 0.0f;  // back to zero
+        for (int j = r + TM::kThreads; j < a.k; j += TM::kThreads) {
+          const int e = a.ids[t * a.k + j];
+          if (e >= 0 && e < E) g[e] = 0.0f;
+        }
+        TM::sync();
       }
       if (a.func == kSoftmax) {
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
-          const int e = TM::expert(i, r);
-          dl[i] = B[i] + (a.dw && e < E ? g[e] : 0.0f);
-          dot = fmaf(dl[i], p[i], dot);
+          dl[i] += B[i];
+          dot = fmaf(dl[i], l[i], dot);
         }
-        dot = TM::sum(dot, red);
+        dot = TM::sum(dot, red) * inv;
         const float shift = zc * lse - dot;
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) dl[i] = p[i] * (dl[i] + shift);
+        for (int i = 0; i < EPL; ++i) dl[i] = l[i] * inv * (dl[i] + shift);
       } else {
-        float ssum = 0.0f, bsum = 0.0f;
-        float d[EPL];
+        if (losses) {
+          float ssum = 0.0f, bsum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-          const int e = TM::expert(i, r);
-          d[i] = 0.0f;
-          if (e < E) {
-            const float s = score_of(a.func, l[i], &d[i]);
-            ssum += s;
-            bsum = fmaf(B[i], s, bsum);
+          for (int i = 0; i < EPL; ++i) {
+            ssum += s[i];
+            bsum = fmaf(B[i], s[i], bsum);
           }
-        }
-        if (a.counts) {
           ssum = TM::sum(ssum, red);
           bsum = TM::sum(bsum, red);
+          const float is = ssum == 0.0f ? 0.0f : 1.0f / ssum;
+          const float mean = bsum * is;
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) dl[i] = fmaf(B[i] - mean, is, dl[i]);
         }
-        const float is = a.counts && ssum != 0.0f ? 1.0f / ssum : 0.0f;
-        const float mean = bsum * is;
+        const float zl = zc * lse * inv;
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
-          const int e = TM::expert(i, r);
-          const float gs = a.dw && e < E ? g[e] : 0.0f;
-          dl[i] = fmaf(B[i] - mean, is, gs) * d[i];
-          if (zc != 0.0f) dl[i] = fmaf(zc * lse, p[i], dl[i]);
+          dl[i] *= d[i];
+          if (zc != 0.0f) dl[i] = fmaf(zl, l[i], dl[i]);
         }
-      }
-      if (a.dw) {  // g back to zero
-        TM::sync();
-        for (int j = r; j < a.k; j += TM::kThreads) {
-          const int e = a.ids[t * a.k + j];
-          if (e >= 0 && e < E) g[e] = 0.0f;
-        }
-        TM::sync();
       }
     }
     float* o = a.out + t * a.ld_out;
@@ -642,11 +764,13 @@ int check_router(const char* action, size_t T, size_t E, size_t k, size_t S, int
   return OBJB_OK;
 }
 
-// Blocks of the partial pass: two per SM at most, at least 16 tokens each.
+// Blocks of the partial pass: three per SM at most (what its registers allow).
+// Up to 128 tokens one block does it, and, with few experts and sequences, the
+// finish too (no second launch); beyond, 16 tokens or more in each.
 BalancePlan plan_balance(size_t T, size_t E, size_t S, int sms) {
   BalancePlan p;
-  const size_t most = static_cast<size_t>(2) * sms;
-  const size_t want = std::max<size_t>(1, std::min(most, (T + 15) / 16));
+  const size_t most = static_cast<size_t>(3) * sms;
+  const size_t want = T <= 128 ? 1 : std::min(most, (T + 15) / 16);
   p.chunk = static_cast<long long>(std::max<size_t>(1, (T + want - 1) / want));
   p.chunks = (T + p.chunk - 1) / p.chunk;
   p.rows = p.chunks + S;
@@ -755,6 +879,7 @@ int objb_balance_loss_device(const float* d_logits, size_t logits_stride, const 
   a.part_z = reinterpret_cast<double*>(b + p.z);
   a.part_n = reinterpret_cast<int32_t*>(b + p.n);
   f.groups = static_cast<int>(p.groups);
+  f.alone = p.chunks <= 1 && num_seqs * p.groups <= 8;
   f.bal_part = reinterpret_cast<double*>(b + p.bal);
   f.seq_z = reinterpret_cast<double*>(b + p.seqz);
   f.counts = d_counts;
@@ -765,11 +890,12 @@ int objb_balance_loss_device(const float* d_logits, size_t logits_stride, const 
   const int grid = static_cast<int>(std::max<size_t>(1, p.chunks));
   OBJB_TRY(with_team(num_experts, v4, [&](auto epl, auto wpt, auto v) {
     constexpr int EPL = decltype(epl)::value, WPT = decltype(wpt)::value;
-    constexpr int THREADS = WPT == 1 && EPL <= 8 ? 512 : 256;
+    constexpr int THREADS = 256;
     const size_t teams = WPT == 1 ? THREADS / 32 : 0;
     const size_t smem = ((num_experts + 3) / 4 * 4 + teams * num_experts) * 4;
-    return launch_pdl(dev::balance_partial_kernel<EPL, WPT, decltype(v)::value, THREADS>, grid, THREADS, smem, st, a);
+    return launch_pdl(dev::balance_partial_kernel<EPL, WPT, decltype(v)::value, THREADS>, grid, THREADS, smem, st, f);
   }));
+  if (f.alone) return OBJB_OK;
   return launch_pdl(dev::balance_finish_kernel, static_cast<int>(num_seqs * p.groups), 256, 0, st, f);
 }
 
@@ -824,8 +950,8 @@ int objb_router_backward_device(const float* d_logits, size_t logits_stride, con
   return with_team(num_experts, v4, [&](auto epl, auto wpt, auto v) {
     constexpr int EPL = decltype(epl)::value, WPT = decltype(wpt)::value;
     const size_t teams = 8 / WPT;
-    // up to four blocks per SM, each team a run of consecutive tokens
-    const size_t most = static_cast<size_t>(4) * props.sm_count * teams;
+    // up to three blocks per SM (what the registers allow), each team a run of consecutive tokens
+    const size_t most = static_cast<size_t>(EPL <= 8 ? 3 : 1) * props.sm_count * teams;
     a.per_team = static_cast<long long>((num_tokens + most - 1) / most);
     const size_t per_block = teams * a.per_team;
     const size_t smem = teams * ((num_experts + 3) / 4 * 4) * 4;

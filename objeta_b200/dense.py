@@ -10,9 +10,10 @@ that type.  Any sizes, row strides and element-aligned addresses.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from . import _lib
-from ._launch import launch, on_device, row_stride
+from ._launch import launch, matrix, on_device
 
 c_size = ctypes.c_size_t
 c_int = ctypes.c_int
@@ -22,15 +23,20 @@ c_void_p = ctypes.c_void_p
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 _DX, _DW, _DBIAS = 1, 2, 4
+# objb_linear_desc and objb_linear_backward_desc, field by field
+_LINEAR = struct.Struct("@3N6i5N")
+_BACKWARD = struct.Struct("@3N8i6N")
 
 
 class _LinearDesc(ctypes.Structure):
+    """objb_linear_desc (what _LINEAR packs)."""
     _fields_ = ([(n, c_size) for n in ("tokens", "in_features", "out_features")]
                 + [(n, c_int32) for n in ("x_dtype", "w_dtype", "y_dtype", "bias_dtype", "activation", "reserved")]
                 + [(n, c_size) for n in ("x_stride", "w_stride", "y_stride", "residual_stride", "z_stride")])
 
 
 class _LinearBackwardDesc(ctypes.Structure):
+    """objb_linear_backward_desc (what _BACKWARD packs)."""
     _fields_ = ([(n, c_size) for n in ("tokens", "in_features", "out_features")]
                 + [(n, c_int32) for n in ("x_dtype", "w_dtype", "dy_dtype", "dw_dtype", "activation", "outputs",
                                           "accumulate", "reserved")]
@@ -47,39 +53,31 @@ _lib.register_signatures({
                                             c_void_p, c_void_p, c_float, c_void_p, c_size, c_void_p]),
 })
 
-_codes = None
+_codes: dict = {}
 
 
 def _dtype_code(name, dtype):
-    global _codes
-    if _codes is None:
+    if not _codes:
         import torch
-        _codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    if dtype not in _codes:
+        _codes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    code = _codes.get(dtype)
+    if code is None:
         raise ValueError(f"{name} is {dtype}, expected torch.float32, torch.float16 or torch.bfloat16")
-    return _codes[dtype]
+    return code
 
 
 def _activation(name):
-    if name not in ACTIVATIONS:
+    code = ACTIVATIONS.get(name)
+    if code is None:
         raise ValueError(f"unknown activation {name!r}, expected one of {', '.join(ACTIVATIONS)}")
-    return ACTIVATIONS[name]
-
-
-def _p(t):
-    return t.data_ptr() if t is not None else None
-
-
-def _rows(name, t, device, shape=None):
-    on_device(name, t, device, shape=shape, contiguous=False)
-    return row_stride(name, t)
+    return code
 
 
 def _scratch(call, device, *args):
     import torch
     n = c_size()
     _lib.call(call, *args, ctypes.byref(n))
-    return torch.empty(int(n.value), dtype=torch.uint8, device=device) if n.value else None
+    return torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
 
 
 def linear(d_x, d_w, d_bias=None, activation: str = "none", d_residual=None, out_dtype=None, d_y=None, d_z=None,
@@ -93,35 +91,37 @@ def linear(d_x, d_w, d_bias=None, activation: str = "none", d_residual=None, out
     ``linear_backward``.
     """
     import torch
-    dev = on_device("d_x", d_x, contiguous=False)
-    ldx = _rows("d_x", d_x, dev)
-    T, K = d_x.shape
-    ldw = _rows("d_w", d_w, dev)
-    N = d_w.shape[0]
-    if d_w.shape[1] != K:
+    T, K, ldx = matrix("d_x", d_x)
+    dev = d_x.device
+    N, kw, ldw = matrix("d_w", d_w, dev)
+    if kw != K:
         raise ValueError(f"d_w has shape {tuple(d_w.shape)}, expected (out, {K})")
+    xdt, wdt = _dtype_code("d_x", d_x.dtype), _dtype_code("d_w", d_w.dtype)
+    act = _activation(activation)
     with launch(dev, stream) as st:
         if d_y is None:
             d_y = torch.empty(T, N, dtype=out_dtype or d_x.dtype, device=dev)
-        elif out_dtype is not None and d_y.dtype != out_dtype:
-            raise ValueError(f"d_y is {d_y.dtype}, out_dtype {out_dtype}")
-        d = _LinearDesc(tokens=T, in_features=K, out_features=N, x_dtype=_dtype_code("d_x", d_x.dtype),
-                        w_dtype=_dtype_code("d_w", d_w.dtype), y_dtype=_dtype_code("d_y", d_y.dtype),
-                        activation=_activation(activation), x_stride=ldx, w_stride=ldw,
-                        y_stride=_rows("d_y", d_y, dev, (T, N)))
+            ldy = N
+        else:
+            ldy = matrix("d_y", d_y, dev, None if out_dtype is None else (out_dtype,), (T, N))[2]
+        ydt = d_y.dtype
+        bdt = ldr = ldz = 0
+        bias = res = z = scratch = None
         if d_bias is not None:
             on_device("d_bias", d_bias, dev, shape=(N,))
-            d.bias_dtype = _dtype_code("d_bias", d_bias.dtype)
+            bdt, bias = _dtype_code("d_bias", d_bias.dtype), d_bias.data_ptr()
         if d_residual is not None:
-            on_device("d_residual", d_residual, dev, (d_y.dtype,), contiguous=False)
-            d.residual_stride = _rows("d_residual", d_residual, dev, (T, N))
+            ldr = matrix("d_residual", d_residual, dev, (ydt,), (T, N))[2]
+            res = d_residual.data_ptr()
         if d_z is not None:
-            on_device("d_z", d_z, dev, (d_y.dtype,), contiguous=False)
-            d.z_stride = _rows("d_z", d_z, dev, (T, N))
-        ref = ctypes.byref(d)
-        scratch = _scratch("objb_linear_scratch_bytes", dev, ref, d_x.data_ptr(), d_w.data_ptr())
-        _lib.call("objb_linear_device", ref, d_x.data_ptr(), d_w.data_ptr(), _p(d_bias), _p(d_residual),
-                  d_y.data_ptr(), _p(d_z), _p(scratch), scratch.numel() if scratch is not None else 0, st)
+            ldz = matrix("d_z", d_z, dev, (ydt,), (T, N))[2]
+            z = d_z.data_ptr()
+        x, w = d_x.data_ptr(), d_w.data_ptr()
+        desc = _LINEAR.pack(T, K, N, xdt, wdt, _dtype_code("d_y", ydt), bdt, act, 0, ldx, ldw, ldy, ldr, ldz)
+        if xdt == 0 or (x | w) & 15 or (ldx | ldw) & 7:  # an operand that has to be laid out again
+            scratch = _scratch("objb_linear_scratch_bytes", dev, desc, x, w)
+        _lib.call("objb_linear_device", desc, x, w, bias, res, d_y.data_ptr(), z,
+                  *((None, 0) if scratch is None else (scratch.data_ptr(), scratch.numel())), st)
     return d_y
 
 
@@ -138,53 +138,50 @@ def linear_backward(d_dy, d_x, d_w, d_z=None, activation: str = "none", need_dx:
     rounded to that type unless dw is f32; dbias sums it unrounded.
     """
     import torch
-    dev = on_device("d_dy", d_dy, contiguous=False)
-    lddy = _rows("d_dy", d_dy, dev)
-    T, N = d_dy.shape
-    ldw = _rows("d_w", d_w, dev)
-    if d_w.shape[0] != N:
+    T, N, lddy = matrix("d_dy", d_dy)
+    dev = d_dy.device
+    nw, K, ldw = matrix("d_w", d_w, dev)
+    if nw != N:
         raise ValueError(f"d_w has shape {tuple(d_w.shape)}, expected ({N}, in)")
-    K = d_w.shape[1]
-    ldx = _rows("d_x", d_x, dev, (T, K))
+    ldx = matrix("d_x", d_x, dev, None, (T, K))[2]
+    xdt, wdt = _dtype_code("d_x", d_x.dtype), _dtype_code("d_w", d_w.dtype)
     act = _activation(activation)
     if act and d_z is None:
         raise ValueError(f"the gradient of {activation!r} needs d_z")
     if accumulate and ((need_dw and d_dw is None) or (need_dbias and d_dbias is None)):
         raise ValueError("accumulate needs the d_dw and d_dbias to add to")
     with launch(dev, stream) as st:
+        ldz = lddx = lddw = 0
+        z = dx = dw = db = None
+        outputs = 0
+        gdt = wdt
+        if act:
+            ldz = matrix("d_z", d_z, dev, (d_dy.dtype,), (T, N))[2]
+            z = d_z.data_ptr()
         if need_dx:
             if d_dx is None:
-                d_dx = torch.empty(T, K, dtype=d_x.dtype, device=dev)
+                d_dx, lddx = torch.empty(T, K, dtype=d_x.dtype, device=dev), K
             else:
-                on_device("d_dx", d_dx, dev, (d_x.dtype,), contiguous=False)
+                lddx = matrix("d_dx", d_dx, dev, (d_x.dtype,), (T, K))[2]
+            dx, outputs = d_dx.data_ptr(), _DX
         if need_dw:
             if d_dw is None:
-                d_dw = torch.empty(N, K, dtype=dw_dtype or d_w.dtype, device=dev)
-            elif dw_dtype is not None and d_dw.dtype != dw_dtype:
-                raise ValueError(f"d_dw is {d_dw.dtype}, dw_dtype {dw_dtype}")
+                d_dw, lddw = torch.empty(N, K, dtype=dw_dtype or d_w.dtype, device=dev), K
+            else:
+                lddw = matrix("d_dw", d_dw, dev, None if dw_dtype is None else (dw_dtype,), (N, K))[2]
+            dw, outputs, gdt = d_dw.data_ptr(), outputs | _DW, _dtype_code("d_dw", d_dw.dtype)
         if need_dbias:
             if d_dbias is None:
                 d_dbias = torch.empty(N, dtype=torch.float32, device=dev)
             else:
                 on_device("d_dbias", d_dbias, dev, (torch.float32,), (N,))
-        d = _LinearBackwardDesc(tokens=T, in_features=K, out_features=N, x_dtype=_dtype_code("d_x", d_x.dtype),
-                                w_dtype=_dtype_code("d_w", d_w.dtype), dy_dtype=_dtype_code("d_dy", d_dy.dtype),
-                                dw_dtype=_dtype_code("d_dw", d_dw.dtype if need_dw else d_w.dtype), activation=act,
-                                outputs=_DX * bool(need_dx) | _DW * bool(need_dw) | _DBIAS * bool(need_dbias),
-                                accumulate=int(bool(accumulate)), dy_stride=lddy, x_stride=ldx, w_stride=ldw)
-        if act:
-            on_device("d_z", d_z, dev, (d_dy.dtype,), contiguous=False)
-            d.z_stride = _rows("d_z", d_z, dev, (T, N))
-        if need_dx:
-            d.dx_stride = _rows("d_dx", d_dx, dev, (T, K))
-        if need_dw:
-            d.dw_stride = _rows("d_dw", d_dw, dev, (N, K))
-        ref = ctypes.byref(d)
-        scratch = _scratch("objb_linear_backward_scratch_bytes", dev, ref, d_dy.data_ptr(), d_x.data_ptr(),
-                           d_w.data_ptr())
-        _lib.call("objb_linear_backward_device", ref, d_dy.data_ptr(), _p(d_z) if act else None, d_x.data_ptr(),
-                  d_w.data_ptr(), _p(d_dx) if need_dx else None, _p(d_dw) if need_dw else None,
-                  _p(d_dbias) if need_dbias else None, _p(scratch), scratch.numel() if scratch is not None else 0, st)
+            db, outputs = d_dbias.data_ptr(), outputs | _DBIAS
+        desc = _BACKWARD.pack(T, K, N, xdt, wdt, _dtype_code("d_dy", d_dy.dtype), gdt, act, outputs,
+                              int(bool(accumulate)), 0, lddy, ldz, ldx, ldw, lddx, lddw)
+        dy, x, w = d_dy.data_ptr(), d_x.data_ptr(), d_w.data_ptr()
+        scratch = _scratch("objb_linear_backward_scratch_bytes", dev, desc, dy, x, w)
+        _lib.call("objb_linear_backward_device", desc, dy, z, x, w, dx, dw, db,
+                  *((None, 0) if scratch is None else (scratch.data_ptr(), scratch.numel())), st)
     return d_dx if need_dx else None, d_dw if need_dw else None, d_dbias if need_dbias else None
 
 
@@ -197,11 +194,11 @@ def ffn_bf16_tokens(d_gate, d_up, d_down, d_x, d_residual=None, d_out=None, swig
     throughout, as the one-token call.
     """
     import torch
-    dev = on_device("d_x", d_x, dtypes=(torch.float32,))
+    f32, bf = (torch.float32,), (torch.bfloat16,)
+    dev = on_device("d_x", d_x, None, f32)
     if d_x.dim() != 2:
         raise ValueError(f"d_x has shape {tuple(d_x.shape)}, expected (T, hidden)")
     T, H = d_x.shape
-    bf = (torch.bfloat16,)
     on_device("d_gate", d_gate, dev, bf)
     if d_gate.dim() != 2 or d_gate.shape[1] != H:
         raise ValueError(f"d_gate has shape {tuple(d_gate.shape)}, expected (intermediate, {H})")
@@ -212,15 +209,15 @@ def ffn_bf16_tokens(d_gate, d_up, d_down, d_x, d_residual=None, d_out=None, swig
         raise ValueError(f"d_down has shape {tuple(d_down.shape)}, expected (out, {I})")
     O = d_down.shape[0]
     if d_residual is not None:
-        on_device("d_residual", d_residual, dev, (torch.float32,), (T, O))
+        on_device("d_residual", d_residual, dev, f32, (T, O))
     with launch(dev, stream) as st:
         if d_out is None:
             d_out = torch.empty(T, O, dtype=torch.float32, device=dev)
         else:
-            on_device("d_out", d_out, dev, (torch.float32,), (T, O))
-        scratch = _scratch("objb_ffn_bf16_tokens_scratch_bytes", dev, d_gate.data_ptr(), d_up.data_ptr(),
-                           d_down.data_ptr(), H, I, O, T)
-        _lib.call("objb_ffn_bf16_tokens_device", d_gate.data_ptr(), d_up.data_ptr(), d_down.data_ptr(), H, I, O,
-                  d_x.data_ptr(), T, _p(d_residual), d_out.data_ptr(), float(swiglu_limit), _p(scratch),
-                  scratch.numel() if scratch is not None else 0, st)
+            on_device("d_out", d_out, dev, f32, (T, O))
+        g, u, d = d_gate.data_ptr(), d_up.data_ptr(), d_down.data_ptr()
+        scratch = _scratch("objb_ffn_bf16_tokens_scratch_bytes", dev, g, u, d, H, I, O, T)
+        _lib.call("objb_ffn_bf16_tokens_device", g, u, d, H, I, O, d_x.data_ptr(), T,
+                  None if d_residual is None else d_residual.data_ptr(), d_out.data_ptr(), float(swiglu_limit),
+                  *((None, 0) if scratch is None else (scratch.data_ptr(), scratch.numel())), st)
     return d_out

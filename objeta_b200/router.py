@@ -22,7 +22,7 @@ import ctypes
 from dataclasses import dataclass
 
 from . import _lib
-from ._launch import launch, on_device, row_stride
+from ._launch import launch, matrix, on_device
 from .ep import SOFTMAX
 
 c_size = ctypes.c_size_t
@@ -46,35 +46,43 @@ _lib.register_signatures({
 @dataclass
 class BalanceLoss:
     """What ``balance_loss`` returns; ``router_backward`` takes it back."""
-    balance: object      # f32 scalar tensor
-    z: object            # f32 scalar tensor
     counts: object       # int32 [S, E]: selections of each expert
     tokens: object       # int32 [S]: counted tokens
+    losses: object       # f32 [2]: balance, z
     scales: object       # f32 [S + 1]: gradient factors (E / (k n^2 S'), then 2 / N)
     score_func: int
     seq_offsets: object
     token_mask: object
 
+    @property
+    def balance(self):
+        return self.losses[0]
 
-def _p(t):
-    return t.data_ptr() if t is not None else None
+    @property
+    def z(self):
+        return self.losses[1]
 
 
-def _routing(d_logits, d_ids, score_func, d_seq_offsets, d_token_mask):
+def _routing(d_logits, d_ids, d_seq_offsets, d_token_mask):
     import torch
-    dev = on_device("d_logits", d_logits, dtypes=(torch.float32,), contiguous=False)
-    ld = row_stride("d_logits", d_logits)
-    T, E = d_logits.shape
+    T, E, ld = matrix("d_logits", d_logits, None, (torch.float32,))
+    dev = d_logits.device
     on_device("d_ids", d_ids, dev, (torch.int32,))
-    if d_ids.dim() != 2 or d_ids.shape[0] != T:
-        raise ValueError(f"d_ids has shape {tuple(d_ids.shape)}, expected ({T}, top_k)")
+    size = d_ids.shape
+    if len(size) != 2 or size[0] != T:
+        raise ValueError(f"d_ids has shape {tuple(size)}, expected ({T}, top_k)")
+    mask = off = None
+    S = 1
     if d_token_mask is not None:
         on_device("d_token_mask", d_token_mask, dev, (torch.bool, torch.uint8), (T,))
+        mask = d_token_mask.data_ptr()
     if d_seq_offsets is not None:
         on_device("d_seq_offsets", d_seq_offsets, dev, (torch.int32,))
-        if d_seq_offsets.dim() != 1 or d_seq_offsets.numel() < 2:
+        S = d_seq_offsets.numel() - 1
+        if d_seq_offsets.dim() != 1 or S < 1:
             raise ValueError("d_seq_offsets: expected [num_seqs + 1] offsets")
-    return dev, ld, T, E, d_ids.shape[1], 1 if d_seq_offsets is None else d_seq_offsets.numel() - 1
+        off = d_seq_offsets.data_ptr()
+    return dev, ld, T, E, size[1], S, mask, off
 
 
 def balance_loss(d_logits, d_ids, score_func: int = SOFTMAX, d_seq_offsets=None, d_token_mask=None,
@@ -97,19 +105,19 @@ def balance_loss(d_logits, d_ids, score_func: int = SOFTMAX, d_seq_offsets=None,
     the same call gives the same bits.
     """
     import torch
-    dev, ld, T, E, k, S = _routing(d_logits, d_ids, score_func, d_seq_offsets, d_token_mask)
+    dev, ld, T, E, k, S, mask, off = _routing(d_logits, d_ids, d_seq_offsets, d_token_mask)
     with launch(dev, stream) as st:
         n = c_size()
         _lib.call("objb_balance_loss_scratch_bytes", T, E, S, ctypes.byref(n))
-        scratch = torch.empty(int(n.value), dtype=torch.uint8, device=dev)
-        ints = torch.empty(S * (E + 1), dtype=torch.int32, device=dev)
-        floats = torch.empty(S + 3, dtype=torch.float32, device=dev)
-        counts, tokens = ints[:S * E].view(S, E), ints[S * E:]
-        losses, scales = floats[:2], floats[2:]
-        _lib.call("objb_balance_loss_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), _p(d_token_mask),
-                  _p(d_seq_offsets), S, T, E, k, int(score_func), counts.data_ptr(), tokens.data_ptr(),
-                  losses.data_ptr(), scales.data_ptr(), scratch.data_ptr(), scratch.numel(), st)
-    return BalanceLoss(losses[0], losses[1], counts, tokens, scales, int(score_func), d_seq_offsets, d_token_mask)
+        scratch = torch.empty(n.value, dtype=torch.uint8, device=dev)
+        counts = torch.empty(S, E, dtype=torch.int32, device=dev)
+        tokens = torch.empty(S, dtype=torch.int32, device=dev)
+        losses = torch.empty(2, dtype=torch.float32, device=dev)
+        scales = torch.empty(S + 1, dtype=torch.float32, device=dev)
+        _lib.call("objb_balance_loss_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), mask, off, S, T, E, k,
+                  int(score_func), counts.data_ptr(), tokens.data_ptr(), losses.data_ptr(), scales.data_ptr(),
+                  scratch.data_ptr(), n.value, st)
+    return BalanceLoss(counts, tokens, losses, scales, int(score_func), d_seq_offsets, d_token_mask)
 
 
 def router_backward(d_logits, d_ids, d_dweights=None, score_func: int = SOFTMAX, renormalize: bool = False,
@@ -128,28 +136,29 @@ def router_backward(d_logits, d_ids, d_dweights=None, score_func: int = SOFTMAX,
     ``d_dlogits`` may be ``d_logits`` itself.
     """
     import torch
-    off = None
+    d_off = None
     if balance is not None:
         if int(score_func) != balance.score_func:
             raise ValueError(f"score_func {score_func} differs from the balance loss's {balance.score_func}")
         if d_token_mask is not None:
             raise ValueError("the token mask of a call with a balance loss is the balance loss's")
-        off, d_token_mask = balance.seq_offsets, balance.token_mask
-    dev, ld, T, E, k, S = _routing(d_logits, d_ids, score_func, off, d_token_mask)
+        d_off, d_token_mask = balance.seq_offsets, balance.token_mask
+    dev, ld, T, E, k, S, mask, off = _routing(d_logits, d_ids, d_off, d_token_mask)
+    counts = scales = dw = None
     if balance is not None:
         on_device("balance.counts", balance.counts, dev, (torch.int32,), (S, E))
+        counts, scales = balance.counts.data_ptr(), balance.scales.data_ptr()
     if d_dweights is not None:
         on_device("d_dweights", d_dweights, dev, (torch.float32,), (T, k))
+        dw = d_dweights.data_ptr()
     with launch(dev, stream) as st:
         if d_dlogits is None:
-            d_dlogits = torch.empty(T, E, dtype=torch.float32, device=dev)
+            d_dlogits, ldo = torch.empty(T, E, dtype=torch.float32, device=dev), E
         else:
-            on_device("d_dlogits", d_dlogits, dev, (torch.float32,), (T, E), contiguous=False)
-        _lib.call("objb_router_backward_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), _p(d_dweights),
-                  _p(d_token_mask), _p(off), S, _p(balance.counts) if balance is not None else None,
-                  _p(balance.scales) if balance is not None else None, T, E, k, int(score_func),
-                  int(bool(renormalize)), float(route_scale), float(balance_grad), float(z_grad),
-                  d_dlogits.data_ptr(), row_stride("d_dlogits", d_dlogits), st)
+            ldo = matrix("d_dlogits", d_dlogits, dev, (torch.float32,), (T, E))[2]
+        _lib.call("objb_router_backward_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), dw, mask, off, S, counts,
+                  scales, T, E, k, int(score_func), int(bool(renormalize)), float(route_scale), float(balance_grad),
+                  float(z_grad), d_dlogits.data_ptr(), ldo, st)
     return d_dlogits
 
 
@@ -158,18 +167,21 @@ def moe_combine_backward(d_dout, d_v, slot_row, d_dw=None, stream=None):
     d_dout[t, o] * d_v[slot_row[t, j], o], f32 [T, k].  A row outside d_v is
     read as row 0 and flagged (device error word bit 8), as the combine does."""
     import torch
-    dev = on_device("d_dout", d_dout, dtypes=(torch.float32,))
-    on_device("d_v", d_v, dev, (torch.float32,))
+    f32 = (torch.float32,)
+    dev = on_device("d_dout", d_dout, None, f32)
+    on_device("d_v", d_v, dev, f32)
     on_device("slot_row", slot_row, dev, (torch.int32,))
     if d_dout.dim() != 2 or d_v.dim() != 2 or slot_row.dim() != 2:
         raise ValueError("expected d_dout [T, O], d_v [V, O] and slot_row [T, k]")
     T, k = slot_row.shape
-    on_device("d_dout", d_dout, dev, shape=(T, d_v.shape[1]))
+    V, O = d_v.shape
+    if d_dout.shape != (T, O):
+        raise ValueError(f"d_dout has shape {tuple(d_dout.shape)}, expected ({T}, {O})")
     with launch(dev, stream) as st:
         if d_dw is None:
             d_dw = torch.empty(T, k, dtype=torch.float32, device=dev)
         else:
-            on_device("d_dw", d_dw, dev, (torch.float32,), (T, k))
-        _lib.call("objb_moe_combine_backward_device", d_dout.data_ptr(), d_v.data_ptr(), d_v.shape[0],
-                  slot_row.data_ptr(), T, k, d_v.shape[1], d_dw.data_ptr(), st)
+            on_device("d_dw", d_dw, dev, f32, (T, k))
+        _lib.call("objb_moe_combine_backward_device", d_dout.data_ptr(), d_v.data_ptr(), V, slot_row.data_ptr(), T, k,
+                  O, d_dw.data_ptr(), st)
     return d_dw
