@@ -212,17 +212,16 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   if (warp == 0) {
     if (lane == 0) {
       // ---- producer
-      int it = 0;
+      int issued = 0, st = 0;
+      uint32_t phase = 1;  // of empty[st]: the first round finds every stage free
       bool ok = true;
       for (int t = first; t < ntiles && ok; t += step) {
         int tm, tn;
         lin_tile(g, t, &tm, &tn);
         const int m0 = GATED ? tm * 64 : (tm * CG + (CG == 2 ? rank : 0)) * 128;
         const int n0 = tn * BN + (CG == 2 ? rank * BNC : 0);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int st = it % g.nstages;
-          if (it >= g.nstages &&
-              !mbar_wait_bounded(&empty[st], (it / g.nstages - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait_bounded(&empty[st], phase, g.err, kErrEmptyWaitTimeout, &s_abort)) {
             ok = false;
             break;
           }
@@ -249,11 +248,13 @@ __global__ void __launch_bounds__(kLinThreads, 1)
               lin_tma<CG>(dst, &map_b, kb * 64, n0, p, bar);
             }
           }
+          ++issued;
+          if (++st == g.nstages) st = 0, phase ^= 1;
         }
       }
       if (*reinterpret_cast<volatile unsigned*>(&s_abort)) {
         // a wait ran out: let the copies in flight land before shared memory goes
-        for (int i = it > g.nstages ? it - g.nstages : 0; i < it && (CG == 1 || rank == 0); ++i)
+        for (int i = issued > g.nstages ? issued - g.nstages : 0; i < issued && (CG == 1 || rank == 0); ++i)
           mbar_wait_bounded(&full[i % g.nstages], (i / g.nstages) & 1, g.err, kErrDrainTimeout);
       }
     }
@@ -261,9 +262,12 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   } else if (warp == 1) {
     if (CG == 1 || rank == 0) {
       // ---- MMA issue
-      int it = 0, cc = 0, tt = 0;
+      int st = 0, cc = 0, tt = 0;
+      uint32_t phase = 0;  // of full[st]
       bool ok = true;
       const bool cross = g.pa + g.pb > 2;
+      constexpr uint32_t kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
+      const uint64_t base_a = lin_desc<A_MN>(0), base_b = lin_desc<B_MN>(0);
       for (int t = first; t < ntiles && ok; t += step, ++tt) {
         const uint32_t d_cross = tmem + (2 + (tt & 1)) * BN;
         bool cross_acc = false;
@@ -271,8 +275,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           ok = lin_wait(&c_empty[tt & 1], ((tt >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort);
         for (int kb = kb0; kb < kb1 && ok; ++cc) {
           const int buf = cc & 1;
-          if (cc >= 2 &&
-              !lin_wait(&t_empty[buf], ((cc >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
+          if (cc >= 2 && !lin_wait(&t_empty[buf], ((cc >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
             ok = false;
             break;
           }
@@ -280,28 +283,29 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           const uint32_t d_main = tmem + buf * BN;
           const int end = kb + g.chunk_kb < kb1 ? kb + g.chunk_kb : kb1;
           bool acc = false;
-          for (; kb < end; ++kb, ++it) {
-            const int st = it % g.nstages;
-            if (!lin_wait(&full[st], (it / g.nstages) & 1, g.err, kErrFullWaitTimeout, &s_abort)) {
+          for (; kb < end; ++kb) {
+            if (!lin_wait(&full[st], phase, g.err, kErrFullWaitTimeout, &s_abort)) {
               ok = false;
               break;
             }
             tc_fence_after_sync();
-            const uint32_t sa = smem_u32(stages) + st * stage_bytes, sb = sa + g.pa * kLinAPlane;
+            const uint32_t sa = smem_u32(stages) + st * stage_bytes;
+            // (in a cluster a shared address carries the CTA's rank above the 18 bits a descriptor has room for)
+            const uint64_t da = base_a + ((sa & 0x3FFFFu) >> 4);
+            const uint64_t db = base_b + (((sa + g.pa * kLinAPlane) & 0x3FFFFu) >> 4);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              lin_mma<CG>(d_main, lin_desc<A_MN>(sa + k * (A_MN ? 2048 : 32)),
-                          lin_desc<B_MN>(sb + k * (B_MN ? 2048 : 32)), g.idesc, acc);
+              lin_mma<CG>(d_main, da + k * kStepA, db + k * kStepB, g.idesc, acc);
               acc = true;
             }
             if (PROMOTE && cross) {
               // planes (i, j) with 0 < i + j <= 2: what is left out is below 2^-24
               for (int i = 0; i < g.pa; ++i)
                 for (int j = i ? 0 : 1; j < g.pb && i + j <= 2; ++j) {
+                  const uint64_t ai = da + i * (kLinAPlane >> 4), bj = db + j * (kBPlane >> 4);
 #pragma unroll
                   for (int k = 0; k < 4; ++k) {
-                    lin_mma<CG>(d_cross, lin_desc<A_MN>(sa + i * kLinAPlane + k * (A_MN ? 2048 : 32)),
-                                lin_desc<B_MN>(sb + j * kBPlane + k * (B_MN ? 2048 : 32)), g.idesc, cross_acc);
+                    lin_mma<CG>(d_cross, ai + k * kStepA, bj + k * kStepB, g.idesc, cross_acc);
                     cross_acc = true;
                   }
                 }
@@ -310,6 +314,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
               umma_commit(&empty[st]);
             else
               umma_commit_pair(&empty[st]);
+            if (++st == g.nstages) st = 0, phase ^= 1;
           }
           if constexpr (CG == 1)
             umma_commit(&t_full[buf]);
