@@ -232,37 +232,58 @@ struct Product {
   float swiglu_limit = 0.0f;
 };
 
-constexpr int kLinRing = 200 * 1024;  // bytes of stages
+constexpr size_t kLinRing = 216 * 1024;  // bytes of stages: three of f32 x f32 pair tiles
 
-template <int MAJ, int BN, int CG, bool GATED>
-int launch_gemm(const Product& p, dev::GemmArgs g, int device, const DeviceProps& props, cudaStream_t st) {
-  constexpr int kBPlane = BN / CG * 128;
-  const int mt = (GATED ? 64 : 128) * CG;
+// A product's tile: rm rows per accumulator, mt accumulators and bn columns
+// per CTA or pair, k split over a cluster.
+struct Tile {
+  int rm = 128, bn = 0, split = 1, chunk_kb = 0;
+  size_t ring = kLinRing;
+};
+
+template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE>
+int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProps& props, cudaStream_t st) {
+  dev::GemmArgs g;
+  g.M = static_cast<int>(p.M);
+  g.N = static_cast<long long>(p.N);
+  g.nkb = static_cast<int>((p.K + 63) / 64);
+  g.pa = p.a.planes;
+  g.pb = p.b.planes;
+  g.rm = tile.rm;
+  g.bn = tile.bn;
+  g.split = tile.split;
+  g.chunk_kb = PROMOTE ? tile.chunk_kb : g.nkb;
+  g.swiglu_limit = p.swiglu_limit;
+  g.epi = p.epi;
+  OBJB_TRY(device_error_word(device, &g.err));
+  const size_t mt = static_cast<size_t>(GATED ? 64 : MT * tile.rm) * CG;
   g.tiles_m = static_cast<int>((p.M + mt - 1) / mt);
-  g.tiles_n = static_cast<int>((p.N + BN - 1) / BN);
-  const uint32_t stage = p.a.planes * dev::kLinAPlane + p.b.planes * kBPlane;
-  g.nstages = std::max(2, std::min<int>(dev::kLinStagesMax, kLinRing / static_cast<int>(stage)));
-  const size_t smem = g.nstages * static_cast<size_t>(stage) + 1024;
+  g.tiles_n = static_cast<int>((p.N + tile.bn - 1) / tile.bn);
+  const size_t stage = static_cast<size_t>(g.pa) * MT * dev::kLinABlock + static_cast<size_t>(g.pb) * (tile.bn / CG) * 128;
+  g.nstages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(dev::kLinStagesMax, tile.ring / stage)));
+  size_t smem = g.nstages * stage;
+  if (GATED || tile.split > 1) smem = std::max(smem, static_cast<size_t>(MT) * BN * 512);  // the partial tile
+  smem += 1024;
   const uint32_t half = p.a.dtype == OBJB_DTYPE_F16 ? 0 : 1;
   g.idesc = (1u << 4) | (half << 7) | (half << 10) | (static_cast<uint32_t>(MAJ != dev::kMajKK) << 15) |
-            (static_cast<uint32_t>(MAJ == dev::kMajMN) << 16) | (static_cast<uint32_t>(BN >> 3) << 17) |
+            (static_cast<uint32_t>(MAJ == dev::kMajMN) << 16) | (static_cast<uint32_t>(tile.bn >> 3) << 17) |
             (static_cast<uint32_t>(128 * CG >> 4) << 24);
   CUtensorMap ma, ma2, mb;
-  OBJB_TRY(encode(&ma, p.a, MAJ == dev::kMajKK ? (GATED ? 64 : 128) : 64));
+  OBJB_TRY(encode(&ma, p.a, MAJ == dev::kMajKK && !GATED ? tile.rm : 64));
   if (GATED)
     OBJB_TRY(encode(&ma2, p.a2, 64));
   else
     ma2 = ma;
-  OBJB_TRY(encode(&mb, p.b, MAJ == dev::kMajMN ? 64 : BN / CG));
-  auto kernel = dev::lin_gemm_kernel<MAJ, BN, CG, GATED>;
+  OBJB_TRY(encode(&mb, p.b, MAJ == dev::kMajMN ? 64 : tile.bn / CG));
+  auto kernel = dev::lin_gemm_kernel<MAJ, BN, CG, MT, GATED, PROMOTE>;
   OBJB_TRY(ensure_smem_attr(kernel, device, smem));
   const long long tiles = static_cast<long long>(g.tiles_m) * g.tiles_n;
-  const int csize = CG == 2 ? 2 : g.split;
-  const bool one_each = GATED || g.split > 1;
+  const int csize = CG == 2 ? 2 : tile.split;
+  const bool one_each = GATED || tile.split > 1;
   const long long clusters = one_each ? tiles : std::min<long long>(tiles, props.sm_count / csize);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(clusters * csize));
-  cfg.blockDim = dim3(dev::kLinThreads);
+  cfg.blockDim = dim3(dev::lin_threads(PROMOTE));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -278,66 +299,84 @@ int launch_gemm(const Product& p, dev::GemmArgs g, int device, const DeviceProps
   return OBJB_OK;
 }
 
-// Which tile a product takes.  CTA pairs (256 x 256) where the result has 16
-// bits, the operands one plane and the pairs' tiles fill the SMs; else single
-// CTAs of 128 rows by N up to 128, a tile's k split over a cluster while that
+size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
+
+// Columns of a pair's tile, 256 or fewer: the count (a multiple of 16) whose
+// rounds of the grid take the fewest columns in all.
+int pair_columns(size_t tiles_m, size_t N, int most, int step, int pairs) {
+  int best = most;
+  size_t cost = ~size_t{0};
+  for (int bn = most; bn >= most / 2; bn -= step) {
+    const size_t c = ceil_div(tiles_m * ceil_div(N, bn), pairs) * bn;
+    if (c < cost) cost = c, best = bn;
+  }
+  return best;
+}
+
+// Which tile a product takes.  CTA pairs where their tiles fill most of the
+// SMs: 512 x 256 straight from tensor memory for a 16-bit result of one-plane
+// operands, else 256 x 128 with promoted accumulators.  Otherwise single CTAs
+// of 128 rows by N up to 128, a tile's k split over a cluster while that
 // leaves SMs free.
 int gemm(const Product& p, int device, const DeviceProps& props, cudaStream_t st) {
-  dev::GemmArgs g;
-  g.M = static_cast<int>(p.M);
-  g.N = static_cast<long long>(p.N);
-  g.nkb = static_cast<int>((p.K + 63) / 64);
-  g.pa = p.a.planes;
-  g.pb = p.b.planes;
-  g.split = 1;
-  g.swiglu_limit = p.swiglu_limit;
-  g.epi = p.epi;
-  OBJB_TRY(device_error_word(device, &g.err));
-  const bool y16 = p.epi.y_dtype != OBJB_DTYPE_F32;
-  const size_t pair_tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (!p.gated && y16 && g.pa == 1 && g.pb == 1 && pair_tiles * 4 >= static_cast<size_t>(props.sm_count)) {
-    g.chunk_kb = g.nkb;
+  const size_t sms = static_cast<size_t>(props.sm_count);
+  const int pairs = props.sm_count / 2;
+  const size_t nkb = ceil_div(p.K, 64);
+  const bool y16 = !p.gated && p.epi.y_dtype != OBJB_DTYPE_F32;
+  const bool plain = p.a.planes == 1 && p.b.planes == 1;
+  Tile t;
+#define OBJB_GEMM(MAJ, BN, CG, MT, GATED, PROMOTE) return launch_gemm<MAJ, BN, CG, MT, GATED, PROMOTE>(p, t, device, props, st)
+  if (y16 && plain && ceil_div(p.M, 512) * ceil_div(p.N, 256) * 4 >= sms) {
+    t.bn = pair_columns(ceil_div(p.M, 512), p.N, 256, p.maj == dev::kMajMN ? 128 : 16, pairs);
     switch (p.maj) {
-      case dev::kMajKK: return launch_gemm<dev::kMajKK, 256, 2, false>(p, g, device, props, st);
-      case dev::kMajMK: return launch_gemm<dev::kMajMK, 256, 2, false>(p, g, device, props, st);
-      default: return launch_gemm<dev::kMajMN, 256, 2, false>(p, g, device, props, st);
+      case dev::kMajKK: OBJB_GEMM(dev::kMajKK, 256, 2, 2, false, false);
+      case dev::kMajMK: OBJB_GEMM(dev::kMajMK, 256, 2, 2, false, false);
+      default: OBJB_GEMM(dev::kMajMN, 256, 2, 2, false, false);
+    }
+  }
+  t.chunk_kb = y16 ? 16 : 4;
+  const size_t pair_m = ceil_div(p.M, p.gated ? 128 : 256);
+  if (pair_m * ceil_div(p.N, 128) * 4 >= sms) {
+    t.bn = p.maj == dev::kMajMN ? 128 : pair_columns(pair_m, p.N, 128, 16, pairs);
+    if (p.gated) OBJB_GEMM(dev::kMajKK, 128, 2, 1, true, true);
+    switch (p.maj) {
+      case dev::kMajKK: OBJB_GEMM(dev::kMajKK, 128, 2, 1, false, true);
+      case dev::kMajMK: OBJB_GEMM(dev::kMajMK, 128, 2, 1, false, true);
+      default: OBJB_GEMM(dev::kMajMN, 128, 2, 1, false, true);
     }
   }
   int bn = p.maj == dev::kMajMN ? 64 : 16;
   while (bn < 128 && static_cast<size_t>(bn) < p.N) bn *= 2;
-  const size_t mt = p.gated ? 64 : 128;
-  const size_t tiles = ((p.M + mt - 1) / mt) * ((p.N + bn - 1) / bn);
-  while (g.split < 8 && tiles * g.split * 2 <= static_cast<size_t>(props.sm_count) && g.nkb >= g.split * 2 * 4 &&
-         bn / (g.split * 2) >= 2)
-    g.split *= 2;
-  g.chunk_kb = y16 ? 16 : 4;
-#define OBJB_GEMM(MAJ, BN, GATED) return launch_gemm<MAJ, BN, 1, GATED>(p, g, device, props, st)
+  t.bn = p.maj == dev::kMajMN ? bn : static_cast<int>(std::min<size_t>(bn, ceil_div(p.N, 16) * 16));
+  const size_t tiles = ceil_div(p.M, p.gated ? 64 : 128) * ceil_div(p.N, t.bn);
+  while (t.split < 8 && tiles * t.split * 2 <= sms && nkb >= static_cast<size_t>(t.split) * 8 && bn / (t.split * 2) >= 2)
+    t.split *= 2;
   if (p.gated) {
     switch (bn) {
-      case 16: OBJB_GEMM(dev::kMajKK, 16, true);
-      case 32: OBJB_GEMM(dev::kMajKK, 32, true);
-      case 64: OBJB_GEMM(dev::kMajKK, 64, true);
-      default: OBJB_GEMM(dev::kMajKK, 128, true);
+      case 16: OBJB_GEMM(dev::kMajKK, 16, 1, 1, true, true);
+      case 32: OBJB_GEMM(dev::kMajKK, 32, 1, 1, true, true);
+      case 64: OBJB_GEMM(dev::kMajKK, 64, 1, 1, true, true);
+      default: OBJB_GEMM(dev::kMajKK, 128, 1, 1, true, true);
     }
   }
   switch (p.maj) {
     case dev::kMajKK:
       switch (bn) {
-        case 16: OBJB_GEMM(dev::kMajKK, 16, false);
-        case 32: OBJB_GEMM(dev::kMajKK, 32, false);
-        case 64: OBJB_GEMM(dev::kMajKK, 64, false);
-        default: OBJB_GEMM(dev::kMajKK, 128, false);
+        case 16: OBJB_GEMM(dev::kMajKK, 16, 1, 1, false, true);
+        case 32: OBJB_GEMM(dev::kMajKK, 32, 1, 1, false, true);
+        case 64: OBJB_GEMM(dev::kMajKK, 64, 1, 1, false, true);
+        default: OBJB_GEMM(dev::kMajKK, 128, 1, 1, false, true);
       }
     case dev::kMajMK:
       switch (bn) {
-        case 16: OBJB_GEMM(dev::kMajMK, 16, false);
-        case 32: OBJB_GEMM(dev::kMajMK, 32, false);
-        case 64: OBJB_GEMM(dev::kMajMK, 64, false);
-        default: OBJB_GEMM(dev::kMajMK, 128, false);
+        case 16: OBJB_GEMM(dev::kMajMK, 16, 1, 1, false, true);
+        case 32: OBJB_GEMM(dev::kMajMK, 32, 1, 1, false, true);
+        case 64: OBJB_GEMM(dev::kMajMK, 64, 1, 1, false, true);
+        default: OBJB_GEMM(dev::kMajMK, 128, 1, 1, false, true);
       }
     default:
-      if (bn == 64) OBJB_GEMM(dev::kMajMN, 64, false);
-      OBJB_GEMM(dev::kMajMN, 128, false);
+      if (bn == 64) OBJB_GEMM(dev::kMajMN, 64, 1, 1, false, true);
+      OBJB_GEMM(dev::kMajMN, 128, 1, 1, false, true);
   }
 #undef OBJB_GEMM
 }

@@ -5,22 +5,27 @@
 // its rows' elements (K-major) or with k along its rows (the transposed read
 // of the gradients, MN-major); an f32 operand has three bf16 planes (the upper,
 // middle and lower 8 bits of its significand), whose products are taken pair
-// by pair.  Rows of A are the rows m of an M 128 tcgen05.mma, rows of B its N,
-// so a tensor-memory lane is a row m and a warp's 32 lanes store 32
-// neighbouring elements of D's row n: no transposition on the way out.
+// by pair.  Rows of A are the rows m of a tcgen05.mma, rows of B its N, so a
+// tensor-memory lane is a row m and a warp's 32 lanes store 32 neighbouring
+// elements of D's row n: no transposition on the way out.
 //
 // One warp issues TMA copies into a ring of 128-byte-swizzled stages (64 of k,
-// all planes), one warp the MMAs, eight warps the epilogue (32 rows by half
-// of the columns each):
-//   * Single CTAs (CG 1), N 16..128.  The tensor core adds into its f32
-//     accumulators with truncation, so their error grows with the number of
-//     MMAs in one accumulator; the epilogue warps therefore take the
-//     accumulators into registers every chunk_kb k-blocks (two buffers) and
-//     add there, rounded to nearest.  The planes' cross products are below
-//     2^-8 of the main one and stay in a buffer of their own.
-//   * CTA pairs (CG 2, cta_group::2), M 256, N 256, for large 16-bit results:
-//     straight from tensor memory into the epilogue, two buffers over a
-//     persistent grid.
+// all planes), one warp the MMAs, the others the epilogue.  Accumulators:
+//   * PROMOTE.  The tensor core adds into its f32 accumulators with
+//     truncation, so their error grows with the number of MMAs in one
+//     accumulator; the epilogue warps therefore take the accumulators into
+//     registers every chunk_kb k-blocks (two buffers) and add there, rounded
+//     to nearest.  The planes' cross products are below 2^-8 of the main one
+//     and stay in a buffer of their own.
+//   * else straight from tensor memory into the epilogue, which rounds to 16
+//     bits: two accumulators of 256 columns, all of tensor memory.  The ring
+//     goes on filling while a tile is drained.
+// CTA pairs (CG 2, cta_group::2) share each MMA: M 256, half of B's rows from
+// each CTA's shared memory.  MT accumulators per CTA (rows m0 + a * rm) share
+// B's stage.  An L2-fed SM takes in about 64 bytes per clock, an MMA of 128 x
+// 256 x 64 per CTA pair half lasts 512 clocks: 512 x 256 tiles (48 KB a
+// k-block and CTA, 1024 clocks) are fed in time, 256 x 256 ones (32 KB, 512
+// clocks) were not (140 against 98 us at 4096^3).
 //   * Few tiles (CG 1): `split` CTAs of a cluster share a tile's k-blocks and
 //     fold their partial tiles through distributed shared memory in rank
 //     order: one launch, no atomics, no scratch.
@@ -42,14 +47,17 @@ enum { kMajKK = 0, kMajMK = 1, kMajMN = 2 };  // A, B: K-major both; A MN-major;
 
 constexpr int kLinBK = 64;        // k of a stage: 128 bytes, one swizzle row
 constexpr int kLinStagesMax = 12;
-constexpr int kLinThreads = 320;  // producer, MMA, eight epilogue warps
-constexpr int kLinAPlane = 128 * 128;
+// producer, MMA and eight (PROMOTE) or sixteen epilogue warps
+constexpr int lin_threads(bool promote) { return promote ? 320 : 576; }
+constexpr int kLinABlock = 128 * 128;  // bytes of 128 rows of A in a stage
 
 struct GemmArgs {
   int M;                  // rows of A (GATED: features)
   long long N;            // rows of B
   int nkb;                // k-blocks
   int tiles_m, tiles_n;
+  int rm;                 // rows of an accumulator in use (128, or fewer to even out the rounds of the grid)
+  int bn;                 // columns of a tile in use (at most BN)
   int pa, pb;             // planes
   int split;              // CTAs of a cluster per tile (CG 1)
   int chunk_kb;           // k-blocks per accumulator chunk
@@ -157,21 +165,21 @@ __device__ __forceinline__ void lin_tile(const GemmArgs& g, int t, int* tm, int*
   *tn = b * 8 + r - *tm * width;
 }
 
-template <int MAJ, int BN, int CG, bool GATED>
-__global__ void __launch_bounds__(kLinThreads, 1)
+template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE>
+__global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
     lin_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a2,
                     const __grid_constant__ CUtensorMap map_b, const GemmArgs g) {
   constexpr bool A_MN = MAJ != kMajKK, B_MN = MAJ == kMajMN;
-  constexpr bool PROMOTE = CG == 1;
-  constexpr int BNC = BN / CG;                 // rows of B in this CTA's shared memory
-  constexpr int kBPlane = BNC * 128;
-  constexpr int HN = BN / 2;                   // columns of an epilogue warp
-  constexpr int G = HN < 32 ? HN : 32;         // of one tensor-memory load
-  constexpr int P = G < 16 ? G : 16;           // of one step of the epilogue
-  constexpr uint32_t kCols = PROMOTE ? (4 * BN < 32 ? 32 : 4 * BN) : 2 * BN;  // main x 2 (, cross products x 2)
+  constexpr int kWarps = PROMOTE ? 8 : 16;       // epilogue warps
+  constexpr int HN = MT * BN * 4 / kWarps;       // accumulator columns of each
+  constexpr int G = HN < 32 ? HN : 32;           // of one tensor-memory load
+  constexpr int P = G < 16 ? G : 16;             // of one step of the epilogue
+  constexpr int kWide = MT * BN;                 // columns of one set of accumulators
+  constexpr uint32_t kUsed = PROMOTE ? 4 * kWide : kWide;  // main x 2, cross products x 2
+  constexpr uint32_t kCols = kUsed < 32 ? 32 : kUsed;
   static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0, "tensor memory columns");
-  static_assert(!B_MN || BNC % 64 == 0, "MN-major B comes in 64-row chunks");
-  static_assert(!GATED || (MAJ == kMajKK && CG == 1), "gated products are K-major, single CTAs");
+  static_assert(!GATED || (MAJ == kMajKK && MT == 1 && PROMOTE), "gated products are K-major, one accumulator");
+  static_assert(PROMOTE || (CG == 2 && MT == 2), "direct products are pairs of two accumulators");
 
   extern __shared__ uint8_t lin_smem[];
   __shared__ alignas(8) uint64_t full[kLinStagesMax], empty[kLinStagesMax], t_full[2], t_empty[2], c_empty[2];
@@ -184,7 +192,11 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < g.nstages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&t_full[i], 1), mbar_init(&t_empty[i], 8 * CG), mbar_init(&c_empty[i], 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&t_full[i], 1);
+      mbar_init(&t_empty[i], 8 * CG);  // PROMOTE: all epilogue warps; else the eight of accumulator i
+      mbar_init(&c_empty[i], 8 * CG);
+    }
     s_abort = 0;
     fence_mbar_init();
   }
@@ -207,43 +219,55 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   const int krank = CG == 1 ? static_cast<int>(rank) : 0;
   const int kb0 = static_cast<int>(static_cast<long long>(g.nkb) * krank / g.split);
   const int kb1 = static_cast<int>(static_cast<long long>(g.nkb) * (krank + 1) / g.split);
-  const uint32_t stage_bytes = g.pa * kLinAPlane + g.pb * kBPlane;
+  const uint32_t b_rows = g.bn / CG, b_plane = b_rows * 128;  // of B in this CTA's shared memory
+  constexpr uint32_t kAPlane = MT * kLinABlock;
+  const uint32_t stage_bytes = g.pa * kAPlane + g.pb * b_plane;
+  // first row of A of this CTA's part of tile row tm
+  const int cta_rows = GATED ? 64 : MT * g.rm;
+  auto row0 = [&](int tm) { return (tm * CG + (CG == 2 ? static_cast<int>(rank) : 0)) * cta_rows; };
 
   if (warp == 0) {
     if (lane == 0) {
       // ---- producer
+      const uint32_t tx = CG * (g.pa * MT * g.rm * 128 + g.pb * b_plane);
       int issued = 0, st = 0;
       uint32_t phase = 1;  // of empty[st]: the first round finds every stage free
       bool ok = true;
       for (int t = first; t < ntiles && ok; t += step) {
         int tm, tn;
         lin_tile(g, t, &tm, &tn);
-        const int m0 = GATED ? tm * 64 : (tm * CG + (CG == 2 ? rank : 0)) * 128;
-        const int n0 = tn * BN + (CG == 2 ? rank * BNC : 0);
+        const int m0 = row0(tm);
+        const int n0 = tn * g.bn + (CG == 2 ? rank * b_rows : 0);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait_bounded(&empty[st], phase, g.err, kErrEmptyWaitTimeout, &s_abort)) {
             ok = false;
             break;
           }
           uint32_t bar = smem_u32(&full[st]);
-          if (rank == 0 || CG == 1) mbar_arrive_expect_tx(&full[st], stage_bytes * CG);
+          if (rank == 0 || CG == 1) mbar_arrive_expect_tx(&full[st], tx);
           if (CG == 2) bar = lin_mapa(bar, 0);
           uint32_t dst = smem_u32(stages) + st * stage_bytes;
-          for (int p = 0; p < g.pa; ++p, dst += kLinAPlane) {
+          for (int p = 0; p < g.pa; ++p) {
             if constexpr (GATED) {
               lin_tma<CG>(dst, &map_a, kb * 64, m0, p, bar);
               lin_tma<CG>(dst + 8192, &map_a2, kb * 64, m0, p, bar);
-            } else if constexpr (A_MN) {
-              lin_tma<CG>(dst, &map_a, m0, kb * 64, p, bar);
-              lin_tma<CG>(dst + 8192, &map_a, m0 + 64, kb * 64, p, bar);
+              dst += kLinABlock;
             } else {
-              lin_tma<CG>(dst, &map_a, kb * 64, m0, p, bar);
+#pragma unroll
+              for (int a = 0; a < MT; ++a, dst += kLinABlock) {
+                if constexpr (A_MN) {
+                  lin_tma<CG>(dst, &map_a, m0 + a * 128, kb * 64, p, bar);
+                  lin_tma<CG>(dst + 8192, &map_a, m0 + a * 128 + 64, kb * 64, p, bar);
+                } else {
+                  lin_tma<CG>(dst, &map_a, kb * 64, m0 + a * g.rm, p, bar);
+                }
+              }
             }
           }
-          for (int p = 0; p < g.pb; ++p, dst += kBPlane) {
+          for (int p = 0; p < g.pb; ++p, dst += b_plane) {
             if constexpr (B_MN) {
-#pragma unroll
-              for (int c = 0; c < BNC / 64; ++c) lin_tma<CG>(dst + c * 8192, &map_b, n0 + c * 64, kb * 64, p, bar);
+              for (int c = 0; c < static_cast<int>(b_rows); c += 64)
+                lin_tma<CG>(dst + c * 128, &map_b, n0 + c, kb * 64, p, bar);
             } else {
               lin_tma<CG>(dst, &map_b, kb * 64, n0, p, bar);
             }
@@ -269,18 +293,20 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       constexpr uint32_t kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
       const uint64_t base_a = lin_desc<A_MN>(0), base_b = lin_desc<B_MN>(0);
       for (int t = first; t < ntiles && ok; t += step, ++tt) {
-        const uint32_t d_cross = tmem + (2 + (tt & 1)) * BN;
+        const uint32_t d_cross = tmem + (2 + (tt & 1)) * kWide;
         bool cross_acc = false;
-        if (cross && tt >= 2)
+        if (PROMOTE && cross && tt >= 2)
           ok = lin_wait(&c_empty[tt & 1], ((tt >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort);
         for (int kb = kb0; kb < kb1 && ok; ++cc) {
-          const int buf = cc & 1;
-          if (cc >= 2 && !lin_wait(&t_empty[buf], ((cc >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
+          // PROMOTE: chunk cc into buffer cc & 1; else the tile into both accumulators
+          const int buf = PROMOTE ? cc & 1 : 0;
+          if (PROMOTE && cc >= 2 &&
+              !lin_wait(&t_empty[buf], ((cc >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t d_main = tmem + buf * BN;
+          const uint32_t d_main = tmem + buf * kWide;
           const int end = kb + g.chunk_kb < kb1 ? kb + g.chunk_kb : kb1;
           bool acc = false;
           for (; kb < end; ++kb) {
@@ -292,22 +318,32 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             const uint32_t sa = smem_u32(stages) + st * stage_bytes;
             // (in a cluster a shared address carries the CTA's rank above the 18 bits a descriptor has room for)
             const uint64_t da = base_a + ((sa & 0x3FFFFu) >> 4);
-            const uint64_t db = base_b + (((sa + g.pa * kLinAPlane) & 0x3FFFFu) >> 4);
+            const uint64_t db = base_b + (((sa + g.pa * kAPlane) & 0x3FFFFu) >> 4);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              lin_mma<CG>(d_main, da + k * kStepA, db + k * kStepB, g.idesc, acc);
-              acc = true;
+            for (int a = 0; a < MT; ++a) {
+              if (!PROMOTE && !acc && tt >= 1) {  // accumulator a of the tile before is drained
+                if (!lin_wait(&t_empty[a], (tt - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) ok = false;
+                tc_fence_after_sync();
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                lin_mma<CG>(d_main + a * BN, da + a * (kLinABlock >> 4) + k * kStepA, db + k * kStepB, g.idesc,
+                            acc || k > 0);
+              if (!PROMOTE && kb + 1 == kb1) umma_commit_pair(&t_full[a]);
             }
+            acc = true;
             if (PROMOTE && cross) {
               // planes (i, j) with 0 < i + j <= 2: what is left out is below 2^-24
               for (int i = 0; i < g.pa; ++i)
                 for (int j = i ? 0 : 1; j < g.pb && i + j <= 2; ++j) {
-                  const uint64_t ai = da + i * (kLinAPlane >> 4), bj = db + j * (kBPlane >> 4);
+                  const uint64_t ai = da + i * (kAPlane >> 4), bj = db + j * (b_plane >> 4);
 #pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    lin_mma<CG>(d_cross, ai + k * kStepA, bj + k * kStepB, g.idesc, cross_acc);
-                    cross_acc = true;
-                  }
+                  for (int a = 0; a < MT; ++a)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                      lin_mma<CG>(d_cross + a * BN, ai + a * (kLinABlock >> 4) + k * kStepA, bj + k * kStepB, g.idesc,
+                                  cross_acc || k > 0);
+                  cross_acc = true;
                 }
             }
             if constexpr (CG == 1)
@@ -316,27 +352,43 @@ __global__ void __launch_bounds__(kLinThreads, 1)
               umma_commit_pair(&empty[st]);
             if (++st == g.nstages) st = 0, phase ^= 1;
           }
-          if constexpr (CG == 1)
-            umma_commit(&t_full[buf]);
-          else
-            umma_commit_pair(&t_full[buf]);
+          if constexpr (PROMOTE) {
+            if constexpr (CG == 1)
+              umma_commit(&t_full[buf]);
+            else
+              umma_commit_pair(&t_full[buf]);
+          }
         }
       }
     }
   } else {
     // ---- epilogue
-    const int quarter = warp & 3;  // tensor-memory lanes 32 quarter ..
-    const int col0 = warp < 6 ? 0 : HN;
-    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + col0;
+    const int quarter = warp & 3;                 // tensor-memory lanes 32 quarter ..
+    const int part = (warp - 2) >> 2;             // of the accumulator columns
+    const int a = part * HN / BN;                 // accumulator
+    const int col0 = part * HN - a * BN;          // and column in it
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * HN;
     const int row = quarter * 32 + lane;
     int cc = 0, tt = 0;
     bool ok = true;
     const bool cross = g.pa + g.pb > 2;
+    auto release = [&](uint64_t* bar) {
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 1)
+          mbar_arrive(bar);
+        else
+          mbar_arrive_cta_relaxed(bar, 0);
+      }
+    };
     for (int t = first; t < ntiles && ok; t += step, ++tt) {
       int tm, tn;
       lin_tile(g, t, &tm, &tn);
-      const long long n0 = static_cast<long long>(tn) * BN + col0;
-      const int m = GATED ? tm * 64 + (row & 63) : (tm * CG + (CG == 2 ? static_cast<int>(rank) : 0)) * 128 + row;
+      const long long n0 = static_cast<long long>(tn) * g.bn;
+      const long long n_end = n0 + g.bn < g.N ? n0 + g.bn : g.N;
+      const int m = GATED ? 0 : row0(tm) + a * g.rm + row;
+      const bool m_ok = row < g.rm && m < g.M;
       if constexpr (PROMOTE) {
         float acc[HN];
 #pragma unroll
@@ -350,8 +402,6 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 #pragma unroll
             for (int i = 0; i < G; ++i) acc[c + i] += v[i];
           }
-          tc_fence_before_sync();
-          __syncwarp();
         };
         for (int kb = kb0; kb < kb1; kb += g.chunk_kb, ++cc) {
           const int buf = cc & 1;
@@ -360,30 +410,29 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             break;
           }
           tc_fence_after_sync();
-          take(t_lane + buf * BN);
-          if (lane == 0) mbar_arrive(&t_empty[buf]);
+          take(t_lane + buf * kWide);
+          release(&t_empty[buf]);
         }
         if (cross && ok) {
-          take(t_lane + (2 + (tt & 1)) * BN);
-          if (lane == 0) mbar_arrive(&c_empty[tt & 1]);
+          take(t_lane + (2 + (tt & 1)) * kWide);
+          release(&c_empty[tt & 1]);
         }
         if (GATED || g.split > 1) {
-          // one tile per CTA: its stages are done with, the partial tile goes there as [n][row]
-          float* ex = reinterpret_cast<float*>(stages) + col0 * 128 + row;
+          // one tile per CTA: its stages are done with, the partial tile goes there as [column][row]
+          float* ex = reinterpret_cast<float*>(stages) + part * HN * 128 + row;
 #pragma unroll
           for (int i = 0; i < HN; ++i) ex[i * 128] = acc[i];
-        } else if (ok && m < g.M) {
+        } else if (ok && m_ok) {
 #pragma unroll
           for (int c = 0; c < HN; c += P) {
             float v[P];
 #pragma unroll
             for (int i = 0; i < P; ++i) v[i] = acc[c + i];
-            g.epi.put_columns<P>(m, n0 + c, g.N, v);
+            g.epi.put_columns<P>(m, n0 + col0 + c, n_end, v);
           }
         }
       } else {
-        const int buf = tt & 1;
-        if (!lin_wait(&t_full[buf], (tt >> 1) & 1, g.err, kErrFullWaitTimeout, &s_abort)) {
+        if (!lin_wait(&t_full[a], tt & 1, g.err, kErrFullWaitTimeout, &s_abort)) {
           ok = false;
           break;
         }
@@ -391,14 +440,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 #pragma unroll 1
         for (int c = 0; c < HN; c += P) {
           float v[P];
-          tmem_ldf<P>(t_lane + buf * BN + c, v);
+          tmem_ldf<P>(t_lane + c, v);
           tmem_wait_ld();
-          if (c + P == HN) {  // the accumulator is read: the next tile may have it
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cta_relaxed(&t_empty[buf], 0);
-          }
-          if (m < g.M) g.epi.put_columns<P>(m, n0 + c, g.N, v);
+          if (c + P == HN) release(&t_empty[a]);  // read: the next tile may have the accumulator
+          if (m_ok) g.epi.put_columns<P>(m, n0 + col0 + c, n_end, v);
         }
       }
     }
@@ -411,25 +456,31 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       int tm, tn;
       lin_tile(g, first, &tm, &tn);
       const uint32_t ex = smem_u32(stages);
-      const int per = BN / g.split, c0 = static_cast<int>(rank) * per;
-      const long long n0 = static_cast<long long>(tn) * BN;
+      const long long n0 = static_cast<long long>(tn) * g.bn;
+      const long long n_end = n0 + g.bn < g.N ? n0 + g.bn : g.N;
+      const int krank_cols = CG == 1 ? kWide / g.split : kWide, c0 = krank * krank_cols;
       if constexpr (GATED) {
-        const int tid = threadIdx.x - 64, f = tid & 63, m = tm * 64 + f;
-        for (int c = c0 + (tid >> 6); c < c0 + per; c += 4) {
+        const int tid = threadIdx.x - 64, f = tid & 63, m = row0(tm) + f;
+        for (int c = c0 + (tid >> 6); c < c0 + krank_cols; c += 4) {
+          if (m >= g.M || n0 + c >= n_end) continue;
           float gate = 0.0f, up = 0.0f;
           for (int s = 0; s < g.split; ++s) {
             const uint32_t at = (g.split > 1 ? lin_mapa(ex, s) : ex) + (c * 128 + f) * 4;
             gate += lin_ld_cluster(at);
             up += lin_ld_cluster(at + 256);
           }
-          if (m < g.M && n0 + c < g.N) g.epi.put_planes(m, n0 + c, swiglu(gate, up, g.swiglu_limit));
+          g.epi.put_planes(m, n0 + c, swiglu(gate, up, g.swiglu_limit));
         }
       } else {
         // threads of 128 rows by two halves of this CTA's columns
-        const int tid = threadIdx.x - 64, row = tid & 127, m = tm * 128 + row;
+        const int tid = threadIdx.x - 64, row = tid & 127;
         auto fold = [&](auto cnt) {
           constexpr int C = decltype(cnt)::value;
-          for (int c = c0 + (tid >> 7) * C; c < c0 + per; c += 2 * C) {
+          for (int c = c0 + (tid >> 7) * C; c < c0 + krank_cols; c += 2 * C) {
+            const int a = c / BN;
+            const int m = row0(tm) + a * g.rm + row;
+            const long long n = n0 + c - a * BN;
+            if (row >= g.rm || m >= g.M || n >= n_end) continue;
             float v[C];
 #pragma unroll
             for (int i = 0; i < C; ++i) v[i] = 0.0f;
@@ -438,10 +489,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 #pragma unroll
               for (int i = 0; i < C; ++i) v[i] += lin_ld_cluster(at + i * 512);
             }
-            if (m < g.M) g.epi.put_columns<C>(m, n0 + c, g.N, v);
+            g.epi.put_columns<C>(m, n, n_end, v);
           }
         };
-        if (per % 8 == 0)
+        if (krank_cols % 8 == 0)
           fold(std::integral_constant<int, 4>{});
         else
           fold(std::integral_constant<int, 1>{});

@@ -327,26 +327,35 @@ def test_c_entry_with_the_streams_workspace(cuda_device):
     assert torch.equal(y, linear(x, w))
 
 
-@pytest.mark.parametrize("dt", ["bf16", "f16"])
-def test_large_tiles(cuda_device, dt):
-    """Results that fill the SMs with 256 x 256 tiles, ragged on both sides,
+@pytest.mark.parametrize("xd,wd,yd", PAIRS)
+def test_large_tiles(cuda_device, xd, wd, yd):
+    """Results that fill the SMs with the largest tiles, ragged on both sides,
     more tiles than the grid holds at once, one k-block and many."""
     from objeta_b200.dense import linear
-    for T, K, N, act in ((1500, 200, 1800, "none"), (2049, 40, 1537, "silu"), (2600, 1000, 2570, "gelu_tanh"),
-                         (8000, 64, 1000, "relu")):
-        x, w = _case(T, K, N, dt, dt, 4)
-        yt = U.DT[dt]
-        b, r = U.randn((N,), yt, seed=8), U.randn((T, N), yt, seed=9)
+    for T, K, N, act in ((1500, 200, 1800, "none"), (2049, 40, 1537, "silu"), (2600, 1000, 5000, "gelu_tanh"),
+                         (8000, 64, 1000, "relu"), (4100, 72, 4100, "none")):
+        x, w = _case(T, K, N, xd, wd, 4)
+        yt = U.DT[yd]
+        b, r = U.randn((N,), U.DT[wd], seed=8), U.randn((T, N), yt, seed=9)
         z = torch.empty(T, N, dtype=yt, device="cuda")
-        y = linear(x, w, b, activation=act, d_residual=r, d_z=z)
+        y = linear(x, w, b, activation=act, d_residual=r, d_z=z, out_dtype=yt)
         rz, bz, ry, by = U.linear_ref(x, w, b, act, r, yt)
         U.check(z, rz, bz, "z")
         U.check(y, ry, by, "y")
-        assert torch.equal(y, linear(x, w, b, activation=act, d_residual=r))
+        assert torch.equal(y, linear(x, w, b, activation=act, d_residual=r, out_dtype=yt))
 
 
-@pytest.mark.parametrize("dt", ["bf16", "f16"])
-def test_large_tiles_backward(cuda_device, dt):
-    _run_backward(1600, 1704, 1601, dt, dt, dt, dt, "none", 3)
-    _run_backward(1603, 1801, 2056, dt, dt, dt, dt, "silu", 4)
-    _run_backward(130, 2700, 2600, dt, dt, dt, dt, "none", 5)
+@pytest.mark.parametrize("xd,wd,yd,dwd", BPAIRS)
+def test_large_tiles_backward(cuda_device, xd, wd, yd, dwd):
+    _run_backward(1600, 1704, 1601, xd, wd, yd, dwd, "none", 3)
+    _run_backward(2603, 1801, 4056, xd, wd, yd, dwd, "silu", 4)
+    _run_backward(130, 2700, 2600, xd, wd, yd, dwd, "none", 5)
+
+
+def test_large_tiles_ffn(cuda_device):
+    from objeta_b200.dense import ffn_bf16_tokens
+    for T, H, I, O in ((700, 264, 800, 1000), (1001, 72, 1500, 136)):
+        x, r = U.randn((T, H), seed=1), U.randn((T, O), seed=5)
+        g, u = U.randn((I, H), torch.bfloat16, 1 / math.sqrt(H), 2), U.randn((I, H), torch.bfloat16, 1 / math.sqrt(H), 3)
+        d = U.randn((O, I), torch.bfloat16, 1 / math.sqrt(I), 4)
+        U.check(ffn_bf16_tokens(g, u, d, x, d_residual=r), *_ffn_ref(g, u, d, x, r, 0.0), "out")
