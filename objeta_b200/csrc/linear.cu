@@ -11,41 +11,67 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
+#include <map>
 #include <mutex>
 #include <string>
 
 #include "objb_common.h"
 #include "objb_host_launch.cuh"
 #include "objb_launch.h"
-#include "objb_linear_gemm.cuh"
+#include "objb_linear_launch.cuh"
 
 namespace objb {
 namespace dev {
 
-// 8 neighbouring elements as f32; VEC: their address is 16-byte aligned.
-template <bool VEC>
-__device__ __forceinline__ void load8(const void* p, int dtype, size_t at, int n, float (&v)[8]) {
-  if constexpr (VEC) {
-    if (n >= 8) {
-      if (dtype == OBJB_DTYPE_F32) {
-        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-        const float4 a = q[0], b = q[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-      } else {
-        const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
-        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+// 8 neighbouring elements in flight; T: float, __nv_bfloat16 or __half.  VEC:
+// their address is 16-byte aligned and all 8 exist.
+template <class T, bool VEC>
+struct Oct {
+  uint4 q[sizeof(T) / 2];
+  T e[VEC ? 1 : 8];
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if constexpr (VEC) {
+      const uint4* s = reinterpret_cast<const uint4*>(p);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint16_t h = static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)));
-          v[i] = dtype == OBJB_DTYPE_BF16 ? __uint_as_float(static_cast<uint32_t>(h) << 16)
-                                          : __half2float(__ushort_as_half(h));
-        }
-      }
-      return;
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) q[i] = __ldg(s + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : T(0.0f);
     }
   }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    if constexpr (!VEC) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < n ? load_elem(p, dtype, at + i) : 0.0f;
+      for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(e[i]);
+    } else if constexpr (sizeof(T) == 4) {
+      v[0] = __uint_as_float(q[0].x), v[1] = __uint_as_float(q[0].y), v[2] = __uint_as_float(q[0].z);
+      v[3] = __uint_as_float(q[0].w), v[4] = __uint_as_float(q[1].x), v[5] = __uint_as_float(q[1].y);
+      v[6] = __uint_as_float(q[1].z), v[7] = __uint_as_float(q[1].w);
+    } else {
+      const uint32_t u[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint16_t h = static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)));
+        if constexpr (std::is_same<T, __half>::value)
+          v[i] = __half2float(__ushort_as_half(h));
+        else
+          v[i] = __uint_as_float(static_cast<uint32_t>(h) << 16);
+      }
+    }
+  }
+};
+
+// f(T, VEC) for an element type; vec: rows of aligned octs.
+template <class F>
+auto with_elements(int dtype, bool vec, F&& f) {
+  using std::integral_constant;
+  if (dtype == OBJB_DTYPE_F32)
+    return vec ? f(float{}, integral_constant<bool, true>{}) : f(float{}, integral_constant<bool, false>{});
+  if (dtype == OBJB_DTYPE_BF16)
+    return vec ? f(__nv_bfloat16{}, integral_constant<bool, true>{})
+               : f(__nv_bfloat16{}, integral_constant<bool, false>{});
+  return vec ? f(__half{}, integral_constant<bool, true>{}) : f(__half{}, integral_constant<bool, false>{});
 }
 
 // 8 elements of an image row (its pitch is a whole number of 16-byte quads):
@@ -74,51 +100,102 @@ __device__ __forceinline__ void store_image8(uint16_t* img, size_t plane, size_t
       *reinterpret_cast<uint4*>(img + j * plane + at) = make_uint4(u[j][0], u[j][1], u[j][2], u[j][3]);
 }
 
-// An operand laid out for the copy engine: rows of `pitch` elements (a multiple
-// of 8), f32 in planes.  8 elements per thread.
-template <bool VEC>
-__global__ void __launch_bounds__(256) image_kernel(const void* src, int dtype, size_t ld, long long rows, int cols,
-                                                    uint16_t* img, int pitch, int planes) {
+// Up to two operands laid out for the copy engine in one launch: rows of
+// `pitch` elements (a multiple of 8), f32 in planes.  8 elements per thread; a
+// block takes 256 >> log_width rows at a time, two in flight.
+struct ImageJob {
+  const void* src;
+  uint16_t* img;
+  size_t ld;
+  long long rows;
+  int cols, pitch, planes, dtype, vec, log_width;
+};
+template <class T, bool VEC>
+__device__ __forceinline__ void image_run(const ImageJob& j) {
+  const int width = 1 << j.log_width, per = 256 >> j.log_width;
+  const int tx = threadIdx.x & (width - 1), ty = threadIdx.x >> j.log_width;
+  const size_t plane = j.rows * static_cast<size_t>(j.pitch);
+  const T* src = static_cast<const T*>(j.src);
+  for (long long r = static_cast<long long>(blockIdx.x) * per * 2 + ty; r < j.rows;
+       r += static_cast<long long>(gridDim.x) * per * 2) {
+    const bool two = r + per < j.rows;
+    for (int c = tx * 8; c < j.pitch; c += width * 8) {
+      Oct<T, VEC> a, b;
+      float v[8];
+      a.load(src + r * j.ld + c, j.cols - c);
+      if (two) b.load(src + (r + per) * j.ld + c, j.cols - c);
+      a.values(v);
+      store_image8(j.img, plane, r * static_cast<size_t>(j.pitch) + c, j.planes, j.dtype, v);
+      if (two) {
+        b.values(v);
+        store_image8(j.img, plane, (r + per) * static_cast<size_t>(j.pitch) + c, j.planes, j.dtype, v);
+      }
+    }
+  }
+}
+__global__ void __launch_bounds__(256) image_kernel(const ImageJob first, const ImageJob second) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int quads = pitch / 8;
-  const long long n = rows * quads;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
-    const long long r = i / quads;
-    const int c = static_cast<int>(i - r * quads) * 8;
-    float v[8];
-    load8<VEC>(src, dtype, r * ld + c, cols - c, v);
-    store_image8(img, rows * static_cast<size_t>(pitch), r * static_cast<size_t>(pitch) + c, planes, dtype, v);
-  }
+  const ImageJob j = blockIdx.y ? second : first;
+  if (j.dtype == OBJB_DTYPE_F32)
+    j.vec ? image_run<float, true>(j) : image_run<float, false>(j);
+  else if (j.dtype == OBJB_DTYPE_BF16)
+    j.vec ? image_run<__nv_bfloat16, true>(j) : image_run<__nv_bfloat16, false>(j);
+  else
+    j.vec ? image_run<__half, true>(j) : image_run<__half, false>(j);
 }
 
 // dz = dy act'(z) as an image (may be null: only its sums), and the column
-// sums of each run of rows.  A block: 256 columns (8 per thread), 8 rows at a
-// time; the 8 row lanes are folded in order.
-template <bool VEC>
-__global__ void __launch_bounds__(256) dz_kernel(const void* dy, size_t ldy, const void* z, size_t ldz, int dtype,
-                                                 int act, long long T, int N, uint16_t* img, int pitch, int planes,
+// sums of each run of rows.  A block: 256 columns (8 per thread), 8 row lanes
+// with four rows in flight; the lanes are folded in order.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) dz_kernel(const T* dy, size_t ldy, const T* z, size_t ldz, int dtype, int act,
+                                                 long long rows, int N, uint16_t* img, int pitch, int planes,
                                                  long long rows_per, float* part) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   __shared__ float sm[8][256];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 256 + tx * 8;
-  const long long r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < T ? r0 + rows_per : T;
+  const long long r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < rows ? r0 + rows_per : rows;
   float s[8] = {};
   if (c < N) {
-    for (long long r = r0 + ty; r < r1; r += 8) {
-      float v[8];
-      load8<VEC>(dy, dtype, r * ldy + c, N - c, v);
-      if (act != OBJB_ACT_NONE) {
-        float zz[8];
-        load8<VEC>(z, dtype, r * ldz + c, N - c, zz);
+    constexpr int R = sizeof(T) == 4 ? 2 : 4;
+    for (long long r = r0 + ty; r < r1; r += 8 * R) {
+      Oct<T, VEC> d[R], a[R];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= act_grad(act, zz[i]);
-      }
-      if (img) store_image8(img, T * static_cast<size_t>(pitch), r * static_cast<size_t>(pitch) + c, planes, dtype, v);
+      for (int q = 0; q < R; ++q)
+        if (r + 8 * q < r1) {
+          d[q].load(dy + (r + 8 * q) * ldy + c, N - c);
+          if (act != OBJB_ACT_NONE) a[q].load(z + (r + 8 * q) * ldz + c, N - c);
+        }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] += v[i];
+      for (int q = 0; q < R; ++q)
+        if (r + 8 * q < r1) {
+          float v[8];
+          d[q].values(v);
+          if (act != OBJB_ACT_NONE) {
+            float zz[8];
+            a[q].values(zz);
+            switch (act) {
+#define OBJB_GRAD_CASE(A) \
+  case A:                 \
+    _Pragma("unroll") for (int i = 0; i < 8; ++i) v[i] *= act_grad(A, zz[i]); \
+    break
+              OBJB_GRAD_CASE(OBJB_ACT_RELU);
+              OBJB_GRAD_CASE(OBJB_ACT_SILU);
+              OBJB_GRAD_CASE(OBJB_ACT_GELU);
+              OBJB_GRAD_CASE(OBJB_ACT_GELU_TANH);
+#undef OBJB_GRAD_CASE
+              default: break;
+            }
+          }
+          if (img)
+            store_image8(img, rows * static_cast<size_t>(pitch), (r + 8 * q) * static_cast<size_t>(pitch) + c, planes,
+                         dtype, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[i] += v[i];
+        }
     }
   }
   if (!part) return;
@@ -133,15 +210,25 @@ __global__ void __launch_bounds__(256) dz_kernel(const void* dy, size_t ldy, con
   part[static_cast<size_t>(blockIdx.y) * N + col] = sum;
 }
 
-__global__ void __launch_bounds__(256) dbias_kernel(const float* part, int parts, int N, float* db, int accumulate) {
+// The runs' sums folded: 32 columns per block, 32 interleaved runs, those in order.
+__global__ void __launch_bounds__(1024) dbias_kernel(const float* part, int parts, int N, float* db, int accumulate) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= N) return;
+  __shared__ float sm[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + tx;
   float s = 0.0f;
-#pragma unroll 8
-  for (int i = 0; i < parts; ++i) s += part[static_cast<size_t>(i) * N + c];
-  db[c] = accumulate ? db[c] + s : s;
+  if (c < N) {
+#pragma unroll 4
+    for (int i = ty; i < parts; i += 32) s += part[static_cast<size_t>(i) * N + c];
+  }
+  sm[ty][tx] = s;
+  __syncthreads();
+  s = sm[tx][ty];  // column ty, run tx
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  const int col = blockIdx.x * 32 + ty;
+  if (tx == 0 && col < N) db[col] = accumulate ? db[col] + s : s;
 }
 
 }  // namespace dev
@@ -150,18 +237,10 @@ namespace {
 
 constexpr size_t kMaxSize = size_t{1} << 24;    // in / out features
 constexpr size_t kMaxTokens = size_t{1} << 30;
+constexpr size_t kMaxStride = size_t{1} << 28;
 
 size_t r256(size_t b) { return (b + 255) / 256 * 256; }
 size_t elem_bytes(int dtype) { return dtype == OBJB_DTYPE_F32 ? 4 : 2; }
-
-// A 16-bit matrix as the copy engine reads it: 16-byte aligned, rows of `ld`
-// elements (a multiple of 8), `planes` of them `rows * ld` apart.
-struct Image {
-  const void* p = nullptr;
-  size_t ld = 0, rows = 0, cols = 0;
-  int planes = 1;
-  int dtype = 0;  // OBJB_DTYPE_BF16 or F16
-};
 
 // How an operand becomes an image: as it lies, or laid out in the scratch.
 struct ImagePlan {
@@ -178,28 +257,63 @@ ImagePlan plan_image(const void* p, int dtype, size_t ld, size_t rows, size_t co
   return i;
 }
 
-int make_image(const ImagePlan& pl, const void* p, int dtype, size_t ld, size_t rows, size_t cols, void* scratch,
-               const DeviceProps& props, cudaStream_t st, Image* out) {
-  out->rows = rows;
-  out->cols = cols;
-  out->planes = pl.planes;
-  out->ld = pl.pitch;
-  out->dtype = pl.planes > 1 || dtype == OBJB_DTYPE_F32 ? OBJB_DTYPE_BF16 : dtype;
-  if (pl.direct) {
-    out->p = p;
+// The images of up to two operands, laid out by one launch where they are not
+// direct.
+class Images {
+ public:
+  Image take(const ImagePlan& pl, const void* p, int dtype, size_t ld, size_t rows, size_t cols, void* scratch) {
+    Image im;
+    im.rows = rows;
+    im.cols = cols;
+    im.planes = pl.planes;
+    im.ld = pl.pitch;
+    im.dtype = pl.planes > 1 || dtype == OBJB_DTYPE_F32 ? OBJB_DTYPE_BF16 : dtype;
+    im.p = pl.direct ? p : scratch;
+    if (!pl.direct) {
+      dev::ImageJob& j = jobs_[n_++];
+      j.src = p;
+      j.img = static_cast<uint16_t*>(scratch);
+      j.ld = ld;
+      j.rows = static_cast<long long>(rows);
+      j.cols = static_cast<int>(cols);
+      j.pitch = static_cast<int>(pl.pitch);
+      j.planes = pl.planes;
+      j.dtype = dtype;
+      j.vec = aligned16(p) && ld % 8 == 0 && cols % 8 == 0;
+      j.log_width = 0;
+      while (j.log_width < 8 && (8u << j.log_width) < pl.pitch) ++j.log_width;
+      blocks_ = std::max(blocks_, ceil_div(rows, size_t{512} >> j.log_width));
+    }
+    return im;
+  }
+  int launch(const DeviceProps& props, cudaStream_t st) {
+    if (!n_) return OBJB_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(blocks_, static_cast<size_t>(props.sm_count) * 8)),
+                       static_cast<unsigned>(n_));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    n_ = 0;
+    blocks_ = 0;
+    OBJB_CUDA(cudaLaunchKernelEx(&cfg, dev::image_kernel, jobs_[0], jobs_[1]), "launch operand image");
     return OBJB_OK;
   }
-  out->p = scratch;
-  const size_t n = rows * (pl.pitch / 8);
-  const int grid = static_cast<int>(std::min<size_t>((n + 255) / 256, static_cast<size_t>(props.sm_count) * 16));
-  const bool vec = aligned16(p) && ld % 8 == 0;
-  auto k = vec ? dev::image_kernel<true> : dev::image_kernel<false>;
-  return launch_pdl(k, grid, 256, 0, st, p, dtype, ld, static_cast<long long>(rows), static_cast<int>(cols),
-                    static_cast<uint16_t*>(scratch), static_cast<int>(pl.pitch), pl.planes);
-}
 
-// The tensor map of an image: box of 64 elements by `box_rows` rows.
-int encode(CUtensorMap* map, const Image& im, int box_rows) {
+ private:
+  dev::ImageJob jobs_[2] = {};
+  int n_ = 0;
+  size_t blocks_ = 0;
+};
+
+// The tensor map of an image: box of 64 elements by `box_rows` rows, all planes.
+}  // namespace
+
+int linear_encode(CUtensorMap* map, const Image& im, int box_rows) {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -212,7 +326,7 @@ int encode(CUtensorMap* map, const Image& im, int box_rows) {
   if (!fn) return OBJB_FAIL(OBJB_ERR_DRIVER, "dense product", "cuTensorMapEncodeTiled is not available");
   const cuuint64_t dims[3] = {im.cols, im.rows, static_cast<cuuint64_t>(im.planes)};
   const cuuint64_t strides[2] = {im.ld * 2, im.rows * im.ld * 2};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(im.planes)};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r =
       fn(map, im.dtype == OBJB_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
@@ -223,162 +337,173 @@ int encode(CUtensorMap* map, const Image& im, int box_rows) {
   return OBJB_OK;
 }
 
-struct Product {
-  int maj = dev::kMajKK;
-  Image a, a2, b;  // a2: the up rows of a gated product
-  bool gated = false;
-  size_t M = 0, N = 0, K = 0;
-  dev::LinearEpilogue epi;
-  float swiglu_limit = 0.0f;
+namespace {
+
+struct Choice {
+  TileKind kind = kSingle;
+  Tile tile;
 };
 
-constexpr size_t kLinRing = 216 * 1024;  // bytes of stages: three of f32 x f32 pair tiles
-
-// A product's tile: rm rows per accumulator, mt accumulators and bn columns
-// per CTA or pair, k split over a cluster.
-struct Tile {
-  int rm = 128, bn = 0, split = 1, chunk_kb = 0;
-  size_t ring = kLinRing;
+// Clusters of 1, 2, 4 and 8 single CTAs that the device holds at once, one and
+// two CTAs per SM (clusters do not straddle its SM groups, so that four or
+// eight CTAs leave SMs over).
+struct Room {
+  int clusters[2][4] = {};
 };
 
-template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE>
-int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProps& props, cudaStream_t st) {
-  dev::GemmArgs g;
-  g.M = static_cast<int>(p.M);
-  g.N = static_cast<long long>(p.N);
-  g.nkb = static_cast<int>((p.K + 63) / 64);
-  g.pa = p.a.planes;
-  g.pb = p.b.planes;
-  g.rm = tile.rm;
-  g.bn = tile.bn;
-  g.split = tile.split;
-  g.chunk_kb = PROMOTE ? tile.chunk_kb : g.nkb;
-  g.swiglu_limit = p.swiglu_limit;
-  g.epi = p.epi;
-  OBJB_TRY(device_error_word(device, &g.err));
-  const size_t mt = static_cast<size_t>(GATED ? 64 : MT * tile.rm) * CG;
-  g.tiles_m = static_cast<int>((p.M + mt - 1) / mt);
-  g.tiles_n = static_cast<int>((p.N + tile.bn - 1) / tile.bn);
-  const size_t stage = static_cast<size_t>(g.pa) * MT * dev::kLinABlock + static_cast<size_t>(g.pb) * (tile.bn / CG) * 128;
-  g.nstages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(dev::kLinStagesMax, tile.ring / stage)));
-  size_t smem = g.nstages * stage;
-  if (GATED || tile.split > 1) smem = std::max(smem, static_cast<size_t>(MT) * BN * 512);  // the partial tile
-  smem += 1024;
-  const uint32_t half = p.a.dtype == OBJB_DTYPE_F16 ? 0 : 1;
-  g.idesc = (1u << 4) | (half << 7) | (half << 10) | (static_cast<uint32_t>(MAJ != dev::kMajKK) << 15) |
-            (static_cast<uint32_t>(MAJ == dev::kMajMN) << 16) | (static_cast<uint32_t>(tile.bn >> 3) << 17) |
-            (static_cast<uint32_t>(128 * CG >> 4) << 24);
-  CUtensorMap ma, ma2, mb;
-  OBJB_TRY(encode(&ma, p.a, MAJ == dev::kMajKK && !GATED ? tile.rm : 64));
-  if (GATED)
-    OBJB_TRY(encode(&ma2, p.a2, 64));
-  else
-    ma2 = ma;
-  OBJB_TRY(encode(&mb, p.b, MAJ == dev::kMajMN ? 64 : tile.bn / CG));
-  auto kernel = dev::lin_gemm_kernel<MAJ, BN, CG, MT, GATED, PROMOTE>;
-  OBJB_TRY(ensure_smem_attr(kernel, device, smem));
-  const long long tiles = static_cast<long long>(g.tiles_m) * g.tiles_n;
-  const int csize = CG == 2 ? 2 : tile.split;
-  const bool one_each = GATED || tile.split > 1;
-  const long long clusters = one_each ? tiles : std::min<long long>(tiles, props.sm_count / csize);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(clusters * csize));
-  cfg.blockDim = dim3(dev::lin_threads(PROMOTE));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = csize;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = csize > 1 ? 2 : 1;
-  OBJB_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, ma2, mb, g), "launch dense product");
-  return OBJB_OK;
+// Nanoseconds that a product takes, about, from rates measured on B200: a
+// producer iteration (wait, expected bytes) 145 and a copy 35; an MMA of 16 of
+// k 20 or bn / 2 clocks, a stage's wait and commit 150; 131 bytes taken in per
+// SM from L2; 1000 (direct: 1500) to drain a tile; launch, set-up and exit
+// 3000, a fold over a cluster 2200.
+double nanoseconds(const Product& p, TileKind kind, const Tile& t, size_t sms, const Room& room) {
+  const size_t cg = kind == kSingle ? 1 : 2, mt = kind == kDirect ? 2 : 1;
+  const bool two = t.ring < kLinRing;
+  const size_t rows = p.gated ? 64 : mt * t.rm;
+  const double tiles = static_cast<double>(ceil_div(p.M, rows * cg)) * ceil_div(p.N, t.bn);
+  const int log_split = t.split == 1 ? 0 : t.split == 2 ? 1 : t.split == 4 ? 2 : 3;
+  const double width = kind == kSingle ? room.clusters[two][log_split] : sms / 2;
+  const double share = two ? std::min(2.0, std::max(1.0, tiles * t.split / sms)) : 1.0;  // CTAs at work per SM
+  // clocks of a k-step's MMAs: side by side (N 3 bn, 2 bn, bn), or one per pair of planes
+  const int pa = p.a.planes, pb = p.b.planes;
+  auto one = [](double n) { return std::max(39.0, n / 2); };
+  double clocks = mt * one(t.bn);
+  if (pb > 1 && kind == kSingle)
+    clocks = one(3.0 * t.bn) + (pa > 1 ? one(2.0 * t.bn) : 0.0) + (pa > 2 ? one(t.bn) : 0.0);
+  else if (pb > 1)
+    clocks = (pa == 1 ? 3 : pa == 2 ? 5 : 6) * one(t.bn);
+  const double mma = 4.0 * clocks / 1.7;
+  const double copies = mt * (p.maj == dev::kMajKK && !p.gated ? 1 : 2) +
+                        (p.maj == dev::kMajMN ? ceil_div(t.bn / cg, 64) : 1);
+  const double bytes = 128.0 * (p.a.planes * (p.gated ? 128 : mt * t.rm) + p.b.planes * t.bn / cg);
+  const double kb = std::max(std::max(145.0 / t.unit + 35.0 * copies, std::max(mma * share, 150.0 / t.unit + mma / 2)),
+                             bytes / (kind == kSingle ? 125.0 : 90.0) * share);
+  const double kbs = std::ceil(static_cast<double>(ceil_div(p.K, 64)) / t.split);
+  return std::ceil(tiles / width) * (kbs * kb + (kind == kDirect ? 1500.0 : 1000.0)) + 3000.0 +
+         (t.split > 1 ? 2200.0 : 0.0);
 }
 
-size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
-
-// Columns of a pair's tile, 256 or fewer: the count (a multiple of 16) whose
-// rounds of the grid take the fewest columns in all.
-int pair_columns(size_t tiles_m, size_t N, int most, int step, int pairs) {
-  int best = most;
-  size_t cost = ~size_t{0};
-  for (int bn = most; bn >= most / 2; bn -= step) {
-    const size_t c = ceil_div(tiles_m * ceil_div(N, bn), pairs) * bn;
-    if (c < cost) cost = c, best = bn;
-  }
+// Which tile a product takes: the one of the fewest nanoseconds() among
+//   * direct: pairs, 512 x up to 256 columns, for 16-bit results of one-plane operands;
+//   * pairs of 256 rows x up to 128 columns;
+//   * single CTAs of 128 rows x up to 128 columns, k split over a cluster, one
+//     per SM or (up to 64 columns) two.
+// Rows below 128 (K-major A) and columns below the most even out the rounds;
+// stages of several k-blocks save the producer's and the MMA warp's turns.
+Choice choose_tile(const Product& p, bool y16, size_t sms, const Room& room) {
+  const size_t nkb = ceil_div(p.K, 64);
+  const bool mn = p.maj == dev::kMajMN, rows_free = p.maj == dev::kMajKK && !p.gated;
+  Choice best;
+  double least = 1e300;
+  auto consider = [&](TileKind k, const Tile& c) {
+    const double v = nanoseconds(p, k, c, sms, room);
+    if (v < least) {
+      least = v;
+      best.kind = k;
+      best.tile = c;
+    }
+  };
+  // columns: what N needs, rounded to a step of the layout, at most `most` and then down to `least_bn`
+  auto each_bn = [&](int most, int step, int least_bn, auto f) {
+    const int need = static_cast<int>(std::min<size_t>(most, ceil_div(p.N, step) * step));
+    for (int bn = need; bn >= std::min(need, least_bn); bn -= step) f(bn);
+  };
+  // rows, and units whose stages leave the ring at least three
+  auto each_row_unit = [&](TileKind k, Tile c, int cg) {
+    for (c.rm = 128; c.rm >= (rows_free ? 64 : 128); c.rm -= 8)
+      for (c.unit = 1; c.unit <= 4; c.unit *= 2)
+        if (c.unit == 1 || c.unit * 128u * (p.a.planes * 128 + p.b.planes * c.bn / cg) * 3 <= c.ring) consider(k, c);
+  };
+  Tile c;
+  if (y16 && p.a.planes == 1 && p.b.planes == 1)
+    each_bn(256, mn ? 128 : 16, 144, [&](int bn) {
+      c.bn = bn;
+      consider(kDirect, c);
+    });
+  each_bn(128, mn ? 128 : 16, 80, [&](int bn) {
+    c.bn = bn;
+    each_row_unit(kPair, c, 2);
+  });
+  each_bn(single_columns(p.maj, p.b.planes), mn ? 64 : 16, 16, [&](int bn) {
+    c.bn = bn;
+    for (c.split = 1; c.split <= 8 && nkb >= static_cast<size_t>(c.split); c.split *= 2)
+      for (size_t ring : {kLinRing, kLinRingTwo}) {
+        if (ring == kLinRingTwo && bn > two_columns(p.maj, p.b.planes)) continue;
+        c.ring = ring;
+        each_row_unit(kSingle, c, 1);
+      }
+  });
   return best;
 }
 
-// Which tile a product takes.  CTA pairs where their tiles fill most of the
-// SMs: 512 x 256 straight from tensor memory for a 16-bit result of one-plane
-// operands, else 256 x 128 with promoted accumulators.  Otherwise single CTAs
-// of 128 rows by N up to 128, a tile's k split over a cluster while that
-// leaves SMs free.
+int room_of(int device, size_t sms, Room* out) {
+  static std::mutex mu;
+  static std::map<int, Room> rooms;
+  std::lock_guard<std::mutex> lk(mu);
+  auto it = rooms.find(device);
+  if (it == rooms.end()) {
+    auto kernel = dev::lin_gemm_kernel<dev::kMajKK, 32, 1, 1, false, true, 1>;
+    Room r;
+    for (int two = 0; two < 2; ++two) {
+      const size_t smem = (two ? kLinRingTwo : kLinRing) + 1024;
+      OBJB_TRY(ensure_smem_attr(kernel, device, smem));
+      for (int i = 0; i < 4; ++i) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(8 * sms));
+        cfg.blockDim = dim3(dev::lin_threads(true));
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 1u << i;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        OBJB_CUDA(cudaOccupancyMaxActiveClusters(&r.clusters[two][i], kernel, &cfg), "query clusters per device");
+        r.clusters[two][i] = std::max(1, r.clusters[two][i]);
+      }
+    }
+    it = rooms.emplace(device, r).first;
+  }
+  *out = it->second;
+  return OBJB_OK;
+}
+
+// The choice is a function of these alone; trying all tiles takes the host
+// several microseconds, so each thread keeps its last choices.
+struct ChoiceKey {
+  size_t M, N, K, sms;  // (devices of one process with as many SMs are alike)
+  int maj, pa, pb, flags;
+  bool operator==(const ChoiceKey& o) const {
+    return M == o.M && N == o.N && K == o.K && sms == o.sms && maj == o.maj && pa == o.pa && pb == o.pb &&
+           flags == o.flags;
+  }
+};
+
 int gemm(const Product& p, int device, const DeviceProps& props, cudaStream_t st) {
-  const size_t sms = static_cast<size_t>(props.sm_count);
-  const int pairs = props.sm_count / 2;
-  const size_t nkb = ceil_div(p.K, 64);
   const bool y16 = !p.gated && p.epi.y_dtype != OBJB_DTYPE_F32;
-  const bool plain = p.a.planes == 1 && p.b.planes == 1;
-  Tile t;
-#define OBJB_GEMM(MAJ, BN, CG, MT, GATED, PROMOTE) return launch_gemm<MAJ, BN, CG, MT, GATED, PROMOTE>(p, t, device, props, st)
-  if (y16 && plain && ceil_div(p.M, 512) * ceil_div(p.N, 256) * 4 >= sms) {
-    t.bn = pair_columns(ceil_div(p.M, 512), p.N, 256, p.maj == dev::kMajMN ? 128 : 16, pairs);
-    switch (p.maj) {
-      case dev::kMajKK: OBJB_GEMM(dev::kMajKK, 256, 2, 2, false, false);
-      case dev::kMajMK: OBJB_GEMM(dev::kMajMK, 256, 2, 2, false, false);
-      default: OBJB_GEMM(dev::kMajMN, 256, 2, 2, false, false);
-    }
+  const ChoiceKey key{p.M, p.N, p.K, static_cast<size_t>(props.sm_count), p.maj, p.a.planes, p.b.planes,
+                      (y16 ? 1 : 0) | (p.gated ? 2 : 0)};
+  struct Kept {
+    ChoiceKey key{};
+    Choice choice;
+  };
+  thread_local Kept kept[64];
+  Kept& k = kept[(p.M * 31 + p.N * 7 + p.K * 3 + static_cast<size_t>(p.maj)) % 64];
+  if (!(k.key == key)) {
+    Room room;
+    OBJB_TRY(room_of(device, key.sms, &room));
+    k.choice = choose_tile(p, y16, key.sms, room);
+    k.key = key;
   }
+  const TileKind kind = k.choice.kind;
+  Tile t = k.choice.tile;
   t.chunk_kb = y16 ? 16 : 4;
-  const size_t pair_m = ceil_div(p.M, p.gated ? 128 : 256);
-  if (pair_m * ceil_div(p.N, 128) * 4 >= sms) {
-    t.bn = p.maj == dev::kMajMN ? 128 : pair_columns(pair_m, p.N, 128, 16, pairs);
-    if (p.gated) OBJB_GEMM(dev::kMajKK, 128, 2, 1, true, true);
-    switch (p.maj) {
-      case dev::kMajKK: OBJB_GEMM(dev::kMajKK, 128, 2, 1, false, true);
-      case dev::kMajMK: OBJB_GEMM(dev::kMajMK, 128, 2, 1, false, true);
-      default: OBJB_GEMM(dev::kMajMN, 128, 2, 1, false, true);
-    }
-  }
-  int bn = p.maj == dev::kMajMN ? 64 : 16;
-  while (bn < 128 && static_cast<size_t>(bn) < p.N) bn *= 2;
-  t.bn = p.maj == dev::kMajMN ? bn : static_cast<int>(std::min<size_t>(bn, ceil_div(p.N, 16) * 16));
-  const size_t tiles = ceil_div(p.M, p.gated ? 64 : 128) * ceil_div(p.N, t.bn);
-  while (t.split < 8 && tiles * t.split * 2 <= sms && nkb >= static_cast<size_t>(t.split) * 8 && bn / (t.split * 2) >= 2)
-    t.split *= 2;
-  if (p.gated) {
-    switch (bn) {
-      case 16: OBJB_GEMM(dev::kMajKK, 16, 1, 1, true, true);
-      case 32: OBJB_GEMM(dev::kMajKK, 32, 1, 1, true, true);
-      case 64: OBJB_GEMM(dev::kMajKK, 64, 1, 1, true, true);
-      default: OBJB_GEMM(dev::kMajKK, 128, 1, 1, true, true);
-    }
-  }
   switch (p.maj) {
-    case dev::kMajKK:
-      switch (bn) {
-        case 16: OBJB_GEMM(dev::kMajKK, 16, 1, 1, false, true);
-        case 32: OBJB_GEMM(dev::kMajKK, 32, 1, 1, false, true);
-        case 64: OBJB_GEMM(dev::kMajKK, 64, 1, 1, false, true);
-        default: OBJB_GEMM(dev::kMajKK, 128, 1, 1, false, true);
-      }
-    case dev::kMajMK:
-      switch (bn) {
-        case 16: OBJB_GEMM(dev::kMajMK, 16, 1, 1, false, true);
-        case 32: OBJB_GEMM(dev::kMajMK, 32, 1, 1, false, true);
-        case 64: OBJB_GEMM(dev::kMajMK, 64, 1, 1, false, true);
-        default: OBJB_GEMM(dev::kMajMK, 128, 1, 1, false, true);
-      }
-    default:
-      if (bn == 64) OBJB_GEMM(dev::kMajMN, 64, 1, 1, false, true);
-      OBJB_GEMM(dev::kMajMN, 128, 1, 1, false, true);
+    case dev::kMajKK: return launch_kk(p, kind, t, device, props, st);
+    case dev::kMajMK: return launch_mk(p, kind, t, device, props, st);
+    default: return launch_mn(p, kind, t, device, props, st);
   }
-#undef OBJB_GEMM
 }
 
 int device_here(int* device, DeviceProps* props) {
@@ -411,6 +536,8 @@ int check_types(const char* action, int x, int w, int y, const char* y_name) {
 
 int check_stride(const char* action, const char* name, size_t stride, size_t cols, size_t* out) {
   *out = stride ? stride : cols;
+  if (*out > kMaxStride)
+    return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, std::string(name) + " is above 2^28 elements");
   if (*out < cols)
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, std::string(name) + " is below the row's " + std::to_string(cols) +
                                                          " elements");
@@ -565,8 +692,10 @@ int objb_linear_device(const objb_linear_desc* desc, const void* d_x, const void
   uint8_t* ws = nullptr;
   OBJB_TRY(take_scratch(action, d_scratch, scratch_bytes, pl.total, st, &ws));
   Product p;
-  OBJB_TRY(make_image(pl.w, d_w, d.w_dtype, ldw, d.out_features, d.in_features, ws, props, st, &p.a));
-  OBJB_TRY(make_image(pl.x, d_x, d.x_dtype, ldx, d.tokens, d.in_features, ws + pl.w.bytes, props, st, &p.b));
+  Images images;
+  p.a = images.take(pl.w, d_w, d.w_dtype, ldw, d.out_features, d.in_features, ws);
+  p.b = images.take(pl.x, d_x, d.x_dtype, ldx, d.tokens, d.in_features, ws + pl.w.bytes);
+  OBJB_TRY(images.launch(props, st));
   p.M = d.out_features;
   p.N = d.tokens;
   p.K = d.in_features;
@@ -574,11 +703,11 @@ int objb_linear_device(const objb_linear_desc* desc, const void* d_x, const void
   e.bias = d_bias;
   e.bias_dtype = d.bias_dtype;
   e.residual = d_residual;
-  e.ldr = ldr;
+  e.ldr = static_cast<uint32_t>(ldr);
   e.y = d_y;
-  e.ldy = ldy;
+  e.ldy = static_cast<uint32_t>(ldy);
   e.z = d_z;
-  e.ldz = ldz;
+  e.ldz = static_cast<uint32_t>(ldz);
   e.y_dtype = d.y_dtype;
   e.act = d.activation;
   return gemm(p, device, props, st);
@@ -651,53 +780,61 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
   dz.dtype = pl.dz.planes > 1 ? OBJB_DTYPE_BF16 : d.dy_dtype;
   const bool image = products && !pl.dz_direct;
   if (image || want_db) {
-    const bool vec = aligned16(d_dy) && lddy % 8 == 0 && (!pl.has_act || (aligned16(d_z) && ldz % 8 == 0));
-    const dim3 grid((N + 255) / 256, pl.parts);
-    auto k = vec ? dev::dz_kernel<true> : dev::dz_kernel<false>;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    const bool vec = aligned16(d_dy) && lddy % 8 == 0 && N % 8 == 0 && (!pl.has_act || (aligned16(d_z) && ldz % 8 == 0));
     float* part = want_db ? reinterpret_cast<float*>(ws_part) : nullptr;
-    OBJB_CUDA(cudaLaunchKernelEx(&cfg, k, d_dy, lddy, d_z, ldz, static_cast<int>(d.dy_dtype),
-                                 static_cast<int>(d.activation), static_cast<long long>(d.tokens), N,
-                                 image ? reinterpret_cast<uint16_t*>(ws_dz) : nullptr, static_cast<int>(pl.dz.pitch),
-                                 pl.dz.planes, pl.rows_per, part),
-              "launch dz");
+    OBJB_TRY(dev::with_elements(d.dy_dtype, vec, [&](auto elem, auto v) -> int {
+      using T = decltype(elem);
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((N + 255) / 256, pl.parts);
+      cfg.blockDim = dim3(256);
+      cfg.stream = st;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[0].val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      OBJB_CUDA(cudaLaunchKernelEx(&cfg, dev::dz_kernel<T, decltype(v)::value>, static_cast<const T*>(d_dy), lddy,
+                                   static_cast<const T*>(d_z), ldz, static_cast<int>(d.dy_dtype),
+                                   static_cast<int>(d.activation), static_cast<long long>(d.tokens), N,
+                                   image ? reinterpret_cast<uint16_t*>(ws_dz) : nullptr,
+                                   static_cast<int>(pl.dz.pitch), pl.dz.planes, pl.rows_per, part),
+                "launch dz");
+      return OBJB_OK;
+    }));
     if (want_db)
-      OBJB_TRY(launch_pdl(dev::dbias_kernel, (N + 255) / 256, 256, 0, st, static_cast<const float*>(part), pl.parts, N,
+      OBJB_TRY(launch_pdl(dev::dbias_kernel, (N + 31) / 32, 1024, 0, st, static_cast<const float*>(part), pl.parts, N,
                           d_dbias, static_cast<int>(d.accumulate)));
   }
+  Images images;
+  Image w, x;
+  if (want_dx) w = images.take(pl.w, d_w, d.w_dtype, ldw, d.out_features, d.in_features, ws_w);
+  if (want_dw) x = images.take(pl.x, d_x, d.x_dtype, ldx, d.tokens, d.in_features, ws_x);
+  OBJB_TRY(images.launch(props, st));
   if (want_dx) {
     Product p;
     p.maj = dev::kMajMK;
-    OBJB_TRY(make_image(pl.w, d_w, d.w_dtype, ldw, d.out_features, d.in_features, ws_w, props, st, &p.a));
+    p.a = w;
     p.b = dz;
     p.M = d.in_features;
     p.N = d.tokens;
     p.K = d.out_features;
     p.epi.y = d_dx;
-    p.epi.ldy = lddx;
+    p.epi.ldy = static_cast<uint32_t>(lddx);
     p.epi.y_dtype = d.x_dtype;
     OBJB_TRY(gemm(p, device, props, st));
   }
   if (want_dw) {
     Product p;
     p.maj = dev::kMajMN;
-    OBJB_TRY(make_image(pl.x, d_x, d.x_dtype, ldx, d.tokens, d.in_features, ws_x, props, st, &p.a));
+    p.a = x;
     p.b = dz;
     p.M = d.in_features;
     p.N = d.out_features;
     p.K = d.tokens;
     p.epi.y = d_dw;
-    p.epi.ldy = lddw;
+    p.epi.ldy = static_cast<uint32_t>(lddw);
     p.epi.y_dtype = d.dw_dtype;
-    if (d.accumulate) p.epi.residual = d_dw, p.epi.ldr = lddw;
+    if (d.accumulate) p.epi.residual = d_dw, p.epi.ldr = static_cast<uint32_t>(lddw);
     OBJB_TRY(gemm(p, device, props, st));
   }
   return OBJB_OK;
@@ -738,21 +875,24 @@ int objb_ffn_bf16_tokens_device(const void* d_gate, const void* d_up, const void
   const int bf = OBJB_DTYPE_BF16;
   Product gu;
   gu.gated = true;
-  OBJB_TRY(make_image(pl.gate, d_gate, bf, hidden, intermediate, hidden, ws, props, st, &gu.a));
+  Images images;
+  gu.a = images.take(pl.gate, d_gate, bf, hidden, intermediate, hidden, ws);
   ws += pl.gate.bytes;
-  OBJB_TRY(make_image(pl.up, d_up, bf, hidden, intermediate, hidden, ws, props, st, &gu.a2));
+  gu.a2 = images.take(pl.up, d_up, bf, hidden, intermediate, hidden, ws);
   ws += pl.up.bytes;
+  OBJB_TRY(images.launch(props, st));
   Product dn;
-  OBJB_TRY(make_image(pl.down, d_down, bf, intermediate, out_dim, intermediate, ws, props, st, &dn.a));
+  dn.a = images.take(pl.down, d_down, bf, intermediate, out_dim, intermediate, ws);
   ws += pl.down.bytes;
-  OBJB_TRY(make_image(pl.x, d_x, OBJB_DTYPE_F32, hidden, num_tokens, hidden, ws, props, st, &gu.b));
+  gu.b = images.take(pl.x, d_x, OBJB_DTYPE_F32, hidden, num_tokens, hidden, ws);
   ws += pl.x.bytes;
+  OBJB_TRY(images.launch(props, st));
   gu.M = intermediate;
   gu.N = num_tokens;
   gu.K = hidden;
   gu.swiglu_limit = swiglu_limit;
   gu.epi.y = ws;  // the activations, as the planes that the down product reads
-  gu.epi.ldy = pl.act.pitch;
+  gu.epi.ldy = static_cast<uint32_t>(pl.act.pitch);
   gu.epi.plane = num_tokens * pl.act.pitch;
   OBJB_TRY(gemm(gu, device, props, st));
   dn.b.p = ws;
@@ -765,9 +905,9 @@ int objb_ffn_bf16_tokens_device(const void* d_gate, const void* d_up, const void
   dn.N = num_tokens;
   dn.K = intermediate;
   dn.epi.y = d_out;
-  dn.epi.ldy = out_dim;
+  dn.epi.ldy = static_cast<uint32_t>(out_dim);
   dn.epi.residual = d_residual;
-  dn.epi.ldr = out_dim;
+  dn.epi.ldr = static_cast<uint32_t>(out_dim);
   dn.epi.y_dtype = OBJB_DTYPE_F32;
   return gemm(dn, device, props, st);
 }

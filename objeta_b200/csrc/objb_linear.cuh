@@ -31,19 +31,28 @@ constexpr float kSqrt2OverPi = 0.79788456080286536f;
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 
-// 1 / (1 + exp(-v)) without overflow on either side.
-__device__ __forceinline__ float sigmoid(float v) {
-  const float t = expf(-fabsf(v));
-  const float r = 1.0f / (1.0f + t);
-  return v >= 0.0f ? r : t * r;
+// exp2 and 1 / v by the special-function unit (2 ulp and 1 ulp).
+__device__ __forceinline__ float ex2_sfu(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
+__device__ __forceinline__ float rcp_sfu(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// 1 / (1 + exp(-v)): five instructions, since a tile's epilogue is not hidden
+// behind its MMAs (the IEEE division alone takes twenty).  Overflow of the
+// exponential gives the right 0.
+__device__ __forceinline__ float sigmoid(float v) { return rcp_sfu(1.0f + ex2_sfu(v * -1.4426950408889634f)); }
 
 __device__ __forceinline__ float act_value(int act, float v) {
   switch (act) {
     case OBJB_ACT_RELU: return v > 0.0f ? v : (v == v ? 0.0f : v);
     case OBJB_ACT_SILU: return v * sigmoid(v);
     case OBJB_ACT_GELU: return 0.5f * v * erfcf(-v * kSqrtHalf);  // exact tails
-    case OBJB_ACT_GELU_TANH: return v * sigmoid(2.0f * kSqrt2OverPi * (v + 0.044715f * v * v * v));
+    case OBJB_ACT_GELU_TANH: return v * sigmoid(v * fmaf(v * v, 2.0f * kSqrt2OverPi * 0.044715f, 2.0f * kSqrt2OverPi));
     default: return v;
   }
 }
@@ -54,12 +63,15 @@ __device__ __forceinline__ float act_grad(int act, float v) {
     case OBJB_ACT_RELU: return v > 0.0f ? 1.0f : 0.0f;
     case OBJB_ACT_SILU: {
       const float s = sigmoid(v);
-      return s * (1.0f + v * (1.0f - s));
+      return s * fmaf(v, 1.0f - s, 1.0f);
     }
-    case OBJB_ACT_GELU: return 0.5f * erfcf(-v * kSqrtHalf) + v * kInvSqrt2Pi * expf(-0.5f * v * v);
+    case OBJB_ACT_GELU:
+      return 0.5f * erfcf(-v * kSqrtHalf) + v * kInvSqrt2Pi * ex2_sfu(v * v * (-0.5f * 1.4426950408889634f));
     case OBJB_ACT_GELU_TANH: {
-      const float s = sigmoid(2.0f * kSqrt2OverPi * (v + 0.044715f * v * v * v));
-      return s + 2.0f * v * s * (1.0f - s) * kSqrt2OverPi * (1.0f + 3.0f * 0.044715f * v * v);
+      const float q = v * v;
+      const float s = sigmoid(v * fmaf(q, 2.0f * kSqrt2OverPi * 0.044715f, 2.0f * kSqrt2OverPi));
+      const float d = v * (1.0f - s) * fmaf(q, 6.0f * kSqrt2OverPi * 0.044715f, 2.0f * kSqrt2OverPi);
+      return fmaf(s, d, s);
     }
     default: return 1.0f;
   }
@@ -85,56 +97,44 @@ struct LinearEpilogue {
   const void* residual = nullptr;
   void* y = nullptr;
   void* z = nullptr;
-  size_t ldr = 0, ldy = 0, ldz = 0;
+  uint32_t ldr = 0, ldy = 0, ldz = 0;
   size_t plane = 0;  // put_planes: elements between y's planes
   int bias_dtype = 0, y_dtype = 0, act = 0;
 
-  template <class T, int C>
-  __device__ __forceinline__ void store(T* p, size_t ld, int m, long long n, long long N, const float (&v)[C]) const {
-    p += static_cast<size_t>(n) * ld + m;
+  __device__ __forceinline__ float bias_of(int m) const { return bias ? load_elem(bias, bias_dtype, m) : 0.0f; }
+
+  // FULL: all C columns exist.
+  template <class T, int C, bool FULL>
+  __device__ __forceinline__ static void store(T* p, uint32_t ld, int m, long long n, int left, const float (&v)[C]) {
+    char* at = reinterpret_cast<char*>(p + n * ld + m);
+    const uint32_t pitch = ld * static_cast<uint32_t>(sizeof(T));
 #pragma unroll
     for (int i = 0; i < C; ++i)
-      if (n + i < N) {
+      if (FULL || i < left) {
+        T* q = reinterpret_cast<T*>(at + static_cast<uint64_t>(pitch) * i);
         if constexpr (sizeof(T) == 4)
-          p[i * ld] = v[i];
+          *q = v[i];
         else if constexpr (std::is_same<T, __half>::value)
-          p[i * ld] = __float2half_rn(v[i]);
+          *q = __float2half_rn(v[i]);
         else
-          p[i * ld] = __float2bfloat16_rn(v[i]);
+          *q = __float2bfloat16_rn(v[i]);
       }
   }
-  template <class T, int C>
-  __device__ __forceinline__ void add(const T* p, size_t ld, int m, long long n, long long N, float (&v)[C]) const {
-    p += static_cast<size_t>(n) * ld + m;
+  template <class T, int C, bool FULL>
+  __device__ __forceinline__ static void add(const T* p, uint32_t ld, int m, long long n, int left, float (&v)[C]) {
+    const char* at = reinterpret_cast<const char*>(p + n * ld + m);
+    const uint32_t pitch = ld * static_cast<uint32_t>(sizeof(T));
     T r[C];
 #pragma unroll
     for (int i = 0; i < C; ++i)
-      if (n + i < N) r[i] = p[i * ld];
+      if (FULL || i < left) r[i] = *reinterpret_cast<const T*>(at + static_cast<uint64_t>(pitch) * i);
 #pragma unroll
     for (int i = 0; i < C; ++i)
-      if (n + i < N) v[i] += static_cast<float>(r[i]);
+      if (FULL || i < left) v[i] += static_cast<float>(r[i]);
   }
-  template <int C>
-  __device__ __forceinline__ void store_any(void* p, size_t ld, int m, long long n, long long N,
-                                            const float (&v)[C]) const {
-    if (y_dtype == OBJB_DTYPE_F32)
-      store(static_cast<float*>(p), ld, m, n, N, v);
-    else if (y_dtype == OBJB_DTYPE_BF16)
-      store(static_cast<__nv_bfloat16*>(p), ld, m, n, N, v);
-    else
-      store(static_cast<__half*>(p), ld, m, n, N, v);
-  }
-
-  // C neighbouring n of one m (those below N).
-  template <int C>
-  __device__ __forceinline__ void put_columns(int m, long long n, long long N, float (&v)[C]) const {
-    if (n >= N) return;
-    if (bias) {
-      const float b = load_elem(bias, bias_dtype, m);
-#pragma unroll
-      for (int i = 0; i < C; ++i) v[i] += b;
-    }
-    if (z) store_any(z, ldz, m, n, N, v);
+  template <class T, int C, bool FULL>
+  __device__ __forceinline__ void put_typed(int m, long long n, int left, float (&v)[C]) const {
+    if (z) store<T, C, FULL>(static_cast<T*>(z), ldz, m, n, left, v);
     switch (act) {
 #define OBJB_ACT_CASE(A)                                          \
   case A:                                                         \
@@ -147,15 +147,30 @@ struct LinearEpilogue {
 #undef OBJB_ACT_CASE
       default: break;
     }
-    if (residual) {
-      if (y_dtype == OBJB_DTYPE_F32)
-        add(static_cast<const float*>(residual), ldr, m, n, N, v);
-      else if (y_dtype == OBJB_DTYPE_BF16)
-        add(static_cast<const __nv_bfloat16*>(residual), ldr, m, n, N, v);
-      else
-        add(static_cast<const __half*>(residual), ldr, m, n, N, v);
-    }
-    store_any(y, ldy, m, n, N, v);
+    if (residual) add<T, C, FULL>(static_cast<const T*>(residual), ldr, m, n, left, v);
+    store<T, C, FULL>(static_cast<T*>(y), ldy, m, n, left, v);
+  }
+  template <class T, int C>
+  __device__ __forceinline__ void put_left(int m, long long n, int left, float (&v)[C]) const {
+    if (left >= C)
+      put_typed<T, C, true>(m, n, left, v);
+    else
+      put_typed<T, C, false>(m, n, left, v);
+  }
+
+  // C neighbouring n of one m, those below n_end; b = bias_of(m).
+  template <int C>
+  __device__ __forceinline__ void put_columns(int m, long long n, long long n_end, float b, float (&v)[C]) const {
+    if (n >= n_end) return;
+    const int left = n_end - n < C ? static_cast<int>(n_end - n) : C;
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] += b;
+    if (y_dtype == OBJB_DTYPE_F32)
+      put_left<float>(m, n, left, v);
+    else if (y_dtype == OBJB_DTYPE_BF16)
+      put_left<__nv_bfloat16>(m, n, left, v);
+    else
+      put_left<__half>(m, n, left, v);
   }
 
   // One f32 value as the three planes of the next product's operand.

@@ -9,14 +9,24 @@
 // tensor-memory lane is a row m and a warp's 32 lanes store 32 neighbouring
 // elements of D's row n: no transposition on the way out.
 //
-// One warp issues TMA copies into a ring of 128-byte-swizzled stages (64 of k,
-// all planes), one warp the MMAs, the others the epilogue.  Accumulators:
+// One warp issues TMA copies into a ring of 128-byte-swizzled stages (`unit`
+// k-blocks of 64, all planes), one warp the MMAs, the others the epilogue.
+// A turn of the producer costs about 145 ns and a copy 35 more, a turn of the
+// MMA warp 150, whatever the tile: small tiles take several k-blocks per stage
+// (16.4 -> 11.6 us for one token by 4096 x 4096 in 64 CTAs).  Accumulators:
 //   * PROMOTE.  The tensor core adds into its f32 accumulators with
 //     truncation, so their error grows with the number of MMAs in one
 //     accumulator; the epilogue warps therefore take the accumulators into
 //     registers every chunk_kb k-blocks (two buffers) and add there, rounded
-//     to nearest.  The planes' cross products are below 2^-8 of the main one
-//     and stay in a buffer of their own.
+//     to nearest.  Products of planes i and j are 2^-8 (i + j) of the main one;
+//     those of i + j > 2 are below f32 and left out.
+//     CG 1, planes side by side: B's planes lie behind one another, so one MMA
+//     of N = 3 bn takes a plane of A against all of them, plane 1 against two
+//     of them into columns bn.. (the products of i + j = 1 and 2), plane 2
+//     against one into columns 2 bn..; an MMA takes 39 clocks or more, so a
+//     third (half) of the MMAs is what counts up to bn 64.
+//     CG 2: one MMA per pair of planes, the cross products into a buffer of
+//     their own that is read once per tile; twice the columns per tile.
 //   * else straight from tensor memory into the epilogue, which rounds to 16
 //     bits: two accumulators of 256 columns, all of tensor memory.  The ring
 //     goes on filling while a tile is drained.
@@ -49,7 +59,6 @@ constexpr int kLinBK = 64;        // k of a stage: 128 bytes, one swizzle row
 constexpr int kLinStagesMax = 12;
 // producer, MMA and eight (PROMOTE) or sixteen epilogue warps
 constexpr int lin_threads(bool promote) { return promote ? 320 : 576; }
-constexpr int kLinABlock = 128 * 128;  // bytes of 128 rows of A in a stage
 
 struct GemmArgs {
   int M;                  // rows of A (GATED: features)
@@ -58,23 +67,23 @@ struct GemmArgs {
   int tiles_m, tiles_n;
   int rm;                 // rows of an accumulator in use (128, or fewer to even out the rounds of the grid)
   int bn;                 // columns of a tile in use (at most BN)
-  int pa, pb;             // planes
+  int pa;                 // planes of A
   int split;              // CTAs of a cluster per tile (CG 1)
-  int chunk_kb;           // k-blocks per accumulator chunk
-  int nstages;
+  int chunk_kb;           // k-blocks per accumulator chunk, a multiple of unit
+  int nstages, unit;      // stages of `unit` k-blocks
   uint32_t idesc;
   float swiglu_limit;
   unsigned* err;
   LinearEpilogue epi;
 };
 
-// SWIZZLE_128B operand tiles.  K-major: rows of 128 bytes, 8-row groups 1024
-// bytes apart.  MN-major: 64 rows x 64 k as 64 k rows of 128 bytes; 8-k groups
-// 1024 bytes apart (stride offset), the next 64 rows 8192 bytes (leading).
+// SWIZZLE_128B operand tiles, without their address.  K-major: rows of 128
+// bytes, 8-row groups 1024 bytes apart.  MN-major: 64 rows x 64 k as 64 k rows
+// of 128 bytes; 8-k groups 1024 bytes apart (stride offset), the next 64 rows
+// behind this chunk's planes (leading offset).
 template <bool MN>
-__device__ __forceinline__ uint64_t lin_desc(uint32_t saddr) {
-  uint64_t d = static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>((MN ? 8192 : 16) >> 4) << 16;
+__device__ __forceinline__ uint64_t lin_desc(int planes) {
+  uint64_t d = static_cast<uint64_t>((MN ? 8192 * planes : 16) >> 4) << 16;
   d |= static_cast<uint64_t>(1024 >> 4) << 32;
   d |= static_cast<uint64_t>(1) << 46;
   d |= static_cast<uint64_t>(2) << 61;
@@ -95,7 +104,7 @@ __device__ __forceinline__ void lin_mma(uint32_t d_tmem, uint64_t a, uint64_t b,
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u));
 }
 
-// 3-D tiled load (x along a row, row, plane).  x is a multiple of 64 elements.
+// 3-D tiled load (x along a row, row; the box holds all planes).  x is a multiple of 64 elements.
 // With CG 2 the bytes are counted on the even CTA's barrier.
 template <int CG>
 __device__ __forceinline__ void lin_tma(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -165,21 +174,35 @@ __device__ __forceinline__ void lin_tile(const GemmArgs& g, int t, int* tm, int*
   *tn = b * 8 + r - *tm * width;
 }
 
-template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE>
-__global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
+// BN: columns of a tile at most; PB: planes of B.
+template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE, int PB>
+struct LinShape {
+  static constexpr bool kWideB = CG == 1 && PB > 1;         // planes side by side in N
+  static constexpr int kSet = MT * BN * (kWideB ? PB : 1);  // accumulator columns of one set
+  static constexpr int kUsed = PROMOTE ? (CG == 2 && PB > 1 ? 4 : 2) * kSet : kSet;
+  static constexpr int pow2(int v) { return v <= 32 ? 32 : v <= 64 ? 64 : v <= 128 ? 128 : v <= 256 ? 256 : 512; }
+  static constexpr int kCols = pow2(kUsed);
+  static constexpr int kThreads = lin_threads(PROMOTE);
+  static constexpr int kBlocks = PROMOTE && CG == 1 && BN <= 64 && kCols <= 256 ? 2 : 1;  // CTAs an SM has room for
+  static_assert(kUsed <= 512, "tensor memory columns");
+  static_assert(!GATED || (MAJ == kMajKK && MT == 1 && PROMOTE), "gated products are K-major, one accumulator");
+  static_assert(!(kWideB && MAJ == kMajMN) || BN < 128, "planes side by side of one 64-row chunk");
+  static_assert(PROMOTE ? MT == 1 : CG == 2 && MT == 2 && PB == 1, "one promoted accumulator, or a pair of two direct ones");
+};
+
+template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE, int PB>
+__global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>::kThreads,
+                                  LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>::kBlocks)
     lin_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a2,
                     const __grid_constant__ CUtensorMap map_b, const GemmArgs g) {
+  using SH = LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>;
   constexpr bool A_MN = MAJ != kMajKK, B_MN = MAJ == kMajMN;
-  constexpr int kWarps = PROMOTE ? 8 : 16;       // epilogue warps
-  constexpr int HN = MT * BN * 4 / kWarps;       // accumulator columns of each
-  constexpr int G = HN < 32 ? HN : 32;           // of one tensor-memory load
-  constexpr int P = G < 16 ? G : 16;             // of one step of the epilogue
-  constexpr int kWide = MT * BN;                 // columns of one set of accumulators
-  constexpr uint32_t kUsed = PROMOTE ? 4 * kWide : kWide;  // main x 2, cross products x 2
-  constexpr uint32_t kCols = kUsed < 32 ? 32 : kUsed;
-  static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0, "tensor memory columns");
-  static_assert(!GATED || (MAJ == kMajKK && MT == 1 && PROMOTE), "gated products are K-major, one accumulator");
-  static_assert(PROMOTE || (CG == 2 && MT == 2), "direct products are pairs of two accumulators");
+  constexpr int kWarps = PROMOTE ? 8 : 16;        // epilogue warps
+  constexpr int HN = MT * BN * 4 / kWarps;        // columns of each
+  constexpr int G = HN % 32 == 0 ? 32 : HN % 16 == 0 ? 16 : 8;  // of one tensor-memory load
+  constexpr int P = G < 16 ? G : 16;              // of one step of the epilogue
+  constexpr int kSet = SH::kSet;
+  constexpr uint32_t kCols = SH::kCols;
 
   extern __shared__ uint8_t lin_smem[];
   __shared__ alignas(8) uint64_t full[kLinStagesMax], empty[kLinStagesMax], t_full[2], t_empty[2], c_empty[2];
@@ -219,9 +242,12 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
   const int krank = CG == 1 ? static_cast<int>(rank) : 0;
   const int kb0 = static_cast<int>(static_cast<long long>(g.nkb) * krank / g.split);
   const int kb1 = static_cast<int>(static_cast<long long>(g.nkb) * (krank + 1) / g.split);
-  const uint32_t b_rows = g.bn / CG, b_plane = b_rows * 128;  // of B in this CTA's shared memory
-  constexpr uint32_t kAPlane = MT * kLinABlock;
-  const uint32_t stage_bytes = g.pa * kAPlane + g.pb * b_plane;
+  // A k-block of a stage: A's accumulators (all planes of each: K-major planes
+  // of rm rows; MN-major two 64-row chunks of planes), then B's planes.
+  const uint32_t b_rows = g.bn / CG;  // of B in this CTA's shared memory
+  const uint32_t a_plane = A_MN || GATED ? 8192 : g.rm * 128, b_plane = B_MN ? 8192 : b_rows * 128;
+  const uint32_t a_acc = g.pa * (A_MN || GATED ? 16384 : a_plane);
+  const uint32_t b_at = MT * a_acc, kb_bytes = b_at + PB * b_rows * 128, stage_bytes = g.unit * kb_bytes;
   // first row of A of this CTA's part of tile row tm
   const int cta_rows = GATED ? 64 : MT * g.rm;
   auto row0 = [&](int tm) { return (tm * CG + (CG == 2 ? static_cast<int>(rank) : 0)) * cta_rows; };
@@ -229,7 +255,6 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
   if (warp == 0) {
     if (lane == 0) {
       // ---- producer
-      const uint32_t tx = CG * (g.pa * MT * g.rm * 128 + g.pb * b_plane);
       int issued = 0, st = 0;
       uint32_t phase = 1;  // of empty[st]: the first round finds every stage free
       bool ok = true;
@@ -238,38 +263,35 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
         lin_tile(g, t, &tm, &tn);
         const int m0 = row0(tm);
         const int n0 = tn * g.bn + (CG == 2 ? rank * b_rows : 0);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = kb0; kb < kb1;) {
           if (!mbar_wait_bounded(&empty[st], phase, g.err, kErrEmptyWaitTimeout, &s_abort)) {
             ok = false;
             break;
           }
           uint32_t bar = smem_u32(&full[st]);
-          if (rank == 0 || CG == 1) mbar_arrive_expect_tx(&full[st], tx);
+          const int n = kb1 - kb < g.unit ? kb1 - kb : g.unit;
+          if (rank == 0 || CG == 1) mbar_arrive_expect_tx(&full[st], CG * n * kb_bytes);
           if (CG == 2) bar = lin_mapa(bar, 0);
           uint32_t dst = smem_u32(stages) + st * stage_bytes;
-          for (int p = 0; p < g.pa; ++p) {
-            if constexpr (GATED) {
-              lin_tma<CG>(dst, &map_a, kb * 64, m0, p, bar);
-              lin_tma<CG>(dst + 8192, &map_a2, kb * 64, m0, p, bar);
-              dst += kLinABlock;
-            } else {
+          for (const int end = kb + n; kb < end; ++kb, dst += kb_bytes) {
 #pragma unroll
-              for (int a = 0; a < MT; ++a, dst += kLinABlock) {
-                if constexpr (A_MN) {
-                  lin_tma<CG>(dst, &map_a, m0 + a * 128, kb * 64, p, bar);
-                  lin_tma<CG>(dst + 8192, &map_a, m0 + a * 128 + 64, kb * 64, p, bar);
-                } else {
-                  lin_tma<CG>(dst, &map_a, kb * 64, m0 + a * g.rm, p, bar);
-                }
+            for (int a = 0; a < MT; ++a) {
+              const uint32_t to = dst + a * a_acc;
+              if constexpr (GATED) {
+                lin_tma<CG>(to, &map_a, kb * 64, m0, 0, bar);
+                lin_tma<CG>(to + 8192, &map_a2, kb * 64, m0, 0, bar);
+              } else if constexpr (A_MN) {
+                lin_tma<CG>(to, &map_a, m0 + a * 128, kb * 64, 0, bar);
+                lin_tma<CG>(to + g.pa * 8192, &map_a, m0 + a * 128 + 64, kb * 64, 0, bar);
+              } else {
+                lin_tma<CG>(to, &map_a, kb * 64, m0 + a * g.rm, 0, bar);
               }
             }
-          }
-          for (int p = 0; p < g.pb; ++p, dst += b_plane) {
             if constexpr (B_MN) {
-              for (int c = 0; c < static_cast<int>(b_rows); c += 64)
-                lin_tma<CG>(dst + c * 128, &map_b, n0 + c, kb * 64, p, bar);
+              for (uint32_t c = 0; c < b_rows; c += 64)
+                lin_tma<CG>(dst + b_at + c * 128 * PB, &map_b, n0 + c, kb * 64, 0, bar);
             } else {
-              lin_tma<CG>(dst, &map_b, kb * 64, n0, p, bar);
+              lin_tma<CG>(dst + b_at, &map_b, kb * 64, n0, 0, bar);
             }
           }
           ++issued;
@@ -289,13 +311,16 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
       int st = 0, cc = 0, tt = 0;
       uint32_t phase = 0;  // of full[st]
       bool ok = true;
-      const bool cross = g.pa + g.pb > 2;
+      constexpr bool kCross = CG == 2 && PB > 1;
       constexpr uint32_t kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
-      const uint64_t base_a = lin_desc<A_MN>(0), base_b = lin_desc<B_MN>(0);
+      const uint64_t base_a = lin_desc<A_MN>(g.pa), base_b = lin_desc<B_MN>(SH::kWideB ? 1 : PB);
+      // (side by side, an MN-major B is one 64-row chunk and its planes are the next rows)
+      const uint32_t acc_step = a_acc >> 4, plane_a = a_plane >> 4, plane_b = b_plane >> 4;
+      const uint32_t n_step = static_cast<uint32_t>(g.bn >> 3) << 17;  // bn columns in the instruction descriptor
       for (int t = first; t < ntiles && ok; t += step, ++tt) {
-        const uint32_t d_cross = tmem + (2 + (tt & 1)) * kWide;
+        const uint32_t d_cross = tmem + (2 + (tt & 1)) * kSet;
         bool cross_acc = false;
-        if (PROMOTE && cross && tt >= 2)
+        if (kCross && tt >= 2)
           ok = lin_wait(&c_empty[tt & 1], ((tt >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort);
         for (int kb = kb0; kb < kb1 && ok; ++cc) {
           // PROMOTE: chunk cc into buffer cc & 1; else the tile into both accumulators
@@ -306,45 +331,75 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
             break;
           }
           tc_fence_after_sync();
-          const uint32_t d_main = tmem + buf * kWide;
+          const uint32_t d_main = tmem + buf * kSet;
           const int end = kb + g.chunk_kb < kb1 ? kb + g.chunk_kb : kb1;
           bool acc = false;
-          for (; kb < end; ++kb) {
+          while (kb < end) {
             if (!lin_wait(&full[st], phase, g.err, kErrFullWaitTimeout, &s_abort)) {
               ok = false;
               break;
             }
             tc_fence_after_sync();
-            const uint32_t sa = smem_u32(stages) + st * stage_bytes;
             // (in a cluster a shared address carries the CTA's rank above the 18 bits a descriptor has room for)
-            const uint64_t da = base_a + ((sa & 0x3FFFFu) >> 4);
-            const uint64_t db = base_b + (((sa + g.pa * kAPlane) & 0x3FFFFu) >> 4);
+            uint32_t sa = (smem_u32(stages) + st * stage_bytes) & 0x3FFFFu;
+            for (int u = 0; u < g.unit && kb < end; ++u, ++kb, sa += kb_bytes) {
+              const uint64_t da = base_a + (sa >> 4), db = base_b + ((sa + b_at) >> 4);
+              if constexpr (!PROMOTE) {
 #pragma unroll
-            for (int a = 0; a < MT; ++a) {
-              if (!PROMOTE && !acc && tt >= 1) {  // accumulator a of the tile before is drained
-                if (!lin_wait(&t_empty[a], (tt - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) ok = false;
-                tc_fence_after_sync();
-              }
+                for (int a = 0; a < MT; ++a) {
+                  if (!acc && tt >= 1) {  // accumulator a of the tile before is drained
+                    if (!lin_wait(&t_empty[a], (tt - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) ok = false;
+                    tc_fence_after_sync();
+                  }
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                lin_mma<CG>(d_main + a * BN, da + a * (kLinABlock >> 4) + k * kStepA, db + k * kStepB, g.idesc,
-                            acc || k > 0);
-              if (!PROMOTE && kb + 1 == kb1) umma_commit_pair(&t_full[a]);
-            }
-            acc = true;
-            if (PROMOTE && cross) {
-              // planes (i, j) with 0 < i + j <= 2: what is left out is below 2^-24
-              for (int i = 0; i < g.pa; ++i)
-                for (int j = i ? 0 : 1; j < g.pb && i + j <= 2; ++j) {
-                  const uint64_t ai = da + i * (kAPlane >> 4), bj = db + j * (b_plane >> 4);
+                  for (int k = 0; k < 4; ++k)
+                    lin_mma<CG>(d_main + a * BN, da + a * acc_step + k * kStepA, db + k * kStepB, g.idesc,
+                                acc || k > 0);
+                  if (kb + 1 == kb1) umma_commit_pair(&t_full[a]);
+                }
+              } else if constexpr (SH::kWideB) {
+                // plane i of A against B's planes 0 .. PB - 1 - i, into the columns of i + j
+                const uint32_t wide = g.idesc + (PB - 1) * n_step;
 #pragma unroll
-                  for (int a = 0; a < MT; ++a)
+                for (int k = 0; k < 4; ++k)
+                  lin_mma<CG>(d_main, da + k * kStepA, db + k * kStepB, wide, acc || k > 0);
+                if (g.pa > 1) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k)
+                    lin_mma<CG>(d_main + g.bn, da + plane_a + k * kStepA, db + k * kStepB, wide - n_step, true);
+                }
+                if (g.pa > 2) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k)
+                    lin_mma<CG>(d_main + 2 * g.bn, da + 2 * plane_a + k * kStepA, db + k * kStepB, g.idesc, true);
+                }
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  lin_mma<CG>(d_main, da + k * kStepA, db + k * kStepB, g.idesc, acc || k > 0);
+                if constexpr (kCross) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k)
+                    lin_mma<CG>(d_cross, da + k * kStepA, db + plane_b + k * kStepB, g.idesc, cross_acc || k > 0);
+                  cross_acc = true;
+#pragma unroll
+                  for (int k = 0; k < 4; ++k)
+                    lin_mma<CG>(d_cross, da + k * kStepA, db + 2 * plane_b + k * kStepB, g.idesc, true);
+                  if (g.pa > 1) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                      for (int k = 0; k < 4; ++k)
+                        lin_mma<CG>(d_cross, da + plane_a + k * kStepA, db + j * plane_b + k * kStepB, g.idesc, true);
+                  }
+                  if (g.pa > 2) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                      lin_mma<CG>(d_cross + a * BN, ai + a * (kLinABlock >> 4) + k * kStepA, bj + k * kStepB, g.idesc,
-                                  cross_acc || k > 0);
-                  cross_acc = true;
+                      lin_mma<CG>(d_cross, da + 2 * plane_a + k * kStepA, db + k * kStepB, g.idesc, true);
+                  }
                 }
+              }
+              acc = true;
             }
             if constexpr (CG == 1)
               umma_commit(&empty[st]);
@@ -364,14 +419,15 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
   } else {
     // ---- epilogue
     const int quarter = warp & 3;                 // tensor-memory lanes 32 quarter ..
-    const int part = (warp - 2) >> 2;             // of the accumulator columns
-    const int a = part * HN / BN;                 // accumulator
-    const int col0 = part * HN - a * BN;          // and column in it
-    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * HN;
+    const int part = (warp - 2) >> 2;             // of the columns
+    // PROMOTE: half of the tile's bn columns; else HN columns of accumulator a
+    const int a = PROMOTE ? 0 : part * HN / BN;
+    const int half = PROMOTE ? g.bn / 2 : HN;
+    const int col0 = part * half - a * BN;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * half;
     const int row = quarter * 32 + lane;
     int cc = 0, tt = 0;
     bool ok = true;
-    const bool cross = g.pa + g.pb > 2;
     auto release = [&](uint64_t* bar) {
       tc_fence_before_sync();
       __syncwarp();
@@ -386,10 +442,13 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
       int tm, tn;
       lin_tile(g, t, &tm, &tn);
       const long long n0 = static_cast<long long>(tn) * g.bn;
-      const long long n_end = n0 + g.bn < g.N ? n0 + g.bn : g.N;
+      long long n_end = n0 + g.bn < g.N ? n0 + g.bn : g.N;
       const int m = GATED ? 0 : row0(tm) + a * g.rm + row;
       const bool m_ok = row < g.rm && m < g.M;
+      const float bias = !GATED && m_ok ? g.epi.bias_of(m) : 0.0f;
       if constexpr (PROMOTE) {
+        // (columns past the half hold other columns or nothing: never stored)
+        if (n_end > n0 + col0 + half) n_end = n0 + col0 + half;
         float acc[HN];
 #pragma unroll
         for (int i = 0; i < HN; ++i) acc[i] = 0.0f;
@@ -410,25 +469,31 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
             break;
           }
           tc_fence_after_sync();
-          take(t_lane + buf * kWide);
+          if constexpr (SH::kWideB) {
+#pragma unroll 1
+            for (int j = PB - 1; j >= 0; --j) take(t_lane + buf * kSet + j * g.bn);
+          } else {
+            take(t_lane + buf * kSet);
+          }
           release(&t_empty[buf]);
         }
-        if (cross && ok) {
-          take(t_lane + (2 + (tt & 1)) * kWide);
+        if (CG == 2 && PB > 1 && ok) {
+          take(t_lane + (2 + (tt & 1)) * kSet);
           release(&c_empty[tt & 1]);
         }
         if (GATED || g.split > 1) {
           // one tile per CTA: its stages are done with, the partial tile goes there as [column][row]
-          float* ex = reinterpret_cast<float*>(stages) + part * HN * 128 + row;
+          float* ex = reinterpret_cast<float*>(stages) + part * half * 128 + row;
 #pragma unroll
-          for (int i = 0; i < HN; ++i) ex[i * 128] = acc[i];
+          for (int i = 0; i < HN; ++i)
+            if (i < half) ex[i * 128] = acc[i];
         } else if (ok && m_ok) {
 #pragma unroll
           for (int c = 0; c < HN; c += P) {
             float v[P];
 #pragma unroll
             for (int i = 0; i < P; ++i) v[i] = acc[c + i];
-            g.epi.put_columns<P>(m, n0 + col0 + c, n_end, v);
+            g.epi.put_columns<P>(m, n0 + col0 + c, n_end, bias, v);
           }
         }
       } else {
@@ -443,7 +508,7 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
           tmem_ldf<P>(t_lane + c, v);
           tmem_wait_ld();
           if (c + P == HN) release(&t_empty[a]);  // read: the next tile may have the accumulator
-          if (m_ok) g.epi.put_columns<P>(m, n0 + col0 + c, n_end, v);
+          if (m_ok) g.epi.put_columns<P>(m, n0 + col0 + c, n_end, bias, v);
         }
       }
     }
@@ -458,7 +523,7 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
       const uint32_t ex = smem_u32(stages);
       const long long n0 = static_cast<long long>(tn) * g.bn;
       const long long n_end = n0 + g.bn < g.N ? n0 + g.bn : g.N;
-      const int krank_cols = CG == 1 ? kWide / g.split : kWide, c0 = krank * krank_cols;
+      const int krank_cols = g.bn / g.split, c0 = krank * krank_cols;
       if constexpr (GATED) {
         const int tid = threadIdx.x - 64, f = tid & 63, m = row0(tm) + f;
         for (int c = c0 + (tid >> 6); c < c0 + krank_cols; c += 4) {
@@ -477,9 +542,8 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
         auto fold = [&](auto cnt) {
           constexpr int C = decltype(cnt)::value;
           for (int c = c0 + (tid >> 7) * C; c < c0 + krank_cols; c += 2 * C) {
-            const int a = c / BN;
-            const int m = row0(tm) + a * g.rm + row;
-            const long long n = n0 + c - a * BN;
+            const int m = row0(tm) + row;
+            const long long n = n0 + c;
             if (row >= g.rm || m >= g.M || n >= n_end) continue;
             float v[C];
 #pragma unroll
@@ -489,7 +553,7 @@ __global__ void __launch_bounds__(lin_threads(PROMOTE), 1)
 #pragma unroll
               for (int i = 0; i < C; ++i) v[i] += lin_ld_cluster(at + i * 512);
             }
-            g.epi.put_columns<C>(m, n, n_end, v);
+            g.epi.put_columns<C>(m, n, n_end, g.epi.bias_of(m), v);
           }
         };
         if (krank_cols % 8 == 0)

@@ -1,0 +1,123 @@
+// objb_linear_launch.cuh -- host side of the tensor-core product: operands as
+// the copy engine reads them, tiles, and the launch of one (instantiated per
+// operand layout in linear_kk.cu, linear_mk.cu and linear_mn.cu).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "objb_common.h"
+#include "objb_host_launch.cuh"
+#include "objb_launch.h"
+#include "objb_linear_gemm.cuh"
+
+namespace objb {
+
+// A 16-bit matrix as the copy engine reads it: 16-byte aligned, rows of `ld`
+// elements (a multiple of 8), `planes` of them `rows * ld` apart.
+struct Image {
+  const void* p = nullptr;
+  size_t ld = 0, rows = 0, cols = 0;
+  int planes = 1;
+  int dtype = 0;  // OBJB_DTYPE_BF16 or F16
+};
+
+// The tensor map of an image: box of 64 elements by `box_rows` rows, all planes.
+int linear_encode(CUtensorMap* map, const Image& im, int box_rows);
+
+// One product: A (a2: the up rows of a gated one), B, D's epilogue.
+struct Product {
+  int maj = dev::kMajKK;
+  Image a, a2, b;
+  bool gated = false;
+  size_t M = 0, N = 0, K = 0;
+  dev::LinearEpilogue epi;
+  float swiglu_limit = 0.0f;
+};
+
+constexpr size_t kLinRing = 216 * 1024;    // bytes of stages: three of f32 x f32 pair tiles
+constexpr size_t kLinRingTwo = 104 * 1024;  // the same with two CTAs per SM
+
+inline size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
+
+// A product's tile: rm rows per accumulator, mt accumulators and bn columns
+// per CTA or pair, k split over a cluster.
+struct Tile {
+  int rm = 128, bn = 0, split = 1, chunk_kb = 0, unit = 1;
+  size_t ring = kLinRing;
+};
+
+enum TileKind { kDirect, kPair, kSingle };
+
+template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE, int PB>
+int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProps& props, cudaStream_t st) {
+  using SH = dev::LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>;
+  dev::GemmArgs g;
+  g.M = static_cast<int>(p.M);
+  g.N = static_cast<long long>(p.N);
+  g.nkb = static_cast<int>((p.K + 63) / 64);
+  g.pa = p.a.planes;
+  g.rm = tile.rm;
+  g.bn = tile.bn;
+  g.split = tile.split;
+  g.chunk_kb = PROMOTE ? tile.chunk_kb : g.nkb;
+  g.swiglu_limit = p.swiglu_limit;
+  g.epi = p.epi;
+  OBJB_TRY(device_error_word(device, &g.err));
+  const size_t mt = static_cast<size_t>(GATED ? 64 : MT * tile.rm) * CG;
+  g.tiles_m = static_cast<int>((p.M + mt - 1) / mt);
+  g.tiles_n = static_cast<int>((p.N + tile.bn - 1) / tile.bn);
+  const size_t a_rows = static_cast<size_t>(MT) * (MAJ != dev::kMajKK || GATED ? 128 : tile.rm);
+  g.unit = PROMOTE ? tile.unit : 1;
+  const size_t stage = g.unit * 128 * (g.pa * a_rows + static_cast<size_t>(PB) * (tile.bn / CG));
+  g.nstages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(dev::kLinStagesMax, tile.ring / stage)));
+  size_t smem = g.nstages * stage;
+  if (GATED || tile.split > 1) smem = std::max(smem, static_cast<size_t>(tile.bn) * 512);  // the partial tile
+  smem += 1024 + (128 - tile.rm) * 128;  // an MMA reads 128 rows, those past rm for nothing
+  const uint32_t half = p.a.dtype == OBJB_DTYPE_F16 ? 0 : 1;
+  g.idesc = (1u << 4) | (half << 7) | (half << 10) | (static_cast<uint32_t>(MAJ != dev::kMajKK) << 15) |
+            (static_cast<uint32_t>(MAJ == dev::kMajMN) << 16) | (static_cast<uint32_t>(tile.bn >> 3) << 17) |
+            (static_cast<uint32_t>(128 * CG >> 4) << 24);
+  CUtensorMap ma, ma2, mb;
+  OBJB_TRY(linear_encode(&ma, p.a, MAJ == dev::kMajKK && !GATED ? tile.rm : 64));
+  if (GATED)
+    OBJB_TRY(linear_encode(&ma2, p.a2, 64));
+  else
+    ma2 = ma;
+  OBJB_TRY(linear_encode(&mb, p.b, MAJ == dev::kMajMN ? 64 : tile.bn / CG));
+  auto kernel = dev::lin_gemm_kernel<MAJ, BN, CG, MT, GATED, PROMOTE, PB>;
+  OBJB_TRY(ensure_smem_attr(kernel, device, smem));
+  const long long tiles = static_cast<long long>(g.tiles_m) * g.tiles_n;
+  const int csize = CG == 2 ? 2 : tile.split;
+  const bool one_each = GATED || tile.split > 1;
+  const long long at_once = static_cast<long long>(props.sm_count) * (tile.ring < kLinRing ? 2 : 1) / csize;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((one_each ? tiles : std::min(tiles, at_once)) * csize));
+  cfg.blockDim = dim3(SH::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = csize;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = csize > 1 ? 2 : 1;
+  OBJB_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, ma2, mb, g), "launch dense product");
+  return OBJB_OK;
+}
+
+// The kernel that a tile of this layout takes (linear_kk.cu, linear_mk.cu, linear_mn.cu).
+int launch_kk(const Product& p, TileKind kind, const Tile& t, int device, const DeviceProps& props, cudaStream_t st);
+int launch_mk(const Product& p, TileKind kind, const Tile& t, int device, const DeviceProps& props, cudaStream_t st);
+int launch_mn(const Product& p, TileKind kind, const Tile& t, int device, const DeviceProps& props, cudaStream_t st);
+
+// Most columns of a single CTA's tile, and with two CTAs on an SM.
+inline int single_columns(int maj, int pb) { return pb == 1 ? 128 : maj == dev::kMajMN ? 64 : 80; }
+inline int two_columns(int maj, int pb) { return pb == 1 ? 64 : maj == dev::kMajMN ? 0 : 32; }
+
+}  // namespace objb
