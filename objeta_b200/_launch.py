@@ -4,24 +4,22 @@ from __future__ import annotations
 
 import contextlib
 
+import torch
 
-class _Here:
-    """The current device already fits: nothing to change."""
-    __slots__ = ("handle",)
 
-    def __init__(self, handle):
-        self.handle = handle
-
-    def __enter__(self):
-        return self.handle
-
-    def __exit__(self, *exc):
-        return False
+# torch's own getters of the current device and of the raw handle of its
+# current stream where it has them (a fraction of the time of the public ones,
+# which build objects), else the public ones
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 @contextlib.contextmanager
-def _there(device, stream):
-    import torch
+def launch(device, stream=None):
+    """A context whose value is the stream's handle: ``stream`` (a torch stream
+    or a handle), or the current torch stream of ``device``.  Inside it
+    ``device`` is current and new tensors belong to the stream."""
     with torch.cuda.device(device):
         if stream is None:
             yield torch.cuda.current_stream(device).cuda_stream
@@ -36,32 +34,16 @@ def _there(device, stream):
             yield stream.cuda_stream
 
 
-_raw_stream = None  # device index -> handle of torch's current stream
-
-
-def _raw_stream_getter():
-    """torch's own getter of the raw handle where it has one (a tenth of the
-    time of building a Stream object), else the public one."""
-    global _raw_stream
-    import torch
-    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
-                          lambda index: torch.cuda.current_stream(index).cuda_stream)
-    return _raw_stream
-
-
-def launch(device, stream=None):
-    """A context whose value is the stream's handle: ``stream`` (a torch stream
-    or a handle), or the current torch stream of ``device``.  Inside it
-    ``device`` is current and new tensors belong to the stream."""
-    import torch
-    index = device.index
-    if stream is None and torch.cuda.current_device() == index:
-        return _Here((_raw_stream or _raw_stream_getter())(index))
-    return _there(device, stream)
+def run(device, stream, fn, *args):
+    """fn(stream handle, *args) inside ``launch``; directly where the current
+    device and stream already fit."""
+    if stream is None and device.index == current_device():
+        return fn(raw_stream(device.index), *args)
+    with launch(device, stream) as st:
+        return fn(st, *args)
 
 
 def _refuse(name, t, device, dtypes, shape, contiguous):
-    import torch
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA tensor")
     if device is not None and t.device != device:

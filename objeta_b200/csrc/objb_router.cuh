@@ -1,0 +1,248 @@
+// objb_router.cuh -- what the router-training kernels share: teams of threads
+// that hold a token's experts, the scores, sequences and arguments.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "objb_common.h"
+#include "objb_host_launch.cuh"
+#include "objb_launch.h"
+#include "objb_pipe.cuh"
+
+namespace objb {
+namespace dev {
+
+// A token belongs to a team of L threads: 8 up to 64 experts, 16 up to 128, a
+// warp up to 1024, a block of 8 warps up to 8192; a thread holds EPL of its
+// experts in registers.  Small teams share a warp's instructions between two
+// or four tokens and reduce in fewer shuffles (32768 tokens of 64 experts: 24
+// and 22 us with a warp per token, 12 and 11 so).  With V4 (rows of whole
+// 16-byte quads) a thread's experts come in quads.  Teams of a warp run in
+// step: every lane takes part in every shuffle.
+constexpr int kTeamWarps = 8;  // warps of a block-wide team
+
+template <int LANES, int E_PER_LANE, bool V4>
+struct Team {
+  static constexpr int L = LANES, EPL = E_PER_LANE;
+  static constexpr bool kBlock = L > 32, kQuads = V4;
+  static __device__ __forceinline__ int rank() { return kBlock ? threadIdx.x : threadIdx.x & (L - 1); }
+  static __device__ __forceinline__ int expert(int i, int r) {
+    return V4 ? (i >> 2) * (4 * L) + r * 4 + (i & 3) : i * L + r;
+  }
+  static __device__ __forceinline__ void sync() {
+    if (kBlock)
+      __syncthreads();
+    else
+      __syncwarp();
+  }
+  // The lanes of this thread's team in its warp.
+  static __device__ __forceinline__ unsigned lanes() {
+    return L >= 32 ? 0xFFFFFFFFu : ((1u << (L & 31)) - 1u) << (threadIdx.x & 31 & ~(L - 1));
+  }
+  // v of every lane becomes the team's maximum / sum (fixed order).
+  static __device__ __forceinline__ float max(float v, float* red) {
+#pragma unroll
+    for (int o = (kBlock ? 32 : L) / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    if (kBlock) {
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = red[0];
+      for (int w = 1; w < kTeamWarps; ++w) v = fmaxf(v, red[w]);
+    }
+    return v;
+  }
+  static __device__ __forceinline__ float sum(float v, float* red) {
+#pragma unroll
+    for (int o = (kBlock ? 32 : L) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    if (kBlock) {
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = red[0];
+      for (int w = 1; w < kTeamWarps; ++w) v += red[w];
+    }
+    return v;
+  }
+  // Experts past E read as `fill`.
+  static __device__ __forceinline__ void load(const float* row, int E, float fill, float (&l)[EPL]) {
+    const int r = rank();
+    if constexpr (V4) {
+#pragma unroll
+      for (int i = 0; i < EPL; i += 4) {
+        const int e = expert(i, r);
+        float4 q = make_float4(fill, fill, fill, fill);
+        if (e < E) q = *reinterpret_cast<const float4*>(row + e);
+        l[i] = q.x, l[i + 1] = q.y, l[i + 2] = q.z, l[i + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        const int e = expert(i, r);
+        l[i] = e < E ? row[e] : fill;
+      }
+    }
+  }
+};
+
+enum { kSoftmax = 0, kSigmoid = 1, kSqrtSoftplus = 2 };
+
+__device__ __forceinline__ float neg_inf() { return -__int_as_float(0x7F800000); }
+
+// exp by the special-function unit: 2 ulp, plus |x| half steps from the product.
+__device__ __forceinline__ float exp_sfu(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+__device__ __forceinline__ float rcp_sfu(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The gate's sigmoid and sqrt-softplus scores and their derivatives.  The
+// sqrt-softplus keeps the gate's branches, log1p(exp(-l)) below -20 among
+// them, so the derivative is that of the score as it is computed.
+__device__ __forceinline__ float score_of(int func, float l, float* d) {
+  if (func == kSigmoid) {
+    const float t = exp_sfu(-fabsf(l));
+    const float r = rcp_sfu(1.0f + t);
+    *d = t * r * r;
+    return l >= 0.0f ? r : t * r;
+  }
+  if (l > 20.0f) {
+    const float s = sqrtf(l);
+    *d = 0.5f / s;
+    return s;
+  }
+  const bool low = l < -20.0f;
+  const float ex = expf(low ? -l : l);
+  const float s = sqrtf(log1pf(ex));
+  const float sg = low ? 1.0f / (1.0f + expf(l)) : ex / (1.0f + ex);
+  *d = (low ? -0.5f : 0.5f) * sg / s;
+  return s;
+}
+
+// A token's logits l become exp(l - base); returns their sum.  Where none is
+// above 64 and one above -64 (every trained router), base is 0: no maximum has
+// to be found first, and the exponentials serve the sigmoid too (*direct).
+template <class TM>
+__device__ __forceinline__ float exponentials(float (&l)[TM::EPL], float* red, float* base, bool* direct) {
+  float m = l[0];
+#pragma unroll
+  for (int i = 1; i < TM::EPL; ++i) m = fmaxf(m, l[i]);
+  *direct = false;
+  *base = 0.0f;
+  if (!TM::kBlock) {
+    const unsigned high = __ballot_sync(0xFFFFFFFFu, m > 64.0f), seen = __ballot_sync(0xFFFFFFFFu, m > -64.0f);
+    *direct = !(high & TM::lanes()) && (seen & TM::lanes());
+  }
+  if (TM::kBlock || !__all_sync(0xFFFFFFFFu, *direct)) {
+    m = TM::max(m, red);
+    if (!*direct) *base = m > neg_inf() ? m : 0.0f;  // a row of -inf: every exponential is 0
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < TM::EPL; ++i) {
+    l[i] = exp_sfu(l[i] - *base);
+    sum += l[i];
+  }
+  return TM::sum(sum, red);
+}
+
+// The sequence of token t: -1 before the first, S behind the last.  Offsets
+// off[0..S] ascend; without a table every token is of sequence 0.
+__device__ __forceinline__ int sequence_of(const int32_t* off, int S, long long t) {
+  if (!off) return 0;
+  int lo = -1, hi = S + 1;  // off[lo] <= t < off[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (off[mid] <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+struct BalanceArgs {
+  const float* logits;
+  size_t ld;
+  const int32_t* ids;
+  const uint8_t* mask;
+  const int32_t* off;
+  int S;
+  long long T;
+  int E, k, func;
+  long long chunk;  // tokens per block
+  // partial rows, one per (block, sequence it meets): index block + sequence,
+  // which is its own for every pair (both only ascend along the tokens)
+  float* part_p;       // [rows][E] sums of p
+  int32_t* part_c;     // [rows][E] selections
+  double* part_z;      // [rows] sums of lse^2
+  int32_t* part_n;     // [rows] counted tokens
+  unsigned* ticket;
+};
+
+struct BalanceFinishArgs {
+  BalanceArgs a;
+  int groups;          // 32-expert groups
+  bool alone;          // one block does the partial pass and this one
+  double* bal_part;    // [S][groups] sum_e c P
+  double* seq_z;       // [S]
+  int32_t* counts;     // [S][E]
+  int32_t* tokens;     // [S]
+  float* losses;       // balance, z
+  float* scales;       // [S + 1]: E / (k n_q^2 S'), then 2 / N
+};
+
+struct RouterBackwardArgs {
+  const float* logits;
+  size_t ld;
+  const int32_t* ids;
+  const float* dw;        // may be null
+  const uint8_t* mask;
+  const int32_t* off;
+  int S;
+  const int32_t* counts;  // null: no losses
+  const float* scales;
+  long long T;
+  int E, k, func, renorm;
+  float route_scale, balance_grad, z_grad;
+  float* out;
+  size_t ld_out;
+  int per_team;           // consecutive tokens of a team
+};
+
+}  // namespace dev
+
+// f(Team) for E experts; v4: rows of whole aligned quads.
+template <class F>
+int with_team(size_t E, bool v4, F&& f) {
+  if (E <= 8) return f(dev::Team<8, 1, false>{});
+  if (E <= 16) return f(dev::Team<8, 2, false>{});
+  if (E <= 32) return f(dev::Team<8, 4, false>{});
+  if (E <= 64) return v4 ? f(dev::Team<8, 8, true>{}) : f(dev::Team<8, 8, false>{});
+  if (E <= 128) return v4 ? f(dev::Team<16, 8, true>{}) : f(dev::Team<16, 8, false>{});
+  if (E <= 256) return v4 ? f(dev::Team<32, 8, true>{}) : f(dev::Team<32, 8, false>{});
+  if (E <= 512) return v4 ? f(dev::Team<32, 16, true>{}) : f(dev::Team<32, 16, false>{});
+  if (E <= 1024) return f(dev::Team<32, 32, false>{});
+  return f(dev::Team<32 * dev::kTeamWarps, 32, false>{});
+}
+
+template <class F>
+int with_func(int func, F&& f) {
+  using std::integral_constant;
+  if (func == dev::kSoftmax) return f(integral_constant<int, dev::kSoftmax>{});
+  if (func == dev::kSigmoid) return f(integral_constant<int, dev::kSigmoid>{});
+  return f(integral_constant<int, dev::kSqrtSoftplus>{});
+}
+
+// router_partial.cu, router_backward.cu
+int launch_balance_partial(const dev::BalanceFinishArgs& f, int grid, bool v4, cudaStream_t st);
+int launch_router_backward(dev::RouterBackwardArgs a, bool v4, const DeviceProps& props, cudaStream_t st);
+
+}  // namespace objb

@@ -19,674 +19,19 @@
 #include <algorithm>
 #include <string>
 
-#include "objb_common.h"
-#include "objb_host_launch.cuh"
-#include "objb_launch.h"
-#include "objb_pipe.cuh"
+#include "objb_router.cuh"
+#include "objb_router_finish.cuh"
 
 namespace objb {
 namespace dev {
 
-// A token belongs to a team: one warp up to 1024 experts, a block of 8 warps
-// up to 8192.  Each thread holds EPL experts of the token in registers.  With
-// V4 (EPL >= 4, rows of whole 16-byte quads) a thread's experts come in quads.
-constexpr int kTeamWarps = 8;  // warps of a block-wide team
+constexpr int kFinishWarps = 32;
 
-template <int EPL, int WPT, bool V4>
-struct Team {
-  static constexpr int kThreads = 32 * WPT;
-  static __device__ __forceinline__ int rank() { return WPT == 1 ? (threadIdx.x & 31) : threadIdx.x; }
-  static __device__ __forceinline__ int expert(int i, int r) {
-    return V4 ? (i >> 2) * (4 * kThreads) + r * 4 + (i & 3) : i * kThreads + r;
-  }
-  static __device__ __forceinline__ void sync() {
-    if (WPT == 1)
-      __syncwarp();
-    else
-      __syncthreads();
-  }
-  // v of every lane becomes the team's maximum / sum (fixed order).
-  static __device__ __forceinline__ float max(float v, float* red) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    if (WPT > 1) {
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-      __syncthreads();
-      v = red[0];
-      for (int w = 1; w < WPT; ++w) v = fmaxf(v, red[w]);
-    }
-    return v;
-  }
-  static __device__ __forceinline__ float sum(float v, float* red) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    if (WPT > 1) {
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-      __syncthreads();
-      v = red[0];
-      for (int w = 1; w < WPT; ++w) v += red[w];
-    }
-    return v;
-  }
-  // Experts past E read as `fill`.
-  static __device__ __forceinline__ void load(const float* row, int E, float fill, float (&l)[EPL]) {
-    const int r = rank();
-    if constexpr (V4) {
-#pragma unroll
-      for (int i = 0; i < EPL; i += 4) {
-        const int e = expert(i, r);
-        float4 q = make_float4(fill, fill, fill, fill);
-        if (e < E) q = *reinterpret_cast<const float4*>(row + e);
-        l[i] = q.x, l[i + 1] = q.y, l[i + 2] = q.z, l[i + 3] = q.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        const int e = expert(i, r);
-        l[i] = e < E ? row[e] : fill;
-      }
-    }
-  }
-};
-
-enum { kSoftmax = 0, kSigmoid = 1, kSqrtSoftplus = 2 };
-
-__device__ __forceinline__ float neg_inf() { return -__int_as_float(0x7F800000); }
-
-// exp by the special-function unit: 2 ulp, plus |x| half steps from the product.
-__device__ __forceinline__ float exp_sfu(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
-  return r;
-}
-__device__ __forceinline__ float rcp_sfu(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// The gate's sigmoid and sqrt-softplus scores and their derivatives.  The
-// sqrt-softplus keeps the gate's branches, log1p(exp(-l)) below -20 among
-// them, so the derivative is that of the score as it is computed.
-__device__ __forceinline__ float score_of(int func, float l, float* d) {
-  if (func == kSigmoid) {
-    const float t = exp_sfu(-fabsf(l));
-    const float r = rcp_sfu(1.0f + t);
-    *d = t * r * r;
-    return l >= 0.0f ? r : t * r;
-  }
-  if (l > 20.0f) {
-    const float s = sqrtf(l);
-    *d = 0.5f / s;
-    return s;
-  }
-  const bool low = l < -20.0f;
-  const float ex = expf(low ? -l : l);
-  const float s = sqrtf(log1pf(ex));
-  const float sg = low ? 1.0f / (1.0f + expf(l)) : ex / (1.0f + ex);
-  *d = (low ? -0.5f : 0.5f) * sg / s;
-  return s;
-}
-
-// A token's logits l become exp(l - base); returns their sum.  Where none is
-// above 64 and one above -64 (every trained router), base is 0: no maximum has
-// to be found first, and the exponentials serve the sigmoid too (*direct).
-template <class TM, int EPL>
-__device__ __forceinline__ float exponentials(float (&l)[EPL], float* red, float* base, bool* direct) {
-  *base = 0.0f;
-  *direct = false;
-  if (TM::kThreads == 32) {
-    float m = l[0];
-#pragma unroll
-    for (int i = 1; i < EPL; ++i) m = fmaxf(m, l[i]);
-    *direct = !__any_sync(0xFFFFFFFFu, m > 64.0f) && __any_sync(0xFFFFFFFFu, m > -64.0f);
-  }
-  if (!*direct) {
-    float m = neg_inf();
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) m = fmaxf(m, l[i]);
-    m = TM::max(m, red);
-    *base = m > neg_inf() ? m : 0.0f;  // a row of -inf: every exponential is 0
-  }
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    l[i] = exp_sfu(l[i] - *base);
-    sum += l[i];
-  }
-  return TM::sum(sum, red);
-}
-
-// The sequence of token t: -1 before the first, S behind the last.  Offsets
-// off[0..S] ascend; without a table every token is of sequence 0.
-__device__ __forceinline__ int sequence_of(const int32_t* off, int S, long long t) {
-  if (!off) return 0;
-  int lo = -1, hi = S + 1;  // off[lo] <= t < off[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (off[mid] <= t)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return lo;
-}
-
-struct BalanceArgs {
-  const float* logits;
-  size_t ld;
-  const int32_t* ids;
-  const uint8_t* mask;
-  const int32_t* off;
-  int S;
-  long long T;
-  int E, k, func;
-  long long chunk;  // tokens per block
-  // partial rows, one per (block, sequence it meets): index block + sequence,
-  // which is its own for every pair (both only ascend along the tokens)
-  float* part_p;       // [rows][E] sums of p
-  int32_t* part_c;     // [rows][E] selections
-  double* part_z;      // [rows] sums of lse^2
-  int32_t* part_n;     // [rows] counted tokens
-  unsigned* ticket;
-};
-
-struct BalanceFinishArgs {
-  BalanceArgs a;
-  int groups;          // 32-expert groups
-  bool alone;          // one block does the partial pass and this one
-  double* bal_part;    // [S][groups] sum_e c P
-  double* seq_z;       // [S]
-  int32_t* counts;     // [S][E]
-  int32_t* tokens;     // [S]
-  float* losses;       // balance, z
-  float* scales;       // [S + 1]: E / (k n_q^2 S'), then 2 / N
-};
-
-// Sums of up to four values per thread over the block, in a fixed order.
-template <int N>
-__device__ __forceinline__ void block_sums(double (&v)[N], double (*red)[32]) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], o);
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (lane == 0) red[i][w] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = 0.0;
-    for (int j = 0; j < warps; ++j) v[i] += red[i][j];
-  }
-}
-
-struct FinishSmem {
-  double p[16][32];
-  int c[16][32];
-  double red[4][32];
-  bool last;
-};
-
-// One (sequence, 32 experts) item per block and turn: the partial rows of the
-// sequence are summed in block order (interleaved over the warps, the runs
-// folded in order), in double.  The block that finishes last (`alone`: the
-// only one) folds the sequences' sums into the losses.
-__device__ __forceinline__ void balance_finish(const BalanceFinishArgs& f, FinishSmem& sm, bool alone) {
-  const BalanceArgs& a = f.a;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  for (int item = alone ? 0 : blockIdx.x; item < a.S * f.groups; item += alone ? 1 : gridDim.x) {
-    const int q = item / f.groups, g = item - q * f.groups;
-    const int e = g * 32 + lane;
-    long long b = a.off ? a.off[q] : 0, end = a.off ? a.off[q + 1] : a.T;
-    b = b > 0 ? b : 0;
-    end = end < a.T ? end : a.T;
-    const int c0 = static_cast<int>(b / a.chunk), c1 = end > b ? static_cast<int>((end - 1) / a.chunk) : c0 - 1;
-    double p = 0.0;
-    int c = 0;
-    if (e < a.E) {
-      const float* pp = a.part_p + (static_cast<size_t>(c0) + q) * a.E + e;
-      const int32_t* pc = a.part_c + (static_cast<size_t>(c0) + q) * a.E + e;
-#pragma unroll 8
-      for (int i = w; i <= c1 - c0; i += warps) {
-        p += pp[static_cast<size_t>(i) * a.E];
-        c += pc[static_cast<size_t>(i) * a.E];
-      }
-    }
-    sm.p[w][lane] = p;
-    sm.c[w][lane] = c;
-    if (g == 0) {
-      double zn[2] = {};
-      for (int i = c0 + threadIdx.x; i <= c1; i += blockDim.x) {
-        zn[0] += a.part_z[static_cast<size_t>(i) + q];
-        zn[1] += a.part_n[static_cast<size_t>(i) + q];
-      }
-      block_sums(zn, sm.red);
-      if (threadIdx.x == 0) {
-        f.seq_z[q] = zn[0];
-        f.tokens[q] = static_cast<int32_t>(zn[1]);
-      }
-    }
-    __syncthreads();
-    if (w == 0) {
-      for (int i = 1; i < warps; ++i) p += sm.p[i][lane], c += sm.c[i][lane];
-      if (e < a.E) f.counts[static_cast<size_t>(q) * a.E + e] = c;
-      double v = p * c;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-      if (lane == 0) f.bal_part[item] = v;
-    }
-    __syncthreads();
-  }
-  if (!alone) {
-    if (threadIdx.x == 0) {
-      __threadfence();
-      sm.last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
-      __threadfence();
-    }
-    __syncthreads();
-    if (!sm.last) return;
-  }
-  double t[4] = {};  // S', N, sum of z, sum of the sequences' balances
-  for (int i = threadIdx.x; i < a.S; i += blockDim.x) {
-    const int n = __ldcg(f.tokens + i);
-    if (n == 0) continue;
-    t[0] += 1.0;
-    t[1] += n;
-    t[2] += __ldcg(f.seq_z + i);
-    double v = 0.0;
-    for (int j = 0; j < f.groups; ++j) v += __ldcg(f.bal_part + static_cast<size_t>(i) * f.groups + j);
-    t[3] += v * a.E / (static_cast<double>(a.k) * n * n);
-  }
-  block_sums(t, sm.red);
-  for (int i = threadIdx.x; i < a.S; i += blockDim.x) {
-    const double n = __ldcg(f.tokens + i);
-    f.scales[i] = n > 0.0 ? static_cast<float>(a.E / (a.k * n * n * t[0])) : 0.0f;
-  }
-  if (threadIdx.x == 0) {
-    f.losses[0] = t[0] > 0.0 ? static_cast<float>(t[3] / t[0]) : 0.0f;
-    f.losses[1] = t[1] > 0.0 ? static_cast<float>(t[2] / t[1]) : 0.0f;
-    f.scales[a.S] = t[1] > 0.0 ? static_cast<float>(2.0 / t[1]) : 0.0f;
-  }
-}
-
-__global__ void __launch_bounds__(256) balance_finish_kernel(const BalanceFinishArgs f) {
-  __shared__ FinishSmem sm;
+__global__ void __launch_bounds__(32 * kFinishWarps) balance_finish_kernel(const BalanceFinishArgs f) {
+  __shared__ FinishSmem<kFinishWarps> sm;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   balance_finish(f, sm, false);
-}
-
-template <int EPL, int WPT, bool V4, int THREADS>
-__global__ void __launch_bounds__(THREADS, EPL <= 8 ? 3 : 1) balance_partial_kernel(const BalanceFinishArgs f) {
-  using TM = Team<EPL, WPT, V4>;
-  constexpr int kTeams = THREADS / TM::kThreads;
-  extern __shared__ __align__(16) uint8_t router_smem[];
-  const BalanceArgs& a = f.a;
-  int32_t* hist = reinterpret_cast<int32_t*>(router_smem);             // [E]
-  float* acc_sm = reinterpret_cast<float*>(hist + (a.E + 3) / 4 * 4);  // [kTeams][E], warp teams
-  __shared__ float red[kTeamWarps];
-  __shared__ double z_sm[kTeams];
-  __shared__ int n_sm[kTeams];
-  __shared__ FinishSmem fin;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
-  const int E = a.E, r = TM::rank();
-  const int team = WPT == 1 ? threadIdx.x >> 5 : 0;
-  const long long t0 = blockIdx.x * a.chunk;
-  const long long t1 = t0 + a.chunk < a.T ? t0 + a.chunk : a.T;
-  long long pos = t0;
-  while (pos < t1) {
-    const int q = sequence_of(a.off, a.S, pos);
-    if (q >= a.S) break;
-    if (q < 0) {
-      pos = a.off[0];
-      continue;
-    }
-    long long end = a.off ? a.off[q + 1] : t1;
-    end = end < t1 ? end : t1;
-    for (int e = threadIdx.x; e < E; e += THREADS) hist[e] = 0;
-    __syncthreads();
-    float acc[EPL];
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) acc[i] = 0.0f;
-    double z = 0.0;
-    int n = 0;
-    float nxt[EPL];
-    int id_nxt = -1;  // slot r of the team's next token
-    bool in_nxt = false;
-    auto fetch = [&](long long t) {
-      if (t >= end) return;
-      TM::load(a.logits + t * a.ld, E, neg_inf(), nxt);
-      id_nxt = r < a.k ? a.ids[t * a.k + r] : -1;
-      in_nxt = !a.mask || a.mask[t];
-    };
-    fetch(pos + team);
-    for (long long t = pos + team; t < end; t += kTeams) {
-      float l[EPL];
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) l[i] = nxt[i];
-      const int id = id_nxt;
-      const bool in = in_nxt;
-      fetch(t + kTeams);
-      if (!in) continue;
-      ++n;
-      if (id >= 0 && id < E) atomicAdd(&hist[id], 1);
-      for (int j = r + TM::kThreads; j < a.k; j += TM::kThreads) {
-        const int e = a.ids[t * a.k + j];
-        if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
-      }
-      float base, s[EPL];
-      bool direct;
-      if (a.func != kSoftmax) {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) s[i] = l[i];
-      }
-      const float sum = exponentials<TM, EPL>(l, red, &base, &direct);
-      float ssum = sum;
-      if (a.func != kSoftmax) {
-        ssum = 0.0f;
-        if (a.func == kSigmoid && direct) {
-#pragma unroll
-          for (int i = 0; i < EPL; ++i) {
-            s[i] = l[i] * rcp_sfu(1.0f + l[i]);
-            ssum += s[i];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < EPL; ++i) {
-            float d;
-            s[i] = TM::expert(i, r) < E ? score_of(a.func, s[i], &d) : 0.0f;
-            ssum += s[i];
-          }
-        }
-        ssum = TM::sum(ssum, red);
-      } else {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) s[i] = l[i];
-      }
-      const float inv = ssum == 0.0f ? 0.0f : 1.0f / ssum;  // nothing to share out: p = 0
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) acc[i] = fmaf(s[i], inv, acc[i]);
-      if (r == 0 && sum != 0.0f) {
-        const float lse = base + logf(sum);
-        z += static_cast<double>(lse) * lse;
-      }
-    }
-    const size_t row = static_cast<size_t>(blockIdx.x) + q;
-    if (r == 0) {
-      z_sm[team] = z;
-      n_sm[team] = n;
-    }
-    if (WPT == 1) {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        const int e = TM::expert(i, r);
-        if (e < E) acc_sm[team * E + e] = acc[i];
-      }
-    }
-    __syncthreads();
-    float* pr = a.part_p + row * E;
-    int32_t* cr = a.part_c + row * E;
-    if (WPT == 1) {
-      for (int e = threadIdx.x; e < E; e += THREADS) {
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kTeams; ++w) v += acc_sm[w * E + e];
-        pr[e] = v;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        const int e = TM::expert(i, r);
-        if (e < E) pr[e] = acc[i];
-      }
-    }
-    for (int e = threadIdx.x; e < E; e += THREADS) cr[e] = hist[e];
-    if (threadIdx.x == 0) {
-      double zz = 0.0;
-      int nn = 0;
-      for (int w = 0; w < kTeams; ++w) zz += z_sm[w], nn += n_sm[w];
-      a.part_z[row] = zz;
-      a.part_n[row] = nn;
-    }
-    __syncthreads();
-    pos = end;
-  }
-  if (f.alone) balance_finish(f, fin, true);  // its own rows are all there are
-}
-
-struct RouterBackwardArgs {
-  const float* logits;
-  size_t ld;
-  const int32_t* ids;
-  const float* dw;        // may be null
-  const uint8_t* mask;
-  const int32_t* off;
-  int S;
-  const int32_t* counts;  // null: no losses
-  const float* scales;
-  long long T;
-  int E, k, func, renorm;
-  float route_scale, balance_grad, z_grad;
-  float* out;
-  size_t ld_out;
-  long long per_team;     // consecutive tokens of a team
-};
-
-template <int EPL, int WPT, bool V4>
-__global__ void __launch_bounds__(256, EPL <= 8 ? 3 : 1) router_backward_kernel(const RouterBackwardArgs a) {
-  using TM = Team<EPL, WPT, V4>;
-  extern __shared__ __align__(16) uint8_t router_smem[];
-  __shared__ float red[kTeamWarps];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int E = a.E, r = TM::rank();
-  const int team = WPT == 1 ? threadIdx.x >> 5 : 0;
-  const int Epad = (E + 3) / 4 * 4;
-  float* g = reinterpret_cast<float*>(router_smem) + static_cast<size_t>(team) * Epad;  // dL/ds of the selected experts
-  for (int e = r; e < Epad; e += TM::kThreads) g[e] = 0.0f;
-  TM::sync();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const long long t0 = (static_cast<long long>(blockIdx.x) * (256 / TM::kThreads) + team) * a.per_team;
-  const long long t1 = t0 + a.per_team < a.T ? t0 + a.per_team : a.T;
-  float B[EPL];
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) B[i] = 0.0f;
-  const bool losses = a.counts != nullptr;
-  const float zc = losses && a.z_grad != 0.0f ? a.z_grad * a.scales[a.S] : 0.0f;
-  // the team's next token: its logits, and its slot r
-  float nxt[EPL], w_nxt = 0.0f;
-  int id_nxt = -1;
-  bool in_nxt = false;
-  auto fetch = [&](long long t) {
-    if (t >= t1) return;
-    TM::load(a.logits + t * a.ld, E, neg_inf(), nxt);
-    in_nxt = !a.mask || a.mask[t];
-    if (a.dw) {
-      id_nxt = r < a.k ? a.ids[t * a.k + r] : -1;
-      w_nxt = r < a.k ? a.dw[t * a.k + r] : 0.0f;
-    }
-  };
-  fetch(t0);
-  int q = -1;
-  long long q_end = t0;  // where the sequence q ends
-  for (long long t = t0; t < t1; ++t) {
-    float l[EPL], s[EPL], d[EPL];
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) l[i] = nxt[i];
-    const int id0 = id_nxt >= 0 && id_nxt < E ? id_nxt : -1;
-    const float w0 = w_nxt;
-    const bool in = in_nxt;
-    const float le0 = a.dw && id0 >= 0 ? a.logits[t * a.ld + id0] : 0.0f;
-    fetch(t + 1);
-    if (t >= q_end) {
-      q = sequence_of(a.off, a.S, t);
-      q_end = !a.off || q >= a.S ? a.T : a.off[q < 0 ? 0 : q + 1];
-      const bool some = losses && q >= 0 && q < a.S;
-      const float c = some ? a.balance_grad * a.scales[q] : 0.0f;
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        const int e = TM::expert(i, r);
-        B[i] = some && e < E ? c * static_cast<float>(a.counts[static_cast<size_t>(q) * E + e]) : 0.0f;
-      }
-    }
-    float dl[EPL];
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) dl[i] = 0.0f;
-    if (in && q >= 0 && q < a.S) {
-      // exponentials, where the score or the z loss wants them
-      float base = 0.0f, inv = 0.0f, lse = 0.0f;
-      bool direct = false;
-      const bool exps = a.func != kSqrtSoftplus || zc != 0.0f;
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) s[i] = l[i];
-      if (exps) {
-        const float sum = exponentials<TM, EPL>(l, red, &base, &direct);
-        inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row of -inf: no probabilities, no gradient
-        if (zc != 0.0f) lse = sum == 0.0f ? 0.0f : base + logf(sum);
-      }
-      // scores and their derivatives
-      if (a.func == kSigmoid) {
-        if (direct) {
-#pragma unroll
-          for (int i = 0; i < EPL; ++i) {
-            const float rc = rcp_sfu(1.0f + l[i]);
-            s[i] = l[i] * rc;
-            d[i] = s[i] * rc;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < EPL; ++i) s[i] = score_of(kSigmoid, s[i], &d[i]);
-        }
-      } else if (a.func == kSqrtSoftplus) {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-          d[i] = 0.0f;
-          s[i] = TM::expert(i, r) < E ? score_of(kSqrtSoftplus, s[i], &d[i]) : 0.0f;
-        }
-      }
-      // dL/ds of the selected experts, scattered into g
-      if (a.dw) {
-        auto score_at = [&](float le) {
-          float dd;
-          return a.func == kSoftmax ? exp_sfu(le - base) * inv : score_of(a.func, le, &dd);
-        };
-        float c = a.route_scale, mean = 0.0f;
-        if (a.renorm) {
-          float Q = 0.0f, GQ = 0.0f;
-          if (id0 >= 0) {
-            Q = score_at(le0);
-            GQ = w0 * Q;
-          }
-          for (int j = r + TM::kThreads; j < a.k; j += TM::kThreads) {
-            const int e = a.ids[t * a.k + j];
-            if (e >= 0 && e < E) {
-              const float v = score_at(a.logits[t * a.ld + e]);
-              Q += v;
-              GQ = fmaf(a.dw[t * a.k + j], v, GQ);
-            }
-          }
-          Q = TM::sum(Q, red);
-          GQ = TM::sum(GQ, red);
-          if (Q > 0.0f) {  // as the gate: a sum of 0 divides nothing
-            const float iq = 1.0f / Q;
-            c *= iq;
-            mean = GQ * iq;
-          }
-        }
-        // 32 slots at a time; equal ids of a group are added in slot order
-        if (WPT == 1 || threadIdx.x < 32) {
-          const int lane = threadIdx.x & 31;
-          for (int j0 = 0; j0 < a.k; j0 += 32) {
-            int e = id0;
-            float v = w0;
-            if (j0) {
-              const int j = j0 + lane;
-              e = j < a.k ? a.ids[t * a.k + j] : -1;
-              if (e < 0 || e >= E) e = -1;
-              v = e >= 0 ? a.dw[t * a.k + j] : 0.0f;
-            }
-            v = c * (v - mean);
-            const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
-            if (__all_sync(0xFFFFFFFFu, (same & (same - 1)) == 0 || e < 0)) {
-              if (e >= 0) g[e] += v;
-            } else {
-              for (int i = 0; i < 32; ++i) {
-                if (lane == i && e >= 0) g[e] += v;
-                __syncwarp();
-              }
-            }
-            __syncwarp();
-          }
-        }
-        TM::sync();
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-          const int e = TM::expert(i, r);
-          dl[i] = e < E ? g[e] : 0.0f;
-        }
-        TM::sync();
-        if (id0 >= 0) g[id0] = 0.0f;  // back to zero
-        for (int j = r + TM::kThreads; j < a.k; j += TM::kThreads) {
-          const int e = a.ids[t * a.k + j];
-          if (e >= 0 && e < E) g[e] = 0.0f;
-        }
-        TM::sync();
-      }
-      if (a.func == kSoftmax) {
-        float dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-          dl[i] += B[i];
-          dot = fmaf(dl[i], l[i], dot);
-        }
-        dot = TM::sum(dot, red) * inv;
-        const float shift = zc * lse - dot;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) dl[i] = l[i] * inv * (dl[i] + shift);
-      } else {
-        if (losses) {
-          float ssum = 0.0f, bsum = 0.0f;
-#pragma unroll
-          for (int i = 0; i < EPL; ++i) {
-            ssum += s[i];
-            bsum = fmaf(B[i], s[i], bsum);
-          }
-          ssum = TM::sum(ssum, red);
-          bsum = TM::sum(bsum, red);
-          const float is = ssum == 0.0f ? 0.0f : 1.0f / ssum;
-          const float mean = bsum * is;
-#pragma unroll
-          for (int i = 0; i < EPL; ++i) dl[i] = fmaf(B[i] - mean, is, dl[i]);
-        }
-        const float zl = zc * lse * inv;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-          dl[i] *= d[i];
-          if (zc != 0.0f) dl[i] = fmaf(zl, l[i], dl[i]);
-        }
-      }
-    }
-    float* o = a.out + t * a.ld_out;
-    if constexpr (V4) {
-#pragma unroll
-      for (int i = 0; i < EPL; i += 4) {
-        const int e = TM::expert(i, r);
-        if (e < E) *reinterpret_cast<float4*>(o + e) = make_float4(dl[i], dl[i + 1], dl[i + 2], dl[i + 3]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        const int e = TM::expert(i, r);
-        if (e < E) o[e] = dl[i];
-      }
-    }
-  }
 }
 
 // dw[t, j] = sum_o dout[t, o] v[slot_row[t, j], o]: WPS warps per slot, each
@@ -801,21 +146,6 @@ int plan_balance_here(size_t T, size_t E, size_t S, BalancePlan* p) {
   return OBJB_OK;
 }
 
-// f(EPL, WPT, V4) for E experts; v4: rows of whole aligned quads.
-template <class F>
-int with_team(size_t E, bool v4, F&& f) {
-  using std::integral_constant;
-#define OBJB_TEAM(EPL, WPT, V) f(integral_constant<int, EPL>{}, integral_constant<int, WPT>{}, integral_constant<bool, V>{})
-  if (E <= 32) return OBJB_TEAM(1, 1, false);
-  if (E <= 64) return OBJB_TEAM(2, 1, false);
-  if (E <= 128) return v4 ? OBJB_TEAM(4, 1, true) : OBJB_TEAM(4, 1, false);
-  if (E <= 256) return v4 ? OBJB_TEAM(8, 1, true) : OBJB_TEAM(8, 1, false);
-  if (E <= 512) return v4 ? OBJB_TEAM(16, 1, true) : OBJB_TEAM(16, 1, false);
-  if (E <= 1024) return v4 ? OBJB_TEAM(32, 1, true) : OBJB_TEAM(32, 1, false);
-  return OBJB_TEAM(32, dev::kTeamWarps, false);
-#undef OBJB_TEAM
-}
-
 }  // namespace
 }  // namespace objb
 
@@ -888,15 +218,9 @@ int objb_balance_loss_device(const float* d_logits, size_t logits_stride, const 
   f.scales = d_scales;
   const bool v4 = aligned16(d_logits) && ld % 4 == 0 && num_experts % 4 == 0;
   const int grid = static_cast<int>(std::max<size_t>(1, p.chunks));
-  OBJB_TRY(with_team(num_experts, v4, [&](auto epl, auto wpt, auto v) {
-    constexpr int EPL = decltype(epl)::value, WPT = decltype(wpt)::value;
-    constexpr int THREADS = 256;
-    const size_t teams = WPT == 1 ? THREADS / 32 : 0;
-    const size_t smem = ((num_experts + 3) / 4 * 4 + teams * num_experts) * 4;
-    return launch_pdl(dev::balance_partial_kernel<EPL, WPT, decltype(v)::value, THREADS>, grid, THREADS, smem, st, f);
-  }));
+  OBJB_TRY(launch_balance_partial(f, grid, v4, st));
   if (f.alone) return OBJB_OK;
-  return launch_pdl(dev::balance_finish_kernel, static_cast<int>(num_seqs * p.groups), 256, 0, st, f);
+  return launch_pdl(dev::balance_finish_kernel, static_cast<int>(num_seqs * p.groups), 32 * dev::kFinishWarps, 0, st, f);
 }
 
 int objb_router_backward_device(const float* d_logits, size_t logits_stride, const int32_t* d_ids,
@@ -947,18 +271,7 @@ int objb_router_backward_device(const float* d_logits, size_t logits_stride, con
   a.out = d_dlogits;
   a.ld_out = ldo;
   const bool v4 = aligned16(d_logits) && aligned16(d_dlogits) && ld % 4 == 0 && ldo % 4 == 0 && num_experts % 4 == 0;
-  return with_team(num_experts, v4, [&](auto epl, auto wpt, auto v) {
-    constexpr int EPL = decltype(epl)::value, WPT = decltype(wpt)::value;
-    const size_t teams = 8 / WPT;
-    // up to three blocks per SM (what the registers allow), each team a run of consecutive tokens
-    const size_t most = static_cast<size_t>(EPL <= 8 ? 3 : 1) * props.sm_count * teams;
-    a.per_team = static_cast<long long>((num_tokens + most - 1) / most);
-    const size_t per_block = teams * a.per_team;
-    const size_t smem = teams * ((num_experts + 3) / 4 * 4) * 4;
-    return launch_pdl(dev::router_backward_kernel<EPL, WPT, decltype(v)::value>,
-                      static_cast<int>((num_tokens + per_block - 1) / per_block), 256, smem,
-                      static_cast<cudaStream_t>(stream), a);
-  });
+  return launch_router_backward(a, v4, props, static_cast<cudaStream_t>(stream));
 }
 
 int objb_moe_combine_backward_device(const float* d_dout, const float* d_v, size_t v_rows, const int32_t* d_slot_row,

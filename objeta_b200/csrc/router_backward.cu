@@ -1,0 +1,253 @@
+// router_backward.cu -- the gradient of the router's logits, through the
+// routing weights and the balance and z losses, in one pass over the logits.
+#include "objb_router.cuh"
+
+namespace objb {
+namespace dev {
+
+template <class TM, int FUNC>
+__global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : 1) router_backward_kernel(const RouterBackwardArgs a) {
+  constexpr int EPL = TM::EPL, L = TM::L;
+  extern __shared__ __align__(16) uint8_t router_smem[];
+  __shared__ float red[kTeamWarps];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int E = a.E, r = TM::rank();
+  const int team = TM::kBlock ? 0 : threadIdx.x / L;
+  const int Epad = (E + 3) / 4 * 4;
+  float* g = reinterpret_cast<float*>(router_smem) + static_cast<size_t>(team) * Epad;  // dL/ds of the selected experts
+  for (int e = r; e < Epad; e += L) g[e] = 0.0f;
+  TM::sync();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long t0 = (static_cast<long long>(blockIdx.x) * (256 / L) + team) * a.per_team;
+  const long long t1 = t0 + a.per_team < a.T ? t0 + a.per_team : a.T;
+  float B[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) B[i] = 0.0f;
+  const bool losses = a.counts != nullptr;
+  const float zc = losses && a.z_grad != 0.0f ? a.z_grad * a.scales[a.S] : 0.0f;
+  // the team's next token: its logits, and its slot r
+  float nxt[EPL], w_nxt = 0.0f;
+  int id_nxt = -1;
+  bool in_nxt = false;
+  auto fetch = [&](long long t) {
+    in_nxt = t < t1 && (!a.mask || a.mask[t]);
+    id_nxt = -1;
+    w_nxt = 0.0f;
+    if (t < t1) {
+      TM::load(a.logits + t * a.ld, E, neg_inf(), nxt);
+      if (a.dw && r < a.k) {
+        id_nxt = a.ids[t * a.k + r];
+        w_nxt = a.dw[t * a.k + r];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) nxt[i] = 0.0f;
+    }
+  };
+  fetch(t0);
+  int q = -1;
+  long long q_end = t0;  // where the sequence q ends
+  for (int step = 0; step < a.per_team; ++step) {  // the teams of a warp in step
+    const long long t = t0 + step;
+    const bool here = t < t1;
+    float l[EPL], s[EPL], d[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) l[i] = nxt[i];
+    const int id0 = id_nxt >= 0 && id_nxt < E ? id_nxt : -1;
+    const float w0 = w_nxt;
+    bool in = in_nxt;
+    const float le0 = id0 >= 0 ? a.logits[t * a.ld + id0] : 0.0f;
+    fetch(t + 1);
+    if (here && t >= q_end) {
+      q = sequence_of(a.off, a.S, t);
+      q_end = !a.off || q >= a.S ? a.T : a.off[q < 0 ? 0 : q + 1];
+      const bool some = losses && q >= 0 && q < a.S;
+      const float c = some ? a.balance_grad * a.scales[q] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        const int e = TM::expert(i, r);
+        B[i] = some && e < E ? c * static_cast<float>(a.counts[static_cast<size_t>(q) * E + e]) : 0.0f;
+      }
+    }
+    in = in && q >= 0 && q < a.S;
+    float dl[EPL];
+    if (TM::kBlock ? in : __any_sync(0xFFFFFFFFu, in)) {
+      // exponentials, where the score or the z loss wants them
+      float base = 0.0f, inv = 0.0f, lse = 0.0f;
+      bool direct = false;
+      if (FUNC != kSoftmax) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) s[i] = l[i];
+      }
+      if (FUNC != kSqrtSoftplus || zc != 0.0f) {
+        const float sum = exponentials<TM>(l, red, &base, &direct);
+        inv = sum == 0.0f ? 0.0f : rcp_sfu(sum);  // a row of -inf: no probabilities, no gradient
+        if (zc != 0.0f) lse = sum == 0.0f ? 0.0f : base + __logf(sum);
+      }
+      // scores and their derivatives
+      if (FUNC == kSigmoid && direct) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+          const float rc = rcp_sfu(1.0f + l[i]);
+          s[i] = l[i] * rc;
+          d[i] = s[i] * rc;
+        }
+      } else if (FUNC != kSoftmax) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+          d[i] = 0.0f;
+          s[i] = TM::expert(i, r) < E ? score_of(FUNC, s[i], &d[i]) : 0.0f;
+        }
+      }
+      __syncwarp();
+      // dL/ds of the selected experts, scattered into g
+      if (a.dw) {
+        auto score_at = [&](float le) {
+          float dd;
+          return FUNC == kSoftmax ? exp_sfu(le - base) * inv : score_of(FUNC, le, &dd);
+        };
+        float c = a.route_scale, mean = 0.0f;
+        if (a.renorm) {
+          float Q = 0.0f, GQ = 0.0f;
+          if (id0 >= 0) {
+            Q = score_at(le0);
+            GQ = w0 * Q;
+          }
+          for (int j = r + L; j < a.k; j += L) {
+            const int e = here ? a.ids[t * a.k + j] : -1;
+            if (e >= 0 && e < E) {
+              const float v = score_at(a.logits[t * a.ld + e]);
+              Q += v;
+              GQ = fmaf(a.dw[t * a.k + j], v, GQ);
+            }
+          }
+          __syncwarp();
+          Q = TM::sum(Q, red);
+          GQ = TM::sum(GQ, red);
+          if (Q > 0.0f) {  // as the gate: a sum of 0 divides nothing
+            const float iq = rcp_sfu(Q);
+            c *= iq;
+            mean = GQ * iq;
+          }
+        }
+        // a team's (a block's first warp's) slots at a time; equal ids among them are added in slot order
+        constexpr int W = TM::kBlock ? 32 : L;
+        if (!TM::kBlock || threadIdx.x < 32) {
+          const int slot = threadIdx.x & (W - 1);
+          for (int j0 = 0; j0 < a.k; j0 += W) {
+            int e = id0;
+            float v = w0;
+            if (j0) {
+              const int j = j0 + slot;
+              e = here && j < a.k ? a.ids[t * a.k + j] : -1;
+              if (e < 0 || e >= E) e = -1;
+              v = e >= 0 ? a.dw[t * a.k + j] : 0.0f;
+            }
+            v = c * (v - mean);
+            const unsigned same = __match_any_sync(0xFFFFFFFFu, e) & TM::lanes();
+            if (__all_sync(0xFFFFFFFFu, (same & (same - 1)) == 0 || e < 0)) {
+              if (e >= 0) g[e] += v;
+            } else {
+              for (int i = 0; i < W; ++i) {
+                if (slot == i && e >= 0) g[e] += v;
+                __syncwarp();
+              }
+            }
+            __syncwarp();
+          }
+        }
+        TM::sync();
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+          const int e = TM::expert(i, r);
+          dl[i] = e < E ? g[e] : 0.0f;
+        }
+        TM::sync();
+        if (id0 >= 0) g[id0] = 0.0f;  // back to zero
+        for (int j = r + L; j < a.k; j += L) {
+          const int e = here ? a.ids[t * a.k + j] : -1;
+          if (e >= 0 && e < E) g[e] = 0.0f;
+        }
+        TM::sync();
+      } else {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) dl[i] = 0.0f;
+      }
+      if (FUNC == kSoftmax) {
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+          dl[i] += B[i];
+          dot = fmaf(dl[i], l[i], dot);
+        }
+        dot = TM::sum(dot, red) * inv;
+        const float shift = fmaf(zc, lse, -dot);
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) dl[i] = l[i] * inv * (dl[i] + shift);
+      } else {
+        if (losses) {
+          float ssum = 0.0f, bsum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) {
+            ssum += s[i];
+            bsum = fmaf(B[i], s[i], bsum);
+          }
+          ssum = TM::sum(ssum, red);
+          bsum = TM::sum(bsum, red);
+          const float is = ssum == 0.0f ? 0.0f : rcp_sfu(ssum);
+          const float less = bsum * is * is;
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) dl[i] += fmaf(B[i], is, -less);
+        }
+        if (zc != 0.0f) {
+          const float zl = zc * lse * inv;
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) dl[i] = fmaf(dl[i], d[i], zl * l[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) dl[i] *= d[i];
+        }
+      }
+    }
+    if (!in) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) dl[i] = 0.0f;
+    }
+    if (here) {
+      float* o = a.out + t * a.ld_out;
+      if constexpr (TM::kQuads) {
+#pragma unroll
+        for (int i = 0; i < EPL; i += 4) {
+          const int e = TM::expert(i, r);
+          if (e < E) *reinterpret_cast<float4*>(o + e) = make_float4(dl[i], dl[i + 1], dl[i + 2], dl[i + 3]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+          const int e = TM::expert(i, r);
+          if (e < E) o[e] = dl[i];
+        }
+      }
+    }
+  }
+}
+
+}  // namespace dev
+
+int launch_router_backward(dev::RouterBackwardArgs a, bool v4, const DeviceProps& props, cudaStream_t st) {
+  return with_team(a.E, v4, [&](auto tm) {
+    return with_func(a.func, [&](auto func) {
+      using TM = decltype(tm);
+      const size_t teams = 256 / TM::L;
+      // up to three blocks per SM (what the registers allow), each team a run of consecutive tokens
+      const size_t most = static_cast<size_t>(TM::EPL <= 8 ? 3 : 1) * props.sm_count * teams;
+      a.per_team = static_cast<int>((static_cast<size_t>(a.T) + most - 1) / most);
+      const size_t per_block = teams * a.per_team;
+      const size_t smem = teams * ((static_cast<size_t>(a.E) + 3) / 4 * 4) * 4;
+      return launch_pdl(dev::router_backward_kernel<TM, decltype(func)::value>,
+                        static_cast<int>((static_cast<size_t>(a.T) + per_block - 1) / per_block), 256, smem, st, a);
+    });
+  });
+}
+
+}  // namespace objb

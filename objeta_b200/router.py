@@ -21,8 +21,10 @@ from __future__ import annotations
 import ctypes
 from dataclasses import dataclass
 
+import torch
+
 from . import _lib
-from ._launch import launch, matrix, on_device
+from ._launch import matrix, on_device, run
 from .ep import SOFTMAX
 
 c_size = ctypes.c_size_t
@@ -43,41 +45,53 @@ _lib.register_signatures({
 })
 
 
+_F32, _I32, _MASK = (torch.float32,), (torch.int32,), (torch.bool, torch.uint8)
+
+
 @dataclass
 class BalanceLoss:
     """What ``balance_loss`` returns; ``router_backward`` takes it back."""
     counts: object       # int32 [S, E]: selections of each expert
-    tokens: object       # int32 [S]: counted tokens
-    losses: object       # f32 [2]: balance, z
-    scales: object       # f32 [S + 1]: gradient factors (E / (k n^2 S'), then 2 / N)
+    sums: object         # f32 [2 S + 3]: balance, z, scales [S + 1], then the bits of tokens [S]
     score_func: int
     seq_offsets: object
     token_mask: object
 
     @property
     def balance(self):
-        return self.losses[0]
+        """f32 scalar tensor."""
+        return self.sums[0]
 
     @property
     def z(self):
-        return self.losses[1]
+        """f32 scalar tensor."""
+        return self.sums[1]
+
+    @property
+    def scales(self):
+        """f32 [S + 1]: the gradients' factors, E / (k n^2 S') and then 2 / N."""
+        return self.sums[2:self.counts.shape[0] + 3]
+
+    @property
+    def tokens(self):
+        """int32 [S]: counted tokens."""
+        return self.sums[self.counts.shape[0] + 3:].view(torch.int32)
 
 
 def _routing(d_logits, d_ids, d_seq_offsets, d_token_mask):
-    import torch
-    T, E, ld = matrix("d_logits", d_logits, None, (torch.float32,))
+    T, E, ld = matrix("d_logits", d_logits, None, _F32)
     dev = d_logits.device
-    on_device("d_ids", d_ids, dev, (torch.int32,))
+    on_device("d_ids", d_ids, dev, _I32)
     size = d_ids.shape
     if len(size) != 2 or size[0] != T:
         raise ValueError(f"d_ids has shape {tuple(size)}, expected ({T}, top_k)")
     mask = off = None
     S = 1
     if d_token_mask is not None:
-        on_device("d_token_mask", d_token_mask, dev, (torch.bool, torch.uint8), (T,))
+        on_device("d_token_mask", d_token_mask, dev, _MASK, (T,))
         mask = d_token_mask.data_ptr()
     if d_seq_offsets is not None:
-        on_device("d_seq_offsets", d_seq_offsets, dev, (torch.int32,))
+        on_device("d_seq_offsets", d_seq_offsets, dev, _I32)
         S = d_seq_offsets.numel() - 1
         if d_seq_offsets.dim() != 1 or S < 1:
             raise ValueError("d_seq_offsets: expected [num_seqs + 1] offsets")
@@ -104,20 +118,21 @@ def balance_loss(d_logits, d_ids, score_func: int = SOFTMAX, d_seq_offsets=None,
     but adds nothing to either.  Sums over tokens are folded in a fixed order:
     the same call gives the same bits.
     """
-    import torch
     dev, ld, T, E, k, S, mask, off = _routing(d_logits, d_ids, d_seq_offsets, d_token_mask)
-    with launch(dev, stream) as st:
-        n = c_size()
-        _lib.call("objb_balance_loss_scratch_bytes", T, E, S, ctypes.byref(n))
-        scratch = torch.empty(n.value, dtype=torch.uint8, device=dev)
-        counts = torch.empty(S, E, dtype=torch.int32, device=dev)
-        tokens = torch.empty(S, dtype=torch.int32, device=dev)
-        losses = torch.empty(2, dtype=torch.float32, device=dev)
-        scales = torch.empty(S + 1, dtype=torch.float32, device=dev)
-        _lib.call("objb_balance_loss_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), mask, off, S, T, E, k,
-                  int(score_func), counts.data_ptr(), tokens.data_ptr(), losses.data_ptr(), scales.data_ptr(),
-                  scratch.data_ptr(), n.value, st)
-    return BalanceLoss(counts, tokens, losses, scales, int(score_func), d_seq_offsets, d_token_mask)
+    counts, sums = run(dev, stream, _balance_loss, d_logits, ld, d_ids, mask, off, S, T, E, k, int(score_func), dev)
+    return BalanceLoss(counts, sums, int(score_func), d_seq_offsets, d_token_mask)
+
+
+def _balance_loss(st, d_logits, ld, d_ids, mask, off, S, T, E, k, func, dev):
+    n = c_size()
+    _lib.call("objb_balance_loss_scratch_bytes", T, E, S, ctypes.byref(n))
+    scratch = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    counts = torch.empty(S, E, dtype=torch.int32, device=dev)
+    sums = torch.empty(2 * S + 3, dtype=torch.float32, device=dev)
+    at = sums.data_ptr()
+    _lib.call("objb_balance_loss_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), mask, off, S, T, E, k, func,
+              counts.data_ptr(), at + 4 * (S + 3), at, at + 8, scratch.data_ptr(), n.value, st)
+    return counts, sums
 
 
 def router_backward(d_logits, d_ids, d_dweights=None, score_func: int = SOFTMAX, renormalize: bool = False,
@@ -135,7 +150,6 @@ def router_backward(d_logits, d_ids, d_dweights=None, score_func: int = SOFTMAX,
     ``d_token_mask``).  Rows of tokens that do not count are zero.
     ``d_dlogits`` may be ``d_logits`` itself.
     """
-    import torch
     d_off = None
     if balance is not None:
         if int(score_func) != balance.score_func:
@@ -146,19 +160,25 @@ def router_backward(d_logits, d_ids, d_dweights=None, score_func: int = SOFTMAX,
     dev, ld, T, E, k, S, mask, off = _routing(d_logits, d_ids, d_off, d_token_mask)
     counts = scales = dw = None
     if balance is not None:
-        on_device("balance.counts", balance.counts, dev, (torch.int32,), (S, E))
-        counts, scales = balance.counts.data_ptr(), balance.scales.data_ptr()
+        on_device("balance.counts", balance.counts, dev, _I32, (S, E))
+        counts, scales = balance.counts.data_ptr(), balance.sums.data_ptr() + 8
     if d_dweights is not None:
-        on_device("d_dweights", d_dweights, dev, (torch.float32,), (T, k))
+        on_device("d_dweights", d_dweights, dev, _F32, (T, k))
         dw = d_dweights.data_ptr()
-    with launch(dev, stream) as st:
-        if d_dlogits is None:
-            d_dlogits, ldo = torch.empty(T, E, dtype=torch.float32, device=dev), E
-        else:
-            ldo = matrix("d_dlogits", d_dlogits, dev, (torch.float32,), (T, E))[2]
-        _lib.call("objb_router_backward_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), dw, mask, off, S, counts,
-                  scales, T, E, k, int(score_func), int(bool(renormalize)), float(route_scale), float(balance_grad),
-                  float(z_grad), d_dlogits.data_ptr(), ldo, st)
+    ldo = E
+    if d_dlogits is not None:
+        ldo = matrix("d_dlogits", d_dlogits, dev, _F32, (T, E))[2]
+    return run(dev, stream, _router_backward, d_logits, ld, d_ids, dw, mask, off, S, counts, scales, T, E, k,
+               int(score_func), int(bool(renormalize)), float(route_scale), float(balance_grad), float(z_grad),
+               d_dlogits, ldo, dev)
+
+
+def _router_backward(st, d_logits, ld, d_ids, dw, mask, off, S, counts, scales, T, E, k, func, renorm, scale, bg, zg,
+                     d_dlogits, ldo, dev):
+    if d_dlogits is None:
+        d_dlogits = torch.empty(T, E, dtype=torch.float32, device=dev)
+    _lib.call("objb_router_backward_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), dw, mask, off, S, counts,
+              scales, T, E, k, func, renorm, scale, bg, zg, d_dlogits.data_ptr(), ldo, st)
     return d_dlogits
 
 
@@ -166,22 +186,23 @@ def moe_combine_backward(d_dout, d_v, slot_row, d_dw=None, stream=None):
     """The routing weights' gradient of ``moe_combine``: dw[t, j] = sum_o
     d_dout[t, o] * d_v[slot_row[t, j], o], f32 [T, k].  A row outside d_v is
     read as row 0 and flagged (device error word bit 8), as the combine does."""
-    import torch
-    f32 = (torch.float32,)
-    dev = on_device("d_dout", d_dout, None, f32)
-    on_device("d_v", d_v, dev, f32)
-    on_device("slot_row", slot_row, dev, (torch.int32,))
-    if d_dout.dim() != 2 or d_v.dim() != 2 or slot_row.dim() != 2:
+    dev = on_device("d_dout", d_dout, None, _F32)
+    on_device("d_v", d_v, dev, _F32)
+    on_device("slot_row", slot_row, dev, _I32)
+    if d_v.dim() != 2 or slot_row.dim() != 2:
         raise ValueError("expected d_dout [T, O], d_v [V, O] and slot_row [T, k]")
     T, k = slot_row.shape
     V, O = d_v.shape
     if d_dout.shape != (T, O):
         raise ValueError(f"d_dout has shape {tuple(d_dout.shape)}, expected ({T}, {O})")
-    with launch(dev, stream) as st:
-        if d_dw is None:
-            d_dw = torch.empty(T, k, dtype=torch.float32, device=dev)
-        else:
-            on_device("d_dw", d_dw, dev, f32, (T, k))
-        _lib.call("objb_moe_combine_backward_device", d_dout.data_ptr(), d_v.data_ptr(), V, slot_row.data_ptr(), T, k,
-                  O, d_dw.data_ptr(), st)
+    if d_dw is not None:
+        on_device("d_dw", d_dw, dev, _F32, (T, k))
+    return run(dev, stream, _combine_backward, d_dout, d_v, V, slot_row, T, k, O, d_dw, dev)
+
+
+def _combine_backward(st, d_dout, d_v, V, slot_row, T, k, O, d_dw, dev):
+    if d_dw is None:
+        d_dw = torch.empty(T, k, dtype=torch.float32, device=dev)
+    _lib.call("objb_moe_combine_backward_device", d_dout.data_ptr(), d_v.data_ptr(), V, slot_row.data_ptr(), T, k, O,
+              d_dw.data_ptr(), st)
     return d_dw
