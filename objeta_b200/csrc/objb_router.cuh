@@ -126,31 +126,37 @@ __device__ __forceinline__ float score_of(int func, float l, float* d) {
   return s;
 }
 
-// A token's logits l become exp(l - base); returns their sum.  Where none is
-// above 64 and one above -64 (every trained router), base is 0: no maximum has
-// to be found first, and the exponentials serve the sigmoid too (*direct).
+// ex = exp(l - base) of a token's logits; returns their sum.  The first try has
+// base 0: its sum says whether any logit was above 69 or all below -64, and only
+// then (no trained router) is there a maximum to find.  *direct: base is 0 and
+// the exponentials serve the sigmoid too.
 template <class TM>
-__device__ __forceinline__ float exponentials(float (&l)[TM::EPL], float* red, float* base, bool* direct) {
-  float m = l[0];
-#pragma unroll
-  for (int i = 1; i < TM::EPL; ++i) m = fmaxf(m, l[i]);
-  *direct = false;
-  *base = 0.0f;
-  if (!TM::kBlock) {
-    const unsigned high = __ballot_sync(0xFFFFFFFFu, m > 64.0f), seen = __ballot_sync(0xFFFFFFFFu, m > -64.0f);
-    *direct = !(high & TM::lanes()) && (seen & TM::lanes());
-  }
-  if (TM::kBlock || !__all_sync(0xFFFFFFFFu, *direct)) {
-    m = TM::max(m, red);
-    if (!*direct) *base = m > neg_inf() ? m : 0.0f;  // a row of -inf: every exponential is 0
-  }
+__device__ __forceinline__ float exponentials(const float (&l)[TM::EPL], float (&ex)[TM::EPL], float* red, float* base,
+                                              bool* direct) {
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < TM::EPL; ++i) {
-    l[i] = exp_sfu(l[i] - *base);
-    sum += l[i];
+    ex[i] = exp_sfu(l[i]);
+    sum += ex[i];
   }
-  return TM::sum(sum, red);
+  sum = TM::sum(sum, red);
+  *base = 0.0f;
+  *direct = sum > 1e-28f && sum < 1e30f;
+  if (TM::kBlock ? !*direct : !__all_sync(0xFFFFFFFFu, *direct)) {
+    float m = neg_inf();
+#pragma unroll
+    for (int i = 0; i < TM::EPL; ++i) m = fmaxf(m, l[i]);
+    m = TM::max(m, red);
+    if (!*direct) *base = m > neg_inf() ? m : 0.0f;  // a row of -inf: every exponential is 0
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < TM::EPL; ++i) {
+      ex[i] = exp_sfu(l[i] - *base);
+      sum += ex[i];
+    }
+    sum = TM::sum(sum, red);
+  }
+  return sum;
 }
 
 // The sequence of token t: -1 before the first, S behind the last.  Offsets
@@ -219,15 +225,16 @@ struct RouterBackwardArgs {
 
 }  // namespace dev
 
-// f(Team) for E experts; v4: rows of whole aligned quads.
-template <class F>
+// f(Team) for E experts; v4: rows of whole aligned quads.  WIDE: the lanes of 129
+// to 256 experts (16, or 32 where registers run short).
+template <int WIDE, class F>
 int with_team(size_t E, bool v4, F&& f) {
   if (E <= 8) return f(dev::Team<8, 1, false>{});
   if (E <= 16) return f(dev::Team<8, 2, false>{});
   if (E <= 32) return f(dev::Team<8, 4, false>{});
   if (E <= 64) return v4 ? f(dev::Team<8, 8, true>{}) : f(dev::Team<8, 8, false>{});
   if (E <= 128) return v4 ? f(dev::Team<16, 8, true>{}) : f(dev::Team<16, 8, false>{});
-  if (E <= 256) return v4 ? f(dev::Team<32, 8, true>{}) : f(dev::Team<32, 8, false>{});
+  if (E <= 256) return v4 ? f(dev::Team<WIDE, 256 / WIDE, true>{}) : f(dev::Team<WIDE, 256 / WIDE, false>{});
   if (E <= 512) return v4 ? f(dev::Team<32, 16, true>{}) : f(dev::Team<32, 16, false>{});
   if (E <= 1024) return f(dev::Team<32, 32, false>{});
   return f(dev::Team<32 * dev::kTeamWarps, 32, false>{});

@@ -6,7 +6,7 @@ namespace objb {
 namespace dev {
 
 template <class TM, int FUNC>
-__global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : 1) router_backward_kernel(const RouterBackwardArgs a) {
+__global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1) router_backward_kernel(const RouterBackwardArgs a) {
   constexpr int EPL = TM::EPL, L = TM::L;
   extern __shared__ __align__(16) uint8_t router_smem[];
   __shared__ float red[kTeamWarps];
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : 1) router_backward_ker
   for (int step = 0; step < a.per_team; ++step) {  // the teams of a warp in step
     const long long t = t0 + step;
     const bool here = t < t1;
-    float l[EPL], s[EPL], d[EPL];
+    float l[EPL], ex[EPL], s[EPL], d[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) l[i] = nxt[i];
     const int id0 = id_nxt >= 0 && id_nxt < E ? id_nxt : -1;
@@ -75,12 +75,8 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : 1) router_backward_ker
       // exponentials, where the score or the z loss wants them
       float base = 0.0f, inv = 0.0f, lse = 0.0f;
       bool direct = false;
-      if (FUNC != kSoftmax) {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) s[i] = l[i];
-      }
       if (FUNC != kSqrtSoftplus || zc != 0.0f) {
-        const float sum = exponentials<TM>(l, red, &base, &direct);
+        const float sum = exponentials<TM>(l, ex, red, &base, &direct);
         inv = sum == 0.0f ? 0.0f : rcp_sfu(sum);  // a row of -inf: no probabilities, no gradient
         if (zc != 0.0f) lse = sum == 0.0f ? 0.0f : base + __logf(sum);
       }
@@ -88,15 +84,15 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : 1) router_backward_ker
       if (FUNC == kSigmoid && direct) {
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
-          const float rc = rcp_sfu(1.0f + l[i]);
-          s[i] = l[i] * rc;
+          const float rc = rcp_sfu(1.0f + ex[i]);
+          s[i] = ex[i] * rc;
           d[i] = s[i] * rc;
         }
       } else if (FUNC != kSoftmax) {
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
           d[i] = 0.0f;
-          s[i] = TM::expert(i, r) < E ? score_of(FUNC, s[i], &d[i]) : 0.0f;
+          s[i] = TM::expert(i, r) < E ? score_of(FUNC, l[i], &d[i]) : 0.0f;
         }
       }
       __syncwarp();
@@ -178,12 +174,12 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : 1) router_backward_ker
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
           dl[i] += B[i];
-          dot = fmaf(dl[i], l[i], dot);
+          dot = fmaf(dl[i], ex[i], dot);
         }
         dot = TM::sum(dot, red) * inv;
         const float shift = fmaf(zc, lse, -dot);
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) dl[i] = l[i] * inv * (dl[i] + shift);
+        for (int i = 0; i < EPL; ++i) dl[i] = ex[i] * inv * (dl[i] + shift);
       } else {
         if (losses) {
           float ssum = 0.0f, bsum = 0.0f;
@@ -202,7 +198,7 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : 1) router_backward_ker
         if (zc != 0.0f) {
           const float zl = zc * lse * inv;
 #pragma unroll
-          for (int i = 0; i < EPL; ++i) dl[i] = fmaf(dl[i], d[i], zl * l[i]);
+          for (int i = 0; i < EPL; ++i) dl[i] = fmaf(dl[i], d[i], zl * ex[i]);
         } else {
 #pragma unroll
           for (int i = 0; i < EPL; ++i) dl[i] *= d[i];
@@ -235,12 +231,12 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : 1) router_backward_ker
 }  // namespace dev
 
 int launch_router_backward(dev::RouterBackwardArgs a, bool v4, const DeviceProps& props, cudaStream_t st) {
-  return with_team(a.E, v4, [&](auto tm) {
+  return with_team<16>(a.E, v4, [&](auto tm) {
     return with_func(a.func, [&](auto func) {
       using TM = decltype(tm);
       const size_t teams = 256 / TM::L;
       // up to three blocks per SM (what the registers allow), each team a run of consecutive tokens
-      const size_t most = static_cast<size_t>(TM::EPL <= 8 ? 3 : 1) * props.sm_count * teams;
+      const size_t most = static_cast<size_t>(TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1) * props.sm_count * teams;
       a.per_team = static_cast<int>((static_cast<size_t>(a.T) + most - 1) / most);
       const size_t per_block = teams * a.per_team;
       const size_t smem = teams * ((static_cast<size_t>(a.E) + 3) / 4 * 4) * 4;

@@ -9,7 +9,7 @@ namespace objb {
 namespace dev {
 
 template <class TM, int FUNC, int THREADS>
-__global__ void __launch_bounds__(THREADS, TM::EPL <= 8 ? 3 : 1) balance_partial_kernel(const BalanceFinishArgs f) {
+__global__ void __launch_bounds__(THREADS, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1) balance_partial_kernel(const BalanceFinishArgs f) {
   constexpr int EPL = TM::EPL, L = TM::L;
   constexpr int kTeams = THREADS / L;
   extern __shared__ __align__(16) uint8_t router_smem[];
@@ -73,30 +73,23 @@ __global__ void __launch_bounds__(THREADS, TM::EPL <= 8 ? 3 : 1) balance_partial
           if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
         }
       }
-      if (FUNC != kSoftmax) {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) s[i] = l[i];
-      }
       float base;
       bool direct;
-      const float sum = exponentials<TM>(l, red, &base, &direct);
+      const float sum = exponentials<TM>(l, s, red, &base, &direct);
       float ssum = sum;
-      if (FUNC == kSoftmax) {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) s[i] = l[i];
-      } else {
+      if (FUNC != kSoftmax) {
         ssum = 0.0f;
         if (FUNC == kSigmoid && direct) {
 #pragma unroll
           for (int i = 0; i < EPL; ++i) {
-            s[i] = l[i] * rcp_sfu(1.0f + l[i]);
+            s[i] *= rcp_sfu(1.0f + s[i]);
             ssum += s[i];
           }
         } else {
 #pragma unroll
           for (int i = 0; i < EPL; ++i) {
             float d;
-            s[i] = TM::expert(i, r) < E ? score_of(FUNC, s[i], &d) : 0.0f;
+            s[i] = TM::expert(i, r) < E ? score_of(FUNC, l[i], &d) : 0.0f;
             ssum += s[i];
           }
         }
@@ -161,7 +154,7 @@ __global__ void __launch_bounds__(THREADS, TM::EPL <= 8 ? 3 : 1) balance_partial
 }  // namespace dev
 
 int launch_balance_partial(const dev::BalanceFinishArgs& f, int grid, bool v4, cudaStream_t st) {
-  return with_team(f.a.E, v4, [&](auto tm) {
+  return with_team<32>(f.a.E, v4, [&](auto tm) {
     return with_func(f.a.func, [&](auto func) {
       using TM = decltype(tm);
       constexpr int THREADS = 256;
