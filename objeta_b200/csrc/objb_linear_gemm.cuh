@@ -57,8 +57,8 @@ enum { kMajKK = 0, kMajMK = 1, kMajMN = 2 };  // A, B: K-major both; A MN-major;
 
 constexpr int kLinBK = 64;        // k of a stage: 128 bytes, one swizzle row
 constexpr int kLinStagesMax = 12;
-// producer, MMA and eight (PROMOTE) or sixteen epilogue warps
-constexpr int lin_threads(bool promote) { return promote ? 320 : 576; }
+// producer, MMA, eight (PROMOTE) or sixteen epilogue warps, second MMA warp
+constexpr int lin_threads(bool promote) { return promote ? 352 : 608; }
 
 struct GemmArgs {
   int M;                  // rows of A (GATED: features)
@@ -158,6 +158,17 @@ __device__ __forceinline__ void tmem_ldf(uint32_t taddr, float (&r)[G]) {
   }
 }
 
+// Whether phase `parity` of a barrier is over, without waiting.
+__device__ __forceinline__ bool lin_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return __all_sync(0xFFFFFFFFu, ok != 0);
+}
+
 // mbar_wait_bounded by a whole warp: all lanes go on or all give up.
 __device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code,
                                          unsigned* abort) {
@@ -183,6 +194,8 @@ struct LinShape {
   static constexpr int pow2(int v) { return v <= 32 ? 32 : v <= 64 ? 64 : v <= 128 ? 128 : v <= 256 ? 256 : 512; }
   static constexpr int kCols = pow2(kUsed);
   static constexpr int kThreads = lin_threads(PROMOTE);
+  static constexpr bool kCross = PROMOTE && CG == 2 && PB > 1;  // cross products in their own accumulators
+  static constexpr bool kTwoIssue = !PROMOTE || kCross;         // a second warp issues MMAs
   static constexpr int kBlocks = PROMOTE && CG == 1 && BN <= 64 && kCols <= 256 ? 2 : 1;  // CTAs an SM has room for
   static_assert(kUsed <= 512, "tensor memory columns");
   static_assert(!GATED || (MAJ == kMajKK && MT == 1 && PROMOTE), "gated products are K-major, one accumulator");
@@ -205,7 +218,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
   constexpr uint32_t kCols = SH::kCols;
 
   extern __shared__ uint8_t lin_smem[];
-  __shared__ alignas(8) uint64_t full[kLinStagesMax], empty[kLinStagesMax], t_full[2], t_empty[2], c_empty[2];
+  __shared__ alignas(8) uint64_t full[kLinStagesMax], empty[kLinStagesMax], t_full[2], t_empty[2], c_full[2], c_empty[2];
   __shared__ uint32_t s_tmem;
   __shared__ unsigned s_abort;
   uint8_t* stages = lin_smem + ((1024u - (smem_u32(lin_smem) & 1023u)) & 1023u);
@@ -214,10 +227,11 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
   const int csize = CG == 2 ? 2 : g.split;
 
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < g.nstages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < g.nstages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], SH::kTwoIssue ? 2 : 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&t_full[i], 1);
       mbar_init(&t_empty[i], 8 * CG);  // PROMOTE: all epilogue warps; else the eight of accumulator i
+      mbar_init(&c_full[i], 1);
       mbar_init(&c_empty[i], 8 * CG);
     }
     s_abort = 0;
@@ -305,114 +319,117 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
       }
     }
     __syncwarp();
-  } else if (warp == 1) {
-    if (CG == 1 || rank == 0) {
-      // ---- MMA issue
+  } else if (warp == 1 || warp == SH::kThreads / 32 - 1) {
+    const int role = warp == 1 ? 0 : 1;
+    if ((CG == 1 || rank == 0) && (role == 0 || SH::kTwoIssue)) {
+      // ---- MMA issue.  The tensor core takes an MMA when the one before it is
+      // nearly done, so whatever a warp does between two MMAs beyond that time
+      // idles it (a turn's 260 clocks of waits, addresses and branches).  So
+      // two warps issue, each for accumulators of its own (the second: direct
+      // accumulator 1, or the cross products), and the next k-block's
+      // bookkeeping is done between this one's MMAs.
       int st = 0, cc = 0, tt = 0;
       uint32_t phase = 0;  // of full[st]
       bool ok = true;
-      constexpr bool kCross = CG == 2 && PB > 1;
       constexpr uint32_t kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
       const uint64_t base_a = lin_desc<A_MN>(g.pa), base_b = lin_desc<B_MN>(SH::kWideB ? 1 : PB);
       // (side by side, an MN-major B is one 64-row chunk and its planes are the next rows)
-      const uint32_t acc_step = a_acc >> 4, plane_a = a_plane >> 4, plane_b = b_plane >> 4;
+      const uint32_t plane_a = a_plane >> 4, plane_b = b_plane >> 4;
       const uint32_t n_step = static_cast<uint32_t>(g.bn >> 3) << 17;  // bn columns in the instruction descriptor
+      const uint32_t ring = smem_u32(stages) & 0x3FFFFu;  // (in a cluster a shared address carries the CTA's rank
+                                                          // above the 18 bits a descriptor has room for)
+      const uint32_t a_at = PROMOTE ? 0 : role * a_acc;
+      uint32_t sa = ring, head = ring;  // this k-block's place, its stage's
+      int left = g.unit;                // k-blocks left in its stage
+      bool ready = false;               // its stage is known to be full
+      const int chunk = PROMOTE && role == 0 ? g.chunk_kb : g.nkb;
       for (int t = first; t < ntiles && ok; t += step, ++tt) {
-        const uint32_t d_cross = tmem + (2 + (tt & 1)) * kSet;
-        bool cross_acc = false;
-        if (kCross && tt >= 2)
+        if (SH::kCross && role == 1 && tt >= 2)
           ok = lin_wait(&c_empty[tt & 1], ((tt >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort);
+        if (!PROMOTE && tt >= 1)  // the accumulator is drained of the tile before
+          ok = lin_wait(&t_empty[role], (tt - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort);
         for (int kb = kb0; kb < kb1 && ok; ++cc) {
-          // PROMOTE: chunk cc into buffer cc & 1; else the tile into both accumulators
+          // PROMOTE: chunk cc into buffer cc & 1; else the tile into accumulator `role`
           const int buf = PROMOTE ? cc & 1 : 0;
-          if (PROMOTE && cc >= 2 &&
+          if (PROMOTE && role == 0 && cc >= 2 &&
               !lin_wait(&t_empty[buf], ((cc >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t d_main = tmem + buf * kSet;
-          const int end = kb + g.chunk_kb < kb1 ? kb + g.chunk_kb : kb1;
+          const uint32_t d = tmem + (!PROMOTE ? role * BN : role == 0 ? buf * kSet : (2 + (tt & 1)) * kSet);
+          const int end = kb + chunk < kb1 ? kb + chunk : kb1;
           bool acc = false;
           while (kb < end) {
-            if (!lin_wait(&full[st], phase, g.err, kErrFullWaitTimeout, &s_abort)) {
+            if (!ready && !lin_wait(&full[st], phase, g.err, kErrFullWaitTimeout, &s_abort)) {
               ok = false;
               break;
             }
             tc_fence_after_sync();
-            // (in a cluster a shared address carries the CTA's rank above the 18 bits a descriptor has room for)
-            uint32_t sa = (smem_u32(stages) + st * stage_bytes) & 0x3FFFFu;
-            for (int u = 0; u < g.unit && kb < end; ++u, ++kb, sa += kb_bytes) {
-              const uint64_t da = base_a + (sa >> 4), db = base_b + ((sa + b_at) >> 4);
-              if constexpr (!PROMOTE) {
-#pragma unroll
-                for (int a = 0; a < MT; ++a) {
-                  if (!acc && tt >= 1) {  // accumulator a of the tile before is drained
-                    if (!lin_wait(&t_empty[a], (tt - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) ok = false;
-                    tc_fence_after_sync();
-                  }
-#pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    lin_mma<CG>(d_main + a * BN, da + a * acc_step + k * kStepA, db + k * kStepB, g.idesc,
-                                acc || k > 0);
-                  if (kb + 1 == kb1) umma_commit_pair(&t_full[a]);
-                }
-              } else if constexpr (SH::kWideB) {
-                // plane i of A against B's planes 0 .. PB - 1 - i, into the columns of i + j
-                const uint32_t wide = g.idesc + (PB - 1) * n_step;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  lin_mma<CG>(d_main, da + k * kStepA, db + k * kStepB, wide, acc || k > 0);
-                if (g.pa > 1) {
-#pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    lin_mma<CG>(d_main + g.bn, da + plane_a + k * kStepA, db + k * kStepB, wide - n_step, true);
-                }
-                if (g.pa > 2) {
-#pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    lin_mma<CG>(d_main + 2 * g.bn, da + 2 * plane_a + k * kStepA, db + k * kStepB, g.idesc, true);
-                }
+            const uint64_t da = base_a + ((sa + a_at) >> 4), db = base_b + ((sa + b_at) >> 4);
+            // the k-block after this one: in this stage, or at the head of the next
+            int next_st = st;
+            uint32_t next_phase = phase, next_sa = sa;
+            bool stage_end = false;
+            auto look_ahead = [&]() {
+              ++kb;
+              stage_end = --left == 0 || kb == kb1;
+              if (stage_end) {
+                left = g.unit;
+                next_st = st + 1;
+                head += stage_bytes;
+                if (next_st == g.nstages) next_st = 0, next_phase ^= 1, head = ring;
+                next_sa = head;
+                ready = lin_test(&full[next_st], next_phase);
               } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  lin_mma<CG>(d_main, da + k * kStepA, db + k * kStepB, g.idesc, acc || k > 0);
-                if constexpr (kCross) {
-#pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    lin_mma<CG>(d_cross, da + k * kStepA, db + plane_b + k * kStepB, g.idesc, cross_acc || k > 0);
-                  cross_acc = true;
-#pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    lin_mma<CG>(d_cross, da + k * kStepA, db + 2 * plane_b + k * kStepB, g.idesc, true);
-                  if (g.pa > 1) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                      for (int k = 0; k < 4; ++k)
-                        lin_mma<CG>(d_cross, da + plane_a + k * kStepA, db + j * plane_b + k * kStepB, g.idesc, true);
-                  }
-                  if (g.pa > 2) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                      lin_mma<CG>(d_cross, da + 2 * plane_a + k * kStepA, db + k * kStepB, g.idesc, true);
-                  }
-                }
+                next_sa = sa + kb_bytes;
+                ready = true;
               }
-              acc = true;
+              asm volatile("" : "+r"(next_sa), "+r"(next_st), "+r"(next_phase));  // here, not behind the MMAs
+            };
+            auto four = [&](uint32_t to, uint64_t a, uint64_t b, uint32_t idesc, bool into) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) lin_mma<CG>(to, a + k * kStepA, b + k * kStepB, idesc, into || k > 0);
+            };
+            auto four_ahead = [&](uint32_t to, uint64_t a, uint64_t b, uint32_t idesc, bool into) {
+              lin_mma<CG>(to, a, b, idesc, into);
+              look_ahead();
+#pragma unroll
+              for (int k = 1; k < 4; ++k) lin_mma<CG>(to, a + k * kStepA, b + k * kStepB, idesc, true);
+            };
+            if constexpr (SH::kWideB) {
+              // plane i of A against B's planes 0 .. PB - 1 - i, into the columns of i + j
+              const uint32_t wide = g.idesc + (PB - 1) * n_step;
+              four_ahead(d, da, db, wide, acc);
+              if (g.pa > 1) four(d + g.bn, da + plane_a, db, wide - n_step, true);
+              if (g.pa > 2) four(d + 2 * g.bn, da + 2 * plane_a, db, g.idesc, true);
+            } else if (role == 0 || !SH::kCross) {
+              four_ahead(d, da, db, g.idesc, acc);
+            } else {
+              four_ahead(d, da, db + plane_b, g.idesc, acc);
+              four(d, da, db + 2 * plane_b, g.idesc, true);
+              if (g.pa > 1) {
+                four(d, da + plane_a, db, g.idesc, true);
+                four(d, da + plane_a, db + plane_b, g.idesc, true);
+              }
+              if (g.pa > 2) four(d, da + 2 * plane_a, db, g.idesc, true);
             }
-            if constexpr (CG == 1)
-              umma_commit(&empty[st]);
-            else
-              umma_commit_pair(&empty[st]);
-            if (++st == g.nstages) st = 0, phase ^= 1;
+            acc = true;
+            if (stage_end) {
+              if constexpr (CG == 1)
+                umma_commit(&empty[st]);
+              else
+                umma_commit_pair(&empty[st]);
+            }
+            st = next_st;
+            phase = next_phase;
+            sa = next_sa;
           }
-          if constexpr (PROMOTE) {
-            if constexpr (CG == 1)
-              umma_commit(&t_full[buf]);
-            else
-              umma_commit_pair(&t_full[buf]);
-          }
+          uint64_t* done = !PROMOTE ? &t_full[role] : role == 0 ? &t_full[buf] : &c_full[tt & 1];
+          if constexpr (CG == 1)
+            umma_commit(done);
+          else
+            umma_commit_pair(done);
         }
       }
     }
@@ -477,9 +494,13 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
           }
           release(&t_empty[buf]);
         }
-        if (CG == 2 && PB > 1 && ok) {
-          take(t_lane + (2 + (tt & 1)) * kSet);
-          release(&c_empty[tt & 1]);
+        if constexpr (SH::kCross) {
+          ok = ok && lin_wait(&c_full[tt & 1], (tt >> 1) & 1, g.err, kErrFullWaitTimeout, &s_abort);
+          if (ok) {
+            tc_fence_after_sync();
+            take(t_lane + (2 + (tt & 1)) * kSet);
+            release(&c_empty[tt & 1]);
+          }
         }
         if (GATED || g.split > 1) {
           // one tile per CTA: its stages are done with, the partial tile goes there as [column][row]
@@ -517,7 +538,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
   if (GATED || (CG == 1 && g.split > 1)) {
     __syncthreads();
     if (g.split > 1) cluster_sync_all();  // every partial tile is in place
-    if (warp >= 2) {
+    if (warp >= 2 && warp < 2 + kWarps) {
       int tm, tn;
       lin_tile(g, first, &tm, &tn);
       const uint32_t ex = smem_u32(stages);

@@ -373,11 +373,16 @@ class ExpertParallelMoe:
     support it), "off" never.  Its rows are within the reference tolerance of
     the CUDA-core ones and, like them, depend only on (expert, token row), so
     the choice -- made from T * k, not from the rank count -- keeps results
-    independent of the number of ranks."""
+    independent of the number of ranks.
+
+    ``shared``: (gate, up, down) bf16 CUDA tensors [I, H], [I, H], [O, I] of a
+    shared expert that every rank holds whole; it runs over this rank's own
+    tokens and is added to the routed output (``ffn_bf16_device`` for one
+    token, ``ffn_bf16_tokens`` for more), with the same ``swiglu_limit``."""
 
     def __init__(self, layer, num_experts: int, top_k: int, rank: int = 0, world: int = 1, group=None,
                  out_dim: int | None = None, compute=None, combine=None, swiglu_limit: float = 0.0,
-                 plan_on_host: bool = False, exchange: str = "device", grouped: str = "auto"):
+                 plan_on_host: bool = False, exchange: str = "device", grouped: str = "auto", shared=None):
         self.layer = layer
         self.num_experts = int(num_experts)
         self.top_k = int(top_k)
@@ -395,6 +400,12 @@ class ExpertParallelMoe:
         if grouped == "on" and (layer is None or not grouped_supported(layer)):
             raise ValueError("grouped='on' needs a Q4_0 layer with hidden, intermediate multiples of 256")
         self.grouped = grouped
+        if shared is not None:
+            gate, up, down = shared
+            if gate.shape != up.shape or down.dim() != 2 or down.shape != (self.out_dim, gate.shape[0]):
+                raise ValueError(f"shared expert shapes {tuple(gate.shape)}, {tuple(up.shape)}, {tuple(down.shape)} "
+                                 f"do not make [I, H], [I, H], [{self.out_dim}, I]")
+        self.shared = shared
         self.last_plan = None
         self.phase_events = None  # a list: forward() appends (phase, CUDA event) boundaries to it
         self._pin = None     # pinned int32 staging for plan arrays (grow-only)
@@ -542,6 +553,24 @@ class ExpertParallelMoe:
         return DispatchPlan.build(ids_all, self.rank, self.world, self.num_experts)
 
     def forward(self, x, ids, w):
+        out = self._forward_routed(x, ids, w)
+        if self.shared is not None and x.shape[0]:
+            self._add_shared(x.contiguous(), out)
+        return out
+
+    def _add_shared(self, x, out):
+        """out += the shared expert of this rank's tokens."""
+        import torch
+        from .dense import ffn_bf16_tokens
+        from .moe import ffn_bf16_device
+        gate, up, down = self.shared
+        if x.shape[0] == 1:
+            ffn_bf16_device(gate, up, down, gate.shape[1], gate.shape[0], down.shape[0], x, out, accumulate=True,
+                            swiglu_limit=self.swiglu_limit, stream=torch.cuda.current_stream(x.device))
+        else:
+            ffn_bf16_tokens(gate, up, down, x, d_residual=out, d_out=out, swiglu_limit=self.swiglu_limit)
+
+    def _forward_routed(self, x, ids, w):
         import torch
         import torch.distributed as dist
         if self.world == 1 and self._device_only:

@@ -359,3 +359,26 @@ def test_large_tiles_ffn(cuda_device):
         g, u = U.randn((I, H), torch.bfloat16, 1 / math.sqrt(H), 2), U.randn((I, H), torch.bfloat16, 1 / math.sqrt(H), 3)
         d = U.randn((O, I), torch.bfloat16, 1 / math.sqrt(I), 4)
         U.check(ffn_bf16_tokens(g, u, d, x, d_residual=r), *_ffn_ref(g, u, d, x, r, 0.0), "out")
+
+
+@pytest.mark.parametrize("T", [1, 5, 40])
+def test_expert_parallel_layer_with_a_shared_expert(cuda_device, T):
+    """ExpertParallelMoe(shared=...): the routed output plus the shared expert."""
+    from objeta_b200.ep import ExpertParallelMoe, router_topk_batched
+    from objeta_b200.moe import MoeLayer
+    from objeta_b200.quant import QGemvShape, QuantBackend, QuantFormat
+    H, I, E, k, Is = 256, 256, 8, 2, 192
+    qb = QuantBackend(0)
+    pack = lambda r, c, s: qb.quantize_matrix_device(QuantFormat.Q4_0, U.randn((r, c), scale=0.05, seed=s),
+                                                     QGemvShape.q4_0(r, c))
+    layer = MoeLayer(QuantFormat.Q4_0, H, I, H, [pack(I, H, 3 * e) for e in range(E)],
+                     [pack(I, H, 3 * e + 1) for e in range(E)], [pack(H, I, 3 * e + 2) for e in range(E)])
+    g, u = U.randn((Is, H), torch.bfloat16, 1 / 16, 91), U.randn((Is, H), torch.bfloat16, 1 / 16, 92)
+    d = U.randn((H, Is), torch.bfloat16, 1 / 14, 93)
+    x = U.randn((T, H), seed=94)
+    ids, w = router_topk_batched(U.randn((T, E), seed=95), k, renormalize=True)
+    routed = ExpertParallelMoe(layer, E, k).forward(x, ids, w)
+    both = ExpertParallelMoe(layer, E, k, shared=(g, u, d)).forward(x, ids, w)
+    U.check(both, *_ffn_ref(g, u, d, x, routed, 0.0))
+    with pytest.raises(ValueError):
+        ExpertParallelMoe(layer, E, k, shared=(g, u, d.t().contiguous()))
