@@ -59,12 +59,12 @@ def _refuse(name, t, device, dtypes, shape, contiguous):
 def on_device(name, t, device=None, dtypes=None, shape=None, contiguous=True):
     """Checks one tensor argument; returns its device."""
     try:
-        ok = t.is_cuda
         dev = t.device
     except AttributeError:
-        ok = False
-    if not ok or (device is not None and dev != device) or (dtypes is not None and t.dtype not in dtypes) or (
-            shape is not None and t.shape != shape) or (contiguous and not t.is_contiguous()):
+        dev = None
+    if dev is None or (dev.type != "cuda" if device is None else dev != device) or (
+            dtypes is not None and t.dtype not in dtypes) or (shape is not None and t.shape != shape) or (
+            contiguous and not t.is_contiguous()):
         _refuse(name, t, device, dtypes, shape, contiguous)
     return dev
 
@@ -72,8 +72,13 @@ def on_device(name, t, device=None, dtypes=None, shape=None, contiguous=True):
 def matrix(name, t, device=None, dtypes=None, shape=None):
     """Checks a 2-D tensor argument whose rows are contiguous (the rows may lie
     apart); returns (rows, cols, elements between rows)."""
-    on_device(name, t, device, dtypes, shape, False)
-    size = t.shape
+    try:
+        size, dev = t.shape, t.device
+    except AttributeError:
+        size = dev = None
+    if dev is None or (dev.type != "cuda" if device is None else dev != device) or (
+            dtypes is not None and t.dtype not in dtypes) or (shape is not None and size != shape):
+        _refuse(name, t, device, dtypes, shape, False)
     if len(size) == 2:
         rows, cols = size
         if t.is_contiguous():

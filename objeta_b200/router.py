@@ -52,7 +52,8 @@ _F32, _I32, _MASK = (torch.float32,), (torch.int32,), (torch.bool, torch.uint8)
 class BalanceLoss:
     """What ``balance_loss`` returns; ``router_backward`` takes it back."""
     counts: object       # int32 [S, E]: selections of each expert
-    sums: object         # f32 [2 S + 3]: balance, z, scales [S + 1], then the bits of tokens [S]
+    sums: object         # f32 [at + 2 S + 3]: from `at` on balance, z, scales [S + 1], the bits of tokens [S]
+    at: int
     score_func: int
     seq_offsets: object
     token_mask: object
@@ -60,22 +61,22 @@ class BalanceLoss:
     @property
     def balance(self):
         """f32 scalar tensor."""
-        return self.sums[0]
+        return self.sums[self.at]
 
     @property
     def z(self):
         """f32 scalar tensor."""
-        return self.sums[1]
+        return self.sums[self.at + 1]
 
     @property
     def scales(self):
         """f32 [S + 1]: the gradients' factors, E / (k n^2 S') and then 2 / N."""
-        return self.sums[2:self.counts.shape[0] + 3]
+        return self.sums[self.at + 2:self.at + self.counts.shape[0] + 3]
 
     @property
     def tokens(self):
         """int32 [S]: counted tokens."""
-        return self.sums[self.counts.shape[0] + 3:].view(torch.int32)
+        return self.sums[self.at + self.counts.shape[0] + 3:].view(torch.int32)
 
 
 def _routing(d_logits, d_ids, d_seq_offsets, d_token_mask):
@@ -119,20 +120,24 @@ def balance_loss(d_logits, d_ids, score_func: int = SOFTMAX, d_seq_offsets=None,
     the same call gives the same bits.
     """
     dev, ld, T, E, k, S, mask, off = _routing(d_logits, d_ids, d_seq_offsets, d_token_mask)
-    counts, sums = run(dev, stream, _balance_loss, d_logits, ld, d_ids, mask, off, S, T, E, k, int(score_func), dev)
-    return BalanceLoss(counts, sums, int(score_func), d_seq_offsets, d_token_mask)
+    counts, sums, at = run(dev, stream, _balance_loss, d_logits, ld, d_ids, mask, off, S, T, E, k, int(score_func),
+                           dev)
+    return BalanceLoss(counts, sums, at, int(score_func), d_seq_offsets, d_token_mask)
 
 
 def _balance_loss(st, d_logits, ld, d_ids, mask, off, S, T, E, k, func, dev):
     n = c_size()
     _lib.call("objb_balance_loss_scratch_bytes", T, E, S, ctypes.byref(n))
-    scratch = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    n = n.value
+    at = n // 4 if n <= 65536 else 0  # a small scratch is in front of the sums: one allocation less
     counts = torch.empty(S, E, dtype=torch.int32, device=dev)
-    sums = torch.empty(2 * S + 3, dtype=torch.float32, device=dev)
-    at = sums.data_ptr()
+    sums = torch.empty(at + 2 * S + 3, dtype=torch.float32, device=dev)
+    base = sums.data_ptr()
+    scratch = base if at else torch.empty(n, dtype=torch.uint8, device=dev)
+    base += 4 * at
     _lib.call("objb_balance_loss_device", d_logits.data_ptr(), ld, d_ids.data_ptr(), mask, off, S, T, E, k, func,
-              counts.data_ptr(), at + 4 * (S + 3), at, at + 8, scratch.data_ptr(), n.value, st)
-    return counts, sums
+              counts.data_ptr(), base + 4 * (S + 3), base, base + 8, scratch if at else scratch.data_ptr(), n, st)
+    return counts, sums, at
 
 
 def router_backward(d_logits, d_ids, d_dweights=None, score_func: int = SOFTMAX, renormalize: bool = False,
@@ -161,7 +166,7 @@ def router_backward(d_logits, d_ids, d_dweights=None, score_func: int = SOFTMAX,
     counts = scales = dw = None
     if balance is not None:
         on_device("balance.counts", balance.counts, dev, _I32, (S, E))
-        counts, scales = balance.counts.data_ptr(), balance.sums.data_ptr() + 8
+        counts, scales = balance.counts.data_ptr(), balance.sums.data_ptr() + 4 * balance.at + 8
     if d_dweights is not None:
         on_device("d_dweights", d_dweights, dev, _F32, (T, k))
         dw = d_dweights.data_ptr()
