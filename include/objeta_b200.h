@@ -641,6 +641,7 @@ int objb_deepseek_gate_device(const float *d_gate_weight, const float *d_gate_bi
  * parts (8 + 8 + 8 bits), so f32 products keep f32's precision.  A non-finite
  * operand makes its row and column of the product non-finite (Inf or NaN).
  * Rows are contiguous; strides are in elements between rows, 0 for contiguous.
+ * Results overlap no operand, but for the residual named below.
  * Any sizes, strides and element-aligned addresses are taken: operands that
  * the copy engine cannot read (16-byte aligned rows) are laid out again in
  * the scratch, which costs one pass over them.  Scratch: 256-byte aligned, at

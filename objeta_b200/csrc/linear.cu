@@ -687,6 +687,7 @@ int objb_linear_device(const objb_linear_desc* desc, const void* d_x, const void
   if (!d_x || !d_w || !d_y) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null device pointer");
   if (d_residual == d_y && ldr != ldy)
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "a residual in place needs y's stride");
+  if (d_z == d_y) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "z and y are the same array");
   int device = 0;
   DeviceProps props;
   OBJB_TRY(device_here(&device, &props));

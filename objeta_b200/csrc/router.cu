@@ -106,6 +106,8 @@ int check_router(const char* action, size_t T, size_t E, size_t k, size_t S, int
   if (S == 0 || S > (1u << 24) || (S != 1 && !off))
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action,
                      "need 1 <= num_seqs <= 2^24, and num_seqs 1 without sequence offsets");
+  if (S * ((E + 31) / 32) > (1u << 30))
+    return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "num_seqs * num_experts is above 2^35");
   return OBJB_OK;
 }
 

@@ -52,6 +52,10 @@ def test_linear_null_descriptor_and_types():
     _fails("InvalidInput", "null descriptor", "objb_linear_device", None, P, P, None, None, P, None, None, 0, None)
     d = dense._LinearDesc(tokens=1, in_features=8, out_features=8, x_dtype=2, w_dtype=2, y_dtype=2, bias_dtype=1)
     _fails("Unsupported", "bias", "objb_linear_device", ctypes.byref(d), P, P, P, None, P, None, None, 0, None)
+    d = dense._LinearDesc(tokens=1, in_features=8, out_features=8, x_dtype=2, w_dtype=2, y_dtype=2)
+    _fails("InvalidInput", "same array", "objb_linear_device", ctypes.byref(d), P, P, None, None, P, P, None, 0, None)
+    d.residual_stride = 9
+    _fails("InvalidInput", "in place", "objb_linear_device", ctypes.byref(d), P, P, None, P, P, None, None, 0, None)
     _fails("InvalidInput", "null output", "objb_linear_scratch_bytes", ctypes.byref(d), P, P, None)
 
 
@@ -103,7 +107,7 @@ def _bwd(E=8, k=2, S=1, func=0, T=4, ld=0, ldo=0, off=None, dw=P, counts=None, s
 @pytest.mark.parametrize("text,f", [
     ("top_k", dict(k=9)), ("top_k", dict(k=0)), ("num_experts", dict(E=0)), ("num_experts", dict(E=8193)),
     ("num_tokens", dict(T=(1 << 30) + 1)), ("score_func", dict(func=3)), ("score_func", dict(func=-1)),
-    ("num_seqs", dict(S=0)), ("num_seqs", dict(S=2)), ("num_seqs", dict(S=(1 << 24) + 1, off=P)),
+    ("num_seqs", dict(S=0)), ("num_seqs", dict(S=2)), ("num_seqs", dict(S=(1 << 24) + 1, off=P)), ("num_seqs", dict(S=1 << 24, E=8192, off=P)),
 ])
 def test_router_refusals(text, f):
     _fails("InvalidInput", text, *_bal(**f))
