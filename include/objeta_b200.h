@@ -644,10 +644,16 @@ int objb_deepseek_gate_device(const float *d_gate_weight, const float *d_gate_bi
  * Results overlap no operand, but for the residual named below.
  * Any sizes, strides and element-aligned addresses are taken: operands that
  * the copy engine cannot read (16-byte aligned rows) are laid out again in
- * the scratch, which costs one pass over them.  Scratch: 256-byte aligned, at
- * least the matching *_scratch_bytes (of the same operands: their alignment
- * counts, nothing is read), in use until the stream has passed the call; NULL takes the per-(device, stream) workspace, under whose rules (no
- * first use under capture; graphs captured on one stream share it). */
+ * the scratch, which costs one pass over them.  tokens <= 2^30, features <=
+ * 2^24, strides <= 2^28.  Scratch: 256-byte aligned, at least the matching
+ * *_scratch_bytes (of the same operands: their alignment counts, nothing is
+ * read), in use until the stream has passed the call; NULL takes the
+ * per-(device, stream) workspace, under its rules (no first use under
+ * capture; graphs captured on one stream share it, so they must not run at
+ * once).  A device's first call is made outside of stream capture (it
+ * allocates the error word).  Every wait of these kernels is bounded: one that
+ * runs out sets a bit of the device error word (objb_device_error_take) and
+ * leaves the results undefined. */
 enum {
   OBJB_ACT_NONE = 0,
   OBJB_ACT_RELU = 1,

@@ -384,7 +384,7 @@ double nanoseconds(const Product& p, TileKind kind, const Tile& t, size_t sms, c
 }
 
 // Which tile a product takes: the one of the fewest nanoseconds() among
-//   * direct: pairs, 512 x up to 256 columns, for 16-bit results of one-plane operands;
+//   * direct: pairs, 512 x up to 256 columns, for 16-bit results of one-plane operands (k up to kDirectK);
 //   * pairs of 256 rows x up to 128 columns;
 //   * single CTAs of 128 rows x up to 128 columns, k split over a cluster, one
 //     per SM or (up to 64 columns) two.
@@ -415,7 +415,7 @@ Choice choose_tile(const Product& p, bool y16, size_t sms, const Room& room) {
         if (c.unit == 1 || c.unit * 128u * (p.a.planes * 128 + p.b.planes * c.bn / cg) * 3 <= c.ring) consider(k, c);
   };
   Tile c;
-  if (y16 && p.a.planes == 1 && p.b.planes == 1)
+  if (y16 && p.a.planes == 1 && p.b.planes == 1 && p.K <= dev::kDirectK)
     each_bn(256, mn ? 128 : 16, 144, [&](int bn) {
       c.bn = bn;
       consider(kDirect, c);

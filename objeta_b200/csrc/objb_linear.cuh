@@ -57,8 +57,11 @@ __device__ __forceinline__ float act_value(int act, float v) {
   }
 }
 
-// d act / d v.  gelu_tanh through tanh(u) = 2 sigmoid(2 u) - 1.
+// d act / d v.  gelu_tanh through tanh(u) = 2 sigmoid(2 u) - 1.  Past 128 (in
+// f32 already before) every one is its limit; a larger v, whose powers
+// overflow, would make 0 * inf of it.
 __device__ __forceinline__ float act_grad(int act, float v) {
+  v = fabsf(v) > 128.0f ? copysignf(128.0f, v) : v;  // (NaN stays)
   switch (act) {
     case OBJB_ACT_RELU: return v > 0.0f ? 1.0f : 0.0f;
     case OBJB_ACT_SILU: {

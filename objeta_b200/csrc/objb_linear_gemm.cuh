@@ -25,10 +25,12 @@
 //     of them into columns bn.. (the products of i + j = 1 and 2), plane 2
 //     against one into columns 2 bn..; an MMA takes 39 clocks or more, so a
 //     third (half) of the MMAs is what counts up to bn 64.
-//     CG 2: one MMA per pair of planes, the cross products into a buffer of
-//     their own that is read once per tile; twice the columns per tile.
+//     CG 2: one MMA per pair of planes, the cross products into two buffers of
+//     their own, each read once per kCrossChunks chunks (their sum is 2^-8 of
+//     the main one, so 16 times the MMAs err less); twice the columns per tile.
 //   * else straight from tensor memory into the epilogue, which rounds to 16
-//     bits: two accumulators of 256 columns, all of tensor memory.  The ring
+//     bits: two accumulators of 256 columns, all of tensor memory, for k up to
+//     65536 (kDirectK).  The ring
 //     goes on filling while a tile is drained.
 // CTA pairs (CG 2, cta_group::2) share each MMA: M 256, half of B's rows from
 // each CTA's shared memory.  MT accumulators per CTA (rows m0 + a * rm) share
@@ -57,6 +59,8 @@ enum { kMajKK = 0, kMajMK = 1, kMajMN = 2 };  // A, B: K-major both; A MN-major;
 
 constexpr int kLinBK = 64;        // k of a stage: 128 bytes, one swizzle row
 constexpr int kLinStagesMax = 12;
+constexpr int kCrossChunks = 16;  // chunks of a cross product's buffer
+constexpr size_t kDirectK = 65536;  // 4096 MMAs in one accumulator lose 1.2e-4 of a sum of one sign: half of f16's rounding
 // producer, MMA, eight (PROMOTE) or sixteen epilogue warps, second MMA warp
 constexpr int lin_threads(bool promote) { return promote ? 352 : 608; }
 
@@ -342,22 +346,23 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
       uint32_t sa = ring, head = ring;  // this k-block's place, its stage's
       int left = g.unit;                // k-blocks left in its stage
       bool ready = false;               // its stage is known to be full
-      const int chunk = PROMOTE && role == 0 ? g.chunk_kb : g.nkb;
+      const int chunk = !PROMOTE ? g.nkb : role == 0 ? g.chunk_kb : kCrossChunks * g.chunk_kb;
+      uint64_t* const chunk_full = role == 0 ? t_full : c_full;
+      uint64_t* const chunk_empty = role == 0 ? t_empty : c_empty;
+      const uint32_t d0 = tmem + (PROMOTE ? 2 * kSet : BN) * role;
       for (int t = first; t < ntiles && ok; t += step, ++tt) {
-        if (SH::kCross && role == 1 && tt >= 2)
-          ok = lin_wait(&c_empty[tt & 1], ((tt >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort);
         if (!PROMOTE && tt >= 1)  // the accumulator is drained of the tile before
           ok = lin_wait(&t_empty[role], (tt - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort);
         for (int kb = kb0; kb < kb1 && ok; ++cc) {
           // PROMOTE: chunk cc into buffer cc & 1; else the tile into accumulator `role`
           const int buf = PROMOTE ? cc & 1 : 0;
-          if (PROMOTE && role == 0 && cc >= 2 &&
-              !lin_wait(&t_empty[buf], ((cc >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
+          if (PROMOTE && cc >= 2 &&
+              !lin_wait(&chunk_empty[buf], ((cc >> 1) - 1) & 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t d = tmem + (!PROMOTE ? role * BN : role == 0 ? buf * kSet : (2 + (tt & 1)) * kSet);
+          const uint32_t d = d0 + buf * kSet;
           const int end = kb + chunk < kb1 ? kb + chunk : kb1;
           bool acc = false;
           while (kb < end) {
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
             phase = next_phase;
             sa = next_sa;
           }
-          uint64_t* done = !PROMOTE ? &t_full[role] : role == 0 ? &t_full[buf] : &c_full[tt & 1];
+          uint64_t* done = PROMOTE ? &chunk_full[buf] : &t_full[role];
           if constexpr (CG == 1)
             umma_commit(done);
           else
@@ -443,7 +448,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
     const int col0 = part * half - a * BN;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * half;
     const int row = quarter * 32 + lane;
-    int cc = 0, tt = 0;
+    int cc = 0, xc = 0, tt = 0;
     bool ok = true;
     auto release = [&](uint64_t* bar) {
       tc_fence_before_sync();
@@ -479,7 +484,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
             for (int i = 0; i < G; ++i) acc[c + i] += v[i];
           }
         };
-        for (int kb = kb0; kb < kb1; kb += g.chunk_kb, ++cc) {
+        for (int kb = kb0, left = kCrossChunks; kb < kb1; kb += g.chunk_kb, ++cc) {
           const int buf = cc & 1;
           if (!lin_wait(&t_full[buf], (cc >> 1) & 1, g.err, kErrFullWaitTimeout, &s_abort)) {
             ok = false;
@@ -493,13 +498,17 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
             take(t_lane + buf * kSet);
           }
           release(&t_empty[buf]);
-        }
-        if constexpr (SH::kCross) {
-          ok = ok && lin_wait(&c_full[tt & 1], (tt >> 1) & 1, g.err, kErrFullWaitTimeout, &s_abort);
-          if (ok) {
+          if constexpr (SH::kCross) {
+            if (--left && kb + g.chunk_kb < kb1) continue;
+            left = kCrossChunks;
+            if (!lin_wait(&c_full[xc & 1], (xc >> 1) & 1, g.err, kErrFullWaitTimeout, &s_abort)) {
+              ok = false;
+              break;
+            }
             tc_fence_after_sync();
-            take(t_lane + (2 + (tt & 1)) * kSet);
-            release(&c_empty[tt & 1]);
+            take(t_lane + (2 + (xc & 1)) * kSet);
+            release(&c_empty[xc & 1]);
+            ++xc;
           }
         }
         if (GATED || g.split > 1) {

@@ -160,6 +160,38 @@ def _run_backward(T, K, N, xd, wd, yd, dwd, act, seed=0):
         U.check(got, *ref[name], f"{name} of {xd} {wd} {yd} {dwd} {act} {T} {K} {N}")
 
 
+def test_backward_activation_range(cuda_device):
+    """Far pre-activations: the powers of z overflow, the derivative is its limit; NaN stays NaN."""
+    from objeta_b200.dense import linear_backward
+    z = torch.tensor([-3e38, -1e30, -1e13, -1e4, -200.0, -129.0, -128.0, -90.0, -30.0, -5.0, -0.0, 0.0, 1e-30, 5.0,
+                      30.0, 90.0, 129.0, 1e4, 1e13, 1e30, 3e38], device="cuda").view(-1, 1)
+    far = torch.tensor([math.inf, -math.inf, math.nan], device="cuda").view(-1, 1)
+    one = torch.ones(1, 1, device="cuda")
+    for act in U.ACTS[1:]:
+        dx = linear_backward(torch.ones_like(z), z, one, d_z=z, activation=act, need_dw=False)[0]
+        ref = U.act_grad64(z, act)
+        # 16 roundings; the exponent's argument, at most a few |z|, is rounded and its exponential off by as much;
+        # below 1e-37 an exponential is flushed to 0
+        bound = (16 + 8 * torch.clamp(z.double().abs(), max=200.0)) * 2.0 ** -24 * ref.abs() + 1e-36
+        U.check(dx, ref, bound, act)
+        dx = linear_backward(torch.ones_like(far), far, one, d_z=far, activation=act, need_dw=False)[0]
+        assert dx[0] == 1 and dx[1] == 0 and (act == "relu" or bool(torch.isnan(dx[2]))), (act, dx)
+
+
+def test_long_k_of_one_sign(cuda_device):
+    """131072 products of one sign in f16: what the accumulators lose stays below the result's rounding."""
+    from objeta_b200.dense import linear
+    T = N = 4096
+    K = 131072
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.rand(T, K, generator=g, device="cuda", dtype=torch.float16) * 0.5
+    w = torch.rand(N, K, generator=g, device="cuda", dtype=torch.float16) * 0.5
+    y = linear(x, w)[::64, ::64]
+    ref = x[::64].double() @ w[::64].double().t()
+    # an accumulator of 64 k-blocks takes 256 MMAs, each off by at most a step (2^-23); then f16's half step
+    U.check(y, ref, (256 * 2.0 ** -23 + 32 * 2.0 ** -24 + 2.0 ** -11) * ref)
+
+
 @pytest.mark.parametrize("xd,wd,yd,dwd", BPAIRS)
 def test_backward_sizes(cuda_device, xd, wd, yd, dwd):
     for T, K, N in ((1, 64, 64), (3, 7, 5), (33, 1000, 257), (129, 520, 136), (400, 136, 256), (1025, 72, 48)):
@@ -343,6 +375,19 @@ def test_large_tiles(cuda_device, xd, wd, yd):
         U.check(z, rz, bz, "z")
         U.check(y, ry, by, "y")
         assert torch.equal(y, linear(x, w, b, activation=act, d_residual=r, out_dtype=yt))
+
+
+@pytest.mark.parametrize("xd,wd", [("f32", "bf16"), ("f32", "f32")])
+def test_long_k_f32(cuda_device, xd, wd):
+    """Hundreds of k-blocks and more tiles than the grid holds at once, forwards and for both gradients."""
+    from objeta_b200.dense import linear
+    x, w = _case(1500, 20000, 2600, xd, wd, 6)
+    _, _, ref, bound = U.linear_ref(x, w, None, "none", None, torch.float32)
+    y = linear(x, w)
+    U.check(y, ref, bound)
+    assert float((y.double() - ref).norm() / ref.norm()) <= 1e-6  # f32 sums, not bf16 steps
+    _run_backward(20000, 2600, 1500, xd, wd, "f32", "f32", "none", 7)
+    _run_backward(1500, 2600, 20000, xd, wd, "f32", "f32", "none", 8)
 
 
 @pytest.mark.parametrize("xd,wd,yd,dwd", BPAIRS)
