@@ -78,26 +78,23 @@ auto with_elements(int dtype, bool vec, F&& f) {
 // one plane of `dtype`, or the first `planes` bf16 parts.
 __device__ __forceinline__ void store_image8(uint16_t* img, size_t plane, size_t at, int planes, int dtype,
                                              const float (&v)[8]) {
-  uint32_t u[3][4] = {};
+  uint32_t u[4][3] = {};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint16_t h[3] = {};
-    if (planes == 1) {
-      h[0] = dtype == OBJB_DTYPE_F16 ? __half_as_ushort(__float2half_rn(v[i]))
-                                     : __bfloat16_as_ushort(__float2bfloat16_rn(v[i]));
+  for (int i = 0; i < 4; ++i) {
+    if (planes > 1) {
+      split3_pair(v[2 * i], v[2 * i + 1], u[i]);
+    } else if (dtype == OBJB_DTYPE_F16) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      u[i][0] = *reinterpret_cast<const uint32_t*>(&h);
     } else {
-      __nv_bfloat16 b[3];
-      split3(v[i], b);
-#pragma unroll
-      for (int j = 0; j < 3; ++j) h[j] = __bfloat16_as_ushort(b[j]);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      u[i][0] = *reinterpret_cast<const uint32_t*>(&h);
     }
-#pragma unroll
-    for (int j = 0; j < 3; ++j) u[j][i >> 1] |= static_cast<uint32_t>(h[j]) << (16 * (i & 1));
   }
 #pragma unroll
   for (int j = 0; j < 3; ++j)
     if (j < planes)
-      *reinterpret_cast<uint4*>(img + j * plane + at) = make_uint4(u[j][0], u[j][1], u[j][2], u[j][3]);
+      *reinterpret_cast<uint4*>(img + j * plane + at) = make_uint4(u[0][j], u[1][j], u[2][j], u[3][j]);
 }
 
 // Up to two operands laid out for the copy engine in one launch: rows of
@@ -111,13 +108,13 @@ struct ImageJob {
   int cols, pitch, planes, dtype, vec, log_width;
 };
 template <class T, bool VEC>
-__device__ __forceinline__ void image_run(const ImageJob& j) {
+__device__ __forceinline__ void image_run(const ImageJob& j, int block, int blocks) {
   const int width = 1 << j.log_width, per = 256 >> j.log_width;
   const int tx = threadIdx.x & (width - 1), ty = threadIdx.x >> j.log_width;
   const size_t plane = j.rows * static_cast<size_t>(j.pitch);
   const T* src = static_cast<const T*>(j.src);
-  for (long long r = static_cast<long long>(blockIdx.x) * per * 2 + ty; r < j.rows;
-       r += static_cast<long long>(gridDim.x) * per * 2) {
+  for (long long r = static_cast<long long>(block) * per * 2 + ty; r < j.rows;
+       r += static_cast<long long>(blocks) * per * 2) {
     const bool two = r + per < j.rows;
     for (int c = tx * 8; c < j.pitch; c += width * 8) {
       Oct<T, VEC> a, b;
@@ -133,47 +130,66 @@ __device__ __forceinline__ void image_run(const ImageJob& j) {
     }
   }
 }
+__device__ __forceinline__ void image_block(const ImageJob& j, int block, int blocks) {
+  if (j.dtype == OBJB_DTYPE_F32)
+    j.vec ? image_run<float, true>(j, block, blocks) : image_run<float, false>(j, block, blocks);
+  else if (j.dtype == OBJB_DTYPE_BF16)
+    j.vec ? image_run<__nv_bfloat16, true>(j, block, blocks) : image_run<__nv_bfloat16, false>(j, block, blocks);
+  else
+    j.vec ? image_run<__half, true>(j, block, blocks) : image_run<__half, false>(j, block, blocks);
+}
 __global__ void __launch_bounds__(256) image_kernel(const ImageJob first, const ImageJob second) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const ImageJob j = blockIdx.y ? second : first;
-  if (j.dtype == OBJB_DTYPE_F32)
-    j.vec ? image_run<float, true>(j) : image_run<float, false>(j);
-  else if (j.dtype == OBJB_DTYPE_BF16)
-    j.vec ? image_run<__nv_bfloat16, true>(j) : image_run<__nv_bfloat16, false>(j);
-  else
-    j.vec ? image_run<__half, true>(j) : image_run<__half, false>(j);
+  image_block(blockIdx.y ? second : first, blockIdx.x, gridDim.x);
 }
 
 // dz = dy act'(z) as an image (may be null: only its sums), and the column
-// sums of each run of rows.  A block: 256 columns (8 per thread), 8 row lanes
-// with four rows in flight; the lanes are folded in order.
+// sums of each run of rows (of one run: dbias itself).  A block: 256 columns (8
+// per thread), 8 row lanes with four rows in flight; the lanes are folded in
+// order.  The blocks behind dz's lay out the other operands, in the same launch.
+struct DzJob {
+  const void *dy, *z;
+  size_t ldy, ldz;
+  long long rows, rows_per;
+  int N, dtype, act, pitch, planes;
+  int cols, blocks;  // blocks of 256 columns, of all
+  uint16_t* img;
+  float* part;
+  bool add;          // one run: part += the sums
+};
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) dz_kernel(const T* dy, size_t ldy, const T* z, size_t ldz, int dtype, int act,
-                                                 long long rows, int N, uint16_t* img, int pitch, int planes,
-                                                 long long rows_per, float* part) {
+__global__ void __launch_bounds__(256) dz_kernel(const DzJob d, const ImageJob first, const ImageJob second,
+                                                 int image_blocks) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   __shared__ float sm[8][256];
+  if (static_cast<int>(blockIdx.x) >= d.blocks) {
+    const int b = blockIdx.x - d.blocks;
+    image_block(b < image_blocks ? first : second, b < image_blocks ? b : b - image_blocks, image_blocks);
+    return;
+  }
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int c = blockIdx.x * 256 + tx * 8;
-  const long long r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < rows ? r0 + rows_per : rows;
+  const int run = blockIdx.x / d.cols, col0 = (blockIdx.x - run * d.cols) * 256;
+  const int c = col0 + tx * 8, N = d.N, act = d.act;
+  const T *dy = static_cast<const T*>(d.dy), *z = static_cast<const T*>(d.z);
+  const long long r0 = run * d.rows_per, r1 = r0 + d.rows_per < d.rows ? r0 + d.rows_per : d.rows;
   float s[8] = {};
   if (c < N) {
     constexpr int R = sizeof(T) == 4 ? 2 : 4;
     for (long long r = r0 + ty; r < r1; r += 8 * R) {
-      Oct<T, VEC> d[R], a[R];
+      Oct<T, VEC> g[R], a[R];
 #pragma unroll
       for (int q = 0; q < R; ++q)
         if (r + 8 * q < r1) {
-          d[q].load(dy + (r + 8 * q) * ldy + c, N - c);
-          if (act != OBJB_ACT_NONE) a[q].load(z + (r + 8 * q) * ldz + c, N - c);
+          g[q].load(dy + (r + 8 * q) * d.ldy + c, N - c);
+          if (act != OBJB_ACT_NONE) a[q].load(z + (r + 8 * q) * d.ldz + c, N - c);
         }
 #pragma unroll
       for (int q = 0; q < R; ++q)
         if (r + 8 * q < r1) {
           float v[8];
-          d[q].values(v);
+          g[q].values(v);
           if (act != OBJB_ACT_NONE) {
             float zz[8];
             a[q].values(zz);
@@ -190,24 +206,25 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* dy, size_t ldy, const 
               default: break;
             }
           }
-          if (img)
-            store_image8(img, rows * static_cast<size_t>(pitch), (r + 8 * q) * static_cast<size_t>(pitch) + c, planes,
-                         dtype, v);
+          if (d.img)
+            store_image8(d.img, d.rows * static_cast<size_t>(d.pitch),
+                         (r + 8 * q) * static_cast<size_t>(d.pitch) + c, d.planes, d.dtype, v);
 #pragma unroll
           for (int i = 0; i < 8; ++i) s[i] += v[i];
         }
     }
   }
-  if (!part) return;
+  if (!d.part) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sm[ty][tx * 8 + i] = s[i];
   __syncthreads();
-  const int col = blockIdx.x * 256 + threadIdx.x;
+  const int col = col0 + threadIdx.x;
   if (col >= N) return;
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum += sm[i][threadIdx.x];
-  part[static_cast<size_t>(blockIdx.y) * N + col] = sum;
+  float* to = d.part + static_cast<size_t>(run) * N + col;
+  *to = d.add ? *to + sum : sum;
 }
 
 // The runs' sums folded: 32 columns per block, 32 interleaved runs, those in order.
@@ -289,8 +306,7 @@ class Images {
   int launch(const DeviceProps& props, cudaStream_t st) {
     if (!n_) return OBJB_OK;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min(blocks_, static_cast<size_t>(props.sm_count) * 8)),
-                       static_cast<unsigned>(n_));
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks(props)), static_cast<unsigned>(n_));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -298,11 +314,17 @@ class Images {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    n_ = 0;
-    blocks_ = 0;
     OBJB_CUDA(cudaLaunchKernelEx(&cfg, dev::image_kernel, jobs_[0], jobs_[1]), "launch operand image");
+    clear();
     return OBJB_OK;
   }
+  // for a launch that does them beside its own work
+  int count() const { return n_; }
+  int blocks(const DeviceProps& props) const {
+    return n_ ? static_cast<int>(std::min(blocks_, static_cast<size_t>(props.sm_count) * 8)) : 0;
+  }
+  const dev::ImageJob& job(int i) const { return jobs_[i]; }
+  void clear() { n_ = 0, blocks_ = 0; }
 
  private:
   dev::ImageJob jobs_[2] = {};
@@ -324,13 +346,20 @@ int linear_encode(CUtensorMap* map, const Image& im, int box_rows) {
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   });
   if (!fn) return OBJB_FAIL(OBJB_ERR_DRIVER, "dense product", "cuTensorMapEncodeTiled is not available");
-  const cuuint64_t dims[3] = {im.cols, im.rows, static_cast<cuuint64_t>(im.planes)};
-  const cuuint64_t strides[2] = {im.ld * 2, im.rows * im.ld * 2};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(im.planes)};
+  const bool f32 = im.dtype == OBJB_DTYPE_F32;
+  const cuuint32_t planes = f32 ? 1 : im.planes;
+  const size_t pitch = im.ld * (f32 ? 4 : 2);
+  const cuuint64_t dims[3] = {im.cols, im.rows, planes};
+  const cuuint64_t strides[2] = {pitch, im.rows * pitch};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), planes};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r =
-      fn(map, im.dtype == OBJB_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-         const_cast<void*>(im.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      fn(map,
+         f32                             ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+         : im.dtype == OBJB_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+         3, const_cast<void*>(im.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         f32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return OBJB_FAIL(OBJB_ERR_DRIVER, "dense product", "cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
@@ -358,7 +387,7 @@ struct Room {
 // 3000, a fold over a cluster 2200.
 double nanoseconds(const Product& p, TileKind kind, const Tile& t, size_t sms, const Room& room) {
   const size_t cg = kind == kSingle ? 1 : 2, mt = kind == kDirect ? 2 : 1;
-  const bool two = t.ring < kLinRing;
+  const bool two = t.ring == kLinRingTwo;
   const size_t rows = p.gated ? 64 : mt * t.rm;
   const double tiles = static_cast<double>(ceil_div(p.M, rows * cg)) * ceil_div(p.N, t.bn);
   const int log_split = t.split == 1 ? 0 : t.split == 2 ? 1 : t.split == 4 ? 2 : 3;
@@ -374,10 +403,12 @@ double nanoseconds(const Product& p, TileKind kind, const Tile& t, size_t sms, c
     clocks = (pa == 1 ? 3 : pa == 2 ? 5 : 6) * one(t.bn);
   const double mma = 4.0 * clocks / 1.7;
   const double copies = mt * (p.maj == dev::kMajKK && !p.gated ? 1 : 2) +
-                        (p.maj == dev::kMajMN ? ceil_div(t.bn / cg, 64) : 1);
+                        (p.raw ? 0 : p.maj == dev::kMajMN ? ceil_div(t.bn / cg, 64) : 1);
   const double bytes = 128.0 * (p.a.planes * (p.gated ? 128 : mt * t.rm) + p.b.planes * t.bn / cg);
-  const double kb = std::max(std::max(145.0 / t.unit + 35.0 * copies, std::max(mma * share, 150.0 / t.unit + mma / 2)),
-                             bytes / (kind == kSingle ? 125.0 : 90.0) * share);
+  // splitting an f32 operand's rows
+  const double convert = p.raw ? 150.0 / t.unit + 5.0 * ((p.raw == 2 ? t.rm : 0) + t.bn) : 0.0;
+  const double kb = std::max(convert, std::max(std::max(145.0 / t.unit + 35.0 * copies, std::max(mma * share, 150.0 / t.unit + mma / 2)),
+                             bytes / (kind == kSingle ? 125.0 : 90.0) * share));
   const double kbs = std::ceil(static_cast<double>(ceil_div(p.K, 64)) / t.split);
   return std::ceil(tiles / width) * (kbs * kb + (kind == kDirect ? 1500.0 : 1000.0)) + 3000.0 +
          (t.split > 1 ? 2200.0 : 0.0);
@@ -408,13 +439,24 @@ Choice choose_tile(const Product& p, bool y16, size_t sms, const Room& room) {
     const int need = static_cast<int>(std::min<size_t>(most, ceil_div(p.N, step) * step));
     for (int bn = need; bn >= std::min(need, least_bn); bn -= step) f(bn);
   };
-  // rows, and units whose stages leave the ring at least three
+  // rows, and units whose stages leave the ring at least three (two of one k-block)
   auto each_row_unit = [&](TileKind k, Tile c, int cg) {
-    for (c.rm = 128; c.rm >= (rows_free ? 64 : 128); c.rm -= 8)
+    for (c.rm = 128; c.rm >= (rows_free ? 64 : 128); c.rm -= 8) {
+      const size_t kb = 128 * (p.a.planes * (rows_free ? c.rm : 128) + p.b.planes * c.bn / cg) +
+                        (p.raw ? 256 * ((p.raw == 2 ? c.rm : 0) + c.bn) : 0);
       for (c.unit = 1; c.unit <= 4; c.unit *= 2)
-        if (c.unit == 1 || c.unit * 128u * (p.a.planes * 128 + p.b.planes * c.bn / cg) * 3 <= c.ring) consider(k, c);
+        if (kb * c.unit * (c.unit == 1 ? 2 : 3) <= c.ring) consider(k, c);
+    }
   };
   Tile c;
+  if (p.raw) {
+    each_bn(single_columns(p.maj, 3), 16, 16, [&](int bn) {
+      c.bn = bn;
+      for (c.split = 1; c.split <= 8 && nkb >= static_cast<size_t>(c.split); c.split *= 2)
+        each_row_unit(kSingle, c, 1);
+    });
+    return best;
+  }
   if (y16 && p.a.planes == 1 && p.b.planes == 1 && p.K <= dev::kDirectK)
     each_bn(256, mn ? 128 : 16, 144, [&](int bn) {
       c.bn = bn;
@@ -442,7 +484,7 @@ int room_of(int device, size_t sms, Room* out) {
   std::lock_guard<std::mutex> lk(mu);
   auto it = rooms.find(device);
   if (it == rooms.end()) {
-    auto kernel = dev::lin_gemm_kernel<dev::kMajKK, 32, 1, 1, false, true, 1>;
+    auto kernel = dev::lin_gemm_kernel<dev::kMajKK, 32, 1, 1, false, true, 1, 0>;
     Room r;
     for (int two = 0; two < 2; ++two) {
       const size_t smem = (two ? kLinRingTwo : kLinRing) + 1024;
@@ -483,7 +525,7 @@ struct ChoiceKey {
 int gemm(const Product& p, int device, const DeviceProps& props, cudaStream_t st) {
   const bool y16 = !p.gated && p.epi.y_dtype != OBJB_DTYPE_F32;
   const ChoiceKey key{p.M, p.N, p.K, static_cast<size_t>(props.sm_count), p.maj, p.a.planes, p.b.planes,
-                      (y16 ? 1 : 0) | (p.gated ? 2 : 0)};
+                      (y16 ? 1 : 0) | (p.gated ? 2 : 0) | p.raw << 2};
   struct Kept {
     ChoiceKey key{};
     Choice choice;
@@ -585,14 +627,49 @@ int check_backward(const char* action, const objb_linear_backward_desc* d) {
   return OBJB_OK;
 }
 
+// Which products split their f32 operands themselves (RAW: no launch before, no
+// scratch, an f32 w read once), where the copy engine can read them as they lie.
+// Every row tile splits x anew and every column tile w, so it pays
+//   * for an f32 w of one narrow column tile (16384 x 4096, 16 tokens: 98 us,
+//     laid out first 182; 64 tokens 180 and 187; 128 tokens 326 and 193);
+//   * for results so small that the launch saved counts (250 tokens by 256 of
+//     2048: 14.1 us a call, laid out first 15.7, launches bound; 512 tokens 18.6
+//     and 15.7).  A column tile has 16 columns at least (bf16 w of 16384 x 4096,
+//     one token: 30.8 and 27.8 us).
+bool raw_pays(size_t T, size_t N, bool w_f32) {
+  return (w_f32 && T <= 32) || std::max<size_t>(T, 16) * N <= (size_t{1} << 16);
+}
+// The same for the gated product (4096 x 2048, 16 tokens: 25.9 and 26.7 us with
+// the down product and one launch less, 64 tokens 35.6 and 31.7).
+constexpr size_t kRawTokensFfn = 16;
+
+bool raw_fits(const void* p, size_t ld) { return aligned16(p) && ld % 4 == 0; }
+Image raw_image(const void* p, size_t ld, size_t rows, size_t cols) {
+  Image im;
+  im.p = p;
+  im.ld = ld;
+  im.rows = rows;
+  im.cols = cols;
+  im.planes = 3;
+  im.dtype = OBJB_DTYPE_F32;
+  return im;
+}
+
 struct LinearPlan {
   ImagePlan x, w;
+  int raw = 0;
   size_t total;
 };
 LinearPlan plan_linear(const objb_linear_desc& d, size_t ldx, size_t ldw, const void* x, const void* w) {
   LinearPlan p;
   p.x = plan_image(x, d.x_dtype, ldx, d.tokens, d.in_features, d.x_dtype == OBJB_DTYPE_F32 ? 3 : 1);
   p.w = plan_image(w, d.w_dtype, ldw, d.out_features, d.in_features, d.w_dtype == OBJB_DTYPE_F32 ? 3 : 1);
+  if (d.x_dtype == OBJB_DTYPE_F32 && raw_pays(d.tokens, d.out_features, d.w_dtype == OBJB_DTYPE_F32) &&
+      raw_fits(x, ldx) && (d.w_dtype != OBJB_DTYPE_F32 || raw_fits(w, ldw))) {
+    p.raw = d.w_dtype == OBJB_DTYPE_F32 ? 2 : 1;
+    p.x.bytes = 0;
+    if (p.raw == 2) p.w.bytes = 0;
+  }
   p.total = p.x.bytes + p.w.bytes;
   return p;
 }
@@ -624,27 +701,32 @@ BackwardPlan plan_backward(const objb_linear_backward_desc& d, size_t lddy, size
   p.w = plan_image(w, d.w_dtype, ldw, d.out_features, d.in_features, planes(d.w_dtype));
   if (!p.want_dw) p.x.bytes = 0;
   if (!p.want_dx) p.w.bytes = 0;
-  // runs of rows of the column sums: enough blocks to fill the SMs, 32 rows or more in each
+  // runs of rows of the column sums: enough blocks to fill the SMs, 32 rows or more in each; up to 256 rows are one
+  // run, whose sums need no folding launch
   const size_t cols = (d.out_features + 255) / 256;
   const size_t want = std::max<size_t>(1, (static_cast<size_t>(sms) * 4 + cols - 1) / cols);
-  p.parts = static_cast<int>(std::max<size_t>(1, std::min(want, (d.tokens + 31) / 32)));
+  p.parts = d.tokens <= 256 ? 1 : static_cast<int>(std::max<size_t>(1, std::min(want, (d.tokens + 31) / 32)));
   p.rows_per = static_cast<long long>((d.tokens + p.parts - 1) / p.parts);
-  p.part_bytes = p.want_db ? r256(static_cast<size_t>(p.parts) * d.out_features * 4) : 0;
+  p.part_bytes = p.want_db && p.parts > 1 ? r256(static_cast<size_t>(p.parts) * d.out_features * 4) : 0;
   p.total = p.x.bytes + p.w.bytes + p.dz.bytes + p.part_bytes;
   return p;
 }
 
 struct FfnPlan {
   ImagePlan gate, up, down, x, act;
+  bool raw;
   size_t total;
 };
-FfnPlan plan_ffn(size_t T, size_t H, size_t I, size_t O, const void* gate, const void* up, const void* down) {
+FfnPlan plan_ffn(size_t T, size_t H, size_t I, size_t O, const void* gate, const void* up, const void* down,
+                 const void* x) {
   FfnPlan p;
+  p.raw = T <= kRawTokensFfn && x && raw_fits(x, H);
   p.gate = plan_image(gate, OBJB_DTYPE_BF16, H, I, H, 1);
   p.up = plan_image(up, OBJB_DTYPE_BF16, H, I, H, 1);
   p.down = plan_image(down, OBJB_DTYPE_BF16, I, O, I, 1);
   p.x = plan_image(nullptr, OBJB_DTYPE_F32, H, T, H, 3);
   p.act = plan_image(nullptr, OBJB_DTYPE_F32, I, T, I, 3);
+  if (p.raw) p.x.bytes = 0;
   p.total = p.gate.bytes + p.up.bytes + p.down.bytes + p.x.bytes + p.act.bytes;
   return p;
 }
@@ -697,8 +779,17 @@ int objb_linear_device(const objb_linear_desc* desc, const void* d_x, const void
   OBJB_TRY(take_scratch(action, d_scratch, scratch_bytes, pl.total, st, &ws));
   Product p;
   Images images;
-  p.a = images.take(pl.w, d_w, d.w_dtype, ldw, d.out_features, d.in_features, ws);
-  p.b = images.take(pl.x, d_x, d.x_dtype, ldx, d.tokens, d.in_features, ws + pl.w.bytes);
+  p.raw = pl.raw;
+  if (pl.raw == 2) {
+    p.a = raw_image(d_w, ldw, d.out_features, d.in_features);
+  } else {
+    p.a = images.take(pl.w, d_w, d.w_dtype, ldw, d.out_features, d.in_features, ws);
+  }
+  if (pl.raw) {
+    p.b = raw_image(d_x, ldx, d.tokens, d.in_features);
+  } else {
+    p.b = images.take(pl.x, d_x, d.x_dtype, ldx, d.tokens, d.in_features, ws + pl.w.bytes);
+  }
   OBJB_TRY(images.launch(props, st));
   p.M = d.out_features;
   p.N = d.tokens;
@@ -783,36 +874,39 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
   dz.planes = pl.dz.planes;
   dz.dtype = pl.dz.planes > 1 ? OBJB_DTYPE_BF16 : d.dy_dtype;
   const bool image = products && !pl.dz_direct;
-  if (image || want_db) {
-    const bool vec = aligned16(d_dy) && lddy % 8 == 0 && N % 8 == 0 && (!pl.has_act || (aligned16(d_z) && ldz % 8 == 0));
-    float* part = want_db ? reinterpret_cast<float*>(ws_part) : nullptr;
-    OBJB_TRY(dev::with_elements(d.dy_dtype, vec, [&](auto elem, auto v) -> int {
-      using T = decltype(elem);
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((N + 255) / 256, pl.parts);
-      cfg.blockDim = dim3(256);
-      cfg.stream = st;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attr[0].val.programmaticStreamSerializationAllowed = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      OBJB_CUDA(cudaLaunchKernelEx(&cfg, dev::dz_kernel<T, decltype(v)::value>, static_cast<const T*>(d_dy), lddy,
-                                   static_cast<const T*>(d_z), ldz, static_cast<int>(d.dy_dtype),
-                                   static_cast<int>(d.activation), static_cast<long long>(d.tokens), N,
-                                   image ? reinterpret_cast<uint16_t*>(ws_dz) : nullptr,
-                                   static_cast<int>(pl.dz.pitch), pl.dz.planes, pl.rows_per, part),
-                "launch dz");
-      return OBJB_OK;
-    }));
-    if (want_db)
-      OBJB_TRY(launch_pdl(dev::dbias_kernel, (N + 31) / 32, 1024, 0, st, static_cast<const float*>(part), pl.parts, N,
-                          d_dbias, static_cast<int>(d.accumulate)));
-  }
   Images images;
   Image w, x;
   if (want_dx) w = images.take(pl.w, d_w, d.w_dtype, ldw, d.out_features, d.in_features, ws_w);
   if (want_dw) x = images.take(pl.x, d_x, d.x_dtype, ldx, d.tokens, d.in_features, ws_x);
+  if (image || want_db) {
+    dev::DzJob j;
+    j.dy = d_dy;
+    j.z = d_z;
+    j.ldy = lddy;
+    j.ldz = ldz;
+    j.rows = static_cast<long long>(d.tokens);
+    j.rows_per = pl.rows_per;
+    j.N = N;
+    j.dtype = d.dy_dtype;
+    j.act = d.activation;
+    j.pitch = static_cast<int>(pl.dz.pitch);
+    j.planes = pl.dz.planes;
+    j.cols = (N + 255) / 256;
+    j.blocks = j.cols * pl.parts;
+    j.img = image ? reinterpret_cast<uint16_t*>(ws_dz) : nullptr;
+    j.part = !want_db ? nullptr : pl.parts > 1 ? reinterpret_cast<float*>(ws_part) : d_dbias;
+    j.add = pl.parts == 1 && d.accumulate;
+    const bool vec = aligned16(d_dy) && lddy % 8 == 0 && N % 8 == 0 && (!pl.has_act || (aligned16(d_z) && ldz % 8 == 0));
+    const int image_blocks = images.blocks(props);
+    OBJB_TRY(dev::with_elements(d.dy_dtype, vec, [&](auto elem, auto v) -> int {
+      return launch_pdl(dev::dz_kernel<decltype(elem), decltype(v)::value>, j.blocks + images.count() * image_blocks, 256,
+                        0, st, j, images.job(0), images.job(1), image_blocks);
+    }));
+    images.clear();
+    if (want_db && pl.parts > 1)
+      OBJB_TRY(launch_pdl(dev::dbias_kernel, (N + 31) / 32, 1024, 0, st, static_cast<const float*>(j.part), pl.parts, N,
+                          d_dbias, static_cast<int>(d.accumulate)));
+  }
   OBJB_TRY(images.launch(props, st));
   if (want_dx) {
     Product p;
@@ -855,7 +949,8 @@ int objb_ffn_bf16_tokens_scratch_bytes(const void* d_gate, const void* d_up, con
   const char* action = "objb_ffn_bf16_tokens_scratch_bytes";
   OBJB_TRY(check_ffn(action, num_tokens, hidden, intermediate, out_dim));
   if (!bytes) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null output pointer");
-  *bytes = plan_ffn(num_tokens, hidden, intermediate, out_dim, d_gate, d_up, d_down).total;
+  // (x is not named here: room for its planes in any case)
+  *bytes = plan_ffn(num_tokens, hidden, intermediate, out_dim, d_gate, d_up, d_down, nullptr).total;
   return OBJB_OK;
 }
 
@@ -873,7 +968,7 @@ int objb_ffn_bf16_tokens_device(const void* d_gate, const void* d_up, const void
   DeviceProps props;
   OBJB_TRY(device_here(&device, &props));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const FfnPlan pl = plan_ffn(num_tokens, hidden, intermediate, out_dim, d_gate, d_up, d_down);
+  const FfnPlan pl = plan_ffn(num_tokens, hidden, intermediate, out_dim, d_gate, d_up, d_down, d_x);
   uint8_t* ws = nullptr;
   OBJB_TRY(take_scratch(action, d_scratch, scratch_bytes, pl.total, st, &ws));
   const int bf = OBJB_DTYPE_BF16;
@@ -888,8 +983,15 @@ int objb_ffn_bf16_tokens_device(const void* d_gate, const void* d_up, const void
   Product dn;
   dn.a = images.take(pl.down, d_down, bf, intermediate, out_dim, intermediate, ws);
   ws += pl.down.bytes;
-  gu.b = images.take(pl.x, d_x, OBJB_DTYPE_F32, hidden, num_tokens, hidden, ws);
-  ws += pl.x.bytes;
+  if (pl.raw) {
+    gu.raw = 1;
+    gu.b = raw_image(d_x, hidden, num_tokens, hidden);
+    // the down weights come while the gated product ends and the next one starts (26.2 -> 25.5 us at 4096 x 2048)
+    if (pl.down.direct) gu.ahead = d_down, gu.ahead_bytes = out_dim * intermediate * 2;
+  } else {
+    gu.b = images.take(pl.x, d_x, OBJB_DTYPE_F32, hidden, num_tokens, hidden, ws);
+    ws += pl.x.bytes;
+  }
   OBJB_TRY(images.launch(props, st));
   gu.M = intermediate;
   gu.N = num_tokens;

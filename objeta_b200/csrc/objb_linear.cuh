@@ -93,6 +93,22 @@ __device__ __forceinline__ void split3(float v, __nv_bfloat16 (&p)[3]) {
   p[2] = __float2bfloat16_rn(r - b);
 }
 
+// The same of two neighbours, part j of both in u[j] (v0 in its lower half).  By
+// byte permutations: the conversion to bf16 takes four times an add's slots.
+__device__ __forceinline__ void split3_pair(float v0, float v1, uint32_t (&u)[3]) {
+  auto rest = [](float v) {  // v without its upper half; 0 for a non-finite v
+    const float r = v - __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
+    return r == r ? r : 0.0f;
+  };
+  auto upper = [](float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); };
+  u[0] = upper(v0 == v0 ? v0 : __int_as_float(0x7FFFFFFF), v1 == v1 ? v1 : __int_as_float(0x7FFFFFFF));
+  v0 = rest(v0), v1 = rest(v1);
+  u[1] = upper(v0, v1);
+  v0 -= __uint_as_float(__float_as_uint(v0) & 0xFFFF0000u);
+  v1 -= __uint_as_float(__float_as_uint(v1) & 0xFFFF0000u);
+  u[2] = upper(v0, v1);
+}
+
 // What happens to the product's element (row m of A, row n of B), whose place
 // in y, z and residual is [n][m]: + bias[m] -> z -> act -> + residual -> y.
 struct LinearEpilogue {

@@ -41,6 +41,11 @@
 //   * Few tiles (CG 1): `split` CTAs of a cluster share a tile's k-blocks and
 //     fold their partial tiles through distributed shared memory in rank
 //     order: one launch, no atomics, no scratch.
+//   * RAW: an f32 operand of few tokens is not laid out in planes by a launch
+//     of its own: a second producer copies it as it lies, eight more warps
+//     split it into the planes of the stages (RAW 1: B; 2: both).  (Copies by
+//     the splitting warps themselves, into registers or shared memory, cost
+//     a memory latency per k-block: the proxy fence waits for them.)
 //   * GATED: A is 64 rows of the gate and the same 64 rows of up; the epilogue
 //     pairs lanes i and i + 64 through shared memory.
 #pragma once
@@ -61,8 +66,10 @@ constexpr int kLinBK = 64;        // k of a stage: 128 bytes, one swizzle row
 constexpr int kLinStagesMax = 12;
 constexpr int kCrossChunks = 16;  // chunks of a cross product's buffer
 constexpr size_t kDirectK = 65536;  // 4096 MMAs in one accumulator lose 1.2e-4 of a sum of one sign: half of f16's rounding
-// producer, MMA, eight (PROMOTE) or sixteen epilogue warps, second MMA warp
-constexpr int lin_threads(bool promote) { return promote ? 352 : 608; }
+constexpr int kConvWarps = 8;
+// producer, MMA, eight (PROMOTE) or sixteen epilogue warps, second MMA warp (RAW: producer of raw k-blocks), RAW: the
+// converting warps
+constexpr int lin_threads(bool promote, bool raw = false) { return promote ? 352 + (raw ? 32 * kConvWarps : 0) : 608; }
 
 struct GemmArgs {
   int M;                  // rows of A (GATED: features)
@@ -75,11 +82,34 @@ struct GemmArgs {
   int split;              // CTAs of a cluster per tile (CG 1)
   int chunk_kb;           // k-blocks per accumulator chunk, a multiple of unit
   int nstages, unit;      // stages of `unit` k-blocks
+  int conv_groups;        // RAW: groups of converting warps, which take the stages in turn; divides nstages
   uint32_t idesc;
   float swiglu_limit;
   unsigned* err;
   LinearEpilogue epi;
+  const uint8_t* ahead;  // bytes that the next product reads, brought into L2 behind this one's own (16-byte
+  size_t ahead_bytes;    // aligned, whole 16-byte quads); may be null
 };
+
+// An oct of 8 f32, and its three planes, `plane` bytes apart.
+__device__ __forceinline__ void raw_take(uint32_t from, float (&v)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v[4 * h]), "=f"(v[4 * h + 1]), "=f"(v[4 * h + 2]), "=f"(v[4 * h + 3])
+                 : "r"(from + h * 16)
+                 : "memory");
+}
+__device__ __forceinline__ void raw_split(const float (&v)[8], uint32_t to, uint32_t plane) {
+  uint32_t u[4][3];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split3_pair(v[2 * i], v[2 * i + 1], u[i]);
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + j * plane), "r"(u[0][j]), "r"(u[1][j]),
+                 "r"(u[2][j]), "r"(u[3][j])
+                 : "memory");
+}
 
 // SWIZZLE_128B operand tiles, without their address.  K-major: rows of 128
 // bytes, 8-row groups 1024 bytes apart.  MN-major: 64 rows x 64 k as 64 k rows
@@ -190,29 +220,30 @@ __device__ __forceinline__ void lin_tile(const GemmArgs& g, int t, int* tm, int*
 }
 
 // BN: columns of a tile at most; PB: planes of B.
-template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE, int PB>
+template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE, int PB, int RAW>
 struct LinShape {
   static constexpr bool kWideB = CG == 1 && PB > 1;         // planes side by side in N
   static constexpr int kSet = MT * BN * (kWideB ? PB : 1);  // accumulator columns of one set
   static constexpr int kUsed = PROMOTE ? (CG == 2 && PB > 1 ? 4 : 2) * kSet : kSet;
   static constexpr int pow2(int v) { return v <= 32 ? 32 : v <= 64 ? 64 : v <= 128 ? 128 : v <= 256 ? 256 : 512; }
   static constexpr int kCols = pow2(kUsed);
-  static constexpr int kThreads = lin_threads(PROMOTE);
+  static constexpr int kThreads = lin_threads(PROMOTE, RAW != 0);
   static constexpr bool kCross = PROMOTE && CG == 2 && PB > 1;  // cross products in their own accumulators
   static constexpr bool kTwoIssue = !PROMOTE || kCross;         // a second warp issues MMAs
-  static constexpr int kBlocks = PROMOTE && CG == 1 && BN <= 64 && kCols <= 256 ? 2 : 1;  // CTAs an SM has room for
+  static constexpr int kBlocks = PROMOTE && CG == 1 && BN <= 64 && kCols <= 256 && !RAW ? 2 : 1;  // CTAs an SM has room for
   static_assert(kUsed <= 512, "tensor memory columns");
   static_assert(!GATED || (MAJ == kMajKK && MT == 1 && PROMOTE), "gated products are K-major, one accumulator");
+  static_assert(!RAW || (MAJ == kMajKK && CG == 1 && PROMOTE && PB == 3 && !(GATED && RAW == 2)), "raw operands");
   static_assert(!(kWideB && MAJ == kMajMN) || BN < 128, "planes side by side of one 64-row chunk");
   static_assert(PROMOTE ? MT == 1 : CG == 2 && MT == 2 && PB == 1, "one promoted accumulator, or a pair of two direct ones");
 };
 
-template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE, int PB>
-__global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>::kThreads,
-                                  LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>::kBlocks)
+template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE, int PB, int RAW>
+__global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, RAW>::kThreads,
+                                  LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, RAW>::kBlocks)
     lin_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a2,
                     const __grid_constant__ CUtensorMap map_b, const GemmArgs g) {
-  using SH = LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>;
+  using SH = LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, RAW>;
   constexpr bool A_MN = MAJ != kMajKK, B_MN = MAJ == kMajMN;
   constexpr int kWarps = PROMOTE ? 8 : 16;        // epilogue warps
   constexpr int HN = MT * BN * 4 / kWarps;        // columns of each
@@ -223,6 +254,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
 
   extern __shared__ uint8_t lin_smem[];
   __shared__ alignas(8) uint64_t full[kLinStagesMax], empty[kLinStagesMax], t_full[2], t_empty[2], c_full[2], c_empty[2];
+  __shared__ alignas(8) uint64_t raw_full[RAW ? kLinStagesMax : 1], raw_empty[RAW ? kLinStagesMax : 1];
   __shared__ uint32_t s_tmem;
   __shared__ unsigned s_abort;
   uint8_t* stages = lin_smem + ((1024u - (smem_u32(lin_smem) & 1023u)) & 1023u);
@@ -231,7 +263,9 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
   const int csize = CG == 2 ? 2 : g.split;
 
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < g.nstages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], SH::kTwoIssue ? 2 : 1);
+    for (int i = 0; i < g.nstages; ++i) mbar_init(&full[i], (RAW < 2 ? 1 : 0) + (RAW ? kConvWarps / g.conv_groups : 0)), mbar_init(&empty[i], SH::kTwoIssue ? 2 : 1);
+    if (RAW)
+      for (int i = 0; i < g.nstages; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], kConvWarps / g.conv_groups);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&t_full[i], 1);
       mbar_init(&t_empty[i], 8 * CG);  // PROMOTE: all epilogue warps; else the eight of accumulator i
@@ -266,12 +300,14 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
   const uint32_t a_plane = A_MN || GATED ? 8192 : g.rm * 128, b_plane = B_MN ? 8192 : b_rows * 128;
   const uint32_t a_acc = g.pa * (A_MN || GATED ? 16384 : a_plane);
   const uint32_t b_at = MT * a_acc, kb_bytes = b_at + PB * b_rows * 128, stage_bytes = g.unit * kb_bytes;
+  const uint32_t raw_kb_bytes = ((RAW == 2 ? g.rm : 0) + b_rows) * 256;  // behind the stages
+  const uint32_t raw_at = smem_u32(stages) + g.nstages * stage_bytes;
   // first row of A of this CTA's part of tile row tm
   const int cta_rows = GATED ? 64 : MT * g.rm;
   auto row0 = [&](int tm) { return (tm * CG + (CG == 2 ? static_cast<int>(rank) : 0)) * cta_rows; };
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (lane == 0 && RAW < 2) {
       // ---- producer
       int issued = 0, st = 0;
       uint32_t phase = 1;  // of empty[st]: the first round finds every stage free
@@ -288,7 +324,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
           }
           uint32_t bar = smem_u32(&full[st]);
           const int n = kb1 - kb < g.unit ? kb1 - kb : g.unit;
-          if (rank == 0 || CG == 1) mbar_arrive_expect_tx(&full[st], CG * n * kb_bytes);
+          if (rank == 0 || CG == 1) mbar_arrive_expect_tx(&full[st], CG * n * (RAW ? b_at : kb_bytes));
           if (CG == 2) bar = lin_mapa(bar, 0);
           uint32_t dst = smem_u32(stages) + st * stage_bytes;
           for (const int end = kb + n; kb < end; ++kb, dst += kb_bytes) {
@@ -305,7 +341,8 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
                 lin_tma<CG>(to, &map_a, kb * 64, m0 + a * g.rm, 0, bar);
               }
             }
-            if constexpr (B_MN) {
+            if constexpr (RAW != 0) {
+            } else if constexpr (B_MN) {
               for (uint32_t c = 0; c < b_rows; c += 64)
                 lin_tma<CG>(dst + b_at + c * 128 * PB, &map_b, n0 + c, kb * 64, 0, bar);
             } else {
@@ -319,11 +356,102 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>:
       if (*reinterpret_cast<volatile unsigned*>(&s_abort)) {
         // a wait ran out: let the copies in flight land before shared memory goes
         for (int i = issued > g.nstages ? issued - g.nstages : 0; i < issued && (CG == 1 || rank == 0); ++i)
-          mbar_wait_bounded(&full[i % g.nstages], (i / g.nstages) & 1, g.err, kErrDrainTimeout);
+          if (!mbar_wait_bounded(&full[i % g.nstages], (i / g.nstages) & 1, g.err, kErrDrainTimeout)) break;
+      }
+      if (g.ahead) {
+        constexpr uint32_t kPiece = 4096;
+        for (size_t at = static_cast<size_t>(blockIdx.x) * kPiece; at < g.ahead_bytes; at += gridDim.x * size_t{kPiece}) {
+          const uint32_t n = g.ahead_bytes - at < kPiece ? static_cast<uint32_t>(g.ahead_bytes - at) : kPiece;
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(g.ahead + at), "r"(n) : "memory");
+        }
       }
     }
     __syncwarp();
-  } else if (warp == 1 || warp == SH::kThreads / 32 - 1) {
+  } else if (RAW && warp == 10) {
+    if (lane == 0) {
+      // ---- producer of raw k-blocks: A's rows (RAW 2), then B's, 256 bytes each
+      int issued = 0, st = 0;
+      uint32_t phase = 1;
+      bool ok = true;
+      for (int t = first; t < ntiles && ok; t += step) {
+        int tm, tn;
+        lin_tile(g, t, &tm, &tn);
+        for (int kb = kb0; kb < kb1;) {
+          if (!mbar_wait_bounded(&raw_empty[st], phase, g.err, kErrEmptyWaitTimeout, &s_abort)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = smem_u32(&raw_full[st]);
+          const int n = kb1 - kb < g.unit ? kb1 - kb : g.unit;
+          mbar_arrive_expect_tx(&raw_full[st], n * raw_kb_bytes);
+          uint32_t dst = raw_at + st * g.unit * raw_kb_bytes;
+          for (const int end = kb + n; kb < end; ++kb, dst += raw_kb_bytes) {
+            if (RAW == 2) lin_tma<1>(dst, &map_a, kb * 64, row0(tm), 0, bar);
+            lin_tma<1>(dst + (RAW == 2 ? g.rm * 256 : 0), &map_b, kb * 64, tn * g.bn, 0, bar);
+          }
+          ++issued;
+          if (++st == g.nstages) st = 0, phase ^= 1;
+        }
+      }
+      if (*reinterpret_cast<volatile unsigned*>(&s_abort))
+        for (int i = issued > g.nstages ? issued - g.nstages : 0; i < issued; ++i)
+          mbar_wait_bounded(&raw_full[i % g.nstages], (i / g.nstages) & 1, g.err, kErrDrainTimeout);
+    }
+    __syncwarp();
+  } else if (RAW && warp > 10) {
+    // ---- converter: the octs of 8 elements of every conv_groups-th stage, a
+    // thread's kConvGroup at a time.  A stage takes about 0.6 us from its
+    // arrival on (waits, splitting, proxy fence), whatever its size: so several
+    // are under way at once.
+    constexpr int kConvGroup = 4;
+    const int kThreads = 32 * kConvWarps / g.conv_groups;
+    const int tid = (threadIdx.x - 352) & (kThreads - 1);
+    const int a_octs = RAW == 2 ? g.rm * 8 : 0, octs = a_octs + static_cast<int>(b_rows) * 8;
+    const int at0 = tid / octs, oct0 = tid - at0 * octs;
+    int st = 0, turn = (threadIdx.x - 352) / kThreads;  // stages until this group's next
+    uint32_t phase = 0;                                 // of raw_full[st]
+    bool ok = true;
+    for (int t = first; t < ntiles && ok; t += step)
+      for (int kb = kb0; kb < kb1; kb += g.unit) {
+        if (turn-- > 0) {
+          if (++st == g.nstages) st = 0, phase ^= 1;
+          continue;
+        }
+        turn = g.conv_groups - 1;
+        if (!lin_wait(&raw_full[st], phase, g.err, kErrFullWaitTimeout, &s_abort) ||
+            !lin_wait(&empty[st], phase ^ 1, g.err, kErrEmptyWaitTimeout, &s_abort)) {
+          ok = false;
+          break;
+        }
+        const int n = kb1 - kb < g.unit ? kb1 - kb : g.unit;
+        const uint32_t from = raw_at + st * g.unit * raw_kb_bytes, to = smem_u32(stages) + st * stage_bytes;
+        int at = at0, oct = oct0;  // this thread's next oct: k-block of the stage, place in it
+        while (at < n) {
+          float v[kConvGroup][8];
+          uint32_t dst[kConvGroup], plane[kConvGroup];
+          bool have[kConvGroup];
+#pragma unroll
+          for (int u = 0; u < kConvGroup; ++u) {
+            have[u] = at < n;
+            if (!have[u]) continue;
+            raw_take(from + at * raw_kb_bytes + oct * 32, v[u]);
+            const bool of_a = oct < a_octs;
+            const int i = of_a ? oct : oct - a_octs, r = i >> 3;
+            dst[u] = to + at * kb_bytes + (of_a ? 0 : b_at) + r * 128 + (((i ^ r) & 7) << 4);
+            plane[u] = of_a ? a_plane : b_plane;
+            oct += kThreads;
+            while (oct >= octs) oct -= octs, ++at;
+          }
+#pragma unroll
+          for (int u = 0; u < kConvGroup; ++u)
+            if (have[u]) raw_split(v[u], dst[u], plane[u]);
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]), mbar_arrive(&raw_empty[st]);
+        if (++st == g.nstages) st = 0, phase ^= 1;
+      }
+  } else if (warp == 1 || (!RAW && warp == SH::kThreads / 32 - 1)) {
     const int role = warp == 1 ? 0 : 1;
     if ((CG == 1 || rank == 0) && (role == 0 || SH::kTwoIssue)) {
       // ---- MMA issue.  The tensor core takes an MMA when the one before it is

@@ -16,12 +16,13 @@
 namespace objb {
 
 // A 16-bit matrix as the copy engine reads it: 16-byte aligned, rows of `ld`
-// elements (a multiple of 8), `planes` of them `rows * ld` apart.
+// elements (a multiple of 8), `planes` of them `rows * ld` apart; or an f32 one
+// as it lies (OBJB_DTYPE_F32, `planes` those it is split into).
 struct Image {
   const void* p = nullptr;
   size_t ld = 0, rows = 0, cols = 0;
   int planes = 1;
-  int dtype = 0;  // OBJB_DTYPE_BF16 or F16
+  int dtype = 0;  // OBJB_DTYPE_*
 };
 
 // The tensor map of an image: box of 64 elements by `box_rows` rows, all planes.
@@ -31,6 +32,9 @@ int linear_encode(CUtensorMap* map, const Image& im, int box_rows);
 struct Product {
   int maj = dev::kMajKK;
   Image a, a2, b;
+  int raw = 0;  // 1: b is f32 as it lies (three planes in the stages), 2: a too
+  const void* ahead = nullptr;  // what the next product reads
+  size_t ahead_bytes = 0;
   bool gated = false;
   size_t M = 0, N = 0, K = 0;
   dev::LinearEpilogue epi;
@@ -51,9 +55,9 @@ struct Tile {
 
 enum TileKind { kDirect, kPair, kSingle };
 
-template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE, int PB>
+template <int MAJ, int BN, int CG, int MT, bool GATED, bool PROMOTE, int PB, int RAW = 0>
 int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProps& props, cudaStream_t st) {
-  using SH = dev::LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB>;
+  using SH = dev::LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, RAW>;
   dev::GemmArgs g;
   g.M = static_cast<int>(p.M);
   g.N = static_cast<long long>(p.N);
@@ -65,6 +69,8 @@ int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProp
   g.chunk_kb = PROMOTE ? tile.chunk_kb : g.nkb;
   g.swiglu_limit = p.swiglu_limit;
   g.epi = p.epi;
+  g.ahead = static_cast<const uint8_t*>(p.ahead);
+  g.ahead_bytes = p.ahead_bytes;
   OBJB_TRY(device_error_word(device, &g.err));
   const size_t mt = static_cast<size_t>(GATED ? 64 : MT * tile.rm) * CG;
   g.tiles_m = static_cast<int>((p.M + mt - 1) / mt);
@@ -72,8 +78,13 @@ int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProp
   const size_t a_rows = static_cast<size_t>(MT) * (MAJ != dev::kMajKK || GATED ? 128 : tile.rm);
   g.unit = PROMOTE ? tile.unit : 1;
   const size_t stage = g.unit * 128 * (g.pa * a_rows + static_cast<size_t>(PB) * (tile.bn / CG));
-  g.nstages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(dev::kLinStagesMax, tile.ring / stage)));
-  size_t smem = g.nstages * stage;
+  const size_t raw = RAW ? g.unit * 256 * ((RAW == 2 ? tile.rm : 0) + static_cast<size_t>(tile.bn)) : 0;
+  g.nstages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(dev::kLinStagesMax, tile.ring / (stage + raw))));
+  // A group keeps to its own stages (a wait for a phase that is not the next one of its barrier falls through), so
+  // that they are a multiple of the groups.
+  g.conv_groups = g.nstages >= dev::kConvWarps ? dev::kConvWarps : g.nstages >= 4 ? 4 : 2;
+  if (RAW) g.nstages -= g.nstages % g.conv_groups;
+  size_t smem = g.nstages * (stage + raw);
   if (GATED || tile.split > 1) smem = std::max(smem, static_cast<size_t>(tile.bn) * 512);  // the partial tile
   smem += 1024 + (128 - tile.rm) * 128;  // an MMA reads 128 rows, those past rm for nothing
   const uint32_t half = p.a.dtype == OBJB_DTYPE_F16 ? 0 : 1;
@@ -87,12 +98,12 @@ int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProp
   else
     ma2 = ma;
   OBJB_TRY(linear_encode(&mb, p.b, MAJ == dev::kMajMN ? 64 : tile.bn / CG));
-  auto kernel = dev::lin_gemm_kernel<MAJ, BN, CG, MT, GATED, PROMOTE, PB>;
+  auto kernel = dev::lin_gemm_kernel<MAJ, BN, CG, MT, GATED, PROMOTE, PB, RAW>;
   OBJB_TRY(ensure_smem_attr(kernel, device, smem));
   const long long tiles = static_cast<long long>(g.tiles_m) * g.tiles_n;
   const int csize = CG == 2 ? 2 : tile.split;
   const bool one_each = GATED || tile.split > 1;
-  const long long at_once = static_cast<long long>(props.sm_count) * (tile.ring < kLinRing ? 2 : 1) / csize;
+  const long long at_once = static_cast<long long>(props.sm_count) * (tile.ring == kLinRingTwo ? 2 : 1) / csize;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((one_each ? tiles : std::min(tiles, at_once)) * csize));
   cfg.blockDim = dim3(SH::kThreads);

@@ -118,6 +118,22 @@ def test_linear_f32_keeps_f32(cuda_device, wd):
     assert rel <= 1e-6, rel
 
 
+@pytest.mark.parametrize("xd,wd,T,K,N", [("f32", "f32", 17, 136, 40000), ("f32", "f32", 32, 5000, 3000),
+                                         ("f32", "f32", 1, 68, 20001), ("f32", "bf16", 1, 8200, 4000),
+                                         ("f32", "bf16", 1000, 136, 65), ("f32", "f32", 100, 260, 600)])
+def test_linear_few_f32_tokens(cuda_device, xd, wd, T, K, N):
+    """f32 operands that the product splits itself: more tiles than the grid holds at once, many k-blocks, ragged
+    ends; rows that the copy engine cannot read give the same."""
+    from objeta_b200.dense import linear
+    x, w = _case(T, K, N, xd, wd, 5)
+    b, r = U.randn((N,), torch.float32, seed=8), U.randn((T, N), seed=9)
+    y = linear(x, w, b, activation="silu", d_residual=r)
+    _, _, ref, bound = U.linear_ref(x, w, b, "silu", r, torch.float32)
+    U.check(y, ref, bound, "y")
+    U.check(linear(U.strided(x, 3, 1), U.strided(w, 5, 1), b, activation="silu", d_residual=r), ref, bound, "strided")
+    U.check(linear(U.strided(x, 4, 4), U.strided(w, 8, 8), b, activation="silu", d_residual=r), ref, bound, "aligned")
+
+
 def test_linear_non_finite(cuda_device):
     """Inf and NaN reach their row (x) or column (w) of y and no other."""
     from objeta_b200.dense import linear
