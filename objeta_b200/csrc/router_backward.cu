@@ -102,29 +102,32 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
           float dd;
           return FUNC == kSoftmax ? exp_sfu(le - base) * inv : score_of(FUNC, le, &dd);
         };
-        float c = a.route_scale, mean = 0.0f;
+        float c = a.route_scale, mean = 0.0f, rest = 0.0f;
         if (a.renorm) {
-          float Q = 0.0f, GQ = 0.0f;
-          if (id0 >= 0) {
-            Q = score_at(le0);
-            GQ = w0 * Q;
-          }
-          for (int j = r + L; j < a.k; j += L) {
-            const int e = here ? a.ids[t * a.k + j] : -1;
-            if (e >= 0 && e < E) {
-              const float v = score_at(a.logits[t * a.ld + e]);
-              Q += v;
-              GQ = fmaf(a.dw[t * a.k + j], v, GQ);
+          // less the weights' mean by score, and less the mean of what that
+          // leaves: what all slots have alike cancels before it is rounded
+          // (one slot: to nothing, beside the small gradients of the losses)
+          const float q0 = id0 >= 0 ? score_at(le0) : 0.0f;
+          auto sums = [&](float less, float* Q) {
+            float q = q0, wq = id0 >= 0 ? q0 * (w0 - less) : 0.0f;
+            for (int j = r + L; j < a.k; j += L) {
+              const int e = here ? a.ids[t * a.k + j] : -1;
+              if (e >= 0 && e < E) {
+                const float v = score_at(a.logits[t * a.ld + e]);
+                q += v;
+                wq = fmaf(a.dw[t * a.k + j] - less, v, wq);
+              }
             }
-          }
-          __syncwarp();
-          Q = TM::sum(Q, red);
-          GQ = TM::sum(GQ, red);
-          if (Q > 0.0f) {  // as the gate: a sum of 0 divides nothing
-            const float iq = rcp_sfu(Q);
-            c *= iq;
-            mean = GQ * iq;
-          }
+            __syncwarp();
+            if (Q) *Q = TM::sum(q, red);
+            return TM::sum(wq, red);
+          };
+          float Q;
+          const float wq = sums(0.0f, &Q);
+          const float iq = Q > 0.0f ? rcp_sfu(Q) : 0.0f;  // as the gate: a sum of 0 divides nothing
+          mean = wq * iq;
+          rest = sums(mean, nullptr) * iq;
+          if (Q > 0.0f) c *= iq;
         }
         // a team's (a block's first warp's) slots at a time; equal ids among them are added in slot order
         constexpr int W = TM::kBlock ? 32 : L;
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
               if (e < 0 || e >= E) e = -1;
               v = e >= 0 ? a.dw[t * a.k + j] : 0.0f;
             }
-            v = c * (v - mean);
+            v = c * ((v - mean) - rest);
             const unsigned same = __match_any_sync(0xFFFFFFFFu, e) & TM::lanes();
             if (__all_sync(0xFFFFFFFFu, (same & (same - 1)) == 0 || e < 0)) {
               if (e >= 0) g[e] += v;

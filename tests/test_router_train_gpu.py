@@ -166,6 +166,29 @@ def test_parts_of_the_gradient(cuda_device):
     assert torch.equal(inplace, router_backward(l, ids, dw, renormalize=True))
 
 
+@pytest.mark.parametrize("func", [SOFTMAX, SIGMOID, SQRT_SOFTPLUS])
+@pytest.mark.parametrize("E,k", [(8, 1), (64, 1), (200, 1), (64, 3), (1500, 1), (1500, 40), (64, 12)])
+def test_equal_weight_gradients_cancel(cuda_device, func, E, k):
+    """Renormalised weights sum to a constant: what their gradients have alike (with one slot, all) leaves
+    nothing beside the losses' small gradients."""
+    from objeta_b200.router import balance_loss, router_backward
+    T = 50
+    l = U.randn((T, E), scale=1.5, seed=E)
+    ids = torch.topk(l, k, dim=1).indices.to(torch.int32)
+    ids[3] = -1
+    b = balance_loss(l, ids, score_func=func)
+    args = dict(score_func=func, balance=b, balance_grad=0.01, z_grad=0.001)
+    want = router_backward(l, ids, None, **args)
+    dw = U.randn((T, 1), seed=1).expand(T, k).contiguous()
+    dw[3] = math.nan  # of no expert: not looked at
+    dl = router_backward(l, ids, dw, renormalize=True, **args)
+    # w - mean is exact, mean wrong by 64 roundings; less the mean of that, 64 roundings of it: 2^-36 of w, which
+    # reaches a logit through 1 / Q and the scores' derivatives, below 32 in all here; then the losses' own sums
+    s = dw.nan_to_num().abs().max().double()
+    U.check(dl, want.double(), 32 * 2.0 ** -36 * s + 64 * 2.0 ** -24 * want.double().abs().amax(1, keepdim=True)
+            .expand(T, E), f"{func} {E} {k}")
+
+
 def test_same_expert_twice(cuda_device):
     """A hash layer's table may name an expert twice: its gradients add up."""
     from objeta_b200.router import balance_loss, router_backward
