@@ -48,6 +48,12 @@
 //     a memory latency per k-block: the proxy fence waits for them.)
 //   * GATED: A is 64 rows of the gate and the same 64 rows of up; the epilogue
 //     pairs lanes i and i + 64 through shared memory.
+//
+// What it comes to (bf16, 4096 x 4096 x 4096): 99 us, 1389 TFLOP/s, tensor pipe
+// 70 % busy over the launch and 95 % in the main loop; the library's product
+// 95 us.  In long runs both are bound by power (117 and 110 us at 1.48 GHz).
+// f32 results: 256 x 128 pair tiles 53 to 55 % busy, bound by the planes that
+// an SM takes in.  Few tokens: bound by w (37 x 2048 x 151936: 6.0 TB/s).
 #pragma once
 
 #include <cuda.h>
