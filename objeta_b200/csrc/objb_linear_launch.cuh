@@ -87,6 +87,9 @@ int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProp
   size_t smem = g.nstages * (stage + raw);
   if (GATED || tile.split > 1) smem = std::max(smem, static_cast<size_t>(tile.bn) * 512);  // the partial tile
   smem += 1024 + (128 - tile.rm) * 128;  // an MMA reads 128 rows, those past rm for nothing
+  // A kernel that takes all of tensor memory leaves no room for another of these on its SM (the least take 78 KB): of
+  // two clusters that share SMs, each might hold what the other waits for.
+  if (SH::kCols == 512) smem = std::max(smem, size_t{152} * 1024);
   const uint32_t half = p.a.dtype == OBJB_DTYPE_F16 ? 0 : 1;
   g.idesc = (1u << 4) | (half << 7) | (half << 10) | (static_cast<uint32_t>(MAJ != dev::kMajKK) << 15) |
             (static_cast<uint32_t>(MAJ == dev::kMajMN) << 16) | (static_cast<uint32_t>(tile.bn >> 3) << 17) |
