@@ -194,10 +194,15 @@ struct BalanceArgs {
   unsigned* ticket;
 };
 
+// Who folds the partial rows: a grid launched behind them; the one block that
+// made them all; the kFinishCluster blocks of one cluster that did.
+enum { kFinishGrid = 0, kFinishAlone = 1, kFinishInCluster = 2 };
+constexpr int kFinishCluster = 8;
+
 struct BalanceFinishArgs {
   BalanceArgs a;
   int groups;          // 32-expert groups
-  bool alone;          // one block does the partial pass and this one
+  int mode;            // kFinishGrid: a launch of its own; else by the blocks of the partial pass
   double* bal_part;    // [S][groups] sum_e c P
   double* seq_z;       // [S]
   int32_t* counts;     // [S][E]

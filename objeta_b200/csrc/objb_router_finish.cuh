@@ -3,6 +3,7 @@
 #pragma once
 
 #include "objb_router.cuh"
+#include "objb_tc.cuh"
 
 namespace objb {
 namespace dev {
@@ -25,14 +26,16 @@ __device__ __forceinline__ double warp_sum(double v) {
 
 // One (sequence, 32 experts) item per block and turn: the partial rows of the
 // sequence are summed in block order (interleaved over the warps, the runs
-// folded in order), in double.  The block that finishes last (`alone`: the
-// only one) folds the sequences' sums into the losses.
+// folded in order), in double.  The block that finishes last (of a cluster the
+// first, behind its barrier; alone the only one) folds the sequences' sums into
+// the losses.
 template <int WARPS>
-__device__ __forceinline__ void balance_finish(const BalanceFinishArgs& f, FinishSmem<WARPS>& sm, bool alone) {
+__device__ __forceinline__ void balance_finish(const BalanceFinishArgs& f, FinishSmem<WARPS>& sm, int mode) {
   const BalanceArgs& a = f.a;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int items = a.S * f.groups;
-  for (int item = alone ? 0 : blockIdx.x; item < items; item += alone ? 1 : gridDim.x) {
+  for (int item = mode == kFinishAlone ? 0 : blockIdx.x; item < items;
+       item += mode == kFinishAlone ? 1 : gridDim.x) {
     const int q = item / f.groups, g = item - q * f.groups;
     const int e = g * 32 + lane;
     long long b = a.off ? a.off[q] : 0, end = a.off ? a.off[q + 1] : a.T;
@@ -77,7 +80,10 @@ __device__ __forceinline__ void balance_finish(const BalanceFinishArgs& f, Finis
     }
     __syncthreads();
   }
-  if (!alone) {
+  if (mode == kFinishInCluster) {
+    cluster_sync_all();
+    if (blockIdx.x != 0) return;
+  } else if (mode == kFinishGrid) {
     if (threadIdx.x == 0) {
       __threadfence();
       sm.last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;

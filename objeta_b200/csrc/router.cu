@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(32 * kFinishWarps) balance_finish_kernel(const
   __shared__ FinishSmem<kFinishWarps> sm;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  balance_finish(f, sm, false);
+  balance_finish(f, sm, kFinishGrid);
 }
 
 // dw[t, j] = sum_o dout[t, o] v[slot_row[t, j], o]: WPS warps per slot, each
@@ -94,6 +94,7 @@ namespace {
 constexpr size_t kMaxExperts = 8192;  // as the router and the gate
 
 struct BalancePlan {
+  int mode;
   long long chunk;
   size_t chunks, rows, groups;
   size_t p, c, z, n, bal, seqz, ticket, total;  // offsets into the workspace
@@ -114,14 +115,25 @@ int check_router(const char* action, size_t T, size_t E, size_t k, size_t S, int
   return OBJB_OK;
 }
 
-// Blocks of the partial pass: three per SM at most (what its registers allow).
-// Up to 128 tokens one block does it, and, with few experts and sequences, the
-// finish too (no second launch); beyond, 16 tokens or more in each.
+// Blocks of the partial pass: three per SM at most (what its registers allow),
+// 16 tokens or more in each (4 in up to 128 blocks that are one team each: 8192
+// experts, 16 tokens 40 -> 28 us).  Few tokens of few experts and sequences need
+// no second launch: one block does the finish too (64 experts: 5.7 us), or a
+// cluster of eight does both while a thread team has at most 16 tokens of 8
+// experts a lane (256 experts, 16 tokens: 6.1 us, alone 10.5; a call's time with
+// 4096 tokens of 64: 13.0, in two launches 16.9; 2048 of 256: 20.9 and 16.4).
 BalancePlan plan_balance(size_t T, size_t E, size_t S, int sms) {
   BalancePlan p;
   const size_t most = static_cast<size_t>(3) * sms;
-  const size_t want = T <= 128 ? 1 : std::min(most, (T + 15) / 16);
-  p.chunk = static_cast<long long>(std::max<size_t>(1, (T + want - 1) / want));
+  const size_t items = S * ((E + 31) / 32), cluster = dev::kFinishCluster;
+  const size_t team = E <= 64 ? 8 : E <= 128 ? 16 : E <= 1024 ? 32 : 256;         // threads of a token
+  const size_t lane = E <= 256 ? 8 : E <= 512 ? 16 : 32;                          // experts of a thread
+  const bool few = T * lane * team <= 16 * 8 * 256 * cluster && items <= 8 * cluster;
+  p.mode = T <= 128 && items <= 2 ? dev::kFinishAlone : few ? dev::kFinishInCluster : dev::kFinishGrid;
+  size_t blocks = (T + 15) / 16;
+  if (team == 256) blocks = std::max(blocks, std::min<size_t>(128, (T + 3) / 4));
+  const size_t want = p.mode == dev::kFinishAlone ? 1 : p.mode == dev::kFinishInCluster ? cluster : std::min(most, blocks);
+  p.chunk = static_cast<long long>(std::max<size_t>(1, T ? (T + want - 1) / want : 0));
   p.chunks = (T + p.chunk - 1) / p.chunk;
   p.rows = p.chunks + S;
   p.groups = (E + 31) / 32;
@@ -214,7 +226,7 @@ int objb_balance_loss_device(const float* d_logits, size_t logits_stride, const 
   a.part_z = reinterpret_cast<double*>(b + p.z);
   a.part_n = reinterpret_cast<int32_t*>(b + p.n);
   f.groups = static_cast<int>(p.groups);
-  f.alone = p.chunks <= 1 && num_seqs * p.groups <= 8;
+  f.mode = p.mode;
   f.bal_part = reinterpret_cast<double*>(b + p.bal);
   f.seq_z = reinterpret_cast<double*>(b + p.seqz);
   f.counts = d_counts;
@@ -222,9 +234,9 @@ int objb_balance_loss_device(const float* d_logits, size_t logits_stride, const 
   f.losses = d_losses;
   f.scales = d_scales;
   const bool v4 = aligned16(d_logits) && ld % 4 == 0 && num_experts % 4 == 0;
-  const int grid = static_cast<int>(std::max<size_t>(1, p.chunks));
+  const int grid = p.mode == dev::kFinishInCluster ? dev::kFinishCluster : static_cast<int>(std::max<size_t>(1, p.chunks));
   OBJB_TRY(launch_balance_partial(f, grid, v4, st));
-  if (f.alone) return OBJB_OK;
+  if (f.mode != dev::kFinishGrid) return OBJB_OK;
   return launch_pdl(dev::balance_finish_kernel, static_cast<int>(num_seqs * p.groups), 32 * dev::kFinishWarps, 0, st, f);
 }
 

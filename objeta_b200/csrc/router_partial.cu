@@ -150,19 +150,37 @@ __global__ void __launch_bounds__(THREADS, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 
     __syncthreads();
     pos = end;
   }
-  if (f.alone) balance_finish(f, fin, true);  // its own rows are all there are
+  if (f.mode == kFinishInCluster) cluster_sync_all();  // the other blocks' rows are in place
+  if (f.mode != kFinishGrid) balance_finish(f, fin, f.mode);
 }
 
 }  // namespace dev
 
 int launch_balance_partial(const dev::BalanceFinishArgs& f, int grid, bool v4, cudaStream_t st) {
   return with_team<32>(f.a.E, v4, [&](auto tm) {
-    return with_func(f.a.func, [&](auto func) {
+    return with_func(f.a.func, [&](auto func) -> int {
       using TM = decltype(tm);
       constexpr int THREADS = 256;
       const size_t teams = TM::kBlock ? 0 : THREADS / TM::L;
       const size_t smem = (static_cast<size_t>(f.a.E + 3) / 4 * 4 + teams * f.a.E) * 4;
-      return launch_pdl(dev::balance_partial_kernel<TM, decltype(func)::value, THREADS>, grid, THREADS, smem, st, f);
+      auto kernel = dev::balance_partial_kernel<TM, decltype(func)::value, THREADS>;
+      if (f.mode != dev::kFinishInCluster) return launch_pdl(kernel, grid, THREADS, smem, st, f);
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(grid);
+      cfg.blockDim = dim3(THREADS);
+      cfg.dynamicSmemBytes = smem;
+      cfg.stream = st;
+      cudaLaunchAttribute attr[2];
+      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[0].val.programmaticStreamSerializationAllowed = 1;
+      attr[1].id = cudaLaunchAttributeClusterDimension;
+      attr[1].val.clusterDim.x = static_cast<unsigned>(grid);
+      attr[1].val.clusterDim.y = 1;
+      attr[1].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 2;
+      OBJB_CUDA(cudaLaunchKernelEx(&cfg, kernel, f), "launch balance loss");
+      return OBJB_OK;
     });
   });
 }

@@ -136,6 +136,15 @@ def test_tokens(cuda_device, func, T):
     run_case(T, 256, 8, min(T, 9) + 1, func, masked=True, renorm=False, seed=T + 1)
 
 
+@pytest.mark.parametrize("T,E,k,S", [(129, 64, 2, 1), (1000, 64, 8, 17), (4096, 33, 3, 30), (300, 500, 4, 4),
+                                     (5, 256, 8, 2), (3, 3, 1, 40), (2048, 128, 8, 16), (2049, 128, 8, 16),
+                                     (1025, 256, 8, 1), (9, 2000, 8, 1), (600, 1100, 3, 2), (1, 1024, 5, 1)])
+def test_who_folds(cuda_device, T, E, k, S):
+    """One block, a cluster of blocks or a launch of its own: sizes at the borders of each."""
+    run_case(T, E, k, S, SOFTMAX, masked=True, seed=T)
+    run_case(T, E, k, S, SIGMOID, renorm=False, dropped=True, seed=T + 1)
+
+
 def test_many_short_sequences(cuda_device):
     run_case(3000, 16, 2, 2900, SOFTMAX, seed=3)
     run_case(40, 8, 2, 200, SIGMOID, masked=True, seed=4)
