@@ -362,6 +362,55 @@ def test_streams_and_graphs(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(want, o))
 
 
+def test_many_streams_at_once(cuda_device):
+    """Products of every kind of tile side by side on the device: the same bits as one after another."""
+    from objeta_b200.dense import ffn_bf16_tokens, linear, linear_backward
+    cases = []
+    for xd, wd, T, K, N in (("f32", "f32", 250, 2048, 256), ("bf16", "bf16", 1, 4096, 4096), ("f32", "bf16", 30, 2048, 512),
+                            ("bf16", "bf16", 1500, 512, 2048), ("f32", "f32", 700, 512, 1024), ("f16", "f16", 60, 1000, 3000)):
+        x, w = _case(T, K, N, xd, wd, T)
+        dy = U.randn((T, N), U.DT[xd], seed=3)
+        cases.append(lambda x=x, w=w: (linear(x, w),))
+        cases.append(lambda x=x, w=w, dy=dy: linear_backward(dy, x, w, need_dbias=True))
+    g, u = (U.randn((512, 1024), torch.bfloat16, 0.03, i) for i in (1, 2))
+    d = U.randn((1024, 512), torch.bfloat16, 0.04, 3)
+    for T in (16, 300):
+        cases.append(lambda x=U.randn((T, 1024), seed=T): (ffn_bf16_tokens(g, u, d, x),))
+    want = [f() for f in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for turn in range(6):
+        for i, f in enumerate(cases):
+            with torch.cuda.stream(streams[(i + turn) % 4]):
+                got.append((i, f()))
+    torch.cuda.synchronize()
+    for i, r in got:
+        assert all(torch.equal(a, b) for a, b in zip(want[i], r)), i
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """Outputs, dz images and strided rows beyond 2^31 elements."""
+    from objeta_b200.dense import linear, linear_backward
+    T, K, N = 70000, 64, 32768
+    x, w = _case(T, K, N, "bf16", "bf16", 1)
+    y = linear(x, w)
+    rows = torch.tensor([0, 65535, 65536, 65537, T - 1], device="cuda")
+    _, _, ref, bound = U.linear_ref(x[rows], w, None, "none", None, torch.bfloat16)
+    U.check(y[rows], ref, bound, "y")
+    dx, _, db = linear_backward(y, x, w, y, activation="relu", need_dw=False, need_dbias=True)
+    r = U.backward_ref(y[rows], x[rows], w, y[rows], "relu", torch.bfloat16)
+    U.check(dx[rows], *r["dx"], "dx")
+    pos = torch.zeros(N, dtype=torch.double, device="cuda")
+    for i in range(0, T, 7000):
+        pos += torch.relu(y[i:i + 7000].double()).sum(0)
+    U.check(db, pos, U.TOL * pos + 1e-30, "db")
+    del y, dx
+    buf = torch.empty(300, 1 << 23, device="cuda", dtype=torch.bfloat16)[:, :K]  # rows 2^23 elements apart
+    buf.copy_(x[:300])
+    assert torch.equal(linear(buf, w[:100]), linear(x[:300].contiguous(), w[:100]))
+
+
 def test_c_entry_with_the_streams_workspace(cuda_device):
     """NULL scratch: the per-stream workspace, as the other device entries."""
     import ctypes

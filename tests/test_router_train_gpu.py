@@ -384,6 +384,32 @@ def test_repeat_streams_and_graphs(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(want, out))
 
 
+def test_offsets_past_32_bits(cuda_device):
+    """Logits, gradients and value rows beyond 2^31 elements."""
+    from objeta_b200.router import balance_loss, moe_combine_backward, router_backward
+    T, E, k = 300, 64, 4
+    l = U.randn((T, E), seed=1)
+    ids = torch.topk(l, k, dim=1).indices.to(torch.int32)
+    dw = U.randn((T, k), seed=2)
+    far = torch.empty(T, 1 << 23, device="cuda")
+    far[:, :E] = l
+    b, c = balance_loss(l, ids), balance_loss(far[:, :E], ids)
+    assert torch.equal(b.counts, c.counts) and torch.equal(b.balance, c.balance) and torch.equal(b.z, c.z)
+    args = dict(renormalize=True, balance=b, balance_grad=0.1, z_grad=0.1)
+    want = router_backward(l, ids, dw, **args)
+    router_backward(far[:, :E], ids, dw, d_dlogits=far[:, :E], **args)
+    assert torch.equal(far[:, :E], want)
+    del far
+    V, O = (1 << 20) + 40, 2048
+    v = torch.empty(V, O, device="cuda")
+    rows = torch.tensor([[0, V - 1], [1 << 20, (1 << 20) - 1]], dtype=torch.int32, device="cuda")
+    v[rows.long()] = U.randn((2, 2, O), seed=4)
+    d = U.randn((2, O), seed=5)
+    got = moe_combine_backward(d, v, rows)
+    ref = (d.double()[:, None] * v[rows.long()].double()).sum(2)
+    U.check(got, ref, U.TOL * (d.double()[:, None] * v[rows.long()].double()).abs().sum(2))
+
+
 def test_argument_checks(cuda_device):
     from objeta_b200.router import balance_loss, moe_combine_backward, router_backward
     l = U.randn((6, 8))
