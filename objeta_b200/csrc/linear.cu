@@ -878,6 +878,7 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
   dz.planes = pl.dz.planes;
   dz.dtype = pl.dz.planes > 1 ? OBJB_DTYPE_BF16 : d.dy_dtype;
   const bool image = products && !pl.dz_direct;
+  dev::BiasFold fold;
   Images images;
   Image w, x;
   if (want_dx) w = images.take(pl.w, d_w, d.w_dtype, ldw, d.out_features, d.in_features, ws_w);
@@ -907,7 +908,9 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
                         0, st, j, images.job(0), images.job(1), image_blocks);
     }));
     images.clear();
-    if (want_db && pl.parts > 1)
+    if (want_db && pl.parts > 1 && products && pl.parts <= dev::kFoldParts)
+      fold = {j.part, d_dbias, pl.parts, N, d.accumulate != 0};
+    else if (want_db && pl.parts > 1)
       OBJB_TRY(launch_pdl(dev::dbias_kernel, (N + 31) / 32, 1024, 0, st, static_cast<const float*>(j.part), pl.parts, N,
                           d_dbias, static_cast<int>(d.accumulate)));
   }
@@ -923,6 +926,8 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
     p.epi.y = d_dx;
     p.epi.ldy = static_cast<uint32_t>(lddx);
     p.epi.y_dtype = d.x_dtype;
+    p.fold = fold;
+    fold.part = nullptr;
     OBJB_TRY(gemm(p, device, props, st));
   }
   if (want_dw) {
@@ -936,6 +941,7 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
     p.epi.y = d_dw;
     p.epi.ldy = static_cast<uint32_t>(lddw);
     p.epi.y_dtype = d.dw_dtype;
+    p.fold = fold;
     if (d.accumulate) p.epi.residual = d_dw, p.epi.ldr = static_cast<uint32_t>(lddw);
     OBJB_TRY(gemm(p, device, props, st));
   }

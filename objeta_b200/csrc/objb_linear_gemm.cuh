@@ -77,6 +77,31 @@ constexpr int kConvWarps = 8;
 // converting warps
 constexpr int lin_threads(bool promote, bool raw = false) { return promote ? 352 + (raw ? 32 * kConvWarps : 0) : 608; }
 
+// The column sums of dz's runs of rows (dz_kernel), folded by the epilogue warps
+// while they wait for their first tile: a launch less.
+struct BiasFold {
+  const float* part = nullptr;  // [parts][n], or null
+  float* to = nullptr;
+  int parts = 0, n = 0;
+  bool add = false;
+};
+constexpr int kFoldParts = 128;  // beyond, the fold would outlast that wait
+
+// Group w of 32 columns: a lane's runs in order.
+__device__ __forceinline__ void fold_bias(const BiasFold& f, int w) {
+  const int c = w * 32 + (threadIdx.x & 31);
+  if (c >= f.n) return;
+  float s = 0.0f;
+  for (int i = 0; i < f.parts; i += 16) {
+    float v[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) v[u] = i + u < f.parts ? f.part[static_cast<size_t>(i + u) * f.n + c] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) s += v[u];
+  }
+  f.to[c] = f.add ? f.to[c] + s : s;
+}
+
 struct GemmArgs {
   int M;                  // rows of A (GATED: features)
   long long N;            // rows of B
@@ -93,6 +118,7 @@ struct GemmArgs {
   float swiglu_limit;
   unsigned* err;
   LinearEpilogue epi;
+  BiasFold fold;
   const uint8_t* ahead;  // bytes that the next product reads, brought into L2 behind this one's own (16-byte
   size_t ahead_bytes;    // aligned, whole 16-byte quads); may be null
 };
@@ -582,6 +608,8 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
     const int col0 = part * half - a * BN;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * half;
     const int row = quarter * 32 + lane;
+    if (g.fold.part)
+      for (int w = blockIdx.x + gridDim.x * (warp - 2); w * 32 < g.fold.n; w += gridDim.x * kWarps) fold_bias(g.fold, w);
     int cc = 0, xc = 0, tt = 0;
     bool ok = true;
     auto release = [&](uint64_t* bar) {

@@ -35,6 +35,7 @@ struct Product {
   int raw = 0;  // 1: b is f32 as it lies (three planes in the stages), 2: a too
   const void* ahead = nullptr;  // what the next product reads
   size_t ahead_bytes = 0;
+  dev::BiasFold fold;
   bool gated = false;
   size_t M = 0, N = 0, K = 0;
   dev::LinearEpilogue epi;
@@ -69,6 +70,7 @@ int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProp
   g.chunk_kb = PROMOTE ? tile.chunk_kb : g.nkb;
   g.swiglu_limit = p.swiglu_limit;
   g.epi = p.epi;
+  g.fold = p.fold;
   g.ahead = static_cast<const uint8_t*>(p.ahead);
   g.ahead_bytes = p.ahead_bytes;
   OBJB_TRY(device_error_word(device, &g.err));
