@@ -124,13 +124,15 @@ struct LinearEpilogue {
 
   // FULL: all C columns exist.
   template <class T, int C, bool FULL>
-  __device__ __forceinline__ static void store(T* p, uint32_t ld, int m, long long n, int left, const float (&v)[C]) {
+  __device__ __forceinline__ static void store(T* p, uint32_t ld, int m, long long n, int left, const float (&v)[C],
+                                               uint32_t lane = 0) {
     char* at = reinterpret_cast<char*>(p + n * ld + m);
+    const uint32_t off = lane * static_cast<uint32_t>(sizeof(T));
     const uint32_t pitch = ld * static_cast<uint32_t>(sizeof(T));
 #pragma unroll
     for (int i = 0; i < C; ++i)
       if (FULL || i < left) {
-        T* q = reinterpret_cast<T*>(at + static_cast<uint64_t>(pitch) * i);
+        T* q = reinterpret_cast<T*>(at + static_cast<uint64_t>(pitch) * i + off);
         if constexpr (sizeof(T) == 4)
           *q = v[i];
         else if constexpr (std::is_same<T, __half>::value)
@@ -140,8 +142,9 @@ struct LinearEpilogue {
       }
   }
   template <class T, int C, bool FULL>
-  __device__ __forceinline__ static void add(const T* p, uint32_t ld, int m, long long n, int left, float (&v)[C]) {
-    const char* at = reinterpret_cast<const char*>(p + n * ld + m);
+  __device__ __forceinline__ static void add(const T* p, uint32_t ld, int m, long long n, int left, float (&v)[C],
+                                             uint32_t lane = 0) {
+    const char* at = reinterpret_cast<const char*>(p + n * ld + m + lane);
     const uint32_t pitch = ld * static_cast<uint32_t>(sizeof(T));
     T r[C];
 #pragma unroll
@@ -152,8 +155,8 @@ struct LinearEpilogue {
       if (FULL || i < left) v[i] += static_cast<float>(r[i]);
   }
   template <class T, int C, bool FULL>
-  __device__ __forceinline__ void put_typed(int m, long long n, int left, float (&v)[C]) const {
-    if (z) store<T, C, FULL>(static_cast<T*>(z), ldz, m, n, left, v);
+  __device__ __forceinline__ void put_typed(int m, long long n, int left, float (&v)[C], uint32_t lane) const {
+    if (z) store<T, C, FULL>(static_cast<T*>(z), ldz, m, n, left, v, lane);
     switch (act) {
 #define OBJB_ACT_CASE(A)                                          \
   case A:                                                         \
@@ -166,30 +169,33 @@ struct LinearEpilogue {
 #undef OBJB_ACT_CASE
       default: break;
     }
-    if (residual) add<T, C, FULL>(static_cast<const T*>(residual), ldr, m, n, left, v);
-    store<T, C, FULL>(static_cast<T*>(y), ldy, m, n, left, v);
+    if (residual) add<T, C, FULL>(static_cast<const T*>(residual), ldr, m, n, left, v, lane);
+    store<T, C, FULL>(static_cast<T*>(y), ldy, m, n, left, v, lane);
   }
   template <class T, int C>
-  __device__ __forceinline__ void put_left(int m, long long n, int left, float (&v)[C]) const {
+  __device__ __forceinline__ void put_left(int m, long long n, int left, float (&v)[C], uint32_t lane) const {
     if (left >= C)
-      put_typed<T, C, true>(m, n, left, v);
+      put_typed<T, C, true>(m, n, left, v, lane);
     else
-      put_typed<T, C, false>(m, n, left, v);
+      put_typed<T, C, false>(m, n, left, v, lane);
   }
 
-  // C neighbouring n of one m, those below n_end; b = bias_of(m).
+  // C neighbouring n of one m, those below n_end; b = bias_of(m).  Where a warp
+  // has 32 neighbouring m, m is the first of them and `lane` the rest: the
+  // addresses but for the lane are the warp's.
   template <int C>
-  __device__ __forceinline__ void put_columns(int m, long long n, long long n_end, float b, float (&v)[C]) const {
+  __device__ __forceinline__ void put_columns(int m, long long n, long long n_end, float b, float (&v)[C],
+                                              uint32_t lane = 0) const {
     if (n >= n_end) return;
     const int left = n_end - n < C ? static_cast<int>(n_end - n) : C;
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] += b;
     if (y_dtype == OBJB_DTYPE_F32)
-      put_left<float>(m, n, left, v);
+      put_left<float>(m, n, left, v, lane);
     else if (y_dtype == OBJB_DTYPE_BF16)
-      put_left<__nv_bfloat16>(m, n, left, v);
+      put_left<__nv_bfloat16>(m, n, left, v, lane);
     else
-      put_left<__half>(m, n, left, v);
+      put_left<__half>(m, n, left, v, lane);
   }
 
   // One f32 value as the three planes of the next product's operand.

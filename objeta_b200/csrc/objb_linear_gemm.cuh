@@ -600,8 +600,9 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
     }
   } else {
     // ---- epilogue
-    const int quarter = warp & 3;                 // tensor-memory lanes 32 quarter ..
-    const int part = (warp - 2) >> 2;             // of the columns
+    const int warp_u = __shfl_sync(0xFFFFFFFFu, warp, 0);  // (known to be the warp's)
+    const int quarter = warp_u & 3;                        // tensor-memory lanes 32 quarter ..
+    const int part = (warp_u - 2) >> 2;                    // of the columns
     // PROMOTE: half of the tile's bn columns; else HN columns of accumulator a
     const int a = PROMOTE ? 0 : part * HN / BN;
     const int half = PROMOTE ? g.bn / 2 : HN;
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
       lin_tile(g, t, &tm, &tn);
       const long long n0 = static_cast<long long>(tn) * g.bn;
       long long n_end = n0 + g.bn < g.N ? n0 + g.bn : g.N;
-      const int m = GATED ? 0 : row0(tm) + a * g.rm + row;
+      const int m_warp = GATED ? 0 : row0(tm) + a * g.rm + quarter * 32, m = m_warp + lane;
       const bool m_ok = row < g.rm && m < g.M;
       const float bias = !GATED && m_ok ? g.epi.bias_of(m) : 0.0f;
       if constexpr (PROMOTE) {
@@ -685,7 +686,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
             float v[P];
 #pragma unroll
             for (int i = 0; i < P; ++i) v[i] = acc[c + i];
-            g.epi.put_columns<P>(m, n0 + col0 + c, n_end, bias, v);
+            g.epi.put_columns<P>(m_warp, n0 + col0 + c, n_end, bias, v, lane);
           }
         }
       } else {
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
           tmem_ldf<P>(t_lane + c, v);
           tmem_wait_ld();
           if (c + P == HN) release(&t_empty[a]);  // read: the next tile may have the accumulator
-          if (m_ok) g.epi.put_columns<P>(m, n0 + col0 + c, n_end, bias, v);
+          if (m_ok) g.epi.put_columns<P>(m_warp, n0 + col0 + c, n_end, bias, v, lane);
         }
       }
     }
