@@ -927,6 +927,7 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
     p.epi.ldy = static_cast<uint32_t>(lddx);
     p.epi.y_dtype = d.x_dtype;
     p.fold = fold;
+    p.next_apart = want_dw;
     fold.part = nullptr;
     OBJB_TRY(gemm(p, device, props, st));
   }
@@ -941,6 +942,7 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
     p.epi.y = d_dw;
     p.epi.ldy = static_cast<uint32_t>(lddw);
     p.epi.y_dtype = d.dw_dtype;
+    p.apart = want_dx;  // beside dx
     p.fold = fold;
     if (d.accumulate) p.epi.residual = d_dw, p.epi.ldr = static_cast<uint32_t>(lddw);
     OBJB_TRY(gemm(p, device, props, st));

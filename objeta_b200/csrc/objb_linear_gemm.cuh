@@ -115,6 +115,11 @@ struct GemmArgs {
   int nstages, unit;      // stages of `unit` k-blocks
   int conv_groups;        // RAW: groups of converting warps, which take the stages in turn; divides nstages
   uint32_t idesc;
+  // Two launches that do not read each other's results run side by side: the
+  // first lets the next one start only when what came before it is complete
+  // (next_apart); the second does not wait but at its end, so that what comes
+  // behind it finds both done (apart).
+  bool next_apart, apart;
   float swiglu_limit;
   unsigned* err;
   LinearEpilogue epi;
@@ -318,8 +323,9 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
   if (csize > 1) cluster_sync_all();  // the peers' barriers exist before any arrival
   tc_fence_after_sync();
   const uint32_t tmem = s_tmem;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!g.next_apart) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!g.apart) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (g.next_apart) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int ntiles = g.tiles_m * g.tiles_n;
   const int first = blockIdx.x / csize, step = gridDim.x / csize;
@@ -766,6 +772,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
     else
       tmem_dealloc_pair(tmem, kCols);
   }
+  if (g.apart) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace dev

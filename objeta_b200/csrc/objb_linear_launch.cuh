@@ -36,6 +36,7 @@ struct Product {
   const void* ahead = nullptr;  // what the next product reads
   size_t ahead_bytes = 0;
   dev::BiasFold fold;
+  bool next_apart = false, apart = false;  // GemmArgs
   bool gated = false;
   size_t M = 0, N = 0, K = 0;
   dev::LinearEpilogue epi;
@@ -71,6 +72,8 @@ int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProp
   g.swiglu_limit = p.swiglu_limit;
   g.epi = p.epi;
   g.fold = p.fold;
+  g.next_apart = p.next_apart;
+  g.apart = p.apart;
   g.ahead = static_cast<const uint8_t*>(p.ahead);
   g.ahead_bytes = p.ahead_bytes;
   OBJB_TRY(device_error_word(device, &g.err));
