@@ -150,6 +150,30 @@ def test_linear_non_finite(cuda_device):
             assert bool((fin == want).all()), (xd, wd, bad)
 
 
+@pytest.mark.parametrize("T,K,N", [(300, 200, 400), (40, 203, 150), (700, 1000, 900)])
+def test_non_finite_of_laid_out_operands(cuda_device, T, K, N):
+    """The same for operands that become planes or images first, forwards and in both gradients."""
+    from objeta_b200.dense import linear, linear_backward
+    for xd, wd, _ in PAIRS:
+        for bad in (math.inf, -math.inf, math.nan):
+            x, w = _case(T, K, N, xd, wd, 2)
+            dy = U.randn((T, N), U.DT[xd], seed=4)
+            want = torch.ones(T, N, dtype=torch.bool, device="cuda")
+            x[7, 11] = bad
+            w[101, 5] = bad
+            want[7, :] = False
+            want[:, 101] = False
+            assert bool((torch.isfinite(linear(x, w)) == want).all()), (xd, wd, bad)
+            x, w = _case(T, K, N, xd, wd, 2)
+            dy[9, 3] = bad  # its row of dx, its row of dw
+            dx, dw, db = linear_backward(dy, x, w, need_dbias=True)
+            rows = torch.isfinite(dx).all(1)
+            assert not bool(torch.isfinite(dx[9]).any()) and int((~rows).sum()) == 1, (xd, wd, bad)
+            rows = torch.isfinite(dw).all(1)
+            assert not bool(torch.isfinite(dw[3]).any()) and int((~rows).sum()) == 1, (xd, wd, bad)
+            assert int((~torch.isfinite(db)).sum()) == 1 and not bool(torch.isfinite(db[3]))
+
+
 def test_linear_empty_and_repeat(cuda_device):
     from objeta_b200.dense import linear
     x, w = _case(0, 64, 32, "bf16", "bf16")
