@@ -47,7 +47,8 @@
 //     the splitting warps themselves, into registers or shared memory, cost
 //     a memory latency per k-block: the proxy fence waits for them.)
 //   * GATED: A is 64 rows of the gate and the same 64 rows of up; the epilogue
-//     pairs lanes i and i + 64 through shared memory.
+//     pairs lanes i and i + 64 through shared memory (behind the stages, where
+//     a CTA has more than one tile, so that the next one's MMAs go on).
 //
 // What it comes to (bf16, 4096 x 4096 x 4096): 99 us, 1389 TFLOP/s, tensor pipe
 // 70 % busy over the launch and 95 % in the main loop; the library's product
@@ -113,6 +114,7 @@ struct GemmArgs {
   int split;              // CTAs of a cluster per tile (CG 1)
   int chunk_kb;           // k-blocks per accumulator chunk, a multiple of unit
   int nstages, unit;      // stages of `unit` k-blocks
+  uint32_t exchange;      // GATED, split: where in the stages' memory a tile is exchanged
   int conv_groups;        // RAW: groups of converting warps, which take the stages in turn; divides nstages
   uint32_t idesc;
   // Two launches that do not read each other's results run side by side: the
@@ -629,7 +631,8 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
           mbar_arrive_cta_relaxed(bar, 0);
       }
     };
-    for (int t = first; t < ntiles && ok; t += step, ++tt) {
+    // (a gated tile's warps meet at a barrier, in every tile, whatever runs out)
+    for (int t = first; t < ntiles && (ok || GATED); t += step, ++tt) {
       int tm, tn;
       lin_tile(g, t, &tm, &tn);
       const long long n0 = static_cast<long long>(tn) * g.bn;
@@ -655,6 +658,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
         };
         for (int kb = kb0, left = kCrossChunks; kb < kb1; kb += g.chunk_kb, ++cc) {
           const int buf = cc & 1;
+          if (!ok) break;
           if (!lin_wait(&t_full[buf], (cc >> 1) & 1, g.err, kErrFullWaitTimeout, &s_abort)) {
             ok = false;
             break;
@@ -681,11 +685,22 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
           }
         }
         if (GATED || g.split > 1) {
-          // one tile per CTA: its stages are done with, the partial tile goes there as [column][row]
-          float* ex = reinterpret_cast<float*>(stages) + part * half * 128 + row;
+          // as [column][row]; where there is one tile per CTA, over its stages, which are done with
+          float* ex = reinterpret_cast<float*>(stages + g.exchange) + part * half * 128 + row;
 #pragma unroll
           for (int i = 0; i < HN; ++i)
             if (i < half) ex[i * 128] = acc[i];
+          if (GATED && g.split == 1) {
+            // gate and up of a feature are 64 lanes apart: they meet here, while the next tile's MMAs run
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const int tid = threadIdx.x - 64, f = tid & 63, mf = row0(tm) + f;
+            const float* e = reinterpret_cast<const float*>(stages + g.exchange) + f;
+            const long long tile_end = n0 + g.bn < g.N ? n0 + g.bn : g.N;
+            if (ok && mf < g.M)
+              for (int c = tid >> 6; n0 + c < tile_end; c += 4)
+                g.epi.put_planes(mf, n0 + c, swiglu(e[c * 128], e[c * 128 + 64], g.swiglu_limit));
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+          }
         } else if (ok && m_ok) {
 #pragma unroll
           for (int c = 0; c < HN; c += P) {
@@ -713,9 +728,9 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
     }
   }
 
-  if (GATED || (CG == 1 && g.split > 1)) {
+  if (CG == 1 && g.split > 1) {
     __syncthreads();
-    if (g.split > 1) cluster_sync_all();  // every partial tile is in place
+    cluster_sync_all();  // every partial tile is in place
     if (warp >= 2 && warp < 2 + kWarps) {
       int tm, tn;
       lin_tile(g, first, &tm, &tn);
@@ -729,7 +744,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
           if (m >= g.M || n0 + c >= n_end) continue;
           float gate = 0.0f, up = 0.0f;
           for (int s = 0; s < g.split; ++s) {
-            const uint32_t at = (g.split > 1 ? lin_mapa(ex, s) : ex) + (c * 128 + f) * 4;
+            const uint32_t at = lin_mapa(ex, s) + (c * 128 + f) * 4;
             gate += lin_ld_cluster(at);
             up += lin_ld_cluster(at + 256);
           }

@@ -84,13 +84,22 @@ int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProp
   g.unit = PROMOTE ? tile.unit : 1;
   const size_t stage = g.unit * 128 * (g.pa * a_rows + static_cast<size_t>(PB) * (tile.bn / CG));
   const size_t raw = RAW ? g.unit * 256 * ((RAW == 2 ? tile.rm : 0) + static_cast<size_t>(tile.bn)) : 0;
-  g.nstages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(dev::kLinStagesMax, tile.ring / (stage + raw))));
+  const long long tiles = static_cast<long long>(g.tiles_m) * g.tiles_n;
+  const int csize = CG == 2 ? 2 : tile.split;
+  const long long at_once = static_cast<long long>(props.sm_count) * (tile.ring == kLinRingTwo ? 2 : 1) / csize;
+  // A tile in f32, exchanged over the stages or, where another tile is on its way into them, behind (1000 tokens of
+  // 4096 x 2048: 139 -> 129 us; with one tile per CTA the stages are worth more: 250 tokens 66.6, over them 61.4).
+  const size_t partial = static_cast<size_t>(tile.bn) * 512;
+  const bool behind = GATED && tile.split == 1 && tiles > at_once;
+  const size_t room = tile.ring - (behind ? partial : 0);
+  g.nstages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(dev::kLinStagesMax, room / (stage + raw))));
   // A group keeps to its own stages (a wait for a phase that is not the next one of its barrier falls through), so
   // that they are a multiple of the groups.
   g.conv_groups = g.nstages >= dev::kConvWarps ? dev::kConvWarps : g.nstages >= 4 ? 4 : 2;
   if (RAW) g.nstages -= g.nstages % g.conv_groups;
   size_t smem = g.nstages * (stage + raw);
-  if (GATED || tile.split > 1) smem = std::max(smem, static_cast<size_t>(tile.bn) * 512);  // the partial tile
+  g.exchange = behind ? static_cast<uint32_t>(smem) : 0;
+  if (GATED || tile.split > 1) smem = std::max(smem, g.exchange + partial);
   smem += 1024 + (128 - tile.rm) * 128;  // an MMA reads 128 rows, those past rm for nothing
   // A kernel that takes all of tensor memory leaves no room for another of these on its SM (the least take 78 KB): of
   // two clusters that share SMs, each might hold what the other waits for.
@@ -108,10 +117,7 @@ int launch_gemm(const Product& p, const Tile& tile, int device, const DeviceProp
   OBJB_TRY(linear_encode(&mb, p.b, MAJ == dev::kMajMN ? 64 : tile.bn / CG));
   auto kernel = dev::lin_gemm_kernel<MAJ, BN, CG, MT, GATED, PROMOTE, PB, RAW>;
   OBJB_TRY(ensure_smem_attr(kernel, device, smem));
-  const long long tiles = static_cast<long long>(g.tiles_m) * g.tiles_n;
-  const int csize = CG == 2 ? 2 : tile.split;
-  const bool one_each = GATED || tile.split > 1;
-  const long long at_once = static_cast<long long>(props.sm_count) * (tile.ring == kLinRingTwo ? 2 : 1) / csize;
+  const bool one_each = tile.split > 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((one_each ? tiles : std::min(tiles, at_once)) * csize));
   cfg.blockDim = dim3(SH::kThreads);
