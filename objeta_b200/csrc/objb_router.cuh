@@ -106,7 +106,10 @@ __device__ __forceinline__ float rcp_sfu(float x) {
 
 // The gate's sigmoid and sqrt-softplus scores and their derivatives.  The
 // sqrt-softplus keeps the gate's branches, log1p(exp(-l)) below -20 among
-// them, so the derivative is that of the score as it is computed.
+// them, so the derivative is that of the score as it is computed.  Below about
+// -88.7 that exponential leaves f32 and the gate's score is no number that
+// shares could be made of: such a logit (-inf and the lowest f32, which masks
+// are made of, among them) has score 0 and derivative 0, as under the other two.
 __device__ __forceinline__ float score_of(int func, float l, float* d) {
   if (func == kSigmoid) {
     const float t = exp_sfu(-fabsf(l));
@@ -121,6 +124,10 @@ __device__ __forceinline__ float score_of(int func, float l, float* d) {
   }
   const bool low = l < -20.0f;
   const float ex = expf(low ? -l : l);
+  if (ex == __int_as_float(0x7F800000)) {
+    *d = 0.0f;
+    return 0.0f;
+  }
   const float s = sqrtf(log1pf(ex));
   const float sg = low ? 1.0f / (1.0f + expf(l)) : ex / (1.0f + ex);
   *d = (low ? -0.5f : 0.5f) * sg / s;

@@ -1,0 +1,77 @@
+"""The router's losses and gradients where scores leave f32's range or
+precision, against 64-bit definitions."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests import _dense_util as U  # noqa: E402
+from tests.test_router_train_gpu import SIGMOID, SOFTMAX, SQRT_SOFTPLUS, reference  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+LOWEST = torch.finfo(torch.float32).min
+
+
+@pytest.mark.parametrize("E,masked", [(40, 20), (200, 3), (1500, 700)])
+@pytest.mark.parametrize("bad", [-math.inf, LOWEST, -100.0])
+def test_masked_experts_of_sqrt_softplus(cuda_device, bad, E, masked):
+    """Logits whose gate score overflows: no share and no gradient there, the
+    other experts as if they were alone."""
+    from objeta_b200.router import balance_loss, router_backward
+    T, k = 12, 3
+    l = U.randn((T, E), seed=5)
+    ids = torch.topk(l[:, masked:], k, dim=1).indices.to(torch.int32) + masked
+    l[:, :masked] = bad
+    dw = U.randn((T, k), seed=6)
+    b = balance_loss(l, ids, score_func=SQRT_SOFTPLUS)
+    dl = router_backward(l, ids, dw, score_func=SQRT_SOFTPLUS, renormalize=True, balance=b, balance_grad=0.5,
+                         z_grad=0.1)
+    assert not dl[:, :masked].any()
+    sub = l[:, masked:].contiguous()
+    n = sub.shape[1]
+    # f has E in place of the n experts that are left
+    _, _, rb, rz, rdl, mag = reference(sub, ids - masked, SQRT_SOFTPLUS, None, None, dw, True, 1.0, 0.5 * E / n, 0.1)
+    assert abs(float(b.balance) - rb * E / n) <= 64 * 2.0 ** -24 * rb * E / n
+    assert abs(float(b.z) - rz) <= 64 * 2.0 ** -24 * (rz + math.sqrt(rz))
+    U.check(dl[:, masked:].contiguous(), rdl, 64 * 2.0 ** -24 * mag + 1e-37)
+
+
+@pytest.mark.parametrize("func", [SOFTMAX, SIGMOID, SQRT_SOFTPLUS])
+def test_row_of_minus_infinity(cuda_device, func):
+    """Such a token counts, and adds nothing to a loss or a gradient; the others' results are theirs alone."""
+    from objeta_b200.router import balance_loss, router_backward
+    l = U.randn((5, 40), seed=5)
+    ids = torch.topk(l, 3, dim=1).indices.to(torch.int32)
+    dw = U.randn((5, 3), seed=6)
+    l[2] = -math.inf
+    b = balance_loss(l, ids, score_func=func)
+    dl = router_backward(l, ids, dw, score_func=func, renormalize=True, balance=b, balance_grad=0.5, z_grad=0.1)
+    assert int(b.tokens[0]) == 5 and not dl[2].any() and bool(torch.isfinite(dl).all())
+    rest = torch.tensor([0, 1, 3, 4], device="cuda")
+    z = torch.logsumexp(l[rest].double(), 1).square().sum() / 5
+    assert abs(float(b.z) - float(z)) <= 64 * 2.0 ** -24 * (float(z) + math.sqrt(float(z)))
+    s = [torch.softmax, lambda v, _: torch.sigmoid(v), lambda v, _: sqrt_softplus(v)][func](l[rest].double(), 1)
+    counts = torch.bincount(ids.reshape(-1).long(), minlength=40).double()
+    bal = (counts * 40 / (3 * 5) * (s / s.sum(1, keepdim=True)).sum(0) / 5).sum()
+    assert abs(float(b.balance) - float(bal)) <= 64 * 2.0 ** -24 * float(bal)
+
+
+def sqrt_softplus(v):
+    return torch.sqrt(torch.nn.functional.softplus(v, threshold=20.0))
+
+
+@pytest.mark.parametrize("l", [-19.9, -20.1, -40.0, -88.0])
+def test_sqrt_softplus_far_branch(cuda_device, l):
+    """Down to -88 the score is the gate's log1p(exp(-l)) branch."""
+    from objeta_b200.router import balance_loss, router_backward
+    v = U.randn((9, 24), seed=3)
+    v[:, 7] = l
+    v[4] = l
+    ids = torch.topk(v, 2, dim=1).indices.to(torch.int32)
+    dw = U.randn((9, 2), seed=4)
+    b = balance_loss(v, ids, score_func=SQRT_SOFTPLUS)
+    dl = router_backward(v, ids, dw, score_func=SQRT_SOFTPLUS, renormalize=True, balance=b, balance_grad=0.5)
+    _, _, rb, _, rdl, mag = reference(v, ids, SQRT_SOFTPLUS, None, None, dw, True, 1.0, 0.5, 0.0)
+    assert abs(float(b.balance) - rb) <= 64 * 2.0 ** -24 * rb
+    U.check(dl, rdl, 64 * 2.0 ** -24 * mag + 1e-37)
