@@ -747,7 +747,8 @@ int objb_balance_loss_device(const float *d_logits, size_t logits_stride, const 
                              void *d_scratch, size_t scratch_bytes, objb_stream_t stream);
 
 /* The whole gradient of the logits in one pass: through the routing weights
- * w_j = route_scale * s[ids_j] (divided by sum_j s[ids_j] when renormalize;
+ * w_j = route_scale * s[ids_j] (divided by sum_j s[ids_j] when renormalize,
+ * whichever ids are given, unless all their scores are 0 or below exp(-128);
  * their gradient d_dweights [num_tokens][top_k] may be NULL), plus
  * balance_grad and z_grad times the gradients of the two losses (d_counts and
  * d_scales of objb_balance_loss_device; both NULL: no losses).  Rows of

@@ -9,8 +9,88 @@
 namespace objb {
 namespace dev {
 
+// A token whose renormalised weights' scores (nearly) underflow: given ids need
+// not be the largest.  With q = exp(l - top) relative to the largest selected (a
+// sigmoid is its exponential there) w = q / sum q and dl = w (dw - mean), not by
+// way of the scores, down to scores of exp(-128), which f32 has long lost; a
+// mask is far below.  One at a time, behind the ordinary tokens and out of
+// line: beside them its registers would cost those 12 % (32768 x 256).
+// `mine`: the team has one (the teams of a warp run in step).  g: zeros, and
+// left as such.
 template <class TM, int FUNC>
-__global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1) router_backward_kernel(const RouterBackwardArgs a) {
+__device__ __noinline__ void far_token(const RouterBackwardArgs& a, long long t, bool mine, float* g, float* red) {
+  const int r = TM::rank(), E = mine ? a.E : 0, k = mine ? a.k : 0;
+  if (!mine) t = 0;
+  const float* l = a.logits + t * a.ld;
+  const int32_t* ids = a.ids + t * a.k;
+  const float* dw = a.dw + t * a.k;
+  auto selected = [&](auto f) {
+    for (int j = r; j < k; j += TM::L) {
+      const int e = ids[j];
+      if (e >= 0 && e < E) f(l[e], dw[j]);
+    }
+    __syncwarp();
+  };
+  auto experts = [&](auto f) {
+    for (int e = r; e < E; e += TM::L) f(e, l[e]);
+    __syncwarp();
+  };
+  // the row's statistics
+  float m = neg_inf(), sum = 0.0f;
+  experts([&](int, float v) { m = fmaxf(m, v); });
+  m = TM::max(m, red);
+  const float base = m > neg_inf() ? m : 0.0f;
+  experts([&](int, float v) { sum += exp_sfu(v - base); });
+  sum = TM::sum(sum, red);
+  const float inv = sum == 0.0f ? 0.0f : rcp_sfu(sum), lse = sum == 0.0f ? 0.0f : base + __logf(sum);
+  // the weights
+  float top = neg_inf(), q = 0.0f, wq = 0.0f, rest = 0.0f;
+  selected([&](float v, float) { top = fmaxf(top, v); });
+  top = TM::max(top, red);
+  const bool some = top - (FUNC == kSoftmax ? lse : 0.0f) > -128.0f;
+  selected([&](float v, float w) {
+    const float x = some ? exp_sfu(v - top) : 0.0f;
+    q += x;
+    wq = fmaf(x, w, wq);
+  });
+  q = TM::sum(q, red);
+  const float iq = some ? rcp_sfu(q) : 0.0f;
+  const float mean = TM::sum(wq, red) * iq;
+  selected([&](float v, float w) { rest = some ? fmaf(exp_sfu(v - top), w - mean, rest) : 0.0f; });
+  rest = TM::sum(rest, red) * iq;
+  if (r == 0 && some)
+    for (int j = 0; j < k; ++j) {
+      const int e = ids[j];
+      if (e >= 0 && e < E) g[e] += a.route_scale * (exp_sfu(l[e] - top) * iq * ((dw[j] - mean) - rest));
+    }
+  // the losses
+  const int seq = mine ? sequence_of(a.off, a.S, t) : 0;
+  const float zc = a.counts && a.z_grad != 0.0f ? a.z_grad * a.scales[a.S] : 0.0f;
+  const float c = a.counts ? a.balance_grad * a.scales[seq] : 0.0f;
+  auto B = [&](int e) { return a.counts ? c * static_cast<float>(a.counts[static_cast<size_t>(seq) * E + e]) : 0.0f; };
+  float ssum = 0.0f, bsum = 0.0f, d;
+  experts([&](int e, float v) {
+    const float s = FUNC == kSoftmax ? exp_sfu(v - base) * inv : score_of(FUNC, v, &d);
+    ssum += s;
+    bsum = fmaf(B(e), s, bsum);
+  });
+  ssum = TM::sum(ssum, red);
+  bsum = TM::sum(bsum, red);
+  const float is = FUNC == kSoftmax ? 1.0f : ssum == 0.0f ? 0.0f : rcp_sfu(ssum);
+  TM::sync();
+  experts([&](int e, float v) {
+    const float p = exp_sfu(v - base) * inv;
+    d = p;
+    if (FUNC != kSoftmax) score_of(FUNC, v, &d);
+    a.out[t * a.ld_out + e] = g[e] + d * (B(e) * is - bsum * is * is) + zc * lse * p;
+    g[e] = 0.0f;
+  });
+  TM::sync();
+}
+
+template <class TM, int FUNC>
+__global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
+    router_backward_kernel(const __grid_constant__ RouterBackwardArgs a) {
   constexpr int EPL = TM::EPL, L = TM::L;
   extern __shared__ __align__(16) uint8_t router_smem[];
   __shared__ float red[kTeamWarps];
@@ -51,6 +131,7 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
   fetch(t0);
   int q = -1;
   long long q_end = t0;  // where the sequence q ends
+  unsigned aside = 0;  // steps of far tokens (per_team is 32 at most)
   for (int step = 0; step < a.per_team; ++step) {  // the teams of a warp in step
     const long long t = t0 + step;
     const bool here = t < t1;
@@ -74,6 +155,7 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
       }
     }
     in = in && q >= 0 && q < a.S;
+    bool far = false;
     float dl[EPL];
     if (TM::kBlock ? in : __any_sync(0xFFFFFFFFu, in)) {
       // exponentials, where the score or the z loss wants them
@@ -132,6 +214,7 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
           mean = wq * iq;
           rest = sums(mean, nullptr) * iq;
           if (Q > 0.0f) c *= iq;
+          far = FUNC != kSqrtSoftplus && in && Q < 1e-30f;
         }
         // a team's (a block's first warp's) slots at a time; equal ids among them are added in slot order
         constexpr int W = TM::kBlock ? 32 : L;
@@ -216,7 +299,7 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
 #pragma unroll
       for (int i = 0; i < EPL; ++i) dl[i] = 0.0f;
     }
-    if (here) {
+    if (here && !far) {
       float* o = a.out + t * a.ld_out;
       if constexpr (TM::kQuads) {
 #pragma unroll
@@ -232,7 +315,13 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
         }
       }
     }
+    if (far) aside |= 1u << step;
   }
+  if (FUNC != kSqrtSoftplus && (TM::kBlock ? aside != 0 : __any_sync(0xFFFFFFFFu, aside)))
+    for (int step = 0; step < a.per_team; ++step) {
+      const bool mine = aside >> step & 1;
+      if (TM::kBlock ? mine : __any_sync(0xFFFFFFFFu, mine)) far_token<TM, FUNC>(a, t0 + step, mine, g, red);
+    }
 }
 
 }  // namespace dev
@@ -242,9 +331,9 @@ int launch_router_backward(dev::RouterBackwardArgs a, bool v4, const DeviceProps
     return with_func(a.func, [&](auto func) {
       using TM = decltype(tm);
       const size_t teams = 256 / TM::L;
-      // up to three blocks per SM (what the registers allow), each team a run of consecutive tokens
+      // up to three blocks per SM (what the registers allow), each team a run of consecutive tokens, 32 at most
       const size_t most = static_cast<size_t>(TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1) * props.sm_count * teams;
-      a.per_team = static_cast<int>((static_cast<size_t>(a.T) + most - 1) / most);
+      a.per_team = static_cast<int>(std::min<size_t>(32, (static_cast<size_t>(a.T) + most - 1) / most));
       const size_t per_block = teams * a.per_team;
       const size_t smem = teams * ((static_cast<size_t>(a.E) + 3) / 4 * 4) * 4;
       return launch_pdl(dev::router_backward_kernel<TM, decltype(func)::value>,

@@ -75,3 +75,62 @@ def test_sqrt_softplus_far_branch(cuda_device, l):
     _, _, rb, _, rdl, mag = reference(v, ids, SQRT_SOFTPLUS, None, None, dw, True, 1.0, 0.5, 0.0)
     assert abs(float(b.balance) - rb) <= 64 * 2.0 ** -24 * rb
     U.check(dl, rdl, 64 * 2.0 ** -24 * mag + 1e-37)
+
+
+@pytest.mark.parametrize("func", [SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("E,k", [(16, 3), (60, 8), (120, 12), (256, 8), (600, 3), (600, 40), (1500, 40)])
+def test_renormalised_weights_of_far_ids(cuda_device, func, E, k):
+    """Given ids (a hash layer's) whose scores underflow beside the others':
+    the renormalised weights are still a share of one another.  Ordinary
+    tokens between them, and the losses' gradients beside."""
+    from objeta_b200.router import balance_loss, router_backward
+    far = [0.0, 60.0, 69.5, 86.0, 87.5, 0.0, 88.5, 90.0, 95.0, 100.0, 101.0, 0.0]
+    T = len(far)
+    l = U.randn((T, E), seed=E)
+    l[:, E - 1] = 1.0
+    gen = torch.Generator().manual_seed(E)
+    ids = torch.stack([torch.randperm(E - 1, generator=gen)[:k] for _ in range(T)]).to(torch.int32).cuda()
+    down = torch.tensor(far, device="cuda")[:, None] + math.log(E) * (func == SIGMOID)
+    l.scatter_(1, ids.long(), (l.gather(1, ids.long()).clamp(min=-1.5, max=1.5) - down).float())
+    dw = U.randn((T, k), seed=6)
+    b = balance_loss(l, ids, score_func=func)
+    for kw, bg, zg in ((dict(), 0.0, 0.0), (dict(balance=b, balance_grad=0.3, z_grad=0.02), 0.3, 0.02)):
+        dl = router_backward(l, ids, dw, score_func=func, renormalize=True, route_scale=2.5, **kw)
+        *_, rdl, mag = reference(l, ids, func, None, None, dw, True, 2.5, bg, zg)
+        # a weight's q is off by its exponent's rounding, at most 12 in size once relative to the largest
+        U.check(dl, rdl, (64 + 24) * 2.0 ** -24 * mag + 1e-37, f"{func} {E} {k}")
+
+
+@pytest.mark.parametrize("func", [SOFTMAX, SIGMOID, SQRT_SOFTPLUS])
+@pytest.mark.parametrize("E,k", [(16, 3), (600, 40), (1500, 40)])
+@pytest.mark.parametrize("bad", [-math.inf, LOWEST, -300.0])
+def test_renormalised_weights_of_nothing(cuda_device, func, E, k, bad):
+    """Selected scores that are all 0 (masked ids): a sum of 0 divides nothing, and nothing flows back."""
+    from objeta_b200.router import router_backward
+    T = 6
+    l = U.randn((T, E), seed=E)
+    ids = torch.arange(k, dtype=torch.int32, device="cuda").expand(T, k).contiguous()
+    l[:, :k] = bad
+    l[3, :k] = 0.5  # an ordinary token among them
+    dw = U.randn((T, k), seed=6)
+    dl = router_backward(l, ids, dw, score_func=func, renormalize=True)
+    rest = torch.arange(T, device="cuda") != 3
+    assert not dl[rest].any() and bool(torch.isfinite(dl).all()) and bool(dl[3].any())
+
+
+@pytest.mark.parametrize("func", [SOFTMAX, SIGMOID])
+def test_far_ids_of_long_runs(cuda_device, func):
+    """More tokens than the teams of one round hold, every seventh with far ids."""
+    from objeta_b200.router import router_backward
+    T, E, k = 6000, 1100, 3
+    l = U.randn((T, E), seed=1)
+    l[::7, :k] -= 95.0
+    ids = torch.topk(l, k, dim=1).indices.to(torch.int32)
+    ids[::7] = torch.arange(k, dtype=torch.int32, device="cuda")
+    dw = U.randn((T, k), seed=2)
+    dl = router_backward(l, ids, dw, score_func=func, renormalize=True)
+    *_, rdl, mag = reference(l, ids, func, None, None, dw, True, 1.0, 0.0, 0.0)
+    U.check(dl, rdl, (64 + 24) * 2.0 ** -24 * mag + 1e-37)
+    inplace = l.clone()
+    router_backward(inplace, ids, dw, score_func=func, renormalize=True, d_dlogits=inplace)
+    assert torch.equal(inplace, dl)
