@@ -112,7 +112,7 @@ __device__ __forceinline__ float rcp_sfu(float x) {
 // are made of, among them) has score 0 and derivative 0, as under the other two.
 __device__ __forceinline__ float score_of(int func, float l, float* d) {
   if (func == kSigmoid) {
-    const float t = exp_sfu(-fabsf(l));
+    const float t = expf(-fabsf(l));  // (of few scores, or of far logits: their exponents are not rounded at |l|)
     const float r = rcp_sfu(1.0f + t);
     *d = t * r * r;
     return l >= 0.0f ? r : t * r;
@@ -135,9 +135,11 @@ __device__ __forceinline__ float score_of(int func, float l, float* d) {
 }
 
 // ex = exp(l - base) of a token's logits; returns their sum.  The first try has
-// base 0: its sum says whether any logit was above 69 or all below -64, and only
-// then (no trained router) is there a maximum to find.  *direct: base is 0 and
-// the exponentials serve the sigmoid too.
+// base 0: its sum says whether the largest logits are within 11.5 of it (1e5,
+// 1e-5), and only else (few trained routers) is there a maximum to find.  An
+// exponent is rounded at |l - base|, so that with base 0 a probability is off
+// by up to 5e-7 instead of 1e-7 (logits around 60: 3e-6, hence the bounds).
+// *direct: base is 0 and the exponentials serve the sigmoid too.
 template <class TM>
 __device__ __forceinline__ float exponentials(const float (&l)[TM::EPL], float (&ex)[TM::EPL], float* red, float* base,
                                               bool* direct) {
@@ -149,7 +151,7 @@ __device__ __forceinline__ float exponentials(const float (&l)[TM::EPL], float (
   }
   sum = TM::sum(sum, red);
   *base = 0.0f;
-  *direct = sum > 1e-28f && sum < 1e30f;
+  *direct = sum > 1e-5f && sum < 1e5f;
   if (TM::kBlock ? !*direct : !__all_sync(0xFFFFFFFFu, *direct)) {
     float m = neg_inf();
 #pragma unroll
