@@ -419,7 +419,7 @@ double nanoseconds(const Product& p, TileKind kind, const Tile& t, size_t sms, c
 }
 
 // Which tile a product takes: the one of the fewest nanoseconds() among
-//   * direct: pairs, 512 x up to 256 columns, for 16-bit results of one-plane operands (k up to kDirectK);
+//   * direct: pairs, 512 x up to 256 columns, for 16-bit results of one-plane operands (k up to direct_k);
 //   * pairs of 256 rows x up to 128 columns;
 //   * single CTAs of 128 rows x up to 128 columns, k split over a cluster, one
 //     per SM or (up to 64 columns) two.
@@ -461,7 +461,7 @@ Choice choose_tile(const Product& p, bool y16, size_t sms, const Room& room) {
     });
     return best;
   }
-  if (y16 && p.a.planes == 1 && p.b.planes == 1 && p.K <= dev::kDirectK)
+  if (y16 && p.a.planes == 1 && p.b.planes == 1 && p.K <= dev::direct_k(p.a.dtype == OBJB_DTYPE_F16))
     each_bn(256, mn ? 128 : 16, 144, [&](int bn) {
       c.bn = bn;
       consider(kDirect, c);
@@ -529,7 +529,7 @@ struct ChoiceKey {
 int gemm(const Product& p, int device, const DeviceProps& props, cudaStream_t st) {
   const bool y16 = !p.gated && p.epi.y_dtype != OBJB_DTYPE_F32;
   const ChoiceKey key{p.M, p.N, p.K, static_cast<size_t>(props.sm_count), p.maj, p.a.planes, p.b.planes,
-                      (y16 ? 1 : 0) | (p.gated ? 2 : 0) | p.raw << 2};
+                      (y16 ? 1 : 0) | (p.gated ? 2 : 0) | p.raw << 2 | (p.a.dtype == OBJB_DTYPE_F16 ? 16 : 0)};
   struct Kept {
     ChoiceKey key{};
     Choice choice;
@@ -544,9 +544,10 @@ int gemm(const Product& p, int device, const DeviceProps& props, cudaStream_t st
   }
   const TileKind kind = k.choice.kind;
   Tile t = k.choice.tile;
-  // MMAs of a chunk err by about 3e-8 of the chunk's sum each: 8 k-blocks keep an f32 result within 5e-7, half
-  // of what f32 sums of 4096 products lose (4 k-blocks: 2.4e-7, 16: 1.0e-6; a chunk's end costs some 400 ns)
-  // (a gated product multiplies two such results: 4)
+  // An MMA into an accumulator takes 2e-8 (bf16) or 8e-8 (f16) of a sum of one sign away: 8 k-blocks (32 MMAs) keep an
+  // f32 result within 7e-7 or 2.5e-6 of it, where f32 sums of 4096 products are off by 8e-7 (relative norm, 1024 x 4096
+  // x 2048); of mixed signs, 4.8e-7 and 6.5e-7 against 6e-7 to 1.1e-6.  (4 k-blocks: half of it, 16: twice; a chunk's
+  // end costs some 400 ns.)  A gated product multiplies two such results: 4.  16-bit results: 2.4e-5 of f16's 4.9e-4.
   t.chunk_kb = y16 ? 64 : p.gated ? 4 : 8;
   switch (p.maj) {
     case dev::kMajKK: return launch_kk(p, kind, t, device, props, st);

@@ -30,8 +30,8 @@
 //     the main one, so 16 times the MMAs err less); twice the columns per tile.
 //   * else straight from tensor memory into the epilogue, which rounds to 16
 //     bits: two accumulators of 256 columns, all of tensor memory, for k up to
-//     65536 (kDirectK).  The ring
-//     goes on filling while a tile is drained.
+//     65536 (bf16) or 16384 (f16; direct_k).  The ring goes on filling while a
+//     tile is drained.
 // CTA pairs (CG 2, cta_group::2) share each MMA: M 256, half of B's rows from
 // each CTA's shared memory.  MT accumulators per CTA (rows m0 + a * rm) share
 // B's stage.  An L2-fed SM takes in about 64 bytes per clock, an MMA of 128 x
@@ -72,7 +72,10 @@ enum { kMajKK = 0, kMajMK = 1, kMajMN = 2 };  // A, B: K-major both; A MN-major;
 constexpr int kLinBK = 64;        // k of a stage: 128 bytes, one swizzle row
 constexpr int kLinStagesMax = 12;
 constexpr int kCrossChunks = 16;  // chunks of a cross product's buffer
-constexpr size_t kDirectK = 65536;  // 4096 MMAs in one accumulator lose 1.2e-4 of a sum of one sign: half of f16's rounding
+// Longest k of one accumulator that is not promoted: what truncation takes from a sum of one sign stays below a fifth of
+// the result's half step.  f16 (2^-11, 4.9e-4): 8.9e-5 at 16384, 3.9e-4 at 65536; bf16 (2^-9 at least, 2e-3), whose
+// products need fewer bits: 1.2e-4 at 65536.
+constexpr size_t direct_k(bool f16) { return f16 ? 16384 : 65536; }
 constexpr int kConvWarps = 8;
 // producer, MMA, eight (PROMOTE) or sixteen epilogue warps, second MMA warp (RAW: producer of raw k-blocks), RAW: the
 // converting warps

@@ -1,0 +1,51 @@
+"""The dense products where accumulators are longest and values are not finite,
+against 64-bit products."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests import _dense_util as U  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dt,K", [("f16", 16384), ("f16", 16448), ("f16", 65536), ("f16", 65600), ("bf16", 65536),
+                                  ("bf16", 65600)])
+def test_longest_accumulators_of_one_sign(cuda_device, dt, K):
+    """Products of one sign over the longest k of an accumulator that is not promoted, and one k-block more, where
+    the tiles fill the device: what truncation takes is a fraction of the result's rounding, and one-sided, so
+    that the mean error shows it."""
+    from objeta_b200.dense import linear
+    T = N = 4096
+    t = U.DT[dt]
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.rand(T, K, generator=g, device="cuda", dtype=t)
+    w = torch.rand(N, K, generator=g, device="cuda", dtype=t) * 0.25
+    y = linear(x, w)[::64, ::64]
+    ref = x[::64].double() @ w[::64].double().t()
+    half = torch.finfo(t).eps / 2
+    loss = half / 4  # f16: a quarter of its half step (1.2e-4); bf16: of its largest (9.8e-4)
+    U.check(y, ref, (half + loss) * ref, "y")
+    # 4096 elements, each off by a rounding of at most half a step: their mean by half / sqrt(3) / 64 in a deviation,
+    # six of which make half / 18
+    mean = float(((y.double() - ref) / ref).mean())
+    assert abs(mean) <= loss + half / 18, mean
+
+
+def test_choice_of_tile_knows_the_type(cuda_device):
+    """The same sizes in both 16-bit types, one after the other: each has its own longest accumulator."""
+    from objeta_b200.dense import linear
+    T = N = 2048
+    K = 40000
+    for dt in ("bf16", "f16", "bf16", "f16"):
+        t = U.DT[dt]
+        g = torch.Generator(device="cuda").manual_seed(7)
+        x = torch.rand(T, K, generator=g, device="cuda", dtype=t)
+        w = torch.rand(N, K, generator=g, device="cuda", dtype=t) * 0.25
+        y = linear(x, w)[::32, ::32]
+        ref = x[::32].double() @ w[::32].double().t()
+        half = torch.finfo(t).eps / 2
+        U.check(y, ref, 1.25 * half * ref, dt)
+        assert abs(float(((y.double() - ref) / ref).mean())) <= half / 4 + half / 18, dt
