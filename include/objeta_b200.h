@@ -708,7 +708,9 @@ int objb_linear_backward_device(const objb_linear_backward_desc *desc, const voi
 
 /* objb_ffn_bf16_device for num_tokens tokens (the shared expert of a batch):
  * out[t] = residual[t] + down SwiGLU(gate x_t, up x_t), the SwiGLU (and its
- * limit) as silu_mul computes it (moe.cu:2-22).  x [tokens][hidden], out and
+ * limit) as silu_mul computes it (moe.cu:2-22), but for NaN, which stays NaN
+ * (silu_mul and the one-token call clamp it to the limit; infinities are
+ * clamped here too).  x [tokens][hidden], out and
  * residual [tokens][out_dim] f32, contiguous; residual may be NULL, or out
  * itself (routed output + shared output); weights bf16 as there. */
 int objb_ffn_bf16_tokens_scratch_bytes(const void *d_gate, const void *d_up, const void *d_down,

@@ -153,6 +153,12 @@ __device__ __forceinline__ void raw_split(const float (&v)[8], uint32_t to, uint
                  : "memory");
 }
 
+// swiglu's clamps (fminf, fmaxf, as the reference has them) turn NaN into the limit: a bad token would come out finite.
+__device__ __forceinline__ float swiglu_keeping_nan(float g, float u, float limit) {
+  const float v = swiglu(g, u, limit);
+  return g == g && u == u ? v : g + u;
+}
+
 // SWIZZLE_128B operand tiles, without their address.  K-major: rows of 128
 // bytes, 8-row groups 1024 bytes apart.  MN-major: 64 rows x 64 k as 64 k rows
 // of 128 bytes; 8-k groups 1024 bytes apart (stride offset), the next 64 rows
@@ -701,7 +707,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
             const long long tile_end = n0 + g.bn < g.N ? n0 + g.bn : g.N;
             if (ok && mf < g.M)
               for (int c = tid >> 6; n0 + c < tile_end; c += 4)
-                g.epi.put_planes(mf, n0 + c, swiglu(e[c * 128], e[c * 128 + 64], g.swiglu_limit));
+                g.epi.put_planes(mf, n0 + c, swiglu_keeping_nan(e[c * 128], e[c * 128 + 64], g.swiglu_limit));
             asm volatile("bar.sync 1, 256;" ::: "memory");
           }
         } else if (ok && m_ok) {
@@ -751,7 +757,7 @@ __global__ void __launch_bounds__(LinShape<MAJ, BN, CG, MT, GATED, PROMOTE, PB, 
             gate += lin_ld_cluster(at);
             up += lin_ld_cluster(at + 256);
           }
-          g.epi.put_planes(m, n0 + c, swiglu(gate, up, g.swiglu_limit));
+          g.epi.put_planes(m, n0 + c, swiglu_keeping_nan(gate, up, g.swiglu_limit));
         }
       } else {
         // threads of 128 rows by two halves of this CTA's columns

@@ -199,7 +199,8 @@ def ffn_bf16_tokens(d_gate, d_up, d_down, d_x, d_residual=None, d_out=None, swig
 
     d_gate, d_up [I, H] and d_down [O, I] bf16, d_x f32 [T, H], d_residual f32
     [T, O] or None; ``d_out`` may be ``d_residual`` itself.  f32 precision
-    throughout, as the one-token call.
+    throughout, as the one-token call.  With ``swiglu_limit`` infinities are
+    clamped and NaN stays NaN (the one-token call clamps it, as the reference).
     """
     dev = on_device("d_x", d_x, None, _F32)
     if d_x.dim() != 2:

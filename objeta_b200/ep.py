@@ -378,7 +378,8 @@ class ExpertParallelMoe:
     ``shared``: (gate, up, down) bf16 CUDA tensors [I, H], [I, H], [O, I] of a
     shared expert that every rank holds whole; it runs over this rank's own
     tokens and is added to the routed output (``ffn_bf16_device`` for one
-    token, ``ffn_bf16_tokens`` for more), with the same ``swiglu_limit``."""
+    token, ``ffn_bf16_tokens`` for more), with the same ``swiglu_limit``
+    (under which the call for one token clamps NaN, that for more keeps it)."""
 
     def __init__(self, layer, num_experts: int, top_k: int, rank: int = 0, world: int = 1, group=None,
                  out_dim: int | None = None, compute=None, combine=None, swiglu_limit: float = 0.0,

@@ -49,3 +49,25 @@ def test_choice_of_tile_knows_the_type(cuda_device):
         half = torch.finfo(t).eps / 2
         U.check(y, ref, 1.25 * half * ref, dt)
         assert abs(float(((y.double() - ref) / ref).mean())) <= half / 4 + half / 18, dt
+
+
+@pytest.mark.parametrize("limit", [0.0, 1.0])
+@pytest.mark.parametrize("T,H,I,O", [(2, 256, 128, 64), (16, 512, 300, 200), (17, 128, 64, 64), (300, 256, 192, 256),
+                                     (700, 264, 800, 1000)])
+def test_ffn_keeps_nan(cuda_device, T, H, I, O, limit):
+    """NaN in a token makes its row NaN, also through the limited SwiGLU, and no other; in a weight all rows."""
+    from objeta_b200.dense import ffn_bf16_tokens
+    x = U.randn((T, H), seed=1)
+    g, u = (U.randn((I, H), torch.bfloat16, 1 / math.sqrt(H), s) for s in (2, 3))
+    d = U.randn((O, I), torch.bfloat16, 1 / math.sqrt(I), 4)
+    want = ffn_bf16_tokens(g, u, d, x, swiglu_limit=limit)
+    assert bool(torch.isfinite(want).all())
+    bad = x.clone()
+    bad[1, 5] = math.nan
+    out = ffn_bf16_tokens(g, u, d, bad, swiglu_limit=limit)
+    rest = torch.arange(T, device="cuda") != 1
+    assert bool(torch.isnan(out[1]).all()) and torch.equal(out[rest], want[rest])
+    for i in range(2):
+        w = [g.clone(), u.clone()]
+        w[i][I - 1, H - 1] = math.nan
+        assert bool(torch.isnan(ffn_bf16_tokens(w[0], w[1], d, x, swiglu_limit=limit)).all()), i
