@@ -379,7 +379,10 @@ class ExpertParallelMoe:
     shared expert that every rank holds whole; it runs over this rank's own
     tokens and is added to the routed output (``ffn_bf16_device`` for one
     token, ``ffn_bf16_tokens`` for more), with the same ``swiglu_limit``
-    (under which the call for one token clamps NaN, that for more keeps it)."""
+    (under which the call for one token clamps NaN, that for more keeps it).
+    Its kernels and the order of its sums are chosen from T: bit-identity
+    over rank counts is the routed part's, the shared one's bits hold for
+    one T."""
 
     def __init__(self, layer, num_experts: int, top_k: int, rank: int = 0, world: int = 1, group=None,
                  out_dim: int | None = None, compute=None, combine=None, swiglu_limit: float = 0.0,
@@ -402,16 +405,25 @@ class ExpertParallelMoe:
             raise ValueError("grouped='on' needs a Q4_0 layer with hidden, intermediate multiples of 256")
         self.grouped = grouped
         if shared is not None:
-            gate, up, down = shared
-            if gate.shape != up.shape or down.dim() != 2 or down.shape != (self.out_dim, gate.shape[0]):
-                raise ValueError(f"shared expert shapes {tuple(gate.shape)}, {tuple(up.shape)}, {tuple(down.shape)} "
-                                 f"do not make [I, H], [I, H], [{self.out_dim}, I]")
+            self._check_shared(*shared)
         self.shared = shared
         self.last_plan = None
         self.phase_events = None  # a list: forward() appends (phase, CUDA event) boundaries to it
         self._pin = None     # pinned int32 staging for plan arrays (grow-only)
         self._dmeta = None   # device copy (grow-only)
         self._slot_cache = {}
+
+    def _check_shared(self, gate, up, down):
+        import torch
+        if gate.dim() != 2 or gate.shape != up.shape or down.shape != (self.out_dim, gate.shape[0]):
+            raise ValueError(f"shared expert shapes {tuple(gate.shape)}, {tuple(up.shape)}, {tuple(down.shape)} "
+                             f"do not make [I, H], [I, H], [{self.out_dim}, I]")
+        if self.layer is not None and gate.shape[1] != self.layer.hidden:
+            raise ValueError(f"shared expert of hidden size {gate.shape[1]} beside a layer of {self.layer.hidden}")
+        for name, t in zip(("gate", "up", "down"), (gate, up, down)):
+            if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != gate.device or not t.is_cuda:
+                raise ValueError(f"shared expert {name}: expected contiguous bf16 CUDA tensors on one device, got "
+                                 f"{t.dtype} on {t.device}, strides {t.stride()}")
 
     def _stage(self, arrays, dev):
         """One H2D copy of the int32 plan arrays; returns device views.  The

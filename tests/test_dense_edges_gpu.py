@@ -71,3 +71,34 @@ def test_ffn_keeps_nan(cuda_device, T, H, I, O, limit):
         w = [g.clone(), u.clone()]
         w[i][I - 1, H - 1] = math.nan
         assert bool(torch.isnan(ffn_bf16_tokens(w[0], w[1], d, x, swiglu_limit=limit)).all()), i
+
+
+def test_expert_parallel_shared_expert_of_every_batch(cuda_device):
+    """Checks of the shared expert's weights, and the same tokens in batches of several sizes: within the bound of
+    one another (the shared part's bits go with the batch)."""
+    from objeta_b200.ep import ExpertParallelMoe, router_topk_batched
+    from objeta_b200.moe import MoeLayer
+    from objeta_b200.quant import QGemvShape, QuantBackend, QuantFormat
+    from tests.test_dense_gpu import _ffn_ref
+    T, H, I, E, k, Is = 40, 256, 256, 8, 2, 192
+    qb = QuantBackend(0)
+    pack = lambda r, c, s: qb.quantize_matrix_device(QuantFormat.Q4_0, U.randn((r, c), scale=0.05, seed=s),
+                                                     QGemvShape.q4_0(r, c))
+    layer = MoeLayer(QuantFormat.Q4_0, H, I, H, [pack(I, H, 3 * e) for e in range(E)],
+                     [pack(I, H, 3 * e + 1) for e in range(E)], [pack(H, I, 3 * e + 2) for e in range(E)])
+    g, u = U.randn((Is, H), torch.bfloat16, 1 / 16, 91), U.randn((Is, H), torch.bfloat16, 1 / 16, 92)
+    d = U.randn((H, Is), torch.bfloat16, 1 / 14, 93)
+    x = U.randn((T, H), seed=94)
+    ids, w = router_topk_batched(U.randn((T, E), seed=95), k, renormalize=True)
+    moe = ExpertParallelMoe(layer, E, k, shared=(g, u, d))
+    routed = ExpertParallelMoe(layer, E, k).forward(x, ids, w)
+    ref = _ffn_ref(g, u, d, x, routed, 0.0)
+    at = 0
+    for n in (1, 3, 16, 20):
+        rows = slice(at, at + n)
+        U.check(moe.forward(x[rows], ids[rows], w[rows]), ref[0][rows], ref[1][rows], f"{n} tokens")
+        at += n
+    for bad in ((g.half(), u.half(), d.half()), (g.float(), u.float(), d.float()), (g, u, d.t().contiguous().t()),
+                (g.cpu(), u.cpu(), d.cpu()), (g[:, :128].contiguous(), u[:, :128].contiguous(), d)):
+        with pytest.raises(ValueError, match="shared expert"):
+            ExpertParallelMoe(layer, E, k, shared=bad)

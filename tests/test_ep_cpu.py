@@ -232,3 +232,29 @@ def test_grouped_path_selection():
             E.ExpertParallelMoe(bad, 256, 8, grouped="on")
     with pytest.raises(ValueError):
         E.ExpertParallelMoe(ok, 256, 8, grouped="yes")
+
+
+def test_shared_expert_refusals():
+    """The shared expert's weights are checked once, whatever T a step has (the one-token call reads bare pointers)."""
+    import torch
+    from objeta_b200.ep import ExpertParallelMoe
+
+    def make(gate, up, down):
+        return ExpertParallelMoe(None, 4, 2, out_dim=16, compute=lambda *a: None, combine=lambda *a: None,
+                                 shared=(gate, up, down))
+
+    b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="shapes"):
+        make(b(8, 32), b(8, 31), b(16, 8))
+    with pytest.raises(ValueError, match="shapes"):
+        make(b(8, 32), b(8, 32), b(8, 16))
+    with pytest.raises(ValueError, match="shapes"):
+        make(b(8), b(8), b(16, 8))
+    with pytest.raises(ValueError, match="gate.*float16"):
+        make(b(8, 32).half(), b(8, 32).half(), b(16, 8).half())
+    with pytest.raises(ValueError, match="down.*float32|gate.*cpu"):
+        make(b(8, 32), b(8, 32), b(16, 8).float())
+    with pytest.raises(ValueError, match="strides"):
+        make(b(32, 8).t(), b(32, 8).t(), b(16, 8))
+    with pytest.raises(ValueError, match="CUDA"):
+        make(b(8, 32), b(8, 32), b(16, 8))
