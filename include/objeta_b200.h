@@ -641,7 +641,9 @@ int objb_deepseek_gate_device(const float *d_gate_weight, const float *d_gate_bi
  * parts (8 + 8 + 8 bits), so f32 products keep f32's precision.  A non-finite
  * operand makes its row and column of the product non-finite (Inf or NaN).
  * Rows are contiguous; strides are in elements between rows, 0 for contiguous.
- * Results overlap no operand, but for the residual named below.
+ * Results overlap neither each other nor what the call reads, but where it is
+ * named below; arrays that plainly do are refused (rows of different strides
+ * lying among one another are not looked through).
  * Any sizes, strides and element-aligned addresses are taken: operands that
  * the copy engine cannot read (16-byte aligned rows) are laid out again in
  * the scratch, which costs one pass over them.  tokens <= 2^30, features <=
@@ -712,7 +714,8 @@ int objb_linear_backward_device(const objb_linear_backward_desc *desc, const voi
  * (silu_mul and the one-token call clamp it to the limit; infinities are
  * clamped here too).  x [tokens][hidden], out and
  * residual [tokens][out_dim] f32, contiguous; residual may be NULL, or out
- * itself (routed output + shared output); weights bf16 as there. */
+ * itself (routed output + shared output), and out may be x; weights bf16 as
+ * there. */
 int objb_ffn_bf16_tokens_scratch_bytes(const void *d_gate, const void *d_up, const void *d_down,
                                        size_t hidden, size_t intermediate, size_t out_dim,
                                        size_t num_tokens, size_t *bytes);

@@ -594,6 +594,10 @@ int check_stride(const char* action, const char* name, size_t stride, size_t col
   return OBJB_OK;
 }
 
+Rows rows_of(const void* p, size_t rows, size_t cols, size_t ld, int dtype) {
+  return {p, rows, cols * elem_bytes(dtype), ld * elem_bytes(dtype)};
+}
+
 // The caller's scratch, or the stream's workspace.
 int take_scratch(const char* action, void* d_scratch, size_t have, size_t need, cudaStream_t st, uint8_t** out) {
   void* ws = d_scratch;
@@ -775,6 +779,14 @@ int objb_linear_device(const objb_linear_desc* desc, const void* d_x, const void
   if (d_residual == d_y && ldr != ldy)
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "a residual in place needs y's stride");
   if (d_z == d_y) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "z and y are the same array");
+  const size_t eb = elem_bytes(d.y_dtype), N = d.out_features;
+  const Rows x = rows_of(d_x, d.tokens, d.in_features, ldx, d.x_dtype), w = rows_of(d_w, N, d.in_features, ldw, d.w_dtype);
+  const Rows bias{d_bias, 1, N * elem_bytes(d.bias_dtype), N * elem_bytes(d.bias_dtype)};
+  const Rows y{d_y, d.tokens, N * eb, ldy * eb}, z{d_z, d.tokens, N * eb, ldz * eb};
+  const Rows res{d_residual, d.tokens, N * eb, ldr * eb};
+  if (overlap(y, x) || overlap(y, w) || overlap(y, bias) || overlap(y, z) || (d_residual != d_y && overlap(y, res)) ||
+      overlap(z, x) || overlap(z, w) || overlap(z, bias) || overlap(z, res))
+    return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "y or z overlaps an operand or the other");
   int device = 0;
   DeviceProps props;
   OBJB_TRY(device_here(&device, &props));
@@ -853,6 +865,21 @@ int objb_linear_backward_device(const objb_linear_backward_desc* desc, const voi
       (d.tokens && (!d_dy || (d.activation != OBJB_ACT_NONE && !d_z) || (want_dw && !d_x) ||
                     (want_dx && (!d_w || !d_dx)))))
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null device pointer");
+  {
+    const size_t T = d.tokens, K = d.in_features, N = d.out_features;
+    const Rows out[3] = {rows_of(want_dx ? d_dx : nullptr, T, K, lddx, d.x_dtype),
+                         rows_of(want_dw ? d_dw : nullptr, N, K, lddw, d.dw_dtype),
+                         rows_of(want_db ? d_dbias : nullptr, 1, N, N, OBJB_DTYPE_F32)};
+    // (what the call reads)
+    const Rows in[4] = {rows_of(d_dy, T, N, lddy, d.dy_dtype),
+                        rows_of(d.activation != OBJB_ACT_NONE ? d_z : nullptr, T, N, ldz, d.dy_dtype),
+                        rows_of(want_dw ? d_x : nullptr, T, K, ldx, d.x_dtype),
+                        rows_of(want_dx ? d_w : nullptr, N, K, ldw, d.w_dtype)};
+    bool bad = overlap(out[0], out[1]) || overlap(out[0], out[2]) || overlap(out[1], out[2]);
+    for (const Rows& o : out)
+      for (const Rows& i : in) bad = bad || overlap(o, i);
+    if (bad) return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "a gradient overlaps an operand or another gradient");
+  }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d.tokens == 0) {  // sums over nothing
     if (want_dw && !d.accumulate)
@@ -977,6 +1004,13 @@ int objb_ffn_bf16_tokens_device(const void* d_gate, const void* d_up, const void
   if (num_tokens == 0) return OBJB_OK;
   if (!d_gate || !d_up || !d_down || !d_x || !d_out)
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null device pointer");
+  // (out may lie over x, which is read before the first result is written)
+  const Rows out = rows_of(d_out, 1, num_tokens * out_dim, num_tokens * out_dim, OBJB_DTYPE_F32);
+  auto weight = [](const void* p, size_t n) { return rows_of(p, 1, n, n, OBJB_DTYPE_BF16); };
+  if (overlap(out, weight(d_gate, intermediate * hidden)) || overlap(out, weight(d_up, intermediate * hidden)) ||
+      overlap(out, weight(d_down, out_dim * intermediate)) ||
+      (d_residual != d_out && overlap(out, rows_of(d_residual, 1, num_tokens * out_dim, num_tokens * out_dim, OBJB_DTYPE_F32))))
+    return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "out overlaps a weight, or the residual without being it");
   int device = 0;
   DeviceProps props;
   OBJB_TRY(device_here(&device, &props));

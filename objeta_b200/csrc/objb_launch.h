@@ -5,6 +5,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <utility>
 
 namespace objb {
 
@@ -56,5 +57,28 @@ size_t pipe_smem_bytes(const RowLayoutHost& L);
 int ensure_smem_attr_ptr(const void* kernel, int device, size_t bytes);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Rows of `width` bytes, `pitch` (>= width) apart; p null: nothing.
+struct Rows {
+  const void* p;
+  size_t rows, width, pitch;
+};
+// Whether two arrays share a byte.  Rows of different pitches that lie among one
+// another are not looked through: false.
+inline bool overlap(Rows a, Rows b) {
+  if (!a.p || !b.p || !a.rows || !b.rows || !a.width || !b.width) return false;
+  for (Rows* r : {&a, &b})
+    if (r->pitch == r->width) r->width *= r->rows, r->rows = 1;
+  auto begin = [](const Rows& r) { return reinterpret_cast<uintptr_t>(r.p); };
+  auto end = [&](const Rows& r) { return begin(r) + (r.rows - 1) * r.pitch + r.width; };
+  if (begin(a) >= end(b) || begin(b) >= end(a)) return false;
+  if (a.rows == 1) std::swap(a, b);
+  if (a.rows == 1) return true;
+  if (b.rows > 1 && b.pitch != a.pitch) return false;
+  // b's first row from the start of a's row at or before it: within that row, or into the next
+  const size_t pitch = a.pitch;
+  const size_t d = begin(b) >= begin(a) ? (begin(b) - begin(a)) % pitch : (pitch - (begin(a) - begin(b)) % pitch) % pitch;
+  return d < a.width || d + b.width > pitch;
+}
 
 }  // namespace objb

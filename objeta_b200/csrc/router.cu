@@ -263,6 +263,14 @@ int objb_router_backward_device(const float* d_logits, size_t logits_stride, con
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "a row stride is below num_experts");
   if (d_logits == d_dlogits && ld != ldo)
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "in place needs equal row strides");
+  {
+    const size_t T = num_tokens, E = num_experts, slots = T * top_k * 4, nc = num_seqs * E * 4, ns = (num_seqs + 1) * 4;
+    const Rows out{d_dlogits, T, E * 4, ldo * 4};
+    if ((d_logits != d_dlogits && overlap(out, {d_logits, T, E * 4, ld * 4})) || overlap(out, {d_ids, 1, slots, slots}) ||
+        overlap(out, {d_dweights, 1, slots, slots}) || overlap(out, {d_counts, 1, nc, nc}) ||
+        overlap(out, {d_scales, 1, ns, ns}) || overlap(out, {d_seq_offsets, 1, ns, ns}) || overlap(out, {d_token_mask, 1, T, T}))
+      return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "dlogits overlaps an operand without being the logits");
+  }
   int device = 0;
   OBJB_TRY(current_device(&device));
   DeviceProps props;
@@ -303,6 +311,12 @@ int objb_moe_combine_backward_device(const float* d_dout, const float* d_v, size
   if (num_tokens == 0) return OBJB_OK;
   if (!d_dout || !d_v || !d_slot_row || !d_dweights || v_rows == 0)
     return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "null device pointer or no value rows");
+  {
+    const size_t n = num_tokens * top_k * 4, o = num_tokens * out_dim * 4, v = v_rows * out_dim * 4;
+    const Rows out{d_dweights, 1, n, n};
+    if (overlap(out, {d_dout, 1, o, o}) || overlap(out, {d_v, 1, v, v}) || overlap(out, {d_slot_row, 1, n, n}))
+      return OBJB_FAIL(OBJB_ERR_INVALID_INPUT, action, "dweights overlaps an operand");
+  }
   int device = 0;
   OBJB_TRY(current_device(&device));
   DeviceProps props;

@@ -5,7 +5,9 @@ The reference's dense paths run one token (``gemv_bf16_device``,
 ``ffn_bf16_device``); these take T of them: the router's projection, the
 shared expert beside ``moe_pairs``, an output head.  Types: x and w both bf16,
 both f16, x f32 with w bf16, or both f32; y f32 or, where x is a 16-bit type,
-that type.  Any sizes, row strides and element-aligned addresses.
+that type.  Any sizes, row strides and element-aligned addresses.  Results
+given by the caller overlap neither each other nor what the call reads, but
+where it says so.
 """
 from __future__ import annotations
 
@@ -198,7 +200,7 @@ def ffn_bf16_tokens(d_gate, d_up, d_down, d_x, d_residual=None, d_out=None, swig
     out[t] = d_residual[t] + down SwiGLU(gate x_t, up x_t).
 
     d_gate, d_up [I, H] and d_down [O, I] bf16, d_x f32 [T, H], d_residual f32
-    [T, O] or None; ``d_out`` may be ``d_residual`` itself.  f32 precision
+    [T, O] or None; ``d_out`` may be ``d_residual`` or ``d_x`` itself.  f32 precision
     throughout, as the one-token call.  With ``swiglu_limit`` infinities are
     clamped and NaN stays NaN (the one-token call clamps it, as the reference).
     """

@@ -102,3 +102,36 @@ def test_expert_parallel_shared_expert_of_every_batch(cuda_device):
                 (g.cpu(), u.cpu(), d.cpu()), (g[:, :128].contiguous(), u[:, :128].contiguous(), d)):
         with pytest.raises(ValueError, match="shared expert"):
             ExpertParallelMoe(layer, E, k, shared=bad)
+
+
+@pytest.mark.parametrize("T,H", [(1, 200), (16, 256), (61, 33), (700, 264)])
+def test_ffn_over_its_input(cuda_device, T, H):
+    """x += ffn(x): x is read before the first result is written."""
+    from objeta_b200.dense import ffn_bf16_tokens
+    I = 136
+    x = U.randn((T, H), seed=1)
+    g, u = (U.randn((I, H), torch.bfloat16, 1 / math.sqrt(H), s) for s in (2, 3))
+    d = U.randn((H, I), torch.bfloat16, 1 / math.sqrt(I), 4)
+    want = ffn_bf16_tokens(g, u, d, x, d_residual=x)
+    for _ in range(3):
+        h = x.clone()
+        assert ffn_bf16_tokens(g, u, d, h, d_residual=h, d_out=h) is h and torch.equal(h, want)
+
+
+def test_results_over_operands_are_refused(cuda_device):
+    from objeta_b200 import CudaError
+    from objeta_b200.dense import linear, linear_backward
+    from objeta_b200.router import router_backward
+    x, w = U.randn((40, 64), torch.bfloat16, seed=1), U.randn((64, 64), torch.bfloat16, seed=2)
+    for kw in (dict(d_y=x), dict(d_y=w[:40]), dict(d_z=x)):
+        with pytest.raises(CudaError, match="overlaps"):
+            linear(x, w, **kw)
+    with pytest.raises(CudaError, match="overlaps"):
+        linear_backward(x, U.randn((40, 64), torch.bfloat16), w, d_dx=x)
+    l = U.randn((41, 8), seed=3)
+    ids = torch.zeros(40, 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(CudaError, match="overlaps"):
+        router_backward(l[:40], ids, U.randn((40, 1)), d_dlogits=l[1:])
+    # side by side in one buffer
+    buf = torch.cat((x, torch.zeros_like(x)), 1)
+    assert torch.equal(linear(buf[:, :64], w, d_y=buf[:, 64:]), linear(x, w))
