@@ -638,8 +638,10 @@ int objb_deepseek_gate_device(const float *d_gate_weight, const float *d_gate_bi
  * F16, x F32 with w BF16, or both F32; y (and residual, z, dy) F32 or, where x
  * is a 16-bit type, that type; bias F32 or w's type.  Products of 16-bit
  * operands are exact and summed in f32; an f32 operand enters as three bf16
- * parts (8 + 8 + 8 bits), so f32 products keep f32's precision.  A non-finite
- * operand makes its row and column of the product non-finite (Inf or NaN).
+ * parts (8 + 8 + 8 bits), so f32 products keep f32's precision (of operands
+ * above 1e-33; what the parts hold ends at 2^-133).  A non-finite operand makes
+ * its row and column of the product non-finite (Inf or NaN: an infinite f32
+ * times a value of fewer bits than three parts is NaN).
  * Rows are contiguous; strides are in elements between rows, 0 for contiguous.
  * Results overlap neither each other nor what the call reads, but where it is
  * named below; arrays that plainly do are refused (rows of different strides

@@ -377,12 +377,12 @@ class ExpertParallelMoe:
 
     ``shared``: (gate, up, down) bf16 CUDA tensors [I, H], [I, H], [O, I] of a
     shared expert that every rank holds whole; it runs over this rank's own
-    tokens and is added to the routed output (``ffn_bf16_device`` for one
-    token, ``ffn_bf16_tokens`` for more), with the same ``swiglu_limit``
-    (under which the call for one token clamps NaN, that for more keeps it).
-    Its kernels and the order of its sums are chosen from T: bit-identity
-    over rank counts is the routed part's, the shared one's bits hold for
-    one T."""
+    tokens and is added to the routed output, with the same ``swiglu_limit``:
+    ``ffn_bf16_device`` for one token where it takes the shapes, else
+    ``ffn_bf16_tokens`` (under a limit the former clamps NaN, the latter keeps
+    it).  Its kernels and the order of its sums are chosen from T:
+    bit-identity over rank counts is the routed part's, the shared one's bits
+    hold for one T."""
 
     def __init__(self, layer, num_experts: int, top_k: int, rank: int = 0, world: int = 1, group=None,
                  out_dim: int | None = None, compute=None, combine=None, swiglu_limit: float = 0.0,
@@ -404,8 +404,13 @@ class ExpertParallelMoe:
         if grouped == "on" and (layer is None or not grouped_supported(layer)):
             raise ValueError("grouped='on' needs a Q4_0 layer with hidden, intermediate multiples of 256")
         self.grouped = grouped
+        self._one_token_shared = False
         if shared is not None:
             self._check_shared(*shared)
+            (I, H), O = shared[0].shape, shared[2].shape[0]
+            # what the one-token call takes: rows of whole 32 columns; unaligned or very long rows up to O <= I
+            self._one_token_shared = (H % 32 == 0 and I % 32 == 0
+                                      and (O <= I or max(H, I) <= 16384 and not any(t.data_ptr() % 16 for t in shared)))
         self.shared = shared
         self.last_plan = None
         self.phase_events = None  # a list: forward() appends (phase, CUDA event) boundaries to it
@@ -577,7 +582,7 @@ class ExpertParallelMoe:
         from .dense import ffn_bf16_tokens
         from .moe import ffn_bf16_device
         gate, up, down = self.shared
-        if x.shape[0] == 1:
+        if x.shape[0] == 1 and self._one_token_shared:
             ffn_bf16_device(gate, up, down, gate.shape[1], gate.shape[0], down.shape[0], x, out, accumulate=True,
                             swiglu_limit=self.swiglu_limit, stream=torch.cuda.current_stream(x.device))
         else:

@@ -135,3 +135,31 @@ def test_results_over_operands_are_refused(cuda_device):
     # side by side in one buffer
     buf = torch.cat((x, torch.zeros_like(x)), 1)
     assert torch.equal(linear(buf[:, :64], w, d_y=buf[:, 64:]), linear(x, w))
+
+
+@pytest.mark.parametrize("Is,shift", [(100, 0), (33, 0), (96, 1), (320, 3), (64, 0)])
+def test_expert_parallel_shared_expert_of_any_width(cuda_device, Is, shift):
+    """Widths and addresses that the one-token call does not take: a step of one token runs as one of more does."""
+    from objeta_b200.ep import ExpertParallelMoe, router_topk_batched
+    from objeta_b200.moe import MoeLayer
+    from objeta_b200.quant import QGemvShape, QuantBackend, QuantFormat
+    from tests.test_dense_gpu import _ffn_ref
+    H, I, E, k = 256, 256, 4, 2
+    qb = QuantBackend(0)
+    pack = lambda r, c, s: qb.quantize_matrix_device(QuantFormat.Q4_0, U.randn((r, c), scale=0.05, seed=s),
+                                                     QGemvShape.q4_0(r, c))
+    layer = MoeLayer(QuantFormat.Q4_0, H, I, H, [pack(I, H, 3 * e) for e in range(E)],
+                     [pack(I, H, 3 * e + 1) for e in range(E)], [pack(H, I, 3 * e + 2) for e in range(E)])
+
+    def at(t):  # `shift` elements off 16-byte alignment
+        buf = torch.empty(t.numel() + shift, dtype=t.dtype, device="cuda")[shift:].view(t.shape)
+        return buf.copy_(t)
+
+    g, u = (at(U.randn((Is, H), torch.bfloat16, 1 / 16, s)) for s in (91, 92))
+    d = at(U.randn((H, Is), torch.bfloat16, 1 / 14, 93))
+    x = U.randn((3, H), seed=94)
+    ids, w = router_topk_batched(U.randn((3, E), seed=95), k, renormalize=True)
+    moe, plain = ExpertParallelMoe(layer, E, k, shared=(g, u, d)), ExpertParallelMoe(layer, E, k)
+    for n in (1, 3):
+        ref, bound = _ffn_ref(g, u, d, x[:n], plain.forward(x[:n], ids[:n], w[:n]), 0.0)
+        U.check(moe.forward(x[:n], ids[:n], w[:n]), ref, bound, f"{Is} {shift} {n}")
