@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(256) image_kernel(const ImageJob first, const 
 // Bound by its bytes: 4096 x 14336 bf16 with SiLU 51.8 us (352 MB), 2048 x 4096
 // f16 with tanh-GELU 12.6 with the fold of the sums.  (Four rows in flight take
 // 80 registers, three blocks an SM: 61 and 13.9; four blocks of 64 registers
-// with as many rows spill: 101.)
+// with as many rows spill so much that they take 101.  The 16-bit kernels as
+// they are spill 32 bytes a thread, 96 where rows are not aligned.)
 struct DzJob {
   const void *dy, *z;
   size_t ldy, ldz;
@@ -384,7 +385,9 @@ struct Room {
   int clusters[2][4] = {};
 };
 
-// Nanoseconds that a product takes, about, from rates measured on B200: a
+// A product's time by a model whose parts were measured apart on B200.  It ranks
+// tiles; its sums do not hold as times (4096^3: 78 us, measured 99; 4096 x 4096 x
+// 14336: 267 and 395; f32 split inside at 16 x 4096 x 16384: 55 and 98).  A
 // producer iteration (wait, expected bytes) 145 and a copy 35; an MMA of 16 of
 // k 20 or bn / 2 clocks, a stage's wait and commit 150; 131 bytes taken in per
 // SM from L2; 1000 (direct: 1500) to drain a tile; launch, set-up and exit
@@ -640,16 +643,18 @@ int check_backward(const char* action, const objb_linear_backward_desc* d) {
 // scratch, an f32 w read once), where the copy engine can read them as they lie.
 // Every row tile splits x anew and every column tile w, so it pays
 //   * for an f32 w of one narrow column tile (16384 x 4096, 16 tokens: 98 us,
-//     laid out first 182; 64 tokens 180 and 187; 128 tokens 326 and 193);
+//     laid out first 182; 64 tokens 180 and 187; 128 tokens 326 and 193; the
+//     border between 16 and 64 was not searched);
 //   * for results so small that the launch saved counts (250 tokens by 256 of
 //     2048: 14.1 us a call, laid out first 15.7, launches bound; 512 tokens 18.6
-//     and 15.7).  A column tile has 16 columns at least (bf16 w of 16384 x 4096,
-//     one token: 30.8 and 27.8 us).
+//     and 15.7; 2^16 results lie between the two).  A column tile has 16 columns
+//     at least (bf16 w of 16384 x 4096, one token: 30.8 and 27.8 us).
 bool raw_pays(size_t T, size_t N, bool w_f32) {
   return (w_f32 && T <= 32) || std::max<size_t>(T, 16) * N <= (size_t{1} << 16);
 }
 // The same for the gated product (4096 x 2048, 16 tokens: 25.9 and 26.7 us with
-// the down product and one launch less, 64 tokens 35.6 and 31.7).
+// the down product and one launch less, 64 tokens 35.6 and 31.7; the border in
+// between was not searched).
 constexpr size_t kRawTokensFfn = 16;
 
 bool raw_fits(const void* p, size_t ld) { return aligned16(p) && ld % 4 == 0; }

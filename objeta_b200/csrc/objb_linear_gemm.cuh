@@ -50,11 +50,16 @@
 //     pairs lanes i and i + 64 through shared memory (behind the stages, where
 //     a CTA has more than one tile, so that the next one's MMAs go on).
 //
-// What it comes to (bf16, 4096 x 4096 x 4096): 99 us, 1389 TFLOP/s, tensor pipe
-// 70 % busy over the launch and 95 % in the main loop; the library's product
-// 95 us.  In long runs both are bound by power (117 and 110 us at 1.48 GHz).
+// What it comes to (bf16, 4096 x 4096 x 4096, 20 launches replayed from a graph):
+// 99 us, 1389 TFLOP/s, tensor pipe 95 % busy in the main loop (alone, with cold
+// caches, 108 us and 70 % over the launch); the library's product 95 us.  In long
+// runs both are bound by power (117 and 110 us at 1.48 GHz).
 // f32 results: 256 x 128 pair tiles 53 to 55 % busy, bound by the planes that
 // an SM takes in.  Few tokens: bound by w (37 x 2048 x 151936: 6.0 TB/s).
+// Registers are capped to what the CTAs on an SM leave, and some kernels spill:
+// the direct 512 x 256 tiles 88 to 92 bytes a thread at 96 registers, two CTAs of
+// 64 columns on an SM 296 at 80 (32 columns: 84), the splitting ones 16 to 72 at
+// 96; the promoted pair and 128- and 80-column tiles none.
 #pragma once
 
 #include <cuda.h>

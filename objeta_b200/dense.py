@@ -7,7 +7,8 @@ shared expert beside ``moe_pairs``, an output head.  Types: x and w both bf16,
 both f16, x f32 with w bf16, or both f32; y f32 or, where x is a 16-bit type,
 that type.  Any sizes, row strides and element-aligned addresses.  Results
 given by the caller overlap neither each other nor what the call reads, but
-where it says so.
+where it says so.  Results carry no autograd graph: a training loop calls
+``linear_backward`` itself.
 """
 from __future__ import annotations
 

@@ -13,6 +13,8 @@ A step over T tokens, beside ``router_topk_batched`` / ``deepseek_gate``,
                               balance_grad=1e-2, z_grad=1e-3)
     _, dw_router, _ = linear_backward(dlogits, x, w_router, need_dx=False)
 
+Results carry no autograd graph; the gradients are these calls' own.
+
 The reference has no training; the scores are those of its router and gate
 (crates/objeta-cuda/src/bin/deepseek_single_layer_moe.rs:720-740, 768-881).
 """
