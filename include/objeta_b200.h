@@ -729,9 +729,9 @@ int objb_ffn_bf16_tokens_device(const void *d_gate, const void *d_up, const void
 
 /* ---- training the router on frozen experts (no counterpart in the reference).
  * score_func: 0 softmax (the router), 1 sigmoid, 2 sqrt-softplus (the gate,
- * with its branches), as objb_deepseek_gate_device.  A logit of -inf or the
- * lowest f32 has score 0 and gradient 0 (2: every logit whose gate score
- * overflows, below about -88.7).  Tokens that count: those
+ * with its branches), as objb_deepseek_gate_device.  A logit of -inf, or of
+ * the lowest f32 beside larger ones, has score 0 and gradient 0 (under 2 every
+ * logit whose gate score overflows, below about -88.7).  Tokens that count: those
  * of a sequence [d_seq_offsets[q], d_seq_offsets[q+1]) (ascending int32
  * [num_seqs + 1]; NULL: all tokens are sequence 0) whose d_token_mask byte
  * (may be NULL) is nonzero.  Ids outside 0..num_experts-1 count nowhere. */

@@ -122,16 +122,13 @@ __device__ __forceinline__ float score_of(int func, float l, float* d) {
     *d = 0.5f / s;
     return s;
   }
-  const bool low = l < -20.0f;
-  const float ex = expf(low ? -l : l);
-  if (ex == __int_as_float(0x7F800000)) {
-    *d = 0.0f;
-    return 0.0f;
-  }
-  const float s = sqrtf(log1pf(ex));
-  const float sg = low ? 1.0f / (1.0f + expf(l)) : ex / (1.0f + ex);
-  *d = (low ? -0.5f : 0.5f) * sg / s;
-  return s;
+  // (below -20, log1p(exp(-l)) is -l to 1e-10 of it, and its sigmoid 1)
+  const bool low = l < -20.0f, lost = l < -88.72283f;
+  const float ex = expf(l);
+  const float s = sqrtf(low ? -l : log1pf(ex));
+  const float sg = low ? -0.5f : 0.5f * ex / (1.0f + ex);
+  *d = lost ? 0.0f : sg / s;
+  return lost ? 0.0f : s;
 }
 
 // ex = exp(l - base) of a token's logits; returns their sum.  The first try has

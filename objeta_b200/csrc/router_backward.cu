@@ -13,12 +13,12 @@ namespace dev {
 // not be the largest.  With q = exp(l - top) relative to the largest selected (a
 // sigmoid is its exponential there) w = q / sum q and dl = w (dw - mean), not by
 // way of the scores, down to scores of exp(-128), which f32 has long lost; a
-// mask is far below.  One at a time, behind the ordinary tokens and out of
-// line: beside them its registers would cost those 12 % (32768 x 256).
-// `mine`: the team has one (the teams of a warp run in step).  g: zeros, and
+// mask is far below.  One at a time, behind the team's ordinary tokens: beside
+// them its registers would cost those 12 % (32768 x 256), a call of its own
+// 25 % where they fill the registers (2000 experts, sigmoid).  `mine`: the team has one (the teams of a warp run in step).  g: zeros, and
 // left as such.
 template <class TM, int FUNC>
-__device__ __noinline__ void far_token(const RouterBackwardArgs& a, long long t, bool mine, float* g, float* red) {
+__device__ __forceinline__ void far_token(const RouterBackwardArgs& a, long long t, bool mine, float* g, float* red) {
   const int r = TM::rank(), E = mine ? a.E : 0, k = mine ? a.k : 0;
   if (!mine) t = 0;
   const float* l = a.logits + t * a.ld;
@@ -90,7 +90,7 @@ __device__ __noinline__ void far_token(const RouterBackwardArgs& a, long long t,
 
 template <class TM, int FUNC>
 __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
-    router_backward_kernel(const __grid_constant__ RouterBackwardArgs a) {
+    router_backward_kernel(const RouterBackwardArgs a) {
   constexpr int EPL = TM::EPL, L = TM::L;
   extern __shared__ __align__(16) uint8_t router_smem[];
   __shared__ float red[kTeamWarps];
@@ -99,7 +99,12 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
   const int team = TM::kBlock ? 0 : threadIdx.x / L;
   const int Epad = (E + 3) / 4 * 4;
   float* g = reinterpret_cast<float*>(router_smem) + static_cast<size_t>(team) * Epad;  // dL/ds of the selected experts
+  auto far_steps = [&]() {  // a bit per step of the team: its far tokens
+    return reinterpret_cast<unsigned*>(router_smem) + 256 / L * ((a.E + 3) / 4 * 4) +
+           (TM::kBlock ? 0 : threadIdx.x / L) * ((a.per_team + 31) >> 5);
+  };
   for (int e = r; e < Epad; e += L) g[e] = 0.0f;
+  for (int i = r; i < (a.per_team + 31) >> 5; i += L) far_steps()[i] = 0;
   TM::sync();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long t0 = (static_cast<long long>(blockIdx.x) * (256 / L) + team) * a.per_team;
@@ -131,7 +136,6 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
   fetch(t0);
   int q = -1;
   long long q_end = t0;  // where the sequence q ends
-  unsigned aside = 0;  // steps of far tokens (per_team is 32 at most)
   for (int step = 0; step < a.per_team; ++step) {  // the teams of a warp in step
     const long long t = t0 + step;
     const bool here = t < t1;
@@ -315,13 +319,19 @@ __global__ void __launch_bounds__(256, TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1)
         }
       }
     }
-    if (far) aside |= 1u << step;
+    if (far && TM::rank() == 0) far_steps()[step >> 5] |= 1u << (step & 31);
   }
-  if (FUNC != kSqrtSoftplus && (TM::kBlock ? aside != 0 : __any_sync(0xFFFFFFFFu, aside)))
-    for (int step = 0; step < a.per_team; ++step) {
-      const bool mine = aside >> step & 1;
-      if (TM::kBlock ? mine : __any_sync(0xFFFFFFFFu, mine)) far_token<TM, FUNC>(a, t0 + step, mine, g, red);
+  if (FUNC != kSqrtSoftplus) {
+    TM::sync();
+    for (int step = 0; step < a.per_team; step += 32) {
+      const unsigned word = far_steps()[step >> 5];
+      if (TM::kBlock ? word != 0 : __any_sync(0xFFFFFFFFu, word))
+        for (int i = 0; i < 32; ++i) {
+          const bool mine = word >> i & 1;
+          if (TM::kBlock ? mine : __any_sync(0xFFFFFFFFu, mine)) far_token<TM, FUNC>(a, t0 + step + i, mine, g, red);
+        }
     }
+  }
 }
 
 }  // namespace dev
@@ -331,11 +341,13 @@ int launch_router_backward(dev::RouterBackwardArgs a, bool v4, const DeviceProps
     return with_func(a.func, [&](auto func) {
       using TM = decltype(tm);
       const size_t teams = 256 / TM::L;
-      // up to three blocks per SM (what the registers allow), each team a run of consecutive tokens, 32 at most
+      // up to three blocks per SM (what the registers allow), each team a run of consecutive tokens
       const size_t most = static_cast<size_t>(TM::EPL <= 8 ? 3 : TM::EPL <= 16 ? 2 : 1) * props.sm_count * teams;
-      a.per_team = static_cast<int>(std::min<size_t>(32, (static_cast<size_t>(a.T) + most - 1) / most));
+      // of 1024 at most (a bit of shared memory each), in rounds of even length
+      const size_t rounds = (static_cast<size_t>(a.T) + most * 1024 - 1) / (most * 1024);
+      a.per_team = static_cast<int>((static_cast<size_t>(a.T) + most * rounds - 1) / (most * rounds));
       const size_t per_block = teams * a.per_team;
-      const size_t smem = teams * ((static_cast<size_t>(a.E) + 3) / 4 * 4) * 4;
+      const size_t smem = teams * ((static_cast<size_t>(a.E) + 3) / 4 * 4 + (a.per_team + 31) / 32) * 4;
       return launch_pdl(dev::router_backward_kernel<TM, decltype(func)::value>,
                         static_cast<int>((static_cast<size_t>(a.T) + per_block - 1) / per_block), 256, smem, st, a);
     });

@@ -118,8 +118,8 @@ def balance_loss(d_logits, d_ids, score_func: int = SOFTMAX, d_seq_offsets=None,
     * z = 1/N sum_t logsumexp(l_t)^2
 
     (both 0 where no token counts).  Masked experts' logits, -inf or the lowest
-    f32 (under sqrt-softplus all below about -88.7, where the gate's
-    log1p(exp(-l)) overflows), have score 0.  A token whose logits are all -inf
+    f32 beside larger ones (under sqrt-softplus all below about -88.7, where
+    the gate's log1p(exp(-l)) overflows), have score 0.  A token whose logits are all -inf
     counts but adds nothing to either loss.  Sums over tokens are folded in a fixed order:
     the same call gives the same bits.
     """
