@@ -15,8 +15,8 @@ namespace dev {
 // way of the scores, down to scores of exp(-128), which f32 has long lost; a
 // mask is far below.  One at a time, behind the team's ordinary tokens: beside
 // them its registers would cost those 12 % (32768 x 256), a call of its own
-// 25 % where they fill the registers (2000 experts, sigmoid).  `mine`: the team has one (the teams of a warp run in step).  g: zeros, and
-// left as such.
+// 25 % where they fill the registers (2000 experts, sigmoid).  `mine`: the team
+// has one (the teams of a warp run in step).  g: zeros, and left as such.
 template <class TM, int FUNC>
 __device__ __forceinline__ void far_token(const RouterBackwardArgs& a, long long t, bool mine, float* g, float* red) {
   const int r = TM::rank(), E = mine ? a.E : 0, k = mine ? a.k : 0;
@@ -82,7 +82,10 @@ __device__ __forceinline__ void far_token(const RouterBackwardArgs& a, long long
     const float p = exp_sfu(v - base) * inv;
     d = p;
     if (FUNC != kSoftmax) score_of(FUNC, v, &d);
-    a.out[t * a.ld_out + e] = g[e] + d * (B(e) * is - bsum * is * is) + zc * lse * p;
+    float dl = g[e];
+    if (a.counts) dl += d * (B(e) * is - bsum * is * is);
+    if (zc != 0.0f) dl += zc * lse * p;
+    a.out[t * a.ld_out + e] = dl;
     g[e] = 0.0f;
   });
   TM::sync();

@@ -2,9 +2,9 @@
 // sequence by sequence, into partial sums of the scores' shares, selections,
 // lse^2 and counted tokens.  Bound by its instructions (about 200 per token
 // and warp at 256 experts, 24 warps an SM), not by the 4 bytes per logit:
-// 32768 x 256 takes 12.4 us (softmax) or 15.8 (sigmoid), 63 % of an
-// active SM's issue slots, where the logits alone take 5.2.  Logits further than 11.5 from 0 take
-// their maximum first (a call of both launches 19 -> 22 and 21 -> 29 us).
+// 32768 x 256 takes 12.4 us (softmax) or 15.8 (sigmoid), 63 % of an active SM's
+// issue slots, where the logits alone take 5.2.  Logits further than 11.5 from 0
+// take their maximum first (a call of both launches 19 -> 22 and 21 -> 29 us).
 #include "objb_router.cuh"
 #include "objb_router_finish.cuh"
 

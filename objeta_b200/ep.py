@@ -423,8 +423,9 @@ class ExpertParallelMoe:
         if gate.dim() != 2 or gate.shape != up.shape or down.shape != (self.out_dim, gate.shape[0]):
             raise ValueError(f"shared expert shapes {tuple(gate.shape)}, {tuple(up.shape)}, {tuple(down.shape)} "
                              f"do not make [I, H], [I, H], [{self.out_dim}, I]")
-        if self.layer is not None and gate.shape[1] != self.layer.hidden:
-            raise ValueError(f"shared expert of hidden size {gate.shape[1]} beside a layer of {self.layer.hidden}")
+        hidden = getattr(self.layer, "hidden", gate.shape[1])
+        if gate.shape[1] != hidden:
+            raise ValueError(f"shared expert of hidden size {gate.shape[1]} beside a layer of {hidden}")
         for name, t in zip(("gate", "up", "down"), (gate, up, down)):
             if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != gate.device or not t.is_cuda:
                 raise ValueError(f"shared expert {name}: expected contiguous bf16 CUDA tensors on one device, got "

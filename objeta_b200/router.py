@@ -119,8 +119,9 @@ def balance_loss(d_logits, d_ids, score_func: int = SOFTMAX, d_seq_offsets=None,
 
     (both 0 where no token counts).  Masked experts' logits, -inf or the lowest
     f32 beside larger ones (under sqrt-softplus all below about -88.7, where
-    the gate's log1p(exp(-l)) overflows), have score 0.  A token whose logits are all -inf
-    counts but adds nothing to either loss.  Sums over tokens are folded in a fixed order:
+    the gate's log1p(exp(-l)) overflows), have score 0.  A token whose logits
+    are all -inf counts but adds nothing to either loss.  Sums over tokens are
+    folded in a fixed order:
     the same call gives the same bits.
     """
     dev, ld, T, E, k, S, mask, off = _routing(d_logits, d_ids, d_seq_offsets, d_token_mask)
